@@ -13,7 +13,10 @@ exports the decode operators built for MI355X:
 * ``paged_attention`` -- MHA / GQA decode over a paged KV cache (``paged.py:20-177``);
 * ``flash_attention_split_kv`` -- flash decoding over contiguous K/V (``split_kv.py:280-344``);
 * ``flash_attention`` -- the forward of ``flash.py:269-300`` through its split-KV decode
-  path (no dropout, no total attention, no backward).
+  path (no dropout, no total attention, no backward);
+* ``flash_attention_varlen`` -- prompt attention over packed sequences of different lengths;
+* ``cache_kv_mxfp4`` / ``gather_kv_mxfp4`` / ``paged_attention_mxfp4`` -- a paged K/V cache in
+  4 bits: its writer, its reader and one-token decode over it.
 
 Every operator runs in ``flagattention_amd/libflagattention_amd.so`` (hand-written HIP for
 gfx950); there is no Triton and no CPU fallback.  The reference's training-path operators
@@ -29,8 +32,13 @@ from flag_attn.mla import (  # noqa: F401
 from flag_attn.paged import attention as paged_attention  # noqa: F401
 from flag_attn.split_kv import attention as flash_attention_split_kv  # noqa: F401
 from flag_attn.flash import attention as flash_attention  # noqa: F401
+from flag_attn.varlen import attention as flash_attention_varlen  # noqa: F401
+from flag_attn.mxfp4 import attention as paged_attention_mxfp4  # noqa: F401
+from flag_attn.mxfp4 import cache_kv as cache_kv_mxfp4  # noqa: F401
+from flag_attn.mxfp4 import gather_kv as gather_kv_mxfp4  # noqa: F401
 
 __all__ = ["get_mla_metadata", "flash_mla_with_kvcache", "concat_and_cache_mla", "topk_indices",
            "paged_attention",
-           "flash_attention_split_kv", "flash_attention"]
+           "flash_attention_split_kv", "flash_attention", "flash_attention_varlen",
+           "cache_kv_mxfp4", "gather_kv_mxfp4", "paged_attention_mxfp4"]
 __version__ = "0.2.0"

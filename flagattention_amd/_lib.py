@@ -1,4 +1,4 @@
-"""ctypes binding of libflagattention_amd.so (the C ABI in include/flagattention_amd.h).
+"""ctypes binding of libflagattention_amd.so (the C ABI in include/flagattention_amd*.h).
 
 The library is loaded on first use.  If it is missing or was built for another ABI
 version, every call raises ``RuntimeError``: there is no fallback path.
@@ -98,6 +98,88 @@ class GqaArgs(ctypes.Structure):
     ]
 
 
+class VarlenArgs(ctypes.Structure):
+    """Mirror of ``fa_varlen_args`` (field order and types must match the header)."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("q_stride_t", ctypes.c_int64),
+        ("q_stride_h", ctypes.c_int64),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_stride_t", ctypes.c_int64),
+        ("k_stride_h", ctypes.c_int64),
+        ("v_stride_t", ctypes.c_int64),
+        ("v_stride_h", ctypes.c_int64),
+        ("cu_seqlens_q", ctypes.c_void_p),
+        ("cu_seqlens_k", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("o_stride_t", ctypes.c_int64),
+        ("o_stride_h", ctypes.c_int64),
+        ("lse", ctypes.c_void_p),
+        ("o_part", ctypes.c_void_p),
+        ("lse_part", ctypes.c_void_p),
+        ("num_seqs", ctypes.c_int32),
+        ("total_q", ctypes.c_int32),
+        ("total_k", ctypes.c_int32),
+        ("h_q", ctypes.c_int32),
+        ("h_kv", ctypes.c_int32),
+        ("d", ctypes.c_int32),
+        ("num_splits", ctypes.c_int32),
+        ("split_tokens", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("causal", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class Mxfp4Cache(ctypes.Structure):
+    """Mirror of ``fa_mxfp4_cache``."""
+
+    _fields_ = [
+        ("k_codes", ctypes.c_void_p),
+        ("k_scales", ctypes.c_void_p),
+        ("v_codes", ctypes.c_void_p),
+        ("v_scales", ctypes.c_void_p),
+        ("code_stride_0", ctypes.c_int64),
+        ("code_stride_h", ctypes.c_int64),
+        ("code_stride_t", ctypes.c_int64),
+        ("scale_stride_0", ctypes.c_int64),
+        ("scale_stride_h", ctypes.c_int64),
+        ("scale_stride_t", ctypes.c_int64),
+        ("num_blocks", ctypes.c_int64),
+        ("block_size", ctypes.c_int32),
+        ("h_kv", ctypes.c_int32),
+        ("d", ctypes.c_int32),
+    ]
+
+
+class Mxfp4DecodeArgs(ctypes.Structure):
+    """Mirror of ``fa_mxfp4_decode_args``."""
+
+    _fields_ = [
+        ("cache", Mxfp4Cache),
+        ("q", ctypes.c_void_p),
+        ("q_stride_b", ctypes.c_int64),
+        ("q_stride_h", ctypes.c_int64),
+        ("block_table", ctypes.c_void_p),
+        ("bt_stride_b", ctypes.c_int64),
+        ("max_blocks_per_seq", ctypes.c_int32),
+        ("seqlens", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("o_stride_b", ctypes.c_int64),
+        ("o_stride_h", ctypes.c_int64),
+        ("o_part", ctypes.c_void_p),
+        ("lse_part", ctypes.c_void_p),
+        ("batch", ctypes.c_int32),
+        ("h_q", ctypes.c_int32),
+        ("num_splits", ctypes.c_int32),
+        ("split_tokens", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
 # name -> (restype, argtypes) for every symbol declared in the header
 SIGNATURES = {
     "fa_abi_version": (ctypes.c_int, []),
@@ -132,6 +214,23 @@ SIGNATURES = {
     "fa_mla_noalloc_scratch_bytes": (ctypes.c_int64, [ctypes.POINTER(DecodeArgs), ctypes.c_int32]),
     "fa_mla_decode_noalloc": (
         ctypes.c_int, [ctypes.POINTER(DecodeArgs), ctypes.c_int32, ctypes.c_void_p]),
+    "fa_varlen_args_size": (ctypes.c_int64, []),
+    "fa_varlen_attention": (ctypes.c_int, [ctypes.POINTER(VarlenArgs), ctypes.c_void_p]),
+    "fa_varlen_combine": (ctypes.c_int, [ctypes.POINTER(VarlenArgs), ctypes.c_void_p]),
+    "fa_mxfp4_cache_size": (ctypes.c_int64, []),
+    "fa_mxfp4_cache_write": (
+        ctypes.c_int,
+        [ctypes.POINTER(Mxfp4Cache), ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
+         ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int32,
+         ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]),
+    "fa_mxfp4_gather": (
+        ctypes.c_int,
+        [ctypes.POINTER(Mxfp4Cache), ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32,
+         ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p,
+         ctypes.c_int32, ctypes.c_void_p]),
+    "fa_mxfp4_decode_args_size": (ctypes.c_int64, []),
+    "fa_mxfp4_decode": (ctypes.c_int, [ctypes.POINTER(Mxfp4DecodeArgs), ctypes.c_void_p]),
+    "fa_mxfp4_combine": (ctypes.c_int, [ctypes.POINTER(Mxfp4DecodeArgs), ctypes.c_void_p]),
 }
 
 _lock = threading.Lock()
@@ -158,16 +257,14 @@ def load() -> ctypes.CDLL:
         ver = lib.fa_abi_version()
         if ver != ABI_VERSION:
             raise RuntimeError(f"flagattention_amd: library ABI {ver} != binding ABI {ABI_VERSION}")
-        size = lib.fa_mla_decode_args_size()
-        if size != ctypes.sizeof(DecodeArgs):
-            raise RuntimeError(
-                f"flagattention_amd: fa_mla_decode_args is {size} bytes in the library, "
-                f"{ctypes.sizeof(DecodeArgs)} in the binding")
-        gsize = lib.fa_gqa_decode_args_size()
-        if gsize != ctypes.sizeof(GqaArgs):
-            raise RuntimeError(
-                f"flagattention_amd: fa_gqa_decode_args is {gsize} bytes in the library, "
-                f"{ctypes.sizeof(GqaArgs)} in the binding")
+        for name, mirror in (("fa_mla_decode_args", DecodeArgs), ("fa_gqa_decode_args", GqaArgs),
+                             ("fa_varlen_args", VarlenArgs), ("fa_mxfp4_cache", Mxfp4Cache),
+                             ("fa_mxfp4_decode_args", Mxfp4DecodeArgs)):
+            size = getattr(lib, name + "_size")()
+            if size != ctypes.sizeof(mirror):
+                raise RuntimeError(
+                    f"flagattention_amd: {name} is {size} bytes in the library, "
+                    f"{ctypes.sizeof(mirror)} in the binding")
         _lib = lib
         return lib
 

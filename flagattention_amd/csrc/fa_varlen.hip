@@ -1,0 +1,480 @@
+// Prompt attention over packed sequences for gfx950: fp16 or bf16, head dim 64, 128, 256.
+//
+// A work-group = 4 waves = 128 query rows of one (sequence, KV head), 32 per wave, which share
+// every K/V tile through LDS.  A query row is a (position, query head of the group) pair, positions
+// outermost.  Row blocks lie inside one sequence, so the grid is the bound that the host knows --
+// every sequence rounds its last block up -- and a work-group finds its sequence from the starts,
+// which only the device knows.
+//
+// Per tile of 64 keys (32 at head dim 256) and wave, all MFMA 32x32x16, fp32 accumulation:
+//   S^T[keys, 32 rows] = K Q^T, softmax down the columns (lane % 32 = row), O^T[D, 32 rows] +=
+//   V^T P^T with P^T the lane's own scores (the k order only has to agree between the operands).
+#include "fa_common.h"
+#include "fa_rows_tile.h"
+#include "fa_wave.h"
+#include "flagattention_amd_packed.h"
+
+namespace fa {
+namespace {
+
+constexpr int kLWaves = 4;
+constexpr int kLThreads = 64 * kLWaves;
+constexpr int kLWaveRows = 32;
+constexpr int kLRows = kLWaves * kLWaveRows;
+// Past this reference (log2 units) the scores are scaled in a pass of their own: a fused
+// multiply-add does not round their product with the scale, which the reference is made of.
+constexpr float kFusedMax = 1024.f;
+
+// Largest |x| of packed 16-bit values as unsigned bit patterns, folded into best.
+__device__ inline void fold_bits(unsigned int& best, uintx4 w) {
+  typedef unsigned short ushortx2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    best = __builtin_bit_cast(
+        unsigned int, __builtin_elementwise_max(__builtin_bit_cast(ushortx2, best),
+                                                __builtin_bit_cast(ushortx2, w[i] & 0x7FFF7FFFu)));
+}
+
+struct Item {
+  int q0, rows;  // first packed position, rows (positions x group) of the sequence
+  int k0, n;     // first packed key, keys
+  int block;     // row block, -1: none left
+};
+
+__device__ inline int clip(int x, int hi) { return min(max(x, 0), hi); }
+
+// The sequence and row block of work item `item`: blocks of the sequences one after the other, the
+// last of a sequence (the longest under a causal mask) first.  The rows behind the last sequence and
+// those before the first are two more, without keys.
+__device__ inline Item find_item(const fa_varlen_args& a, int group, int item) {
+  const int lane = threadIdx.x & 63;
+  for (int base = 0; base <= a.num_seqs + 1; base += 64) {
+    const int s = base + lane;
+    int q0 = 0, m = 0, k0 = 0, n = 0;
+    if (s < a.num_seqs) {
+      q0 = clip(a.cu_seqlens_q[s], a.total_q);
+      m = max(clip(a.cu_seqlens_q[s + 1], a.total_q) - q0, 0);
+      k0 = clip(a.cu_seqlens_k[s], a.total_k);
+      n = max(clip(a.cu_seqlens_k[s + 1], a.total_k) - k0, 0);
+    } else if (s == a.num_seqs) {
+      q0 = clip(a.cu_seqlens_q[s], a.total_q);
+      m = a.total_q - q0;
+    } else if (s == a.num_seqs + 1) {
+      m = clip(a.cu_seqlens_q[0], a.total_q);
+    }
+    const int blocks = cdiv(m * group, kLRows);
+    const int upto = wave_incl_scan(blocks);
+    const unsigned long long past = __ballot(upto > item);
+    if (past != 0ull) {
+      const int l = __builtin_ctzll(past);
+      Item it;
+      it.q0 = __builtin_amdgcn_readlane(q0, l);
+      it.rows = __builtin_amdgcn_readlane(m, l) * group;
+      it.k0 = __builtin_amdgcn_readlane(k0, l);
+      it.n = __builtin_amdgcn_readlane(n, l);
+      it.block = __builtin_amdgcn_readlane(upto, l) - 1 - item;
+      return it;
+    }
+    item -= __builtin_amdgcn_readlane(upto, 63);
+  }
+  return Item{0, 0, 0, 0, -1};
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_args a) {
+  typedef typename PVec<T>::v8 T8;
+  typedef typename PVec<T>::v4 T4;
+  constexpr int C = D / 8;
+  constexpr int kRowB = 2 * D;
+  constexpr int kTok = D <= 128 ? 64 : 32;
+  constexpr int kSub = kTok / 32;
+  constexpr int kTileB = kTok * kRowB;
+  constexpr int kCopies = kTileB / 1024 / kLWaves;
+  constexpr int kRowsPerCopy = 1024 / kRowB;
+  constexpr int kKSteps = D / 16;
+  constexpr int kDimTiles = D / 32;
+  static_assert(kCopies * kLWaves * 1024 == kTileB, "whole copies per wave");
+  // [K, V][tile parity]; the epilogue stages each wave's 32 output rows over them
+  __shared__ __attribute__((aligned(16))) unsigned char bufs[4 * kTileB];
+  static_assert(4 * kTileB >= kLRows * kRowB, "output staging fits the tile buffers");
+  __shared__ int odd_v[2][kLWaves];  // [tile parity][wave]: see below
+
+  const int group = a.h_q / a.h_kv;
+  const int hk = blockIdx.x % a.h_kv;
+  const Item it = find_item(a, group, blockIdx.x / a.h_kv);
+  if (it.block < 0) return;  // uniform
+  const int split = blockIdx.y;
+  const int m = it.rows / group;
+
+  const int wave = wave_id();
+  const int lane = threadIdx.x & 63;
+  const int g = lane >> 5, c32 = lane & 31;
+
+  const int t0 = split * a.split_tokens;
+  const int t1 = split + 1 == a.num_splits ? it.n : min(t0 + a.split_tokens, it.n);
+  // keys visible to a row: [0, n - m + 1 + position) causal, all otherwise
+  auto limit_of = [&](int row) -> int {
+    return a.causal ? min(it.n - m + 1 + row / group, t1) : t1;
+  };
+  const int row0 = it.block * kLRows;
+  const int wg_lim = limit_of(min(row0 + kLRows, it.rows) - 1);
+  const int wg_min = limit_of(row0);
+  const int ntiles = wg_lim > t0 ? cdiv(wg_lim - t0, kTok) : 0;
+  const int wrow0 = row0 + kLWaveRows * wave;
+  const int wave_min = limit_of(min(wrow0, it.rows - 1));
+  const int wave_max = limit_of(min(wrow0 + kLWaveRows, it.rows) - 1);
+  const bool wave_on = wrow0 < it.rows;
+  const int row = min(wrow0 + c32, it.rows - 1);  // past the end: the last row, not stored
+  const int mm = row / group, jj = row - mm * group;
+  const int lim = limit_of(row);
+
+  const float ninf = -__builtin_inff();
+  // The scale is applied inside the exponent, after the mask and the maximum.  That needs a
+  // positive one: otherwise the scores are scaled before either.
+  const bool prescale = !(a.scale > 0.f);  // uniform
+  const float scale_log2 = prescale ? 1.f : a.scale * kLog2e;
+
+  const unsigned char* const kp = static_cast<const unsigned char*>(a.k) +
+                                  2 * (it.k0 * a.k_stride_t + hk * a.k_stride_h);
+  const unsigned char* const vp = static_cast<const unsigned char*>(a.v) +
+                                  2 * (it.k0 * a.v_stride_t + hk * a.v_stride_h);
+  // 32-bit lane offsets inside a tile (host check)
+  const unsigned int k_tb = static_cast<unsigned int>(2 * a.k_stride_t);
+  const unsigned int v_tb = static_cast<unsigned int>(2 * a.v_stride_t);
+  const int crow = lane / C, cslot = lane % C;
+  unsigned int koff[kCopies], voff[kCopies];
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i) {
+    const int r = (kCopies * wave + i) * kRowsPerCopy + crow;
+    koff[i] = r * k_tb + 16 * (cslot ^ fk<C>(r));
+    voff[i] = r * v_tb + 16 * (cslot ^ (fv<C>(r) << 1));
+  }
+  auto issue = [&](int u, int buf) {
+    const int start = t0 + kTok * u;
+    const unsigned char* const ks = kp + static_cast<long long>(start) * k_tb;
+    const unsigned char* const vs = vp + static_cast<long long>(start) * v_tb;
+    unsigned char* const kd = bufs + buf * kTileB + kCopies * wave * 1024;
+    unsigned char* const vd = bufs + (2 + buf) * kTileB + kCopies * wave * 1024;
+    const int last = t1 - 1 - start;  // rows past the end repeat the last one (masked)
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const int r = (kCopies * wave + i) * kRowsPerCopy + crow;
+      const unsigned int back = r > last ? r - last : 0;
+      lds_dma16_off(ks, koff[i] - back * k_tb, (FA_LDS void*)(kd + 1024 * i));
+      lds_dma16_off(vs, voff[i] - back * v_tb, (FA_LDS void*)(vd + 1024 * i));
+    }
+  };
+
+  // Q^T operand: row c32, dims 16kk + 8g..+7
+  T8 qf[kKSteps];
+  {
+    const T* const qrow = static_cast<const T*>(a.q) + (it.q0 + mm) * a.q_stride_t +
+                          (hk * group + jj) * a.q_stride_h + 8 * g;
+#pragma unroll
+    for (int kk = 0; kk < kKSteps; ++kk) qf[kk] = *reinterpret_cast<const T8*>(qrow + 16 * kk);
+  }
+
+  floatx16 acc[kDimTiles];
+#pragma unroll
+  for (int dt = 0; dt < kDimTiles; ++dt) acc[dt] = floatx16{};
+  float mref = ninf, lsum = 0.f;
+
+  // lane offsets of the LDS reads
+  const int kbase = c32 * kRowB + 16 * (g ^ fk<C>(c32));  // chunk 2kk + g: xor 32 kk
+  const int h16 = lane >> 4, e = (lane & 15) >> 2, qd = lane & 3;
+  const int vtok = 4 * g + e;  // token within 8
+  constexpr int kVBases = kDimTiles < 4 ? kDimTiles : 4;  // fv < 8: dt + 4 is 256 bytes on
+  int vbase[kVBases];
+#pragma unroll
+  for (int dt = 0; dt < kVBases; ++dt)
+    vbase[dt] = vtok * kRowB + 32 * ((2 * dt + (h16 & 1)) ^ fv<C>(vtok)) + 16 * (qd >> 1) +
+                8 * (qd & 1);
+
+  if (ntiles > 0) issue(0, 0);
+  for (int u = 0; u < ntiles; ++u) {
+    const int buf = u & 1;
+    const int start = t0 + kTok * u;
+    wait_vmem<0>();  // this wave's copies of tile u (requested one step ago)
+    // A weight of 0 does not hide an infinity or a NaN in V: 0 times either is NaN.  A tile that
+    // some row sees in part is looked through for them (each wave its own copies).
+    const bool part_seen = a.causal && start + kTok > wg_min;  // uniform
+    if (part_seen) {
+      unsigned int best = 0u;
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i)
+        fold_bits(best, *reinterpret_cast<const uintx4*>(bufs + (2 + buf) * kTileB +
+                                                         (kCopies * wave + i) * 1024 + 16 * lane));
+      constexpr unsigned int kInf = __is_same(T, __bf16) ? 0x7F80u : 0x7C00u;
+      const bool any = __ballot((best & 0xFFFFu) >= kInf || (best >> 16) >= kInf) != 0ull;
+      if (lane == 0) odd_v[buf][wave] = any;
+    }
+    barrier();  // everyone's copies; and everyone is done with tile u-1
+    if (u + 1 < ntiles) issue(u + 1, buf ^ 1);
+    const bool odd = part_seen && (odd_v[buf][0] | odd_v[buf][1] | odd_v[buf][2] | odd_v[buf][3]) != 0;
+    // every wave takes its odd values out of its own copies once all have used them
+    auto clean_tile = [&] {
+      barrier();
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        T8* const p = reinterpret_cast<T8*>(bufs + (2 + buf) * kTileB +
+                                            (kCopies * wave + i) * 1024 + 16 * lane);
+        T8 w = *p;
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          w[x] = fabsf(static_cast<float>(w[x])) < __builtin_inff() ? w[x] : static_cast<T>(0.f);
+        *p = w;
+      }
+      barrier();
+    };
+    if (!wave_on || start >= wave_max) {  // uniform: no row of the wave sees a key here
+      if (odd) clean_tile();              // uniform over the work-group
+      continue;
+    }
+    const unsigned char* const kb = bufs + buf * kTileB;
+    const unsigned char* const vb = bufs + (2 + buf) * kTileB;
+
+    floatx16 s[kSub];
+#pragma unroll
+    for (int tt = 0; tt < kSub; ++tt) {
+      s[tt] = floatx16{};
+#pragma unroll
+      for (int kk = 0; kk < kKSteps; ++kk)
+        s[tt] = mfma_32x32x16(
+            *reinterpret_cast<const T8*>(kb + 32 * tt * kRowB + (kbase ^ (32 * kk))), qf[kk], s[tt]);
+    }
+    if (prescale) {
+#pragma unroll
+      for (int tt = 0; tt < kSub; ++tt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[tt][i] *= a.scale * kLog2e;
+    }
+    const bool masked = start + kTok > wave_min;  // uniform: some row does not see the whole tile
+    if (masked) {
+      const int left = lim - start - 4 * g;
+#pragma unroll
+      for (int tt = 0; tt < kSub; ++tt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int j = 32 * tt + 8 * (i >> 2) + (i & 3);  // + 4g: the key of s[tt][i]
+          s[tt][i] = j < left ? s[tt][i] : ninf;
+        }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int tt = 0; tt < kSub; ++tt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[tt][i]);
+    mx = max_xor32(mx) * scale_log2;
+    const float m_new = fmaxf(mref, mx);
+    const float alpha = m_new == ninf ? 1.f : __builtin_amdgcn_exp2f(mref - m_new);
+    lsum *= alpha;
+    mref = m_new;
+#pragma unroll
+    for (int dt = 0; dt < kDimTiles; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[dt][i] *= alpha;
+    const float nm = mref == ninf ? 0.f : -mref;
+    float c = scale_log2;
+    if (__ballot(fabsf(nm) > kFusedMax) != 0ull) {  // uniform
+#pragma unroll
+      for (int tt = 0; tt < kSub; ++tt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[tt][i] *= c;
+      c = 1.f;
+    }
+    T8 pb[2 * kSub];
+    float ps = 0.f;
+#pragma unroll
+    for (int ss = 0; ss < 2 * kSub; ++ss)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float p =
+            __builtin_amdgcn_exp2f(__builtin_fmaf(s[ss >> 1][8 * (ss & 1) + i], c, nm));
+        ps += p;
+        pb[ss][i] = static_cast<T>(p);
+      }
+    lsum += ps;
+    if (odd) {
+      // An infinity or a NaN goes to the rows that see its key as it is, and out of the tile.
+      for (int j = 0; j < kTok; ++j) {
+        const bool sees = start + j < lim;
+#pragma unroll
+        for (int dt = 0; dt < kDimTiles; ++dt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {  // dims 32dt + 8i + 4g..+3: chunk 4dt + i
+            const T4 v4 = *reinterpret_cast<const T4*>(
+                vb + j * kRowB + 16 * ((4 * dt + i) ^ (fv<C>(j) << 1)) + 8 * g);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const float f = static_cast<float>(v4[x]);
+              acc[dt][4 * i + x] += sees && !(fabsf(f) < __builtin_inff()) ? f : 0.f;
+            }
+          }
+      }
+      clean_tile();
+    }
+#pragma unroll
+    for (int ss = 0; ss < 2 * kSub; ++ss)
+#pragma unroll
+      for (int dt = 0; dt < kDimTiles; ++dt) {
+        const unsigned char* const p = vb + 16 * ss * kRowB + 256 * (dt >> 2) + vbase[dt & 3];
+        const T4 lo = lds_tr_read4<T>(p);
+        const T4 hi = lds_tr_read4<T>(p + 8 * kRowB);
+        const T8 va = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        acc[dt] = mfma_32x32x16(va, pb[ss], acc[dt]);
+      }
+  }
+  wait_vmem<0>();
+  barrier();  // the tile buffers are free
+  if (!wave_on) return;
+
+  const float l = sum_xor32(lsum);
+  const bool some = !(l == 0.f);  // else no visible key: out 0, lse -inf (NaN sums stay NaN)
+  const float inv = some ? 1.f / l : 0.f;
+  const float lse = some ? (mref + log2f(l)) * kLn2 : ninf;
+  const int h = hk * group + jj;
+  const long long orow = static_cast<long long>(h) * a.total_q + it.q0 + mm;
+  const bool mine = wrow0 + c32 < it.rows;
+  if (a.num_splits > 1) {
+    if (mine) {
+      const long long prow = orow * a.num_splits + split;
+      float* const op = a.o_part + prow * D + 4 * g;
+#pragma unroll
+      for (int dt = 0; dt < kDimTiles; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          floatx4 w;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) w[x] = some ? acc[dt][4 * i + x] * inv : 0.f;
+          *reinterpret_cast<floatx4*>(op + 32 * dt + 8 * i) = w;
+        }
+      // the merge takes the largest lse, which a NaN would not be
+      if (g == 0) a.lse_part[prow] = lse == lse ? lse : -ninf;
+    }
+    return;
+  }
+  if (mine && g == 0 && a.lse) a.lse[orow] = lse;
+  // whole output rows through LDS (the wave's own 32 rows): 16 bytes per lane and store
+  unsigned char* const st = bufs + wave * kLWaveRows * kRowB;
+#pragma unroll
+  for (int dt = 0; dt < kDimTiles; ++dt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      T4 w;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) w[x] = static_cast<T>(some ? acc[dt][4 * i + x] * inv : 0.f);
+      *reinterpret_cast<T4*>(st + c32 * kRowB + 16 * ((4 * dt + i) ^ (c32 & 7)) + 8 * g) = w;
+    }
+  asm volatile("" ::: "memory");
+  wait_lds();
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < kLWaveRows * kRowB / 1024; ++i) {
+    const int r = i * kRowsPerCopy + crow;
+    const int rr = wrow0 + r;
+    const T8 v = *reinterpret_cast<const T8*>(st + r * kRowB + 16 * (cslot ^ (r & 7)));
+    if (rr < it.rows) {
+      const int m2 = rr / group, j2 = rr - m2 * group;
+      *reinterpret_cast<T8*>(static_cast<T*>(a.out) + (it.q0 + m2) * a.o_stride_t +
+                             (hk * group + j2) * a.o_stride_h + 8 * cslot) = v;
+    }
+  }
+}
+
+// Row blocks per KV head at most: each sequence, and the rows behind the last and before the
+// first, rounds up once.
+long long row_blocks(const fa_varlen_args* a) {
+  return static_cast<long long>(a->total_q) * (a->h_q / a->h_kv) / kLRows + a->num_seqs + 2;
+}
+
+template <typename T>
+void launch_varlen(const fa_varlen_args* a, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(row_blocks(a) * a->h_kv),
+                  static_cast<unsigned>(a->num_splits));
+  if (a->d == 64)
+    hipLaunchKernelGGL((varlen_kernel<T, 64>), grid, dim3(kLThreads), 0, stream, *a);
+  else if (a->d == 128)
+    hipLaunchKernelGGL((varlen_kernel<T, 128>), grid, dim3(kLThreads), 0, stream, *a);
+  else
+    hipLaunchKernelGGL((varlen_kernel<T, 256>), grid, dim3(kLThreads), 0, stream, *a);
+}
+
+bool rows16(const void* p, int64_t s0, int64_t s1) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s0 % 8 == 0 && s1 % 8 == 0;
+}
+
+int check_varlen(const fa_varlen_args* a) {
+  FA_CHECK_ARG(a != nullptr, "args is NULL");
+  FA_CHECK_ARG(a->num_seqs >= 0 && a->total_q >= 1 && a->total_k >= 0,
+               "num_seqs %d / total_q %d / total_k %d invalid", a->num_seqs, a->total_q, a->total_k);
+  FA_CHECK_ARG(a->h_q >= 1 && a->h_kv >= 1 && a->h_q % a->h_kv == 0,
+               "h_q %d is not a multiple of h_kv %d", a->h_q, a->h_kv);
+  FA_CHECK_ARG(a->d == 64 || a->d == 128 || a->d == 256, "head dim %d not in {64, 128, 256}", a->d);
+  FA_CHECK_ARG(a->dtype == 0 || a->dtype == 1, "dtype %d is not 0 (fp16) or 1 (bf16)", a->dtype);
+  FA_CHECK_ARG(a->q && a->out && a->cu_seqlens_q && a->cu_seqlens_k &&
+                   (a->total_k == 0 || (a->k && a->v)),
+               "NULL q / k / v / out / cu_seqlens");
+  FA_CHECK_ARG(rows16(a->q, a->q_stride_t, a->q_stride_h) &&
+                   rows16(a->k, a->k_stride_t, a->k_stride_h) &&
+                   rows16(a->v, a->v_stride_t, a->v_stride_h) &&
+                   rows16(a->out, a->o_stride_t, a->o_stride_h),
+               "q / k / v / out rows must be 16-byte aligned");
+  // 32-bit lane offsets inside a tile
+  FA_CHECK_ARG(a->k_stride_t >= 0 && a->v_stride_t >= 0 && a->k_stride_t < (1ll << 23) &&
+                   a->v_stride_t < (1ll << 23),
+               "k / v token strides must be in [0, 2^23)");
+  FA_CHECK_ARG(static_cast<long long>(a->total_q) * (a->h_q / a->h_kv) < (1ll << 30) &&
+                   row_blocks(a) * a->h_kv < (1ll << 30),
+               "too many query rows or row blocks");
+  FA_CHECK_ARG(a->num_splits >= 1 && a->num_splits <= 65535 && a->split_tokens >= 1 &&
+                   static_cast<int64_t>(a->num_splits - 1) * a->split_tokens <= INT32_MAX,
+               "num_splits %d of %d tokens invalid", a->num_splits, a->split_tokens);
+  FA_CHECK_ARG(a->num_splits == 1 || (a->o_part && a->lse_part),
+               "num_splits %d > 1 needs o_part and lse_part", a->num_splits);
+  // the merge's own limit
+  FA_CHECK_ARG(a->num_splits == 1 ||
+                   a->h_kv * ((static_cast<long long>(a->h_q / a->h_kv) * a->total_q + 15) / 16) <=
+                       65535,
+               "too many query rows for splits");
+  return FA_OK;
+}
+
+}  // namespace
+}  // namespace fa
+
+extern "C" int64_t fa_varlen_args_size(void) { return static_cast<int64_t>(sizeof(fa_varlen_args)); }
+
+extern "C" int fa_varlen_attention(const fa_varlen_args* a, void* stream) {
+  const int rc = fa::check_varlen(a);
+  if (rc != FA_OK) return rc;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (a->dtype == 1)
+    fa::launch_varlen<__bf16>(a, s);
+  else
+    fa::launch_varlen<_Float16>(a, s);
+  FA_CHECK_HIP(hipGetLastError());
+  return FA_OK;
+}
+
+extern "C" int fa_varlen_combine(const fa_varlen_args* a, void* stream) {
+  const int rc = fa::check_varlen(a);
+  if (rc != FA_OK) return rc;
+  FA_CHECK_ARG(a->o_part && a->lse_part, "combine needs o_part and lse_part");
+  fa_gqa_decode_args g = {};  // one batch entry of total_q positions; reads the partial rows alone
+  g.q = g.k = g.v = a->q;
+  g.out = a->out;
+  g.o_stride_h = a->o_stride_h;
+  g.o_stride_m = a->o_stride_t;
+  g.lse = a->lse;
+  g.o_part = a->o_part;
+  g.lse_part = a->lse_part;
+  g.batch = 1;
+  g.h_q = a->h_q;
+  g.h_kv = a->h_kv;
+  g.m = a->total_q;
+  g.d = a->d;
+  g.num_splits = a->num_splits;
+  g.split_tokens = a->split_tokens;
+  g.dtype = a->dtype;
+  return fa_gqa_combine(&g, stream);
+}

@@ -1,0 +1,241 @@
+"""Prompt attention over packed sequences (flag_attn.flash_attention_varlen) against the formula
+in 64 bits, with tolerances made of the roundings it makes (tests/_packed.py)."""
+import math
+
+import pytest
+import torch
+
+import flag_attn
+from flagattention_amd import varlen
+from oracle import packed_oracle as po
+from tests._helpers import DEV, need_gpu, say
+from tests._packed import assert_lse, assert_rows
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float16, torch.bfloat16]
+
+
+def starts(lens):
+    out = [0]
+    for n in lens:
+        out.append(out[-1] + n)
+    return out
+
+
+def inputs(lens_q, lens_k, h, hk, d, dtype, seed=0, extra_q=0, extra_k=0, spread=1.0):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+
+    def rows(n, heads, gain):
+        return (torch.randn((n, heads, d), generator=gen, device=DEV) * gain).to(dtype)
+
+    return (rows(sum(lens_q) + extra_q, h, spread), rows(sum(lens_k) + extra_k, hk, spread),
+            rows(sum(lens_k) + extra_k, hk, 1.0), starts(lens_q), starts(lens_k))
+
+
+def call(q, k, v, cu_q, cu_k, causal, scale=None, max_k=None):
+    cq, ck = (torch.tensor(c, dtype=torch.int32, device=DEV) for c in (cu_q, cu_k))
+    max_q = max((b - a for a, b in zip(cu_q, cu_q[1:])), default=0)
+    if max_k is None:
+        max_k = max((b - a for a, b in zip(cu_k, cu_k[1:])), default=0)
+    return flag_attn.flash_attention_varlen(q, k, v, cq, ck, max_q, max_k, causal, scale,
+                                            return_log_normalizer=True)
+
+
+def check(q, k, v, cu_q, cu_k, causal, scale=None, max_k=None):
+    o, lse = call(q, k, v, cu_q, cu_k, causal, scale, max_k)
+    torch.cuda.synchronize()
+    d = q.shape[-1]
+    ref, ref_lse, a, ds = po.varlen(q, k, v, cu_q, cu_k, d ** -0.5 if scale is None else scale,
+                                    causal)
+    n = max((b - a for a, b in zip(cu_k, cu_k[1:])), default=0)
+    vmax = float(v.float().abs().nan_to_num(0.0, 0.0, 0.0).max()) if v.numel() else 0.0
+    assert o.dtype == q.dtype and o.shape == q.shape and lse.shape == (q.shape[1], q.shape[0])
+    assert_rows(o, ref, a, ds.t(), n, vmax)
+    assert_lse(lse, ref_lse, ds, n, d)
+    return o, lse
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("h,hk,d", [(4, 4, 64), (8, 2, 128), (7, 1, 128), (4, 2, 256), (40, 8, 64)])
+def test_whole_prompts(h, hk, d, dtype, causal):
+    """Lengths around the tiles (one, odd, whole, one more), an empty sequence in the middle."""
+    need_gpu()
+    lens = [1, 31, 64, 65, 0, 127, 200, 2, 32]
+    say(f"varlen prompts h={h} hk={hk} d={d} {dtype} causal={causal}")
+    check(*inputs(lens, lens, h, hk, d, dtype, seed=d + h), causal)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d,dtype", [(64, torch.bfloat16), (128, torch.float16),
+                                     (128, torch.bfloat16), (256, torch.bfloat16)])
+def test_chunks_and_single_tokens(d, dtype, causal):
+    """Chunks behind prefixes, single tokens, and more tokens than keys: the first of those see
+    none (out 0, -inf)."""
+    need_gpu()
+    say(f"varlen chunks d={d} {dtype} causal={causal}")
+    check(*inputs([40, 1, 1, 100, 17, 5], [300, 513, 1, 60, 17, 0], 8, 2, d, dtype, seed=3), causal)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d", varlen.HEAD_DIMS)
+@pytest.mark.parametrize("lens_q,lens_k", [([1], [5000]), ([3, 1], [2111, 40]), ([64], [3001])])
+def test_split_keys(lens_q, lens_k, d, causal):
+    """Few rows over many keys: the keys are split and the parts merged."""
+    need_gpu()
+    say(f"varlen splits {lens_q} {lens_k} d={d} causal={causal}")
+    cu = torch.cuda.get_device_properties(0).multi_processor_count
+    assert varlen.choose_splits(sum(lens_q), len(lens_q), 2, 2, max(lens_k), cu) > 1
+    check(*inputs(lens_q, lens_k, 4, 2, d, torch.bfloat16, seed=9), causal)
+
+
+@pytest.mark.parametrize("max_k", [1, 700, 5000])
+def test_length_bounds_do_not_choose_the_result(max_k):
+    need_gpu()
+    say(f"varlen max_k={max_k}")
+    check(*inputs([2, 5], [2500, 900], 4, 1, 128, torch.float16, seed=1), True, max_k=max_k)
+
+
+def test_rows_of_no_sequence_are_zero():
+    """Rows behind the last sequence and before the first; NaN there and in the keys behind the
+    last sequence reaches nobody."""
+    need_gpu()
+    say("varlen rows of no sequence")
+    for d in varlen.HEAD_DIMS:
+        q, k, v, cq, ck = inputs([70, 130], [70, 130], 4, 2, d, torch.bfloat16, seed=2, extra_q=300,
+                                 extra_k=90)
+        q[200:] = math.nan
+        k[200:] = math.nan
+        v[200:] = math.nan
+        o, lse = call(q, k, v, cq, ck, True)
+        assert bool((o[200:] == 0).all()) and bool(torch.isneginf(lse[:, 200:]).all())
+        ref, ref_lse, a, ds = po.varlen(q[:200], k, v, cq, ck, d ** -0.5, True)
+        assert_rows(o[:200], ref, a, ds.t(), 130, 6.0)
+        assert_lse(lse[:, :200], ref_lse, ds, 130, d)
+        late = [50, 120, 200]
+        o, lse = call(q, k, v, late, ck, False)
+        assert bool((o[:50] == 0).all()) and bool(torch.isneginf(lse[:, :50]).all())
+        o, lse = call(q, k, v, [0], [0], False)
+        assert bool((o == 0).all()) and bool(torch.isneginf(lse).all())
+
+
+@pytest.mark.parametrize("d", varlen.HEAD_DIMS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_odd_values_reach_only_the_rows_that_see_them(d, dtype):
+    """NaN and infinities in K and V at keys that a causal mask hides from earlier tokens."""
+    need_gpu()
+    say(f"varlen odd values d={d} {dtype}")
+    q, k, v, cq, ck = inputs([150, 60, 100], [150, 90, 100], 4, 2, d, dtype, seed=5)
+    v[149, 0, 3] = math.nan
+    v[100, 1, 7] = math.inf
+    v[150 + 70, 1, 0] = -math.inf
+    v[150 + 89, 0, d - 1] = math.inf
+    k[240 + 64, 0, 5] = math.nan
+    o, lse = call(q, k, v, cq, ck, True)
+    ref, ref_lse, a, ds = po.varlen(q, k, v, cq, ck, d ** -0.5, True)
+    assert_rows(o, ref, a, ds.t(), 150, 6.0)
+    assert torch.equal(torch.isnan(lse), torch.isnan(ref_lse))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1e-3, 40.0])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scales(scale, dtype):
+    need_gpu()
+    say(f"varlen scale {scale} {dtype}")
+    check(*inputs([90, 33], [150, 33], 4, 2, 64, dtype, seed=6), True, scale=scale)
+
+
+def test_strided_inputs():
+    """q, k, v as slices of one fused projection, as a transposed tensor, and with rows that are
+    not 16-byte aligned (copied)."""
+    need_gpu()
+    say("varlen strides")
+    lens = [50, 77]
+    cu = starts(lens)
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    fused = torch.randn((127, 8, 128), generator=gen, device=DEV).bfloat16()
+    check(fused[:, :4], fused[:, 4:6], fused[:, 6:], cu, cu, True)
+    by_head = torch.randn((8, 127, 128), generator=gen, device=DEV).half().transpose(0, 1)
+    check(by_head[:, :4], by_head[:, 4:6], by_head[:, 6:], cu, cu, False)
+    odd = torch.randn((127, 4, 65), generator=gen, device=DEV).half()[..., 1:]
+    check(odd, odd[:, :2], odd[:, 2:], cu, cu, True)
+    wide = torch.randn((127, 2, 128), generator=gen, device=DEV).half()
+    check(fused[:, :4].half(), wide.transpose(1, 2).contiguous().transpose(1, 2), wide, cu, cu, True)
+    one = torch.randn((1, 2, 128), generator=gen, device=DEV).half().expand(127, 2, 128)
+    check(fused[:, :4].half(), one, wide, cu, cu, True)
+
+
+def test_equals_the_rectangular_operator_where_both_apply():
+    """Sequences of one length: the same rows as flash_attention, within both tolerances."""
+    need_gpu()
+    say("varlen against flash_attention")
+    q, k, v, cq, ck = inputs([256] * 3, [256] * 3, 8, 2, 128, torch.float16, seed=11)
+    o, lse = check(q, k, v, cq, ck, True)
+    o2, l2 = flag_attn.flash_attention(*(x.view(3, 256, -1, 128).transpose(1, 2) for x in (q, k, v)),
+                                       causal=True, return_log_normalizer=True)[:2]
+    assert float((o.view(3, 256, 8, 128).transpose(1, 2).float() - o2.float()).abs().max()) < 4e-3
+    assert float((lse.view(8, 3, 256).transpose(0, 1) - l2).abs().max()) < 1e-5
+
+
+def test_many_sequences():
+    """More sequences than a wave has lanes, most of a few tokens, some empty."""
+    need_gpu()
+    say("varlen many sequences")
+    gen = torch.Generator().manual_seed(4)
+    lens = torch.randint(0, 40, (200,), generator=gen).tolist()
+    lens[130] = 700
+    check(*inputs(lens, lens, 4, 1, 64, torch.bfloat16, seed=12), True)
+
+
+def test_offsets_past_32_bits():
+    """A key tensor whose last rows lie more than 2^32 bytes behind its first."""
+    need_gpu()
+    say("varlen far offsets")
+    rows, stride = 1400, 1 << 21  # elements: 2.9e9 in all
+    base = torch.empty(rows * stride, dtype=torch.float16, device=DEV)
+    k = base.as_strided((rows, 2, 64), (stride, 64, 1))
+    v = base.as_strided((rows, 2, 64), (stride, 64, 1), 128)
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    k.copy_(torch.randn((rows, 2, 64), generator=gen, device=DEV))
+    v.copy_(torch.randn((rows, 2, 64), generator=gen, device=DEV))
+    q = torch.randn((40, 4, 64), generator=gen, device=DEV).half()
+    check(q, k, v, [0, 10, 40], [0, 1000, 1400], True)
+
+
+def test_replays_and_other_streams():
+    """Two captured calls on changed inputs, replayed in turn, and a call on another stream."""
+    need_gpu()
+    say("varlen graph")
+    lens = [100, 3, 257]
+    a = inputs(lens, lens, 4, 2, 128, torch.float16, seed=1)
+    b = inputs([2], [4000], 4, 2, 128, torch.float16, seed=2)
+    call(*a, True), call(*b, False)
+    torch.cuda.synchronize()
+    cu = [[torch.tensor(c, dtype=torch.int32, device=DEV) for c in x[3:]] for x in (a, b)]
+    graphs, outs = [], []
+    for x, c, mq, mk in ((a, cu[0], 257, 257), (b, cu[1], 2, 4000)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(flag_attn.flash_attention_varlen(*x[:3], *c, mq, mk, True,
+                                                         return_log_normalizer=True))
+        graphs.append(g)
+    for rep in range(3):
+        for x in (a, b):
+            for t in x[:3]:
+                t.copy_(torch.randn_like(t))
+        if rep == 2:  # the lengths are device data
+            cu[0][0].copy_(torch.tensor([0, 200, 203, 360], dtype=torch.int32))
+            cu[0][1].copy_(torch.tensor([0, 180, 203, 360], dtype=torch.int32))
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        got = [[t.clone() for t in o] for o in outs]
+        torch.randn(4096, device=DEV).sum().item()
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            want = [flag_attn.flash_attention_varlen(*x[:3], *c, mq, mk, True,
+                                                     return_log_normalizer=True)
+                    for x, c, mq, mk in ((a, cu[0], 257, 257), (b, cu[1], 2, 4000))]
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(g, w)), rep

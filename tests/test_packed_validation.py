@@ -1,0 +1,192 @@
+"""Refusals of the packed-attention and 4-bit-cache operators, on the Python side and at the C ABI
+-- CPU only: every check runs before any device work."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import flag_attn
+from flagattention_amd import ArgumentError, _lib, mxfp4, varlen
+from oracle import packed_oracle as po
+
+
+def _varlen(dtype=torch.float16):
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    return dict(q=torch.zeros((10, 4, 64), dtype=dtype), k=torch.zeros((12, 2, 64), dtype=dtype),
+                v=torch.zeros((12, 2, 64), dtype=dtype), cu_seqlens_q=i32(0, 4, 10),
+                cu_seqlens_k=i32(0, 6, 12), max_seqlen_q=6, max_seqlen_k=6)
+
+
+@pytest.mark.parametrize("mutate,msg", [
+    (lambda a: a.update(q=a["q"][0]), "tokens, heads, head_dim"),
+    (lambda a: a.update(v=a["v"][:5]), "shapes differ"),
+    (lambda a: a.update(q=torch.zeros((10, 4, 128)).half()), "feature size"),
+    (lambda a: a.update(q=torch.zeros((10, 4, 96)).half(), k=torch.zeros((12, 2, 96)).half(),
+                        v=torch.zeros((12, 2, 96)).half()), "head dim 96"),
+    (lambda a: a.update(q=torch.zeros((10, 3, 64)).half()), "multiple"),
+    (lambda a: a.update(q=torch.zeros((10, 0, 64)).half()), "multiple"),
+    (lambda a: a.update(**{n: a[n].float() for n in "qkv"}), "float16 / bfloat16"),
+    (lambda a: a.update(k=a["k"].bfloat16(), v=a["v"].bfloat16()), "dtypes differ"),
+    (lambda a: a.update(cu_seqlens_q=a["cu_seqlens_q"].long()), "cu_seqlens_q"),
+    (lambda a: a.update(cu_seqlens_q=a["cu_seqlens_q"][:0]), "cu_seqlens_q"),
+    (lambda a: a.update(cu_seqlens_k=a["cu_seqlens_k"][:2]), "cu_seqlens_k"),
+    (lambda a: a.update(max_seqlen_k=-1), "max_seqlen"),
+    (lambda a: a.update(max_seqlen_q=2.0), "max_seqlen"),
+    (lambda a: a.update(sm_scale=math.inf), "finite"),
+    (lambda a: None, "CUDA"),  # valid, but CPU tensors
+])
+def test_varlen_rejects(mutate, msg):
+    args = _varlen()
+    mutate(args)
+    with pytest.raises(ArgumentError, match=msg):
+        flag_attn.flash_attention_varlen(**args)
+
+
+def _cache(blocks=4, hk=2, block=16, d=64):
+    return dict(key_cache=torch.zeros((blocks, hk, block, d // 2), dtype=torch.uint8),
+                key_scales=torch.zeros((blocks, hk, block, d // 32), dtype=torch.uint8),
+                value_cache=torch.zeros((blocks, hk, block, d // 2), dtype=torch.uint8),
+                value_scales=torch.zeros((blocks, hk, block, d // 32), dtype=torch.uint8))
+
+
+def _all(c, f):
+    c.update({n: f(c[n]) for n in ("key_cache", "key_scales", "value_cache", "value_scales")})
+
+
+CACHE_FAULTS = [
+    (lambda c: c.update(key_cache=c["key_cache"][0]), "num_blocks, num_kv_heads"),
+    (lambda c: c.update(value_cache=c["value_cache"][:3]), "num_blocks, num_kv_heads"),
+    (lambda c: c.update(key_scales=c["key_scales"][..., :1]), "head_size / 32"),
+    (lambda c: c.update(value_scales=c["value_scales"][:1]), "head_size / 32"),
+    (lambda c: _all(c, lambda t: t.char()), "uint8"),
+    (lambda c: _all(c, lambda t: t[:0]), "empty"),
+    (lambda c: _all(c, lambda t: t[:, :, :8]), "multiple of 16"),
+    (lambda c: c.update(**_cache(d=96)), "head_size"),
+    (lambda c: c.update(value_cache=c["value_cache"].transpose(0, 1).contiguous().transpose(0, 1)),
+     "same strides"),
+    (lambda c: _all(c, lambda t: t.transpose(2, 3).contiguous().transpose(2, 3)), "contiguous"),
+    (lambda c: c.update(key_cache=torch.zeros(4 * 2 * 16 * 32 + 1, dtype=torch.uint8)[1:].view(
+        4, 2, 16, 32)), "aligned"),
+    (lambda c: None, "CUDA"),
+]
+
+
+@pytest.mark.parametrize("mutate,msg", CACHE_FAULTS)
+def test_every_cache_operator_rejects_a_bad_cache(mutate, msg):
+    c = _cache()
+    mutate(c)
+    d = 2 * c["key_cache"].shape[-1]
+    kv = torch.zeros((3, 2, d)).half()
+    i32 = torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(ArgumentError, match=msg):
+        flag_attn.cache_kv_mxfp4(kv, kv, **c, slot_mapping=i32)
+    with pytest.raises(ArgumentError, match=msg):
+        flag_attn.gather_kv_mxfp4(**c, block_tables=i32.view(1, 3), cu_seqlens=i32[:2],
+                                  total_tokens=5, dtype=torch.float16)
+    with pytest.raises(ArgumentError, match=msg):
+        flag_attn.paged_attention_mxfp4(kv, **c, context_lens=i32, block_tables=i32.view(3, 1),
+                                        attn_scale=1.0, max_context_len=10)
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(key=torch.zeros((3, 64)).half()), "num_tokens"),
+    (dict(value=torch.zeros((2, 2, 64)).half()), "num_tokens"),
+    (dict(key=torch.zeros((3, 2, 64))), "float16"),
+    (dict(value=torch.zeros((3, 2, 64)).bfloat16()), "dtypes differ"),
+    (dict(key=torch.zeros((3, 4, 64)).half(), value=torch.zeros((3, 4, 64)).half()), "CUDA|differ"),
+    (dict(slot_mapping=torch.zeros(2, dtype=torch.int32)), "slot_mapping|CUDA"),
+    (dict(slot_mapping=torch.zeros(3)), "slot_mapping|CUDA"),
+])
+def test_write_rejects(kw, msg):
+    args = dict(key=torch.zeros((3, 2, 64)).half(), value=torch.zeros((3, 2, 64)).half(), **_cache(),
+                slot_mapping=torch.zeros(3, dtype=torch.int64))
+    args.update(kw)
+    with pytest.raises(ArgumentError, match=msg):
+        flag_attn.cache_kv_mxfp4(**args)
+
+
+def test_struct_mirrors_and_c_abi_refusals():
+    lib = _lib.load()
+    for name, mirror in (("fa_varlen_args", _lib.VarlenArgs), ("fa_mxfp4_cache", _lib.Mxfp4Cache),
+                         ("fa_mxfp4_decode_args", _lib.Mxfp4DecodeArgs)):
+        assert getattr(lib, name + "_size")() == ctypes.sizeof(mirror)
+
+    def refused(rc, text):
+        assert rc == -1 and text in lib.fa_last_error(), lib.fa_last_error()
+
+    refused(lib.fa_varlen_attention(None, None), b"NULL")
+    good = dict(q=4096, k=4096, v=4096, out=4096, cu_seqlens_q=4096, cu_seqlens_k=4096, num_seqs=1,
+                total_q=4, total_k=4, h_q=2, h_kv=1, d=64, num_splits=1, split_tokens=1,
+                q_stride_t=128, q_stride_h=64, k_stride_t=64, k_stride_h=64, v_stride_t=64,
+                v_stride_h=64, o_stride_t=128, o_stride_h=64)
+    for change, text in ((dict(total_q=0), b"total_q"), (dict(num_seqs=-1), b"num_seqs"),
+                         (dict(h_q=3, h_kv=2), b"multiple"), (dict(d=32), b"head dim"),
+                         (dict(dtype=2), b"dtype"), (dict(out=None), b"NULL"),
+                         (dict(k=4104), b"aligned"), (dict(o_stride_h=60), b"aligned"),
+                         (dict(k_stride_t=1 << 23), b"token strides"),
+                         (dict(v_stride_t=-64), b"token strides"),
+                         (dict(total_q=1 << 30), b"too many"), (dict(num_splits=0), b"num_splits"),
+                         (dict(num_splits=2), b"o_part"),
+                         (dict(num_splits=9, split_tokens=1 << 29), b"num_splits")):
+        refused(lib.fa_varlen_attention(ctypes.byref(_lib.VarlenArgs(**{**good, **change})), None), text)
+    refused(lib.fa_varlen_combine(ctypes.byref(_lib.VarlenArgs(**good)), None), b"o_part")
+
+    cache = dict(k_codes=4096, k_scales=4096, v_codes=4096, v_scales=4096, code_stride_0=1024,
+                 code_stride_h=512, code_stride_t=32, scale_stride_0=64, scale_stride_h=32,
+                 scale_stride_t=2, num_blocks=4, block_size=16, h_kv=2, d=64)
+    for change, text in ((dict(d=32), b"head dim"), (dict(h_kv=0), b"h_kv"),
+                         (dict(block_size=24), b"block_size"), (dict(num_blocks=0), b"num_blocks"),
+                         (dict(num_blocks=1 << 31), b"num_blocks"), (dict(v_scales=None), b"NULL"),
+                         (dict(k_codes=4100), b"codes"), (dict(code_stride_t=36), b"codes"),
+                         (dict(d=256, scale_stride_h=33), b"scales")):
+        c = _lib.Mxfp4Cache(**{**cache, **change})
+        refused(lib.fa_mxfp4_cache_write(ctypes.byref(c), 4096, 128, 64, 4096, 128, 64, 4096, 1, 3, 0,
+                                         None), text)
+        refused(lib.fa_mxfp4_gather(ctypes.byref(c), 4096, 1, 1, 4096, 1, 3, 4096, 4096, 0, None), text)
+        refused(lib.fa_mxfp4_decode(ctypes.byref(_lib.Mxfp4DecodeArgs(cache=c)), None), text)
+    ok = _lib.Mxfp4Cache(**cache)
+    refused(lib.fa_mxfp4_cache_write(ctypes.byref(ok), 4096, 128, 64, 4096, 128, 64, 4096, 1, -1, 0,
+                                     None), b"num_tokens")
+    refused(lib.fa_mxfp4_cache_write(ctypes.byref(ok), 4096, 128, 64, 4096, 128, 60, 4096, 1, 3, 0,
+                                     None), b"aligned")
+    refused(lib.fa_mxfp4_cache_write(ctypes.byref(ok), 4096, 128, 64, 4096, 128, 64, 4096, 1, 1 << 30, 0,
+                                     None), b"2^31")
+    refused(lib.fa_mxfp4_gather(ctypes.byref(ok), None, 1, 1, 4096, 1, 3, 4096, 4096, 0, None), b"NULL")
+    decode = dict(cache=ok, q=4096, out=4096, block_table=4096, seqlens=4096, max_blocks_per_seq=1,
+                  batch=1, h_q=4, num_splits=1, split_tokens=7, q_stride_b=256, q_stride_h=64)
+    for change, text in ((dict(batch=0), b"batch"), (dict(batch=65536), b"batch"),
+                         (dict(h_q=3), b"multiple"), (dict(dtype=5), b"dtype"),
+                         (dict(num_splits=2, split_tokens=24), b"num_splits"),
+                         (dict(num_splits=2, split_tokens=32), b"o_part"),
+                         (dict(seqlens=None), b"NULL"), (dict(q=4098), b"aligned")):
+        refused(lib.fa_mxfp4_decode(ctypes.byref(_lib.Mxfp4DecodeArgs(**{**decode, **change})), None),
+                text)
+    refused(lib.fa_mxfp4_combine(ctypes.byref(_lib.Mxfp4DecodeArgs(**decode)), None), b"o_part")
+
+
+def test_oracle_formats():
+    """The oracle's writer keeps what a code can say exactly, and is never off by more than half of
+    the widest step, which is the scale itself."""
+    x = torch.tensor(po.MAGNITUDES + tuple(-m for m in po.MAGNITUDES)).repeat(2).view(1, 32) * 8.0
+    codes, scales = po.quantise(x)
+    assert int(scales) == 127 + 3 and torch.equal(po.values(codes, scales), x.double())
+    gen = torch.Generator().manual_seed(0)
+    x = torch.randn((200, 64), generator=gen) * torch.exp(torch.randn((200, 1), generator=gen) * 3)
+    codes, scales = po.quantise(x)
+    err = (po.values(codes, scales) - x.double()).abs().unflatten(-1, (-1, 32)).amax(-1)
+    power = po.pow2(scales)
+    assert bool((err <= power).all())
+    top = x.double().abs().unflatten(-1, (-1, 32)).amax(-1)
+    assert bool((top <= 7 * power).all()) and bool((top > 3.5 * power).all())
+
+
+def test_split_rule():
+    assert varlen.choose_splits(1, 1, 4, 8, 100, 256) == 1
+    assert varlen.choose_splits(100000, 4, 4, 8, 100000, 256) == 1
+    for total, seqs, group, hk, n in ((1, 1, 1, 1, 10000), (64, 1, 8, 2, 300), (5, 4, 4, 1, 70000)):
+        s = varlen.choose_splits(total, seqs, group, hk, n, 256)
+        blocks = hk * max(min(seqs, total), -(-total * group // varlen.ROWS_PER_WG))
+        assert 1 < s <= -(-n // varlen.MIN_SPLIT_TOKENS) and s * blocks < 3 * 256
+        assert hk * -(-group * total // 16) <= 65535  # the merge's limit
+    assert mxfp4.HEAD_DIMS == varlen.HEAD_DIMS == (64, 128, 256)
