@@ -29,6 +29,7 @@
 #include <string>
 
 #include "flagattention_amd.h"
+#include "flagattention_amd_packed.h"
 
 namespace {
 
@@ -633,12 +634,311 @@ PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- packed prompts (varlen.py) and the 4-bit cache (mxfp4.py) ----
+bool packed_dim(int64_t d) { return d == 64 || d == 128 || d == 256; }
+
+// Split count of packed prompts: varlen.choose_splits.
+int64_t varlen_split_count(int64_t total_q, int64_t num_seqs, int64_t group, int64_t h_kv,
+                           int64_t max_k, int64_t cus) {
+  const int64_t blocks = h_kv * std::max<int64_t>({std::min(num_seqs, total_q),
+                                                   cdiv(total_q * group, kPrefillRowsPerWg), 1});
+  if (blocks >= cus || max_k <= kMinSplitTokens) return 1;
+  return std::min(cdiv(2 * cus, blocks), cdiv(max_k, kMinSplitTokens));
+}
+
+// varlen_splits(total_q, num_seqs, group, h_kv, max_k, cus), for the comparison with varlen.py.
+PyObject* varlen_splits(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  int64_t x[6];
+  if (nargs != 6) return none();
+  for (int i = 0; i < 6; ++i)
+    if (!to_int(args[i], &x[i]) || x[i] < 1) return none();
+  return PyLong_FromLongLong(varlen_split_count(x[0], x[1], x[2], x[3], x[4], x[5]));
+}
+
+// varlen(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal, sm_scale,
+//        want_lse): (o, lse) or o
+PyObject* varlen(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 10) return none();
+  const at::Tensor *q = plain(args[0]), *k = plain(args[1]), *v = plain(args[2]),
+                   *cq = plain(args[3]), *ck = plain(args[4]);
+  int64_t max_q, max_k;
+  bool causal, want_lse;
+  if (!q || !k || !v || !cq || !ck || !to_int(args[5], &max_q) || !to_int(args[6], &max_k) ||
+      !to_bool(args[7], &causal) || !to_bool(args[9], &want_lse) || max_q < 0 || max_k < 0)
+    return none();
+  if (q->dim() != 3 || k->dim() != 3 || !v->sizes().equals(k->sizes())) return none();
+  const int64_t total_q = q->size(0), h_q = q->size(1), d = q->size(2);
+  const int64_t total_k = k->size(0), h_kv = k->size(1);
+  double scale = 1.0 / std::sqrt(static_cast<double>(d));
+  if (args[8] != Py_None && !to_double(args[8], &scale)) return none();
+  if (total_q < 1 || total_k < 1 || !packed_dim(d) || k->size(2) != d || h_kv < 1 || h_q < 1 ||
+      h_q % h_kv != 0 || !gqa_dtype(*q) || k->scalar_type() != q->scalar_type() ||
+      v->scalar_type() != q->scalar_type() || !std::isfinite(scale) ||
+      total_q * (h_q / h_kv) >= (int64_t{1} << 30) || total_k >= (int64_t{1} << 31))
+    return none();
+  constexpr int64_t kMaxStride = int64_t{1} << 23;
+  if (q->stride(2) != 1 || k->stride(2) != 1 || v->stride(2) != 1 || !rows16(*q, 2) ||
+      !rows16(*k, 2) || !rows16(*v, 2) || k->stride(0) >= kMaxStride || v->stride(0) >= kMaxStride)
+    return none();
+  if (cq->scalar_type() != at::kInt || cq->dim() != 1 || cq->size(0) < 1 || !cq->is_contiguous() ||
+      ck->scalar_type() != at::kInt || !ck->sizes().equals(cq->sizes()) || !ck->is_contiguous())
+    return none();
+  const c10::Device device = q->device();
+  for (const at::Tensor* t : {k, v, cq, ck})
+    if (t->device() != device) return none();
+  const int cus = cu_count(device.index());
+  if (cus == 0) return none();
+  const int64_t num_seqs = cq->size(0) - 1, longest = std::min(max_k, total_k);
+  const int64_t s = varlen_split_count(total_q, num_seqs, h_q / h_kv, h_kv, longest, cus);
+  at::Tensor out, lse;
+  {
+    NoGil nogil;
+    c10::DeviceGuard guard(device);
+    out = make({total_q, h_q, d}, q->scalar_type(), device);
+    if (want_lse) lse = make({h_q, total_q}, at::kFloat, device);
+    at::Tensor part;
+    fa_varlen_args a = {};
+    a.q = q->data_ptr();
+    a.q_stride_t = q->stride(0);
+    a.q_stride_h = q->stride(1);
+    a.k = k->data_ptr();
+    a.v = v->data_ptr();
+    a.k_stride_t = k->stride(0);
+    a.k_stride_h = k->stride(1);
+    a.v_stride_t = v->stride(0);
+    a.v_stride_h = v->stride(1);
+    a.cu_seqlens_q = cq->data_ptr<int32_t>();
+    a.cu_seqlens_k = ck->data_ptr<int32_t>();
+    a.out = out.data_ptr();
+    a.o_stride_t = out.stride(0);
+    a.o_stride_h = out.stride(1);
+    a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
+    a.num_seqs = static_cast<int32_t>(num_seqs);
+    a.total_q = static_cast<int32_t>(total_q);
+    a.total_k = static_cast<int32_t>(total_k);
+    a.h_q = static_cast<int32_t>(h_q);
+    a.h_kv = static_cast<int32_t>(h_kv);
+    a.d = static_cast<int32_t>(d);
+    a.num_splits = static_cast<int32_t>(s);
+    a.split_tokens = s > 1 ? static_cast<int32_t>(whole_tiles(cdiv(longest, s))) : 1;
+    a.scale = static_cast<float>(scale);
+    a.causal = causal;
+    a.dtype = q->scalar_type() == at::kBFloat16;
+    if (s > 1) {
+      const int64_t n = h_q * total_q * s;
+      part = make({n * (d + 1)}, at::kFloat, device);
+      a.o_part = part.data_ptr<float>();
+      a.lse_part = a.o_part + n * d;
+    }
+    void* const stream = stream_of(device);
+    check(fa_varlen_attention(&a, stream));
+    if (s > 1) check(fa_varlen_combine(&a, stream));
+  }
+  if (!want_lse) return THPVariable_Wrap(std::move(out));
+  PyObject* const o = THPVariable_Wrap(std::move(out));
+  PyObject* const l = THPVariable_Wrap(std::move(lse));
+  PyObject* const both = o && l ? PyTuple_Pack(2, o, l) : nullptr;
+  Py_XDECREF(o);
+  Py_XDECREF(l);
+  return both;
+  END_HANDLE_TH_ERRORS
+}
+
+bool aligned_rows(const at::Tensor& t, int64_t bytes) {
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % static_cast<uintptr_t>(bytes) == 0 &&
+         t.stride(0) % bytes == 0 && t.stride(1) % bytes == 0 && t.stride(2) % bytes == 0;
+}
+
+// The cache of four arguments (mxfp4._check_cache), or false.
+bool mxfp4_cache_of(PyObject* const* args, const at::Tensor** t, fa_mxfp4_cache* c) {
+  for (int i = 0; i < 4; ++i) {
+    t[i] = plain(args[i]);
+    if (!t[i] || t[i]->scalar_type() != at::kByte || t[i]->dim() != 4 ||
+        t[i]->device() != t[0]->device())
+      return false;
+  }
+  const at::Tensor &kc = *t[0], &ks = *t[1], &vc = *t[2], &vs = *t[3];
+  const int64_t d = 2 * kc.size(3);
+  if (!packed_dim(d) || !vc.sizes().equals(kc.sizes()) || !vs.sizes().equals(ks.sizes()) ||
+      ks.size(0) != kc.size(0) || ks.size(1) != kc.size(1) || ks.size(2) != kc.size(2) ||
+      ks.size(3) != d / FA_MXFP4_GROUP || !vc.strides().equals(kc.strides()) ||
+      !vs.strides().equals(ks.strides()) || kc.stride(3) != 1 || ks.stride(3) != 1)
+    return false;
+  const int64_t code_align = std::min<int64_t>(16, d / 8), scale_align = d == 256 ? 2 : 1;
+  if (kc.size(0) < 1 || kc.size(0) > INT32_MAX || kc.size(1) < 1 || kc.size(1) > 65535 ||
+      kc.size(2) < 16 || kc.size(2) % 16 != 0 || kc.size(2) > INT32_MAX ||
+      !aligned_rows(kc, code_align) || !aligned_rows(vc, code_align) ||
+      !aligned_rows(ks, scale_align) || !aligned_rows(vs, scale_align))
+    return false;
+  c->k_codes = kc.data_ptr();
+  c->k_scales = ks.data_ptr();
+  c->v_codes = vc.data_ptr();
+  c->v_scales = vs.data_ptr();
+  c->code_stride_0 = kc.stride(0);
+  c->code_stride_h = kc.stride(1);
+  c->code_stride_t = kc.stride(2);
+  c->scale_stride_0 = ks.stride(0);
+  c->scale_stride_h = ks.stride(1);
+  c->scale_stride_t = ks.stride(2);
+  c->num_blocks = kc.size(0);
+  c->block_size = static_cast<int32_t>(kc.size(2));
+  c->h_kv = static_cast<int32_t>(kc.size(1));
+  c->d = static_cast<int32_t>(d);
+  return true;
+}
+
+// mxfp4_write(key, value, key_cache, key_scales, value_cache, value_scales, slot_mapping): True
+PyObject* mxfp4_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 7) return none();
+  const at::Tensor *k = plain(args[0]), *v = plain(args[1]), *slots = plain(args[6]), *t[4];
+  fa_mxfp4_cache c = {};
+  if (!k || !v || !slots || k->dim() != 3 || !v->sizes().equals(k->sizes()) || !gqa_dtype(*k) ||
+      v->scalar_type() != k->scalar_type() || !mxfp4_cache_of(args + 2, t, &c))
+    return none();
+  const int64_t n = k->size(0);
+  if (n < 1 || k->size(1) != c.h_kv || k->size(2) != c.d || n * c.h_kv > INT32_MAX ||
+      k->stride(2) != 1 || v->stride(2) != 1 || !rows16(*k, 2) || !rows16(*v, 2) ||
+      (slots->scalar_type() != at::kLong && slots->scalar_type() != at::kInt) ||
+      slots->dim() != 1 || slots->size(0) != n || !slots->is_contiguous())
+    return none();
+  const c10::Device device = k->device();
+  if (v->device() != device || slots->device() != device || t[0]->device() != device) return none();
+  {
+    NoGil nogil;
+    c10::DeviceGuard guard(device);
+    check(fa_mxfp4_cache_write(&c, k->data_ptr(), k->stride(0), k->stride(1), v->data_ptr(),
+                               v->stride(0), v->stride(1), slots->data_ptr(),
+                               slots->scalar_type() == at::kLong, static_cast<int32_t>(n),
+                               k->scalar_type() == at::kBFloat16, stream_of(device)));
+  }
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// mxfp4_gather(key_cache, key_scales, value_cache, value_scales, block_tables, cu_seqlens,
+//              total_tokens, is_bf16): (key, value)
+PyObject* mxfp4_gather(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 8) return none();
+  const at::Tensor *bt = plain(args[4]), *cu = plain(args[5]), *t[4];
+  fa_mxfp4_cache c = {};
+  int64_t total;
+  bool bf16;
+  if (!bt || !cu || !to_int(args[6], &total) || !to_bool(args[7], &bf16) ||
+      !mxfp4_cache_of(args, t, &c))
+    return none();
+  if (cu->scalar_type() != at::kInt || cu->dim() != 1 || cu->size(0) < 2 || !cu->is_contiguous() ||
+      bt->scalar_type() != at::kInt || bt->dim() != 2 || bt->size(0) != cu->size(0) - 1 ||
+      bt->size(1) < 1 || bt->stride(1) != 1 || total < 1 || total > INT32_MAX ||
+      total * c.h_kv > INT32_MAX)
+    return none();
+  const c10::Device device = t[0]->device();
+  if (bt->device() != device || cu->device() != device) return none();
+  at::Tensor k, v;
+  {
+    NoGil nogil;
+    c10::DeviceGuard guard(device);
+    k = make({total, c.h_kv, c.d}, bf16 ? at::kBFloat16 : at::kHalf, device);
+    v = make({total, c.h_kv, c.d}, bf16 ? at::kBFloat16 : at::kHalf, device);
+    check(fa_mxfp4_gather(&c, bt->data_ptr<int32_t>(), bt->stride(0),
+                          static_cast<int32_t>(bt->size(1)), cu->data_ptr<int32_t>(),
+                          static_cast<int32_t>(bt->size(0)), static_cast<int32_t>(total),
+                          k.data_ptr(), v.data_ptr(), bf16, stream_of(device)));
+  }
+  PyObject* const a = THPVariable_Wrap(std::move(k));
+  PyObject* const b = THPVariable_Wrap(std::move(v));
+  PyObject* const both = a && b ? PyTuple_Pack(2, a, b) : nullptr;
+  Py_XDECREF(a);
+  Py_XDECREF(b);
+  return both;
+  END_HANDLE_TH_ERRORS
+}
+
+// mxfp4_decode(query, key_cache, key_scales, value_cache, value_scales, context_lens, block_tables,
+//              attn_scale, max_context_len, num_splits)
+PyObject* mxfp4_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 10) return none();
+  const at::Tensor *q = plain(args[0]), *lens = plain(args[5]), *bt = plain(args[6]), *t[4];
+  fa_mxfp4_decode_args a = {};
+  double scale;
+  int64_t max_len, num_splits;
+  if (!q || !lens || !bt || !to_double(args[7], &scale) || !to_int(args[8], &max_len) ||
+      !to_int(args[9], &num_splits) || !mxfp4_cache_of(args + 1, t, &a.cache))
+    return none();
+  if (q->dim() != 3 || !gqa_dtype(*q) || q->size(2) != a.cache.d || q->stride(2) != 1 ||
+      !rows16(*q, 2))
+    return none();
+  const int64_t seqs = q->size(0), h_q = q->size(1), d = q->size(2), h_kv = a.cache.h_kv;
+  if (seqs < 1 || h_q < 1 || h_q % h_kv != 0 || lens->scalar_type() != at::kInt ||
+      lens->dim() != 1 || lens->size(0) != seqs || !lens->is_contiguous() ||
+      bt->scalar_type() != at::kInt || bt->dim() != 2 || bt->size(0) != seqs || bt->size(1) < 1 ||
+      bt->stride(1) != 1)
+    return none();
+  if (num_splits < 0 || max_len < 1 || max_len > (1 << 30) || !std::isfinite(scale)) return none();
+  const c10::Device device = q->device();
+  for (const at::Tensor* x : {lens, bt, t[0]})
+    if (x->device() != device) return none();
+  int64_t split_tokens;
+  if (num_splits == 0) {
+    const int cus = cu_count(device.index());
+    if (cus == 0) return none();
+    split_tokens = whole_tiles(
+        cdiv(max_len, choose_splits(seqs * h_kv, h_q / h_kv, kRowsPerWg, d, max_len, cus)));
+  } else if (num_splits == 1) {
+    split_tokens = max_len;
+  } else {
+    const int64_t each = cdiv(max_len, num_splits);
+    split_tokens = 16;
+    while (split_tokens < each) split_tokens *= 2;
+  }
+  const int64_t s = cdiv(max_len, split_tokens);
+  at::Tensor out;
+  {
+    NoGil nogil;
+    c10::DeviceGuard guard(device);
+    out = make({seqs, h_q, d}, q->scalar_type(), device);
+    at::Tensor part;
+    a.q = q->data_ptr();
+    a.q_stride_b = q->stride(0);
+    a.q_stride_h = q->stride(1);
+    a.block_table = bt->data_ptr<int32_t>();
+    a.bt_stride_b = bt->stride(0);
+    a.max_blocks_per_seq = static_cast<int32_t>(bt->size(1));
+    a.seqlens = lens->data_ptr<int32_t>();
+    a.out = out.data_ptr();
+    a.o_stride_b = out.stride(0);
+    a.o_stride_h = out.stride(1);
+    a.batch = static_cast<int32_t>(seqs);
+    a.h_q = static_cast<int32_t>(h_q);
+    a.num_splits = static_cast<int32_t>(s);
+    a.split_tokens = static_cast<int32_t>(split_tokens);
+    a.scale = static_cast<float>(scale);
+    a.dtype = q->scalar_type() == at::kBFloat16;
+    if (s > 1) {
+      const int64_t n = seqs * h_q * s;
+      part = make({n * (d + 1)}, at::kFloat, device);
+      a.o_part = part.data_ptr<float>();
+      a.lse_part = a.o_part + n * d;
+    }
+    void* const stream = stream_of(device);
+    check(fa_mxfp4_decode(&a, stream));
+    if (s > 1) check(fa_mxfp4_combine(&a, stream));
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 #define FA_METHOD(name)                                                                     \
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, \
    nullptr}
 PyMethodDef g_methods[] = {FA_METHOD(mla_metadata), FA_METHOD(mla_decode),   FA_METHOD(paged),
                            FA_METHOD(contiguous),   FA_METHOD(topk_indices), FA_METHOD(cache_write),
-                           FA_METHOD(split_counts), {nullptr, nullptr, 0, nullptr}};
+                           FA_METHOD(split_counts), FA_METHOD(varlen),   FA_METHOD(varlen_splits),
+                           FA_METHOD(mxfp4_write),  FA_METHOD(mxfp4_gather),
+                           FA_METHOD(mxfp4_decode), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, g_methods};
 
 }  // namespace

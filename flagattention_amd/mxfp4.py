@@ -90,6 +90,10 @@ def cache_kv_mxfp4(
     so that no code is off by more than half of the widest step, and codes of x / scale rounded to
     nearest, ties to the even code.  A group with a NaN or an infinity becomes NaN as a whole.
     """
+    fast = _lib.native()
+    if fast is not None and fast.mxfp4_write(key, value, key_cache, key_scales, value_cache,
+                                             value_scales, slot_mapping):
+        return
     _require(key.dim() == 3 and value.shape == key.shape,
              "key / value must be [num_tokens, num_kv_heads, head_size]")
     code = _dtype_code(key.dtype)
@@ -137,6 +141,12 @@ def gather_kv_mxfp4(
 
     Returns ``(key, value)``, each ``dtype`` (fp16 or bf16) ``[total_tokens, H_kv, D]``.
     """
+    fast = _lib.native() if dtype in (torch.float16, torch.bfloat16) else None
+    if fast is not None:
+        done = fast.mxfp4_gather(key_cache, key_scales, value_cache, value_scales, block_tables,
+                                 cu_seqlens, total_tokens, dtype == torch.bfloat16)
+        if done is not None:
+            return done
     code = _dtype_code(dtype)
     device = key_cache.device
     _, h_kv, _, d = _check_cache(key_cache, key_scales, value_cache, value_scales, device)
@@ -187,6 +197,12 @@ def paged_attention_mxfp4(
 
     Returns ``out`` shaped and typed like ``query``; a sequence without keys gets 0.
     """
+    fast = _lib.native()
+    if fast is not None:
+        done = fast.mxfp4_decode(query, key_cache, key_scales, value_cache, value_scales,
+                                 context_lens, block_tables, attn_scale, max_context_len, num_splits)
+        if done is not None:
+            return done
     _require(query.dim() == 3, "query must be [num_seqs, num_heads, head_size]")
     num_seqs, h_q, d = query.shape
     code = _dtype_code(query.dtype)

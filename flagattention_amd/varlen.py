@@ -30,7 +30,7 @@ def choose_splits(total_q: int, num_seqs: int, group: int, h_kv: int, max_k: int
                   cu_count: int) -> int:
     """Split-KV count: none when the row blocks (at least one per sequence with tokens) give
     every CU a work-group, else enough for about two work-groups per CU, each at least
-    MIN_SPLIT_TOKENS keys long."""
+    MIN_SPLIT_TOKENS keys long (csrc/host/fa_native.cpp has the same rule)."""
     blocks = h_kv * max(min(num_seqs, total_q), -(-total_q * group // ROWS_PER_WG), 1)
     if blocks >= cu_count or max_k <= MIN_SPLIT_TOKENS:
         return 1
@@ -62,6 +62,12 @@ def flash_attention_varlen(
     ``L`` the fp32 natural-log normaliser ``[H, total_q]``.  Tokens that see no key, and rows of
     q that belong to no sequence, get o = 0, L = -inf.
     """
+    fast = _lib.native()
+    if fast is not None:
+        done = fast.varlen(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal,
+                           sm_scale, return_log_normalizer)
+        if done is not None:
+            return done
     _require(q.dim() == 3 and k.dim() == 3, "q, k, v must be [tokens, heads, head_dim]")
     _require(v.shape == k.shape, "k and v shapes differ")
     total_q, h_q, d = q.shape

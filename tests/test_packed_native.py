@@ -1,0 +1,97 @@
+"""The native host path of the packed-attention and 4-bit-cache operators: it takes exactly the calls
+that the Python path would run, with the same results, and leaves every other call to it."""
+import pytest
+import torch
+
+import flag_attn
+from flagattention_amd import _lib, varlen
+from tests._helpers import DEV
+from tests.test_native_host import _both, _same
+
+
+def test_calls_without_gpu_tensors_are_left_to_python():
+    fast = _lib.native()
+    q = torch.zeros((4, 2, 64), dtype=torch.float16)
+    cu = torch.zeros(2, dtype=torch.int32)
+    c = [torch.zeros((2, 2, 16, n), dtype=torch.uint8) for n in (32, 2, 32, 2)]
+    assert fast.varlen(q, q, q, cu, cu, 4, 4, True, None, True) is None
+    assert fast.varlen(q) is None
+    assert fast.mxfp4_write(q, q, *c, cu) is None
+    assert fast.mxfp4_gather(*c, cu.view(1, 2), cu, 4, True) is None
+    assert fast.mxfp4_decode(q, *c, cu, cu.view(1, 2), 1.0, 4, 0) is None
+    assert fast.mxfp4_decode(*[None] * 10) is None
+
+
+def test_split_rule_is_the_python_one():
+    fast = _lib.native()
+    for cus in (64, 256, 304):
+        for total in (1, 2, 16, 31, 32, 33, 100, 511, 1024, 5000):
+            for seqs in (1, 2, 7, 64, 300):
+                for group in (1, 4, 7, 128, 129):
+                    for hk in (1, 8, 40):
+                        for n in (1, 255, 256, 257, 511, 512, 513, 4097, 100000):
+                            assert fast.varlen_splits(total, seqs, group, hk, n, cus) == \
+                                varlen.choose_splits(total, seqs, group, hk, n, cus)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens_q,lens_k,h,hk,d,lse", [
+    ([3, 0, 70], [3, 0, 70], 4, 2, 64, True), ([1], [3000], 8, 1, 128, True),
+    ([200, 1], [200, 900], 8, 8, 256, False)])
+def test_varlen_matches_python_path(monkeypatch, lens_q, lens_k, h, hk, d, lse):
+    def cu(lens):
+        return torch.tensor([0] + lens, device=DEV).cumsum(0).to(torch.int32)
+
+    q = torch.randn((sum(lens_q), h, d), device=DEV).half()
+    kv = torch.randn((sum(lens_k), 2 * hk, d), device=DEV).half()
+    args = (q, kv[:, :hk], kv[:, hk:], cu(lens_q), cu(lens_k), max(lens_q), max(lens_k), True, None, lse)
+    fast = _lib.native()
+    assert fast.varlen(*args) is not None
+    odd = torch.randn((sum(lens_q), h, d + 1), device=DEV).half()[..., 1:]
+    for change in ((0, odd), (0, q.float()), (3, args[3].long()), (5, 1.5), (7, 1), (8, "x")):
+        other = list(args)
+        other[change[0]] = change[1]
+        assert fast.varlen(*other) is None
+    _same(*_both(monkeypatch, lambda: flag_attn.flash_attention_varlen(*args)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d,block", [(64, 16), (128, 48), (256, 64)])
+def test_mxfp4_matches_python_path(monkeypatch, d, block, dtype):
+    hk, blocks, t = 3, 30, 90
+    fast = _lib.native()
+
+    def cache():
+        return [torch.zeros((blocks, hk, block, n), dtype=torch.uint8, device=DEV)
+                for n in (d // 2, d // 32, d // 2, d // 32)]
+
+    k, v = (torch.randn((t, hk, d), device=DEV).to(dtype) for _ in range(2))
+    for slots in (torch.randperm(blocks * block, device=DEV)[:t],
+                  torch.randperm(blocks * block, device=DEV)[:t].int()):
+        assert fast.mxfp4_write(k, v, *cache(), slots) is True
+        assert fast.mxfp4_write(k, v, *cache(), slots.float()) is None
+        assert fast.mxfp4_write(k.float(), v, *cache(), slots) is None
+
+        def write():
+            c = cache()
+            flag_attn.cache_kv_mxfp4(k, v, *c, slots)
+            return tuple(c)
+
+        _same(*_both(monkeypatch, write))
+    c = write()
+    bt = torch.randint(0, blocks, (4, 12), dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, 5, 5, 100, 300], dtype=torch.int32, device=DEV)
+    assert fast.mxfp4_gather(*c, bt, cu, 310, True) is not None
+    assert fast.mxfp4_gather(*c, bt, cu.long(), 310, True) is None
+    assert fast.mxfp4_gather(*c, bt, cu, 0, True) is None
+    _same(*_both(monkeypatch, lambda: flag_attn.gather_kv_mxfp4(*c, bt, cu, 310, dtype)))
+    q = torch.randn((4, 4 * hk, d), device=DEV).to(dtype)
+    lens = torch.tensor([0, 12 * block, 17, 16], dtype=torch.int32, device=DEV)
+    for splits in (0, 1, 3, 40):
+        args = (q, *c, lens, bt, d ** -0.5, 12 * block, splits)
+        assert fast.mxfp4_decode(*args) is not None
+        _same(*_both(monkeypatch, lambda: flag_attn.paged_attention_mxfp4(*args)))
+    assert fast.mxfp4_decode(q, *c, lens, bt, d ** -0.5, 12 * block, -1) is None
+    assert fast.mxfp4_decode(q.float(), *c, lens, bt, d ** -0.5, 12 * block, 0) is None
+    assert fast.mxfp4_decode(q, *c[:3], c[3].half(), lens, bt, d ** -0.5, 12 * block, 0) is None
