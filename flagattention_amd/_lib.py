@@ -229,6 +229,10 @@ SIGNATURES = {
          ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p,
          ctypes.c_int32, ctypes.c_void_p]),
     "fa_mxfp4_decode_args_size": (ctypes.c_int64, []),
+    "fa_mxfp4_decode_plan": (
+        ctypes.c_int,
+        [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+         ctypes.c_int32, ctypes.POINTER(Mxfp4DecodeArgs)]),
     "fa_mxfp4_decode": (ctypes.c_int, [ctypes.POINTER(Mxfp4DecodeArgs), ctypes.c_void_p]),
     "fa_mxfp4_combine": (ctypes.c_int, [ctypes.POINTER(Mxfp4DecodeArgs), ctypes.c_void_p]),
 }

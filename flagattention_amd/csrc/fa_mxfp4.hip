@@ -204,111 +204,174 @@ __global__ __launch_bounds__(kWThreads) void mxfp4_gather_kernel(
 //   V: the values are written to a tile in LDS, private to the wave, and read back transposed.
 // fp16 values are halved on the way (its largest codes, 4 * 2^14, would not fit otherwise) and
 // the scores and the output doubled.
-constexpr int kDThreads = 256;
+constexpr int kWaves = 4;
 constexpr int kDTile = 32;
 constexpr int kDRows = 16;
-
-__device__ __attribute__((aligned(16))) unsigned char g_mxfp4_zero[32];
-
-template <int D>
-__device__ inline int vslot(int r) {  // swizzle of the V tile's 16-byte chunks
-  constexpr int C = D / 8;
-  constexpr int L = C >= 16 ? 1 : 16 / C;
-  constexpr int H = (C < 16 ? C : 16) / 2;
-  return 2 * ((r / L) % H);
-}
 
 template <int kBytes>
 struct CodeWords {
   typedef unsigned int v __attribute__((ext_vector_type(kBytes / 4)));
 };
 
-template <typename T, int D>
-__global__ __launch_bounds__(kDThreads, 2) void mxfp4_decode_kernel(const fa_mxfp4_decode_args a) {
+// scale bytes of a lane's words of a token
+template <int D>
+struct ScaleOf {
+  typedef unsigned char type;
+};
+template <>
+struct ScaleOf<256> {
+  typedef unsigned short type;
+};
+
+#define FA_GLOBAL __attribute__((address_space(1)))
+
+template <typename T, int D, bool kSmallBlocks>
+__global__ __launch_bounds__(64 * kWaves, D == 64 ? 4 : D == 128 ? 3 : 2) void mxfp4_decode_kernel(
+    const fa_mxfp4_decode_args a) {
   typedef typename FVec<T>::v8 T8;
   typedef typename FVec<T>::v4 T4;
-  constexpr int kRowB = 2 * D;            // bytes per token row of the V tile
+  // Bytes per token row of the V tile: 32 more than its values, so that the 8 rows x 32 bytes of a
+  // transposing read's half wave, and the 8 x 16 of a write's, lie in different banks.
+  constexpr int kRowB = 2 * D + 32;
   constexpr int kTileB = kDTile * kRowB;
   constexpr int kWords = D / 32;          // words of codes per lane and token = k-steps of QK
   constexpr int kDimTiles = D / 16;
   constexpr bool kHalved = __is_same(T, _Float16);
   typedef typename CodeWords<4 * kWords>::v Words;
-  __shared__ __attribute__((aligned(16))) unsigned char vbuf[4 * kTileB];
-  __shared__ float ml[8 * kDRows];
-  static_assert(4 * kTileB >= 4 * kDRows * D * 4, "merge area must fit in the tile buffers");
+  typedef typename ScaleOf<D>::type ScaleBytes;
+  __shared__ __attribute__((aligned(16))) unsigned char vbuf[kWaves * kTileB];
+  __shared__ float ml[2 * kWaves * kDRows];
+  static_assert(kTileB >= kDRows * D * 4, "merge area must fit in the tile buffers");
+  // Two tiles of loads in registers at head dim 256 would leave a SIMD one wave.
+  constexpr bool kTwoTiles = D <= 128;
 
   const fa_mxfp4_cache& cache = a.cache;
-  const int split = blockIdx.x;
   const int group = a.h_q / cache.h_kv;
   const int n_rb = cdiv(group, kDRows);
-  const int hk = blockIdx.y / n_rb;
-  const int rb = blockIdx.y - hk * n_rb;
-  const int b = blockIdx.z;
+  const int hk = blockIdx.x / n_rb;
+  const int rb = blockIdx.x - hk * n_rb;
+  const int split = blockIdx.z;
+  // the splits of a long context start away from each other (see launch_decode_d)
+  const int turned = blockIdx.y + split * cdiv(a.batch, a.num_splits);
+  const int b = turned % a.batch;
   const int wave = wave_id();
   const int lane = threadIdx.x & 63;
   const int G = lane >> 4, c16 = lane & 15;
+  const float ninf = -__builtin_inff();
 
   const int seqlen = sload(a.seqlens + b);
   const int t0 = split * a.split_tokens;
   const int t1 = split + 1 == a.num_splits ? seqlen : min(t0 + a.split_tokens, seqlen);
   const int ntok = max(0, t1 - t0);
   const int ntiles = cdiv(ntok, kDTile);
-  const int last = t1 - 1;
+  const int rows = min(group - rb * kDRows, kDRows);
+  const int h0 = hk * group + rb * kDRows;  // query head of row 0
+  if (ntiles == 0 && a.num_splits > 1) {    // the merge does not look at an empty split's rows
+    if (threadIdx.x < rows)
+      a.lse_part[(static_cast<long long>(b) * a.h_q + h0 + threadIdx.x) * a.num_splits + split] =
+          ninf;
+    return;
+  }
 
-  const int rho = rb * kDRows + c16;
-  const bool row_ok = rho < group;
-  const int hq = hk * group + (row_ok ? rho : 0);
-  const float scale_log2 = a.scale * kLog2e * (kHalved ? 2.f : 1.f);
-  const float ninf = -__builtin_inff();
-
+  // The scale is applied inside the exponent, after the maximum, so it has to be positive: a
+  // negative one turns Q's signs instead, and zero makes Q zero.
+  const float mag = fabsf(a.scale) * kLog2e * (kHalved ? 2.f : 1.f);
+  const float scale_log2 = a.scale == 0.f ? 1.f : mag;
   T8 qf[kWords];
+  {
+    const bool row_ok = c16 < rows && a.scale != 0.f;
+    const unsigned int sign = a.scale < 0.f ? 0x80008000u : 0u;
+    const T* const qrow = static_cast<const T*>(a.q) + b * a.q_stride_b +
+                          (h0 + (c16 < rows ? c16 : 0)) * a.q_stride_h + (D / 4) * G;
 #pragma unroll
-  for (int kk = 0; kk < kWords; ++kk)
-    qf[kk] = row_ok ? *reinterpret_cast<const T8*>(static_cast<const T*>(a.q) + b * a.q_stride_b +
-                                                   hq * a.q_stride_h + (D / 4) * G + 8 * kk)
-                    : T8{};
+    for (int kk = 0; kk < kWords; ++kk) {
+      uintx4 w = *reinterpret_cast<const uintx4*>(qrow + 8 * kk);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = row_ok ? w[i] ^ sign : 0u;
+      qf[kk] = __builtin_bit_cast(T8, w);
+    }
+  }
 
   // ---- loads of a tile ----
-  const unsigned char* const kc = static_cast<const unsigned char*>(cache.k_codes);
-  const unsigned char* const vc = static_cast<const unsigned char*>(cache.v_codes);
-  const unsigned char* const ks = static_cast<const unsigned char*>(cache.k_scales);
-  const unsigned char* const vs = static_cast<const unsigned char*>(cache.v_scales);
+  // A tile lies in one block, or in two of 16 tokens (kSmallBlocks).  Where a block's rows are is
+  // worked out for 64 of the wave's blocks at once, a lane each; a tile then takes its scalars
+  // from there, and its loads are a uniform base plus 32-bit lane offsets that never change.
+  // (With scalar page lookups and address arithmetic per tile a step was 430 instructions.)
+  constexpr int kBlocks = kSmallBlocks ? 2 : 1;  // per tile
+  constexpr int kBlockKeys = kDTile / kBlocks;
+  constexpr int kBatch = 64 / kBlocks;           // tiles worked out at once
+  const FA_GLOBAL unsigned char* const kc =
+      (const FA_GLOBAL unsigned char*)cache.k_codes + hk * cache.code_stride_h;
+  const FA_GLOBAL unsigned char* const vc =
+      (const FA_GLOBAL unsigned char*)cache.v_codes + hk * cache.code_stride_h;
+  const FA_GLOBAL unsigned char* const ks =
+      (const FA_GLOBAL unsigned char*)cache.k_scales + hk * cache.scale_stride_h;
+  const FA_GLOBAL unsigned char* const vs =
+      (const FA_GLOBAL unsigned char*)cache.v_scales + hk * cache.scale_stride_h;
   const int32_t* const bt_row = a.block_table + static_cast<long long>(b) * a.bt_stride_b;
-  const int bs_shift = (cache.block_size & (cache.block_size - 1)) == 0
-                           ? __builtin_ctz(static_cast<unsigned int>(cache.block_size))
-                           : -1;
-  Words kw[2], vw[2];
-  unsigned int kse[2], vse[2];
-  bool seen[2];  // the half's page is inside the cache
-  auto issue = [&](int u) {
+  const unsigned int code_t = static_cast<unsigned int>(cache.code_stride_t);
+  const unsigned int scale_t = static_cast<unsigned int>(cache.scale_stride_t);
+  unsigned int code_lane[2], scale_lane[2];  // of a block's first and second 16 tokens
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int start = t0 + kDTile * u + 16 * h;
-      const int first = min(start, last);  // uniform; a half's 16 tokens lie in one block
-      const int blk = bs_shift >= 0 ? first >> bs_shift : first / cache.block_size;
-      const int page = blk < a.max_blocks_per_seq ? sload(bt_row + blk) : -1;
-      seen[h] = page >= 0 && page < cache.num_blocks;
-      const long long row = min(start + c16, last) - blk * cache.block_size;
-      const long long code = page * cache.code_stride_0 + hk * cache.code_stride_h +
-                             row * cache.code_stride_t + (D / 8) * G;
-      const long long sc = page * cache.scale_stride_0 + hk * cache.scale_stride_h +
-                           row * cache.scale_stride_t + (D / 4) * G / FA_MXFP4_GROUP;
-      kw[h] = *reinterpret_cast<const Words*>(seen[h] ? kc + code : g_mxfp4_zero);
-      vw[h] = *reinterpret_cast<const Words*>(seen[h] ? vc + code : g_mxfp4_zero);
-      const unsigned char* const kp = seen[h] ? ks + sc : g_mxfp4_zero;
-      const unsigned char* const vp = seen[h] ? vs + sc : g_mxfp4_zero;
-      if constexpr (D == 256) {
-        kse[h] = *reinterpret_cast<const unsigned short*>(kp);
-        vse[h] = *reinterpret_cast<const unsigned short*>(vp);
-      } else {
-        kse[h] = *kp;
-        vse[h] = *vp;
+  for (int h = 0; h < 2; ++h) {
+    const int r = c16 + (kSmallBlocks ? 0 : 16 * h);
+    code_lane[h] = r * code_t + (D / 8) * G;
+    scale_lane[h] = r * scale_t + (D / 4) * G / FA_MXFP4_GROUP;
+  }
+  unsigned int at_c[2], at_s[2];  // this lane's block: offsets of its codes and scales
+  int at_keys = 0;                // and how many keys it has
+  auto work_out = [&](int i0) {   // blocks of the wave's tiles i0, i0 + 1, ...
+    const int u = wave + kWaves * (i0 + lane / kBlocks);
+    const int start = t0 + kDTile * u + kBlockKeys * (lane % kBlocks);
+    const int blk = start >> __builtin_ctz(static_cast<unsigned int>(cache.block_size));
+    const int id = start < t1 && blk < a.max_blocks_per_seq ? bt_row[blk] : -1;
+    const bool in = id >= 0 && id < cache.num_blocks;
+    // a block outside the cache: the first one instead, all masked
+    const long long page = in ? id : 0;
+    const int row = in ? start & (cache.block_size - 1) : 0;
+    const long long c = page * cache.code_stride_0 + row * cache.code_stride_t;
+    const long long sc = page * cache.scale_stride_0 + row * cache.scale_stride_t;
+    at_c[0] = static_cast<unsigned int>(c);
+    at_c[1] = static_cast<unsigned int>(c >> 32);
+    at_s[0] = static_cast<unsigned int>(sc);
+    at_s[1] = static_cast<unsigned int>(sc >> 32);
+    at_keys = in ? min(t1 - start, kBlockKeys) : 0;
+  };
+  auto lane_of = [&](unsigned int v, int l) -> unsigned int {
+    return static_cast<unsigned int>(__builtin_amdgcn_readlane(static_cast<int>(v), l));
+  };
+  struct Tile {
+    Words k[2], v[2];
+    ScaleBytes ks[2], vs[2];
+    int keys[kBlocks];  // keys of each block, from its first token on (uniform)
+  };
+  auto issue = [&](Tile& x, int i) {  // i: tile of the batch
+#pragma unroll
+    for (int j = 0; j < kBlocks; ++j) {
+      const int l = kBlocks * i + j;
+      const unsigned long long c =
+          (static_cast<unsigned long long>(lane_of(at_c[1], l)) << 32) | lane_of(at_c[0], l);
+      const unsigned long long sc =
+          (static_cast<unsigned long long>(lane_of(at_s[1], l)) << 32) | lane_of(at_s[0], l);
+      x.keys[j] = __builtin_amdgcn_readlane(at_keys, l);
+      const FA_GLOBAL unsigned char *const kcp = kc + c, *const vcp = vc + c;
+      const FA_GLOBAL unsigned char *const ksp = ks + sc, *const vsp = vs + sc;
+#pragma unroll
+      for (int h = j; h < 2; h += kBlocks) {
+        // Seen afresh, a lane offset stays 32 bits beside a scalar base: hoisted as 64 bits it
+        // costs an addition per load and twice the registers.
+        unsigned int co = code_lane[h], so = scale_lane[h];
+        asm volatile("" : "+v"(co), "+v"(so));
+        x.k[h] = __builtin_nontemporal_load((const FA_GLOBAL Words*)(kcp + co));
+        x.v[h] = __builtin_nontemporal_load((const FA_GLOBAL Words*)(vcp + co));
+        x.ks[h] = *(const FA_GLOBAL ScaleBytes*)(ksp + so);
+        x.vs[h] = *(const FA_GLOBAL ScaleBytes*)(vsp + so);
       }
     }
   };
   // the scale of word kk of a lane, from its scale bytes
-  auto word_scale = [&](unsigned int bytes, int kk) -> float {
-    unsigned int e = D == 256 && kk >= 4 ? bytes >> 8 : bytes & 255u;
+  auto word_scale = [&](ScaleBytes bytes, int kk) -> float {
+    unsigned int e = D == 256 && kk >= 4 ? bytes >> 8 : bytes & 255;
     if (kHalved) e = e == 255u ? e : max(e, 1u) - 1u;
     return scale_of(e);
   };
@@ -319,107 +382,176 @@ __global__ __launch_bounds__(kDThreads, 2) void mxfp4_decode_kernel(const fa_mxf
   for (int dt = 0; dt < kDimTiles; ++dt) acc[dt] = floatx4{};
   unsigned char* const vb = vbuf + wave * kTileB;
 
-  if (wave < ntiles) issue(wave);
-  for (int u = wave; u < ntiles; u += 4) {
-    const int tile_start = t0 + kDTile * u;
+  // A tile is taken out of its registers, which the wave's tile after the next is then requested
+  // into: one tile of loads is in flight during all of a step, two during most of it.
+  auto step = [&](Tile& x, int i, bool more) {
+    // keys of the tile's halves (uniform)
+    const int keys0 = kSmallBlocks ? x.keys[0] : min(x.keys[0], 16);
+    const int keys1 = kSmallBlocks ? x.keys[kBlocks - 1] : x.keys[0] - 16;
+    const bool whole = min(keys0, keys1) >= 16;
     floatx4 s[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       s[h] = floatx4{};
 #pragma unroll
       for (int kk = 0; kk < kWords; ++kk)
-        s[h] = mfma_16x16x32(codes8<T>(kw[h][kk], word_scale(kse[h], kk)), qf[kk], s[h]);
+        s[h] = mfma_16x16x32(codes8<T>(x.k[h][kk], word_scale(x.ks[h], kk)), qf[kk], s[h]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    ScaleBytes vse[2] = {x.vs[0], x.vs[1]};
+    if (!whole) {
+      // a masked key's weight is 0, which does not hide a NaN: its scales become the smallest
+      if (c16 >= keys0) vse[0] = 0;
+      if (c16 >= keys1) vse[1] = 0;
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int r = 16 * h + c16;
 #pragma unroll
       for (int kk = 0; kk < kWords; ++kk)
-        *reinterpret_cast<T8*>(vb + r * kRowB + 16 * ((kWords * G + kk) ^ vslot<D>(r))) =
-            codes8<T>(vw[h][kk], word_scale(vse[h], kk));
+        *reinterpret_cast<T8*>(vb + (16 * h + c16) * kRowB + 16 * (kWords * G + kk)) =
+            codes8<T>(x.v[h][kk], word_scale(vse[h], kk));
+      __builtin_amdgcn_sched_barrier(0);
     }
-    const bool seen0 = seen[0], seen1 = seen[1];
-    if (u + 4 < ntiles) issue(u + 4);
-    // softmax down the column: tokens tile_start + 16h + 4G + i
-    float sv[2][4];
-    float tmax = ninf;
+    if (more) issue(x, i + (kTwoTiles ? 2 : 1));
+    __builtin_amdgcn_sched_barrier(0);
+    // softmax down the column: keys 16h + 4G + i of the tile
+    if (!whole) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int left = (h == 0 ? keys0 : keys1) - 4 * G;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[h][i] = i < left ? s[h][i] : ninf;
+      }
+    }
+    float tmax = s[0][0];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool ok = tile_start + 16 * h + 4 * G + i < t1 && (h == 0 ? seen0 : seen1);
-        sv[h][i] = ok ? s[h][i] * scale_log2 : ninf;
-        tmax = fmaxf(tmax, sv[h][i]);
-      }
-    tmax = max_xor32(max_xor16(tmax));
-    const float m_new = fmaxf(m_run, tmax);
-    const float m_use = m_new == ninf ? 0.f : m_new;
-    const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+      for (int i = 0; i < 4; ++i) tmax = fmaxf(tmax, s[h][i]);
+    tmax = max_xor32(max_xor16(tmax)) * scale_log2;
+    // The reference stays while no row's maximum is more than kLag above it: P then reaches
+    // 2^kLag, which rounds no worse, and the accumulators are left alone.
+    constexpr float kLag = 6.f;
+    if (__ballot(tmax > m_run + kLag || (m_run == ninf && tmax != ninf)) != 0ull) {  // uniform
+      const float m_new = fmaxf(m_run, tmax);
+      const float alpha = m_new == ninf ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < kDimTiles; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[dt][i] *= alpha;
+    }
+    const float nm = m_run == ninf ? 0.f : -m_run;
+    float c = scale_log2;
+    // a fused multiply-add does not round the product that a large reference is made of
+    if (__ballot(fabsf(nm) > 1024.f) != 0ull) {  // uniform
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[h][i] *= c;
+      c = 1.f;
+    }
     float psum = 0.f;
     T8 pb;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float p = __builtin_amdgcn_exp2f(sv[h][i] - m_use);
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][i], c, nm));
         psum += p;
         pb[4 * h + i] = static_cast<T>(p);
       }
-    l_run = l_run * alpha + psum;
-    m_run = m_new;
-    const int e = c16 >> 2, qd = c16 & 3;
-    const int r0 = 4 * G + e, r1 = 16 + 4 * G + e;
+    l_run += psum;
+    __builtin_amdgcn_sched_barrier(0);
+    const unsigned char* const vr = vb + (4 * G + (c16 >> 2)) * kRowB + 8 * (c16 & 3);
 #pragma unroll
     for (int dt = 0; dt < kDimTiles; ++dt) {
-      const int chunk = 2 * dt + (qd >> 1);
-      const T4 lo = lds_tr4<T>(vb + r0 * kRowB + 16 * (chunk ^ vslot<D>(r0)) + 8 * (qd & 1));
-      const T4 hi = lds_tr4<T>(vb + r1 * kRowB + 16 * (chunk ^ vslot<D>(r1)) + 8 * (qd & 1));
+      const T4 lo = lds_tr4<T>(vr + 32 * dt);
+      const T4 hi = lds_tr4<T>(vr + 16 * kRowB + 32 * dt);
       const T8 va = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-      floatx4 o = acc[dt];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] *= alpha;
-      acc[dt] = mfma_16x16x32(va, pb, o);
+      acc[dt] = mfma_16x16x32(va, pb, acc[dt]);
+      if (dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  const int mine = wave < ntiles ? (ntiles - wave + kWaves - 1) / kWaves : 0;  // tiles dealt in turn
+  for (int i0 = 0; i0 < mine; i0 += kBatch) {
+    const int n = min(mine - i0, kBatch);
+    Tile x;
+    work_out(i0);
+    issue(x, 0);
+    int i = 0;
+    if constexpr (!kTwoTiles) {
+      for (; i + 1 < n; ++i) step(x, i, true);
+      step(x, i, false);
+    } else {
+      Tile y;
+      if (n > 3) {
+        // Without a condition in front of a request the compiler knows how many are in flight, and
+        // waits for a tile without waiting for the one behind it.
+        issue(y, 1);
+        do {
+          step(x, i, true);
+          step(y, i + 1, true);
+          i += 2;
+        } while (i + 3 < n);
+      } else if (n > 1) {
+        issue(y, 1);
+      }
+      for (;;) {
+        step(x, i, i + 2 < n);
+        if (++i >= n) break;
+        step(y, i, false);
+        if (++i >= n) break;
+      }
     }
   }
 
-  // ---- merge the four waves' states ----
+  // ---- merge the waves' states ----
   const float l_col = sum_xor32(sum_xor16(l_run));
   __syncthreads();
   float* const om = reinterpret_cast<float*>(vbuf);  // [wave][16][D]
   if (G == 0) {
     ml[wave * kDRows + c16] = m_run;
-    ml[(4 + wave) * kDRows + c16] = l_col;
+    ml[(kWaves + wave) * kDRows + c16] = l_col;
   }
 #pragma unroll
   for (int dt = 0; dt < kDimTiles; ++dt)
     *reinterpret_cast<floatx4*>(om + (wave * kDRows + c16) * D + 16 * dt + 4 * G) = acc[dt];
   __syncthreads();
-  for (int idx = threadIdx.x; idx < kDRows * D; idx += kDThreads) {
-    const int r = idx / D, d = idx - r * D;
-    const int rr = rb * kDRows + r;
-    if (rr >= group) break;  // rows are in order: the rest are past the end too
-    float mw[4], M = ninf;
+  for (int idx = threadIdx.x; idx < rows * (D / 4); idx += 64 * kWaves) {
+    const int r = idx / (D / 4), d = 4 * (idx - r * (D / 4));
+    float mw[kWaves], M = ninf;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < kWaves; ++w) {
       mw[w] = ml[w * kDRows + r];
       M = fmaxf(M, mw[w]);
     }
     // no visible key: every weight and sum is 0; NaN sums stay NaN
     const float m_use = M == ninf ? 0.f : M;
-    float L = 0.f, O = 0.f;
+    float L = 0.f;
+    floatx4 O = floatx4{};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < kWaves; ++w) {
       const float f = __builtin_amdgcn_exp2f(mw[w] - m_use);
-      L += ml[(4 + w) * kDRows + r] * f;
-      O += om[(w * kDRows + r) * D + d] * f;
+      L += ml[(kWaves + w) * kDRows + r] * f;
+      const floatx4 o = *reinterpret_cast<const floatx4*>(om + (w * kDRows + r) * D + d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) O[i] += o[i] * f;
     }
-    const int h = hk * group + rr;
-    const float o = L == 0.f ? 0.f : O / L * (kHalved ? 2.f : 1.f);
+    const float inv = L == 0.f ? 0.f : (kHalved ? 2.f : 1.f) / L;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) O[i] *= inv;
+    const int h = h0 + r;
     if (a.num_splits == 1) {
-      static_cast<T*>(a.out)[b * a.o_stride_b + h * a.o_stride_h + d] = static_cast<T>(o);
+      T4 w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = static_cast<T>(O[i]);
+      *reinterpret_cast<T4*>(static_cast<T*>(a.out) + b * a.o_stride_b + h * a.o_stride_h + d) = w;
     } else {
       const long long prow = (static_cast<long long>(b) * a.h_q + h) * a.num_splits + split;
-      a.o_part[prow * D + d] = o;
+      *reinterpret_cast<floatx4*>(a.o_part + prow * D + d) = O;
       // the merge takes the largest lse, which a NaN would not be
       if (d == 0)
         a.lse_part[prow] = L == 0.f ? ninf : L == L ? (M + log2f(L)) * kLn2 : -ninf;
@@ -427,18 +559,55 @@ __global__ __launch_bounds__(kDThreads, 2) void mxfp4_decode_kernel(const fa_mxf
   }
 }
 
+template <typename T, int D>
+void launch_decode_d(const fa_mxfp4_decode_args* a, hipStream_t stream) {
+  const int group = a->h_q / a->cache.h_kv;
+  // Heads vary fastest and splits slowest: work-groups are dealt round-robin over 8 XCDs, and the
+  // late splits of ragged contexts are empty (with splits fastest, 8 of them, one XCD had all the
+  // last ones: 33.7 us instead of 27.3 at 32 sequences of 97 .. 4,096 keys).
+  const dim3 grid(a->cache.h_kv * cdiv(group, kDRows), a->batch, a->num_splits);
+  if (a->cache.block_size < kDTile)
+    hipLaunchKernelGGL((mxfp4_decode_kernel<T, D, true>), grid, dim3(64 * kWaves), 0, stream, *a);
+  else
+    hipLaunchKernelGGL((mxfp4_decode_kernel<T, D, false>), grid, dim3(64 * kWaves), 0, stream, *a);
+}
+
 template <typename T>
 int launch_decode(const fa_mxfp4_decode_args* a, hipStream_t stream) {
-  const int group = a->h_q / a->cache.h_kv;
-  const dim3 grid(a->num_splits, a->cache.h_kv * cdiv(group, kDRows), a->batch);
   if (a->cache.d == 64)
-    hipLaunchKernelGGL((mxfp4_decode_kernel<T, 64>), grid, dim3(kDThreads), 0, stream, *a);
+    launch_decode_d<T, 64>(a, stream);
   else if (a->cache.d == 128)
-    hipLaunchKernelGGL((mxfp4_decode_kernel<T, 128>), grid, dim3(kDThreads), 0, stream, *a);
+    launch_decode_d<T, 128>(a, stream);
   else
-    hipLaunchKernelGGL((mxfp4_decode_kernel<T, 256>), grid, dim3(kDThreads), 0, stream, *a);
+    launch_decode_d<T, 256>(a, stream);
   FA_CHECK_HIP(hipGetLastError());
   return FA_OK;
+}
+
+// Splits of `groups` (sequence, KV head, block of heads) triples of up to max_len keys: the cheapest
+// by a model of the launch.  A work-group takes a step of 128 keys in kStep us by itself; k of them
+// on a CU share its memory bandwidth, from two on, and the sequences of a batch are taken to be
+// half as long as the longest on average; a further work-group on a CU costs 1.4 us, the merge
+// 3.5 us and a little per split.  Measured at 32 heads of 8 KV heads, D = 128: one step 0.72 us
+// with one work-group per CU, 1.48 with two, 2.96 with four; 1,024 work-groups of one key 9.0 us a
+// call, 256 of them 4.7.
+int choose_splits(int64_t groups, int d, int64_t max_len, int64_t cus) {
+  const double step = d == 64 ? 0.5 : d == 128 ? 0.72 : 1.26;
+  const double shared = 0.74 * d / 128;
+  double best = 0;
+  int pick = 1;
+  for (int s : {1, 2, 3, 4, 5, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128}) {
+    if (s > 1 && max_len < 128 * static_cast<int64_t>(s)) break;
+    const double k = static_cast<double>(groups * s) / static_cast<double>(cus);
+    const double steps = static_cast<double>((max_len + 128 * s - 1) / (128 * s));
+    const double t = (k * shared / 2 > step ? k * shared / 2 : step) * steps +
+                     1.4 * (k > 1 ? k - 1 : 0) + (s > 1 ? 3.5 + 0.03 * s : 0);
+    if (s == 1 || t < best) {
+      best = t;
+      pick = s;
+    }
+  }
+  return pick;
 }
 
 bool aligned(const void* p, int64_t bytes) {
@@ -449,8 +618,8 @@ int check_cache(const fa_mxfp4_cache* c) {
   FA_CHECK_ARG(c != nullptr, "cache is NULL");
   FA_CHECK_ARG(c->d == 64 || c->d == 128 || c->d == 256, "head dim %d not in {64, 128, 256}", c->d);
   FA_CHECK_ARG(c->h_kv >= 1 && c->h_kv <= 65535, "h_kv %d not in [1, 65535]", c->h_kv);
-  FA_CHECK_ARG(c->block_size >= 16 && c->block_size % 16 == 0,
-               "block_size %d is not a multiple of 16", c->block_size);
+  FA_CHECK_ARG(c->block_size >= 16 && (c->block_size & (c->block_size - 1)) == 0,
+               "block_size %d is not a power of two of at least 16", c->block_size);
   FA_CHECK_ARG(c->num_blocks >= 1 && c->num_blocks <= INT32_MAX, "num_blocks %lld invalid",
                static_cast<long long>(c->num_blocks));
   FA_CHECK_ARG(c->k_codes && c->k_scales && c->v_codes && c->v_scales, "NULL cache pointer");
@@ -461,6 +630,10 @@ int check_cache(const fa_mxfp4_cache* c) {
   FA_CHECK_ARG(aligned(c->k_scales, sa) && aligned(c->v_scales, sa) && c->scale_stride_0 % sa == 0 &&
                    c->scale_stride_h % sa == 0 && c->scale_stride_t % sa == 0,
                "rows of scales must be %d-byte aligned", static_cast<int>(sa));
+  // 32-bit lane offsets inside 16 tokens
+  FA_CHECK_ARG(c->code_stride_t >= 0 && c->code_stride_t < (1ll << 27) && c->scale_stride_t >= 0 &&
+                   c->scale_stride_t < (1ll << 27),
+               "token strides of the cache must be in [0, 2^27)");
   return FA_OK;
 }
 
@@ -476,7 +649,7 @@ int check_decode(const fa_mxfp4_decode_args* a) {
                "grid too large: h_kv x ceil(group / 16) must be <= 65535");
   FA_CHECK_ARG(a->dtype == 0 || a->dtype == 1, "dtype %d is not 0 (fp16) or 1 (bf16)", a->dtype);
   FA_CHECK_ARG(a->num_splits >= 1 && a->num_splits <= 65535 && a->split_tokens >= 1 &&
-                   (a->num_splits == 1 || a->split_tokens % 16 == 0) &&
+                   (a->num_splits == 1 || a->split_tokens % kDTile == 0) &&
                    static_cast<int64_t>(a->num_splits - 1) * a->split_tokens <= INT32_MAX,
                "num_splits %d of %d tokens invalid", a->num_splits, a->split_tokens);
   FA_CHECK_ARG(a->num_splits == 1 || (a->o_part && a->lse_part),
@@ -485,6 +658,8 @@ int check_decode(const fa_mxfp4_decode_args* a) {
                "NULL q / out / block_table / seqlens or no block per sequence");
   FA_CHECK_ARG(aligned(a->q, 16) && a->q_stride_b % 8 == 0 && a->q_stride_h % 8 == 0,
                "q rows must be 16-byte aligned");
+  FA_CHECK_ARG(aligned(a->out, 8) && a->o_stride_b % 4 == 0 && a->o_stride_h % 4 == 0,
+               "out rows must be 8-byte aligned");
   return FA_OK;
 }
 
@@ -560,6 +735,22 @@ extern "C" int fa_mxfp4_gather(const fa_mxfp4_cache* cache, const int32_t* block
                        cu_seqlens, num_seqs, total, static_cast<_Float16*>(k_out),
                        static_cast<_Float16*>(v_out));
   FA_CHECK_HIP(hipGetLastError());
+  return FA_OK;
+}
+
+extern "C" int fa_mxfp4_decode_plan(int32_t batch, int32_t h_q, int32_t h_kv, int32_t d,
+                                    int32_t max_len, int32_t cu_count, fa_mxfp4_decode_args* a) {
+  FA_CHECK_ARG(a != nullptr, "args is NULL");
+  FA_CHECK_ARG(batch >= 1 && h_q >= 1 && h_kv >= 1 && h_q % h_kv == 0 && max_len >= 1 &&
+                   cu_count >= 1 && (d == 64 || d == 128 || d == 256),
+               "batch %d / h_q %d / h_kv %d / d %d / max_len %d / cu_count %d invalid", batch, h_q,
+               h_kv, d, max_len, cu_count);
+  const int s = fa::choose_splits(
+      static_cast<int64_t>(batch) * h_kv * fa::cdiv(h_q / h_kv, fa::kDRows), d, max_len, cu_count);
+  const int64_t each = (static_cast<int64_t>(max_len) + s - 1) / s;
+  a->split_tokens = static_cast<int32_t>((each + fa::kDTile - 1) / fa::kDTile * fa::kDTile);
+  a->num_splits = static_cast<int32_t>((static_cast<int64_t>(max_len) + a->split_tokens - 1) /
+                                       a->split_tokens);
   return FA_OK;
 }
 

@@ -767,7 +767,8 @@ bool mxfp4_cache_of(PyObject* const* args, const at::Tensor** t, fa_mxfp4_cache*
     return false;
   const int64_t code_align = std::min<int64_t>(16, d / 8), scale_align = d == 256 ? 2 : 1;
   if (kc.size(0) < 1 || kc.size(0) > INT32_MAX || kc.size(1) < 1 || kc.size(1) > 65535 ||
-      kc.size(2) < 16 || kc.size(2) % 16 != 0 || kc.size(2) > INT32_MAX ||
+      kc.size(2) < 16 || (kc.size(2) & (kc.size(2) - 1)) != 0 || kc.size(2) > INT32_MAX ||
+      kc.stride(2) >= (int64_t{1} << 27) || ks.stride(2) >= (int64_t{1} << 27) ||
       !aligned_rows(kc, code_align) || !aligned_rows(vc, code_align) ||
       !aligned_rows(ks, scale_align) || !aligned_rows(vs, scale_align))
     return false;
@@ -881,20 +882,21 @@ PyObject* mxfp4_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const c10::Device device = q->device();
   for (const at::Tensor* x : {lens, bt, t[0]})
     if (x->device() != device) return none();
-  int64_t split_tokens;
+  a.num_splits = 1;
+  a.split_tokens = 1;
   if (num_splits == 0) {
     const int cus = cu_count(device.index());
-    if (cus == 0) return none();
-    split_tokens = whole_tiles(
-        cdiv(max_len, choose_splits(seqs * h_kv, h_q / h_kv, kRowsPerWg, d, max_len, cus)));
-  } else if (num_splits == 1) {
-    split_tokens = max_len;
-  } else {
+    if (cus == 0 || seqs > INT32_MAX || h_q > INT32_MAX) return none();
+    check(fa_mxfp4_decode_plan(static_cast<int32_t>(seqs), static_cast<int32_t>(h_q), a.cache.h_kv,
+                               a.cache.d, static_cast<int32_t>(max_len), cus, &a));
+  } else if (num_splits > 1) {
     const int64_t each = cdiv(max_len, num_splits);
-    split_tokens = 16;
+    int64_t split_tokens = 32;
     while (split_tokens < each) split_tokens *= 2;
+    a.split_tokens = static_cast<int32_t>(split_tokens);
+    a.num_splits = static_cast<int32_t>(cdiv(max_len, split_tokens));
   }
-  const int64_t s = cdiv(max_len, split_tokens);
+  const int64_t s = a.num_splits;
   at::Tensor out;
   {
     NoGil nogil;
@@ -913,8 +915,6 @@ PyObject* mxfp4_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     a.o_stride_h = out.stride(1);
     a.batch = static_cast<int32_t>(seqs);
     a.h_q = static_cast<int32_t>(h_q);
-    a.num_splits = static_cast<int32_t>(s);
-    a.split_tokens = static_cast<int32_t>(split_tokens);
     a.scale = static_cast<float>(scale);
     a.dtype = q->scalar_type() == at::kBFloat16;
     if (s > 1) {

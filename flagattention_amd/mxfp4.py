@@ -21,8 +21,7 @@ from typing import Tuple
 import torch
 
 from . import _lib
-from .gqa import (_aligned, _cu_count, _dtype_code, _next_pow2, _require, choose_splits,
-                  whole_tiles)
+from .gqa import TILE_TOKENS, _aligned, _cu_count, _dtype_code, _next_pow2, _require
 
 HEAD_DIMS = (64, 128, 256)
 GROUP = 32
@@ -42,7 +41,8 @@ def _check_cache(key_cache, key_scales, value_cache, value_scales, device):
     tensors = (key_cache, key_scales, value_cache, value_scales)
     _require(all(t.dtype == torch.uint8 for t in tensors), "the cache must be uint8")
     _require(num_blocks >= 1 and 1 <= h_kv <= 65535, "the cache is empty or has too many heads")
-    _require(block_size >= 16 and block_size % 16 == 0, "block_size must be a multiple of 16")
+    _require(block_size >= 16 and block_size & (block_size - 1) == 0,
+             "block_size must be a power of two of at least 16")
     _require(value_cache.stride() == key_cache.stride()
              and value_scales.stride() == key_scales.stride(),
              "the V cache must have the same strides as the K cache")
@@ -54,6 +54,8 @@ def _check_cache(key_cache, key_scales, value_cache, value_scales, device):
                               (key_scales, scale_align), (value_scales, scale_align))),
              f"rows of codes must be {code_align}-byte aligned, rows of scales "
              f"{scale_align}-byte aligned")
+    _require(key_cache.stride(2) < 1 << 27 and key_scales.stride(2) < 1 << 27,
+             "the cache's rows are too far apart")
     _require(all(t.is_cuda and t.device == device for t in tensors),
              "all tensors must be CUDA (HIP) tensors on one device")
     return num_blocks, h_kv, block_size, d
@@ -193,7 +195,7 @@ def paged_attention_mxfp4(
                   ``block_tables[s, j // block_size]``; a block outside the cache reads as masked
                   keys
     num_splits    0 picks the split count, 1 disables splitting, s > 1 uses partitions of
-                  ``next_pow2(cdiv(max_context_len, s))`` tokens, at least 16
+                  ``next_pow2(cdiv(max_context_len, s))`` tokens, at least 32
 
     Returns ``out`` shaped and typed like ``query``; a sequence without keys gets 0.
     """
@@ -226,24 +228,22 @@ def paged_attention_mxfp4(
         return out
     if block_tables.shape[1] == 0:
         return out.zero_()
-    if num_splits == 0:
-        s = choose_splits(num_seqs, h_kv, h_q // h_kv, max_context_len, _cu_count(device),
-                          head_dim=d)
-        split_tokens = whole_tiles(-(-max_context_len // s))
-    elif num_splits == 1:
-        split_tokens = max_context_len
-    else:
-        split_tokens = max(16, _next_pow2(-(-max_context_len // num_splits)))
-    s = -(-max_context_len // split_tokens)
     args = _lib.Mxfp4DecodeArgs(
         cache=_cache_args(key_cache, key_scales, value_cache, value_scales), q=query.data_ptr(),
         q_stride_b=query.stride(0), q_stride_h=query.stride(1),
         block_table=block_tables.data_ptr(), bt_stride_b=block_tables.stride(0),
         max_blocks_per_seq=block_tables.shape[1], seqlens=context_lens.data_ptr(),
         out=out.data_ptr(), o_stride_b=out.stride(0), o_stride_h=out.stride(1), o_part=None,
-        lse_part=None, batch=num_seqs, h_q=h_q, num_splits=s, split_tokens=split_tokens,
+        lse_part=None, batch=num_seqs, h_q=h_q, num_splits=1, split_tokens=1,
         scale=float(attn_scale), dtype=code)
     lib = _lib.load()
+    if num_splits == 0:
+        _lib.check(lib.fa_mxfp4_decode_plan(num_seqs, h_q, h_kv, d, max_context_len,
+                                            _cu_count(device), ctypes.byref(args)))
+    elif num_splits > 1:
+        args.split_tokens = max(TILE_TOKENS, _next_pow2(-(-max_context_len // num_splits)))
+        args.num_splits = -(-max_context_len // args.split_tokens)
+    s = args.num_splits
     with torch.cuda.device(device):
         stream = torch.cuda.current_stream(device).cuda_stream
         if s > 1:

@@ -67,7 +67,8 @@ int fa_varlen_combine(const fa_varlen_args* args, void* stream);
  * 0.5, 1, 1.5, 2, 3, 4, 6).  Scales: uint8 [num_blocks][h_kv][block_size][d / 32], byte e for
  * 2^(e - 127), 255 for a group that is NaN as a whole.  K and V have the same strides, in bytes;
  * last dimensions are contiguous, rows of codes aligned to min(16, d / 8) bytes, rows of scales to
- * d / 128 bytes (at least 1).  Head dims 64, 128, 256; block_size a multiple of 16.
+ * d / 128 bytes (at least 1).  Head dims 64, 128, 256; block_size a power of
+ * two of at least 16.
  */
 typedef struct fa_mxfp4_cache {
   void* k_codes;
@@ -120,7 +121,7 @@ typedef struct fa_mxfp4_decode_args {
   float* o_part;   /* split workspace fp32 [batch][h_q][num_splits][d] */
   float* lse_part; /* fp32 [batch][h_q][num_splits] */
   int32_t batch, h_q;
-  int32_t num_splits, split_tokens; /* as in fa_gqa_decode_args; split_tokens a multiple of 16
+  int32_t num_splits, split_tokens; /* as in fa_gqa_decode_args; split_tokens a multiple of 32
                                        where there are several */
   float scale;
   int32_t dtype; /* 0 fp16, 1 bf16 */
@@ -128,6 +129,13 @@ typedef struct fa_mxfp4_decode_args {
 
 /* sizeof(fa_mxfp4_decode_args) as compiled into the library. */
 int64_t fa_mxfp4_decode_args_size(void);
+
+/*
+ * Fills in num_splits and split_tokens for sequences of up to max_len keys on a device of
+ * cu_count compute units.
+ */
+int fa_mxfp4_decode_plan(int32_t batch, int32_t h_q, int32_t h_kv, int32_t d, int32_t max_len,
+                         int32_t cu_count, fa_mxfp4_decode_args* args);
 
 /* Decode: writes out with num_splits == 1, else the partials for fa_mxfp4_combine. */
 int fa_mxfp4_decode(const fa_mxfp4_decode_args* args, void* stream);

@@ -61,7 +61,7 @@ CACHE_FAULTS = [
     (lambda c: c.update(value_scales=c["value_scales"][:1]), "head_size / 32"),
     (lambda c: _all(c, lambda t: t.char()), "uint8"),
     (lambda c: _all(c, lambda t: t[:0]), "empty"),
-    (lambda c: _all(c, lambda t: t[:, :, :8]), "multiple of 16"),
+    (lambda c: _all(c, lambda t: t[:, :, :8]), "power of two"),
     (lambda c: c.update(**_cache(d=96)), "head_size"),
     (lambda c: c.update(value_cache=c["value_cache"].transpose(0, 1).contiguous().transpose(0, 1)),
      "same strides"),
