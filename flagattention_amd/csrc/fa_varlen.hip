@@ -24,6 +24,7 @@ constexpr int kLRows = kLWaves * kLWaveRows;
 // Past this reference (log2 units) the scores are scaled in a pass of their own: a fused
 // multiply-add does not round their product with the scale, which the reference is made of.
 constexpr float kFusedMax = 1024.f;
+constexpr float kLag = 6.f;
 
 // Largest |x| of packed 16-bit values as unsigned bit patterns, folded into best.
 __device__ inline void fold_bits(unsigned int& best, uintx4 w) {
@@ -43,45 +44,111 @@ struct Item {
 
 __device__ inline int clip(int x, int hi) { return min(max(x, 0), hi); }
 
-// The sequence and row block of work item `item`: blocks of the sequences one after the other, the
-// last of a sequence (the longest under a causal mask) first.  The rows behind the last sequence and
-// those before the first are two more, without keys.
-__device__ inline Item find_item(const fa_varlen_args& a, int group, int item) {
+// One lane's sequence: lanes go through the sequences, the rows behind the last one and those
+// before the first (two more, without keys).
+struct Seq {
+  int q0, m, k0, n;
+};
+__device__ inline Seq seq_of(const fa_varlen_args& a, int s) {
+  Seq x{0, 0, 0, 0};
+  if (s < a.num_seqs) {
+    x.q0 = clip(a.cu_seqlens_q[s], a.total_q);
+    x.m = max(clip(a.cu_seqlens_q[s + 1], a.total_q) - x.q0, 0);
+    x.k0 = clip(a.cu_seqlens_k[s], a.total_k);
+    x.n = max(clip(a.cu_seqlens_k[s + 1], a.total_k) - x.k0, 0);
+  } else if (s == a.num_seqs) {
+    x.q0 = clip(a.cu_seqlens_q[s], a.total_q);
+    x.m = a.total_q - x.q0;
+  } else if (s == a.num_seqs + 1) {
+    x.m = clip(a.cu_seqlens_q[0], a.total_q);
+  }
+  return x;
+}
+__device__ inline Item item_of(const Seq& x, int l, int group, int block) {
+  Item it;
+  it.q0 = __builtin_amdgcn_readlane(x.q0, l);
+  it.rows = __builtin_amdgcn_readlane(x.m, l) * group;
+  it.k0 = __builtin_amdgcn_readlane(x.k0, l);
+  it.n = __builtin_amdgcn_readlane(x.n, l);
+  it.block = block;
+  return it;
+}
+
+// Inclusive prefix maximum over the lanes (non-negative values), as wave_incl_scan.
+__device__ inline int wave_incl_max(int x) {
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false));  // row_shr:1
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false));  // row_shr:2
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false));  // row_shr:4
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false));  // row_shr:8
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false));  // row_bcast:15
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false));  // row_bcast:31
+  return x;
+}
+
+// The sequence and row block of work item `item`: blocks of the sequences one after the other,
+// each one's last (the longest under a causal mask) first.
+__device__ inline Item find_in_order(const fa_varlen_args& a, int group, int item) {
   const int lane = threadIdx.x & 63;
-  for (int base = 0; base <= a.num_seqs + 1; base += 64) {
-    const int s = base + lane;
-    int q0 = 0, m = 0, k0 = 0, n = 0;
-    if (s < a.num_seqs) {
-      q0 = clip(a.cu_seqlens_q[s], a.total_q);
-      m = max(clip(a.cu_seqlens_q[s + 1], a.total_q) - q0, 0);
-      k0 = clip(a.cu_seqlens_k[s], a.total_k);
-      n = max(clip(a.cu_seqlens_k[s + 1], a.total_k) - k0, 0);
-    } else if (s == a.num_seqs) {
-      q0 = clip(a.cu_seqlens_q[s], a.total_q);
-      m = a.total_q - q0;
-    } else if (s == a.num_seqs + 1) {
-      m = clip(a.cu_seqlens_q[0], a.total_q);
-    }
-    const int blocks = cdiv(m * group, kLRows);
-    const int upto = wave_incl_scan(blocks);
+  for (int base = 0; base < a.num_seqs + 2; base += 64) {
+    const Seq x = seq_of(a, base + lane);
+    const int upto = wave_incl_scan(cdiv(x.m * group, kLRows));
     const unsigned long long past = __ballot(upto > item);
     if (past != 0ull) {
       const int l = __builtin_ctzll(past);
-      Item it;
-      it.q0 = __builtin_amdgcn_readlane(q0, l);
-      it.rows = __builtin_amdgcn_readlane(m, l) * group;
-      it.k0 = __builtin_amdgcn_readlane(k0, l);
-      it.n = __builtin_amdgcn_readlane(n, l);
-      it.block = __builtin_amdgcn_readlane(upto, l) - 1 - item;
-      return it;
+      return item_of(x, l, group, __builtin_amdgcn_readlane(upto, l) - 1 - item);
     }
     item -= __builtin_amdgcn_readlane(upto, 63);
   }
   return Item{0, 0, 0, 0, -1};
 }
 
+// The same with the items ordered by the keys that they walk, the longest first, so that a launch
+// of several work-groups per CU ends with short ones (up to 62 sequences, a lane each).  In units
+// of about a row block's positions, block j of a causal sequence costs low + j, low from its
+// prefix, and a block of a full one low; how many blocks cost c or more is a sum over the
+// sequences, so the item's cost is found by bisection, and its sequence by a scan of those that
+// have a block of that cost.  This takes 1 us longer than going in order.
+__device__ inline Item find_by_cost(const fa_varlen_args& a, int group, int item) {
+  const int lane = threadIdx.x & 63;
+  const Seq x = seq_of(a, lane);
+  const int shift = 31 - __builtin_clz(max(kLRows / group, 1));  // a power of two of positions
+  const int blocks = cdiv(x.m * group, kLRows);
+  const bool rises = a.causal && lane < a.num_seqs;
+  const int low = rises ? (max(x.n - x.m, 0) >> shift) + 1 : cdiv(x.n, 1 << shift);
+  const int end = low + (rises ? blocks : 1);  // past the highest cost
+  auto costing = [&](int c) -> int {           // this lane's blocks that cost c or more
+    return rises ? min(max(end - c, 0), blocks) : low >= c ? blocks : 0;
+  };
+  auto total = [&](int c) -> int {
+    return __builtin_amdgcn_readlane(wave_incl_scan(costing(c)), 63);
+  };
+  if (item >= total(0)) return Item{0, 0, 0, 0, -1};
+  int lo = 0;  // total(lo) > item >= total(hi)
+  int hi = __builtin_amdgcn_readlane(wave_incl_max(blocks > 0 ? end : 0), 63);
+  int above = 0;  // total(hi)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    const int n = total(mid);
+    if (n > item) {
+      lo = mid;
+    } else {
+      hi = mid;
+      above = n;
+    }
+  }
+  const int rank = item - above;  // among the blocks that cost lo
+  const int here = costing(lo) - costing(hi);
+  const int upto = wave_incl_scan(here);
+  const int l = __builtin_ctzll(__ballot(upto > rank));
+  const int before = __builtin_amdgcn_readlane(upto - here, l);
+  const int from = __builtin_amdgcn_readlane(low, l);
+  const bool up = __builtin_amdgcn_readlane(static_cast<int>(rises), l) != 0;
+  return item_of(x, l, group, up ? lo - from : rank - before);
+}
+
 template <typename T, int D>
-__global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_args a) {
+__global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_args a,
+                                                             const int by_cost) {
   typedef typename PVec<T>::v8 T8;
   typedef typename PVec<T>::v4 T4;
   constexpr int C = D / 8;
@@ -101,7 +168,8 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
 
   const int group = a.h_q / a.h_kv;
   const int hk = blockIdx.x % a.h_kv;
-  const Item it = find_item(a, group, blockIdx.x / a.h_kv);
+  const int item = blockIdx.x / a.h_kv;
+  const Item it = by_cost ? find_by_cost(a, group, item) : find_in_order(a, group, item);
   if (it.block < 0) return;  // uniform
   const int split = blockIdx.y;
   const int m = it.rows / group;
@@ -112,22 +180,6 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
 
   const int t0 = split * a.split_tokens;
   const int t1 = split + 1 == a.num_splits ? it.n : min(t0 + a.split_tokens, it.n);
-  // keys visible to a row: [0, n - m + 1 + position) causal, all otherwise
-  auto limit_of = [&](int row) -> int {
-    return a.causal ? min(it.n - m + 1 + row / group, t1) : t1;
-  };
-  const int row0 = it.block * kLRows;
-  const int wg_lim = limit_of(min(row0 + kLRows, it.rows) - 1);
-  const int wg_min = limit_of(row0);
-  const int ntiles = wg_lim > t0 ? cdiv(wg_lim - t0, kTok) : 0;
-  const int wrow0 = row0 + kLWaveRows * wave;
-  const int wave_min = limit_of(min(wrow0, it.rows - 1));
-  const int wave_max = limit_of(min(wrow0 + kLWaveRows, it.rows) - 1);
-  const bool wave_on = wrow0 < it.rows;
-  const int row = min(wrow0 + c32, it.rows - 1);  // past the end: the last row, not stored
-  const int mm = row / group, jj = row - mm * group;
-  const int lim = limit_of(row);
-
   const float ninf = -__builtin_inff();
   // The scale is applied inside the exponent, after the mask and the maximum.  That needs a
   // positive one: otherwise the scores are scaled before either.
@@ -155,15 +207,51 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
     const unsigned char* const vs = vp + static_cast<long long>(start) * v_tb;
     unsigned char* const kd = bufs + buf * kTileB + kCopies * wave * 1024;
     unsigned char* const vd = bufs + (2 + buf) * kTileB + kCopies * wave * 1024;
-    const int last = t1 - 1 - start;  // rows past the end repeat the last one (masked)
+    if (start + kTok <= t1) {  // uniform
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i) {
-      const int r = (kCopies * wave + i) * kRowsPerCopy + crow;
-      const unsigned int back = r > last ? r - last : 0;
-      lds_dma16_off(ks, koff[i] - back * k_tb, (FA_LDS void*)(kd + 1024 * i));
-      lds_dma16_off(vs, voff[i] - back * v_tb, (FA_LDS void*)(vd + 1024 * i));
+      for (int i = 0; i < kCopies; ++i) lds_dma16_off(ks, koff[i], (FA_LDS void*)(kd + 1024 * i));
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) lds_dma16_off(vs, voff[i], (FA_LDS void*)(vd + 1024 * i));
+    } else {  // rows past the end repeat the last one (masked)
+      const int last = t1 - 1 - start;
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const int r = (kCopies * wave + i) * kRowsPerCopy + crow;
+        const unsigned int back = r > last ? r - last : 0;
+        lds_dma16_off(ks, koff[i] - back * k_tb, (FA_LDS void*)(kd + 1024 * i));
+        lds_dma16_off(vs, voff[i] - back * v_tb, (FA_LDS void*)(vd + 1024 * i));
+      }
     }
   };
+
+  if (t1 > t0) issue(0, 0);  // the first tile is on its way from here on
+
+  // Position and query head of the work-group's row r, counted from its first: rows are few, so a
+  // reciprocal and a correction divide them by the group.
+  const int row0 = it.block * kLRows;
+  const int left = min(it.rows - row0, kLRows);  // the work-group's rows
+  const int pos0 = row0 / group, rem0 = row0 - pos0 * group;
+  const float group_inv = __builtin_amdgcn_rcpf(static_cast<float>(group));
+  auto pos_of = [&](int r) -> int {
+    const int x = rem0 + r;
+    int q = static_cast<int>(static_cast<float>(x) * group_inv);
+    q += x - q * group >= group ? 1 : 0;
+    q -= x - q * group < 0 ? 1 : 0;
+    return pos0 + q;
+  };
+  auto head_of = [&](int r, int pos) -> int { return rem0 + r - (pos - pos0) * group; };
+  // keys visible to a position: [0, n - m + 1 + position) causal, all otherwise
+  auto limit_of = [&](int pos) -> int { return a.causal ? min(it.n - m + 1 + pos, t1) : t1; };
+  const int wg_min = limit_of(pos0);
+  const int wg_lim = limit_of(pos_of(left - 1));
+  const int ntiles = wg_lim > t0 ? cdiv(wg_lim - t0, kTok) : 0;
+  const int wrow0 = kLWaveRows * wave;
+  const int wave_min = limit_of(pos_of(min(wrow0, left - 1)));
+  const int wave_max = limit_of(pos_of(min(wrow0 + kLWaveRows, left) - 1));
+  const bool wave_on = wrow0 < left;
+  const int row = min(wrow0 + c32, left - 1);  // past the end: the last row, not stored
+  const int mm = pos_of(row), jj = head_of(row, mm);
+  const int lim = limit_of(mm);
 
   // Q^T operand: row c32, dims 16kk + 8g..+7
   T8 qf[kKSteps];
@@ -190,7 +278,6 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
     vbase[dt] = vtok * kRowB + 32 * ((2 * dt + (h16 & 1)) ^ fv<C>(vtok)) + 16 * (qd >> 1) +
                 8 * (qd & 1);
 
-  if (ntiles > 0) issue(0, 0);
   for (int u = 0; u < ntiles; ++u) {
     const int buf = u & 1;
     const int start = t0 + kTok * u;
@@ -233,14 +320,27 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
     const unsigned char* const kb = bufs + buf * kTileB;
     const unsigned char* const vb = bufs + (2 + buf) * kTileB;
 
+    // K operands one k-step ahead of their MFMAs (the fences keep them there)
     floatx16 s[kSub];
+    T8 ka[2][kSub];
+    auto k_read = [&](int kk, int tt) -> T8 {
+      return *reinterpret_cast<const T8*>(kb + 32 * tt * kRowB + (kbase ^ (32 * kk)));
+    };
 #pragma unroll
     for (int tt = 0; tt < kSub; ++tt) {
       s[tt] = floatx16{};
+      ka[0][tt] = k_read(0, tt);
+    }
 #pragma unroll
-      for (int kk = 0; kk < kKSteps; ++kk)
-        s[tt] = mfma_32x32x16(
-            *reinterpret_cast<const T8*>(kb + 32 * tt * kRowB + (kbase ^ (32 * kk))), qf[kk], s[tt]);
+    for (int kk = 0; kk < kKSteps; ++kk) {
+      if (kk + 1 < kKSteps) {
+#pragma unroll
+        for (int tt = 0; tt < kSub; ++tt) ka[(kk + 1) & 1][tt] = k_read(kk + 1, tt);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int tt = 0; tt < kSub; ++tt) s[tt] = mfma_32x32x16(ka[kk & 1][tt], qf[kk], s[tt]);
+      __builtin_amdgcn_sched_barrier(0);
     }
     if (prescale) {
 #pragma unroll
@@ -250,13 +350,13 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
     }
     const bool masked = start + kTok > wave_min;  // uniform: some row does not see the whole tile
     if (masked) {
-      const int left = lim - start - 4 * g;
+      const int sees = lim - start - 4 * g;
 #pragma unroll
       for (int tt = 0; tt < kSub; ++tt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int j = 32 * tt + 8 * (i >> 2) + (i & 3);  // + 4g: the key of s[tt][i]
-          s[tt][i] = j < left ? s[tt][i] : ninf;
+          s[tt][i] = j < sees ? s[tt][i] : ninf;
         }
     }
     float mx = s[0][0];
@@ -265,14 +365,18 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[tt][i]);
     mx = max_xor32(mx) * scale_log2;
-    const float m_new = fmaxf(mref, mx);
-    const float alpha = m_new == ninf ? 1.f : __builtin_amdgcn_exp2f(mref - m_new);
-    lsum *= alpha;
-    mref = m_new;
+    // The reference stays while no row's maximum is more than kLag above it: P then reaches
+    // 2^kLag, which rounds no worse, and the accumulators are left alone.
+    if (__ballot(mx > mref + kLag || (mref == ninf && mx != ninf)) != 0ull) {  // uniform
+      const float m_new = fmaxf(mref, mx);
+      const float alpha = m_new == ninf ? 1.f : __builtin_amdgcn_exp2f(mref - m_new);
+      lsum *= alpha;
+      mref = m_new;
 #pragma unroll
-    for (int dt = 0; dt < kDimTiles; ++dt)
+      for (int dt = 0; dt < kDimTiles; ++dt)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[dt][i] *= alpha;
+        for (int i = 0; i < 16; ++i) acc[dt][i] *= alpha;
+    }
     const float nm = mref == ninf ? 0.f : -mref;
     float c = scale_log2;
     if (__ballot(fabsf(nm) > kFusedMax) != 0ull) {  // uniform
@@ -334,7 +438,7 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
   const float lse = some ? (mref + log2f(l)) * kLn2 : ninf;
   const int h = hk * group + jj;
   const long long orow = static_cast<long long>(h) * a.total_q + it.q0 + mm;
-  const bool mine = wrow0 + c32 < it.rows;
+  const bool mine = wrow0 + c32 < left;
   if (a.num_splits > 1) {
     if (mine) {
       const long long prow = orow * a.num_splits + split;
@@ -373,8 +477,8 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
     const int r = i * kRowsPerCopy + crow;
     const int rr = wrow0 + r;
     const T8 v = *reinterpret_cast<const T8*>(st + r * kRowB + 16 * (cslot ^ (r & 7)));
-    if (rr < it.rows) {
-      const int m2 = rr / group, j2 = rr - m2 * group;
+    if (rr < left) {
+      const int m2 = pos_of(rr), j2 = head_of(rr, m2);
       *reinterpret_cast<T8*>(static_cast<T*>(a.out) + (it.q0 + m2) * a.o_stride_t +
                              (hk * group + j2) * a.o_stride_h + 8 * cslot) = v;
     }
@@ -391,12 +495,15 @@ template <typename T>
 void launch_varlen(const fa_varlen_args* a, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(row_blocks(a) * a->h_kv),
                   static_cast<unsigned>(a->num_splits));
+  // More work-groups than run at once (2 per CU; 3 at head dim 64): the longest go first.  Under
+  // that their order is all the same and finding it costs 2 us.
+  const int by_cost = a->num_seqs + 2 <= 64 && grid.x * grid.y > (a->d == 64 ? 768u : 512u);
   if (a->d == 64)
-    hipLaunchKernelGGL((varlen_kernel<T, 64>), grid, dim3(kLThreads), 0, stream, *a);
+    hipLaunchKernelGGL((varlen_kernel<T, 64>), grid, dim3(kLThreads), 0, stream, *a, by_cost);
   else if (a->d == 128)
-    hipLaunchKernelGGL((varlen_kernel<T, 128>), grid, dim3(kLThreads), 0, stream, *a);
+    hipLaunchKernelGGL((varlen_kernel<T, 128>), grid, dim3(kLThreads), 0, stream, *a, by_cost);
   else
-    hipLaunchKernelGGL((varlen_kernel<T, 256>), grid, dim3(kLThreads), 0, stream, *a);
+    hipLaunchKernelGGL((varlen_kernel<T, 256>), grid, dim3(kLThreads), 0, stream, *a, by_cost);
 }
 
 bool rows16(const void* p, int64_t s0, int64_t s1) {

@@ -177,14 +177,18 @@ def test_equals_the_rectangular_operator_where_both_apply():
     assert float((lse.view(8, 3, 256).transpose(0, 1) - l2).abs().max()) < 1e-5
 
 
-def test_many_sequences():
-    """More sequences than a wave has lanes, most of a few tokens, some empty."""
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("seqs", [62, 63, 200, 254, 255, 400])
+def test_many_sequences(seqs, causal):
+    """More sequences than a wave has lanes, and than are ordered by their cost; most of a few
+    tokens, some empty."""
     need_gpu()
-    say("varlen many sequences")
+    say(f"varlen {seqs} sequences causal={causal}")
     gen = torch.Generator().manual_seed(4)
-    lens = torch.randint(0, 40, (200,), generator=gen).tolist()
-    lens[130] = 700
-    check(*inputs(lens, lens, 4, 1, 64, torch.bfloat16, seed=12), True)
+    lens = torch.randint(0, 40, (seqs,), generator=gen).tolist()
+    lens[seqs // 2] = 700
+    keys = [n + int(x) for n, x in zip(lens, torch.randint(0, 30, (seqs,), generator=gen))]
+    check(*inputs(lens, keys, 4, 1, 64, torch.bfloat16, seed=12, extra_q=130), causal)
 
 
 def test_offsets_past_32_bits():
