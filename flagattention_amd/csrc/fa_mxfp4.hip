@@ -70,7 +70,34 @@ __device__ inline unsigned int dpp_u32(unsigned int v) {
 }
 
 constexpr int kWThreads = 256;
-constexpr int kWItems = 4;  // 8-dim pieces per thread, all requested before the first is stored
+constexpr int kWTokens = 16;  // tokens per work-group at most
+
+// Rows of a work-group's tokens in the cache: byte offsets of their codes and scales, -1: none.
+struct RowSlots {
+  long long code[kWTokens], scale[kWTokens];
+};
+
+__device__ inline void set_row(RowSlots& rows, int t, const fa_mxfp4_cache& cache, bool in,
+                               long long block, long long row) {
+  rows.code[t] = in ? block * cache.code_stride_0 + row * cache.code_stride_t : -1;
+  rows.scale[t] = in ? block * cache.scale_stride_0 + row * cache.scale_stride_t : -1;
+}
+
+// The n-th 8-dim piece of a work-group's rows [token][head][piece].  Heads divide by a reciprocal
+// and a correction: n / pieces is below 2^20.
+struct Piece {
+  int token, head, piece;
+};
+__device__ inline Piece piece_of(int n, int log_pieces, int h_kv, float h_inv) {
+  Piece p;
+  p.piece = n & ((1 << log_pieces) - 1);
+  const int th = n >> log_pieces;
+  p.token = static_cast<int>(static_cast<float>(th) * h_inv);
+  p.token += th - p.token * h_kv >= h_kv ? 1 : 0;
+  p.token -= th - p.token * h_kv < 0 ? 1 : 0;
+  p.head = th - p.token * h_kv;
+  return p;
+}
 
 // A lane holds 8 dims of a row (16 bytes in, 4 out), four neighbouring lanes a group of 32, whose
 // amax they find with two lane exchanges.  blockIdx.y: K or V.  Bound by memory: it reads
@@ -79,117 +106,145 @@ template <typename T>
 __global__ __launch_bounds__(kWThreads) void mxfp4_write_kernel(
     const fa_mxfp4_cache cache, const T* __restrict__ key, long long key_st, long long key_sh,
     const T* __restrict__ value, long long value_st, long long value_sh, const void* slots,
-    int slots64, int num_tokens) {
+    int slots64, int num_tokens, int tokens) {
   typedef typename FVec<T>::v8 T8;
+  constexpr int kItems = 4;  // requested before the first is stored
+  __shared__ RowSlots rows;
   const bool is_v = blockIdx.y != 0;
-  const T* const src = is_v ? value : key;
   const long long st = is_v ? value_st : key_st, sh = is_v ? value_sh : key_sh;
+  const int tok0 = blockIdx.x * tokens;
+  const T* const src = (is_v ? value : key) + tok0 * st;
   unsigned char* const codes = static_cast<unsigned char*>(is_v ? cache.v_codes : cache.k_codes);
   unsigned char* const scales = static_cast<unsigned char*>(is_v ? cache.v_scales : cache.k_scales);
-  const int pieces = cache.d / 8;
-  const int log_pieces = __builtin_ctz(pieces);
-  const long long total = static_cast<long long>(num_tokens) * cache.h_kv * pieces;
-  const long long first = static_cast<long long>(blockIdx.x) * (kWThreads * kWItems) + threadIdx.x;
-  T8 x[kWItems];
-  long long slot[kWItems];
-  int head[kWItems], piece[kWItems];
-#pragma unroll
-  for (int j = 0; j < kWItems; ++j) {
-    const long long i = min(first + j * kWThreads, total - 1);
-    piece[j] = static_cast<int>(i) & (pieces - 1);
-    const unsigned int th = static_cast<unsigned int>(i >> log_pieces);  // below 2^31 (host)
-    const unsigned int tok = th / static_cast<unsigned int>(cache.h_kv);
-    head[j] = static_cast<int>(th - tok * cache.h_kv);
-    slot[j] = slots64 ? static_cast<const long long*>(slots)[tok]
-                      : static_cast<const int*>(slots)[tok];
-    x[j] = __builtin_nontemporal_load(
-        reinterpret_cast<const T8*>(src + tok * st + head[j] * sh + 8 * piece[j]));
+  const int log_pieces = __builtin_ctz(cache.d / 8);
+  const int mine = min(tokens, num_tokens - tok0);
+  const int n = (mine * cache.h_kv) << log_pieces;
+  const float h_inv = __builtin_amdgcn_rcpf(static_cast<float>(cache.h_kv));
+  if (static_cast<int>(threadIdx.x) < mine) {
+    const int t = tok0 + threadIdx.x;
+    const long long slot =
+        slots64 ? static_cast<const long long*>(slots)[t] : static_cast<const int*>(slots)[t];
+    const long long block = slot >> __builtin_ctz(static_cast<unsigned int>(cache.block_size));
+    set_row(rows, threadIdx.x, cache, slot >= 0 && block < cache.num_blocks, block,
+            slot & (cache.block_size - 1));
   }
+  for (int base = 0; base < n; base += kWThreads * kItems) {
+    const int i0 = base + threadIdx.x;
+    T8 x[kItems];
+    Piece p[kItems];
 #pragma unroll
-  for (int j = 0; j < kWItems; ++j) {
-    // bit patterns of |x|: their unsigned order is the order of the values, and NaN lies above all
-    unsigned int amax = 0u;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      amax = max(amax, __float_as_uint(static_cast<float>(x[j][i])) & 0x7FFFFFFFu);
-    amax = max(amax, dpp_u32<0xB1>(amax));  // quad_perm [1, 0, 3, 2]
-    amax = max(amax, dpp_u32<0x4E>(amax));  // quad_perm [2, 3, 0, 1]
-    // smallest e with amax <= 7 * 2^(e - 127): 7 = 1.75 * 4, so amax's own exponent less 2, and
-    // one more where its fraction is above 1.75 (the addition then carries into the exponent)
-    const int field = static_cast<int>((amax + 0x1FFFFFu) >> 23) - 2;
-    const bool finite = amax < 0x7F800000u;
-    const unsigned int e = finite ? static_cast<unsigned int>(max(field, 0)) : 255u;
-    const float scale = scale_of(e);
-    unsigned int w = 0u;
-    if (finite) {
-      w = to_codes2<T, 0>(w, __builtin_shufflevector(x[j], x[j], 0, 1), scale);
-      w = to_codes2<T, 1>(w, __builtin_shufflevector(x[j], x[j], 2, 3), scale);
-      w = to_codes2<T, 2>(w, __builtin_shufflevector(x[j], x[j], 4, 5), scale);
-      w = to_codes2<T, 3>(w, __builtin_shufflevector(x[j], x[j], 6, 7), scale);
+    for (int j = 0; j < kItems; ++j) {
+      p[j] = piece_of(min(i0 + kWThreads * j, n - 1), log_pieces, cache.h_kv, h_inv);
+      x[j] = __builtin_nontemporal_load(
+          reinterpret_cast<const T8*>(src + p[j].token * st + p[j].head * sh + 8 * p[j].piece));
     }
-    const long long blk = slot[j] >= 0 ? slot[j] / cache.block_size : -1;
-    if (first + j * kWThreads >= total || blk < 0 || blk >= cache.num_blocks) continue;
-    const long long row = slot[j] - blk * cache.block_size;
-    *reinterpret_cast<unsigned int*>(codes + blk * cache.code_stride_0 +
-                                     head[j] * cache.code_stride_h + row * cache.code_stride_t +
-                                     4 * piece[j]) = w;
-    if ((piece[j] & 3) == 0)
-      scales[blk * cache.scale_stride_0 + head[j] * cache.scale_stride_h +
-             row * cache.scale_stride_t + (piece[j] >> 2)] = static_cast<unsigned char>(e);
+    if (base == 0) __syncthreads();  // the rows, whose slots came beside the first values
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) {
+      // bit patterns of |x|: their unsigned order is the order of the values, and NaN lies above all
+      unsigned int amax = 0u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        amax = max(amax, __float_as_uint(static_cast<float>(x[j][i])) & 0x7FFFFFFFu);
+      amax = max(amax, dpp_u32<0xB1>(amax));  // quad_perm [1, 0, 3, 2]
+      amax = max(amax, dpp_u32<0x4E>(amax));  // quad_perm [2, 3, 0, 1]
+      // smallest e with amax <= 7 * 2^(e - 127): 7 = 1.75 * 4, so amax's own exponent less 2, and
+      // one more where its fraction is above 1.75 (the addition then carries into the exponent)
+      const int field = static_cast<int>((amax + 0x1FFFFFu) >> 23) - 2;
+      const bool finite = amax < 0x7F800000u;
+      const unsigned int e = finite ? static_cast<unsigned int>(max(field, 0)) : 255u;
+      const float scale = scale_of(e);
+      unsigned int w = 0u;
+      if (finite) {
+        w = to_codes2<T, 0>(w, __builtin_shufflevector(x[j], x[j], 0, 1), scale);
+        w = to_codes2<T, 1>(w, __builtin_shufflevector(x[j], x[j], 2, 3), scale);
+        w = to_codes2<T, 2>(w, __builtin_shufflevector(x[j], x[j], 4, 5), scale);
+        w = to_codes2<T, 3>(w, __builtin_shufflevector(x[j], x[j], 6, 7), scale);
+      }
+      const long long code = rows.code[p[j].token];
+      if (i0 + kWThreads * j >= n || code < 0) continue;
+      *reinterpret_cast<unsigned int*>(codes + code + p[j].head * cache.code_stride_h +
+                                       4 * p[j].piece) = w;
+      if ((p[j].piece & 3) == 0)
+        scales[rows.scale[p[j].token] + p[j].head * cache.scale_stride_h + (p[j].piece >> 2)] =
+            static_cast<unsigned char>(e);
+    }
   }
 }
 
 // ---- read back ----
 
-// A lane takes 8 dims of a packed row: 4 bytes of codes in, 16 bytes out.
+// A lane takes 8 dims of a packed row: 4 bytes of codes in, 16 bytes out.  A wave finds the
+// sequences of a quarter of the work-group's tokens, 64 starts at a time.
 template <typename T>
 __global__ __launch_bounds__(kWThreads) void mxfp4_gather_kernel(
     const fa_mxfp4_cache cache, const int32_t* __restrict__ block_table, long long bt_stride,
-    int max_blocks, const int32_t* __restrict__ cu, int num_seqs, int total, T* __restrict__ k_out,
-    T* __restrict__ v_out) {
+    int max_blocks, const int32_t* __restrict__ cu, int num_seqs, int total, int tokens,
+    T* __restrict__ k_out, T* __restrict__ v_out) {
   typedef typename FVec<T>::v8 T8;
+  constexpr int kItems = 4;
+  __shared__ RowSlots rows;
   const bool is_v = blockIdx.y != 0;
   const unsigned char* const codes =
       static_cast<const unsigned char*>(is_v ? cache.v_codes : cache.k_codes);
   const unsigned char* const scales =
       static_cast<const unsigned char*>(is_v ? cache.v_scales : cache.k_scales);
-  T* const out = is_v ? v_out : k_out;
-  const int pieces = cache.d / 8;
-  const int log_pieces = __builtin_ctz(pieces);
-  const long long items = static_cast<long long>(total) * cache.h_kv * pieces;
-  const long long i = static_cast<long long>(blockIdx.x) * kWThreads + threadIdx.x;
-  if (i >= items) return;
-  const int piece = static_cast<int>(i) & (pieces - 1);
-  const unsigned int th = static_cast<unsigned int>(i >> log_pieces);
-  const int tok = static_cast<int>(th / static_cast<unsigned int>(cache.h_kv));
-  const int head = static_cast<int>(th - static_cast<unsigned int>(tok) * cache.h_kv);
-  // the last sequence that starts at or before the row
-  int lo = -1, hi = num_seqs;  // cu[lo] <= tok < cu[hi], as far as looked at
-  if (cu[num_seqs] > tok) {
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (cu[mid] <= tok)
-        lo = mid;
-      else
-        hi = mid;
+  const int tok0 = blockIdx.x * tokens;
+  const int mine = min(tokens, total - tok0);
+  const int log_pieces = __builtin_ctz(cache.d / 8);
+  const int n = (mine * cache.h_kv) << log_pieces;
+  const float h_inv = __builtin_amdgcn_rcpf(static_cast<float>(cache.h_kv));
+  {
+    constexpr int kEach = kWTokens / (kWThreads / 64);
+    const int lane = threadIdx.x & 63;
+    const int first = tok0 + kEach * wave_id();
+    int starts[kEach] = {};  // starts at or before the wave's tokens
+    for (int base = 0; base <= num_seqs; base += 64) {
+      const int c = base + lane <= num_seqs ? cu[base + lane] : 0x7FFFFFFF;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) starts[i] += __builtin_popcountll(__ballot(c <= first + i));
+    }
+    int s = -1;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) s = lane == i ? starts[i] - 1 : s;
+    const int t = kEach * wave_id() + lane;
+    if (lane < kEach && t < mine) {
+      bool in = s >= 0 && s < num_seqs;
+      const int pos = in ? tok0 + t - cu[s] : -1;
+      const int blk = pos >> __builtin_ctz(static_cast<unsigned int>(cache.block_size));
+      in = pos >= 0 && blk < max_blocks;
+      const int page = in ? block_table[s * bt_stride + blk] : -1;
+      set_row(rows, t, cache, page >= 0 && page < cache.num_blocks, page,
+              pos & (cache.block_size - 1));
     }
   }
-  T8 w = T8{};
-  if (lo >= 0) {
-    const int pos = tok - cu[lo];
-    const int blk = pos / cache.block_size;
-    const int page = blk < max_blocks ? block_table[lo * bt_stride + blk] : -1;
-    if (page >= 0 && page < cache.num_blocks) {
-      const long long row = pos - blk * cache.block_size;
-      const unsigned int c = *reinterpret_cast<const unsigned int*>(
-          codes + page * cache.code_stride_0 + head * cache.code_stride_h +
-          row * cache.code_stride_t + 4 * piece);
-      const unsigned int e = scales[page * cache.scale_stride_0 + head * cache.scale_stride_h +
-                                    row * cache.scale_stride_t + (piece >> 2)];
-      w = codes8<T>(c, scale_of(e));
+  __syncthreads();
+  T* const out = (is_v ? v_out : k_out) + ((static_cast<long long>(tok0) * cache.h_kv) << log_pieces) * 8;
+  for (int i0 = threadIdx.x; i0 < n; i0 += kWThreads * kItems) {
+    unsigned int w[kItems], e[kItems];
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) {
+      const Piece p = piece_of(min(i0 + kWThreads * j, n - 1), log_pieces, cache.h_kv, h_inv);
+      const long long code = rows.code[p.token], scale = rows.scale[p.token];
+      w[j] = e[j] = 0u;
+      if (code >= 0) {
+        w[j] = __builtin_nontemporal_load(reinterpret_cast<const unsigned int*>(
+            codes + code + p.head * cache.code_stride_h + 4 * p.piece));
+        e[j] = scales[scale + p.head * cache.scale_stride_h + (p.piece >> 2)];
+      }
     }
+#pragma unroll
+    for (int j = 0; j < kItems; ++j)
+      if (i0 + kWThreads * j < n)
+        *reinterpret_cast<T8*>(out + 8ll * (i0 + kWThreads * j)) = codes8<T>(w[j], scale_of(e[j]));
   }
-  *reinterpret_cast<T8*>(out + 8 * i) = w;
+}
+
+// Tokens per work-group of the two: fewer where they would not give every CU work.
+int tokens_per_group(int64_t tokens) {
+  int t = kWTokens;
+  while (t > 1 && tokens < 512 * static_cast<int64_t>(t)) t /= 2;
+  return t;
 }
 
 // ---- decode ----
@@ -688,16 +743,15 @@ extern "C" int fa_mxfp4_cache_write(const fa_mxfp4_cache* cache, const void* key
                "key / value rows must be 16-byte aligned");
   FA_CHECK_ARG(static_cast<int64_t>(num_tokens) * cache->h_kv <= INT32_MAX,
                "num_tokens %d x h_kv %d is 2^31 or more", num_tokens, cache->h_kv);
-  const int64_t items = static_cast<int64_t>(num_tokens) * cache->h_kv * (cache->d / 8);
-  const dim3 grid(static_cast<unsigned>((items + fa::kWThreads * fa::kWItems - 1) /
-                                        (fa::kWThreads * fa::kWItems)), 2);
+  const int tokens = fa::tokens_per_group(num_tokens);
+  const dim3 grid(static_cast<unsigned>(fa::cdiv(num_tokens, tokens)), 2);
   const hipStream_t s = static_cast<hipStream_t>(stream);
 #define FA_WRITE(T)                                                                            \
   hipLaunchKernelGGL(fa::mxfp4_write_kernel<T>, grid, dim3(fa::kWThreads), 0, s, *cache,        \
                      static_cast<const T*>(key), static_cast<long long>(key_stride_t),          \
                      static_cast<long long>(key_stride_h), static_cast<const T*>(value),        \
                      static_cast<long long>(value_stride_t),                                    \
-                     static_cast<long long>(value_stride_h), slots, slots64, num_tokens)
+                     static_cast<long long>(value_stride_h), slots, slots64, num_tokens, tokens)
   if (dtype == 1)
     FA_WRITE(__bf16);
   else
@@ -721,18 +775,18 @@ extern "C" int fa_mxfp4_gather(const fa_mxfp4_cache* cache, const int32_t* block
   FA_CHECK_ARG(fa::aligned(k_out, 16) && fa::aligned(v_out, 16), "outputs must be 16-byte aligned");
   FA_CHECK_ARG(static_cast<int64_t>(total) * cache->h_kv <= INT32_MAX,
                "total %d x h_kv %d is 2^31 or more", total, cache->h_kv);
-  const int64_t items = static_cast<int64_t>(total) * cache->h_kv * (cache->d / 8);
-  const dim3 grid(static_cast<unsigned>((items + fa::kWThreads - 1) / fa::kWThreads), 2);
+  const int tokens = fa::tokens_per_group(total);
+  const dim3 grid(static_cast<unsigned>(fa::cdiv(total, tokens)), 2);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == 1)
     hipLaunchKernelGGL(fa::mxfp4_gather_kernel<__bf16>, grid, dim3(fa::kWThreads), 0, s, *cache,
                        block_table, static_cast<long long>(bt_stride_b), max_blocks_per_seq,
-                       cu_seqlens, num_seqs, total, static_cast<__bf16*>(k_out),
+                       cu_seqlens, num_seqs, total, tokens, static_cast<__bf16*>(k_out),
                        static_cast<__bf16*>(v_out));
   else
     hipLaunchKernelGGL(fa::mxfp4_gather_kernel<_Float16>, grid, dim3(fa::kWThreads), 0, s, *cache,
                        block_table, static_cast<long long>(bt_stride_b), max_blocks_per_seq,
-                       cu_seqlens, num_seqs, total, static_cast<_Float16*>(k_out),
+                       cu_seqlens, num_seqs, total, tokens, static_cast<_Float16*>(k_out),
                        static_cast<_Float16*>(v_out));
   FA_CHECK_HIP(hipGetLastError());
   return FA_OK;
