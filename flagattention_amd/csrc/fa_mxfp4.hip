@@ -296,7 +296,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 4 : D == 128 ? 3 : 2) void m
   typedef typename ScaleOf<D>::type ScaleBytes;
   __shared__ __attribute__((aligned(16))) unsigned char vbuf[kWaves * kTileB];
   __shared__ float ml[2 * kWaves * kDRows];
-  static_assert(kTileB >= kDRows * D * 4, "merge area must fit in the tile buffers");
+  constexpr int kMergeRow = D + 4;  // floats: 16 rows of a write lie in different banks
+  static_assert(kTileB >= kDRows * kMergeRow * 4, "merge area must fit in the tile buffers");
   // Two tiles of loads in registers at head dim 256 would leave a SIMD one wave.
   constexpr bool kTwoTiles = D <= 128;
 
@@ -314,37 +315,19 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 4 : D == 128 ? 3 : 2) void m
   const int G = lane >> 4, c16 = lane & 15;
   const float ninf = -__builtin_inff();
 
-  const int seqlen = sload(a.seqlens + b);
   const int t0 = split * a.split_tokens;
-  const int t1 = split + 1 == a.num_splits ? seqlen : min(t0 + a.split_tokens, seqlen);
-  const int ntok = max(0, t1 - t0);
-  const int ntiles = cdiv(ntok, kDTile);
   const int rows = min(group - rb * kDRows, kDRows);
   const int h0 = hk * group + rb * kDRows;  // query head of row 0
-  if (ntiles == 0 && a.num_splits > 1) {    // the merge does not look at an empty split's rows
-    if (threadIdx.x < rows)
-      a.lse_part[(static_cast<long long>(b) * a.h_q + h0 + threadIdx.x) * a.num_splits + split] =
-          ninf;
-    return;
-  }
-
   // The scale is applied inside the exponent, after the maximum, so it has to be positive: a
   // negative one turns Q's signs instead, and zero makes Q zero.
   const float mag = fabsf(a.scale) * kLog2e * (kHalved ? 2.f : 1.f);
   const float scale_log2 = a.scale == 0.f ? 1.f : mag;
-  T8 qf[kWords];
+  uintx4 q_raw[kWords];
   {
-    const bool row_ok = c16 < rows && a.scale != 0.f;
-    const unsigned int sign = a.scale < 0.f ? 0x80008000u : 0u;
     const T* const qrow = static_cast<const T*>(a.q) + b * a.q_stride_b +
                           (h0 + (c16 < rows ? c16 : 0)) * a.q_stride_h + (D / 4) * G;
 #pragma unroll
-    for (int kk = 0; kk < kWords; ++kk) {
-      uintx4 w = *reinterpret_cast<const uintx4*>(qrow + 8 * kk);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = row_ok ? w[i] ^ sign : 0u;
-      qf[kk] = __builtin_bit_cast(T8, w);
-    }
+    for (int kk = 0; kk < kWords; ++kk) q_raw[kk] = *reinterpret_cast<const uintx4*>(qrow + 8 * kk);
   }
 
   // ---- loads of a tile ----
@@ -375,11 +358,30 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 4 : D == 128 ? 3 : 2) void m
   }
   unsigned int at_c[2], at_s[2];  // this lane's block: offsets of its codes and scales
   int at_keys = 0;                // and how many keys it has
-  auto work_out = [&](int i0) {   // blocks of the wave's tiles i0, i0 + 1, ...
-    const int u = wave + kWaves * (i0 + lane / kBlocks);
-    const int start = t0 + kDTile * u + kBlockKeys * (lane % kBlocks);
-    const int blk = start >> __builtin_ctz(static_cast<unsigned int>(cache.block_size));
-    const int id = start < t1 && blk < a.max_blocks_per_seq ? bt_row[blk] : -1;
+  const int bs_shift = __builtin_ctz(static_cast<unsigned int>(cache.block_size));
+  auto start_of = [&](int i0) -> int {  // this lane's block among those of the wave's tiles i0, ...
+    return t0 + kDTile * (wave + kWaves * (i0 + lane / kBlocks)) + kBlockKeys * (lane % kBlocks);
+  };
+  auto block_id = [&](int i0) -> int {
+    const int blk = start_of(i0) >> bs_shift;
+    return blk < a.max_blocks_per_seq ? bt_row[blk] : -1;
+  };
+  // The length, the first block ids and Q are requested together; only the tiles wait for them.
+  int next_id = block_id(0);
+  const int seqlen = min(sload(a.seqlens + b), 1 << 30);  // positions stay in 32 bits
+  const int t1 = split + 1 == a.num_splits ? seqlen : min(t0 + a.split_tokens, seqlen);
+  const int ntok = max(0, t1 - t0);
+  const int ntiles = cdiv(ntok, kDTile);
+  if (ntiles == 0 && a.num_splits > 1) {    // the merge does not look at an empty split's rows
+    if (threadIdx.x < rows)
+      a.lse_part[(static_cast<long long>(b) * a.h_q + h0 + threadIdx.x) * a.num_splits + split] =
+          ninf;
+    return;
+  }
+
+  auto work_out = [&](int i0, int block) {
+    const int start = start_of(i0);
+    const int id = start < t1 ? block : -1;
     const bool in = id >= 0 && id < cache.num_blocks;
     // a block outside the cache: the first one instead, all masked
     const long long page = in ? id : 0;
@@ -431,6 +433,19 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 4 : D == 128 ? 3 : 2) void m
     return scale_of(e);
   };
 
+  // Q^T operand: row c16, dims (D / 4) G + 8 kk ..; rows past the last are zeros
+  T8 qf[kWords];
+  auto take_q = [&] {
+    const bool row_ok = c16 < rows && a.scale != 0.f;
+    const unsigned int sign = a.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int kk = 0; kk < kWords; ++kk) {
+      uintx4 w = q_raw[kk];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = row_ok ? w[i] ^ sign : 0u;
+      qf[kk] = __builtin_bit_cast(T8, w);
+    }
+  };
   float m_run = ninf, l_run = 0.f;
   floatx4 acc[kDimTiles];
 #pragma unroll
@@ -534,8 +549,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 4 : D == 128 ? 3 : 2) void m
   for (int i0 = 0; i0 < mine; i0 += kBatch) {
     const int n = min(mine - i0, kBatch);
     Tile x;
-    work_out(i0);
+    work_out(i0, next_id);
     issue(x, 0);
+    if (i0 + kBatch < mine) next_id = block_id(i0 + kBatch);
+    if (i0 == 0) take_q();
     int i = 0;
     if constexpr (!kTwoTiles) {
       for (; i + 1 < n; ++i) step(x, i, true);
@@ -566,14 +583,16 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 4 : D == 128 ? 3 : 2) void m
   // ---- merge the waves' states ----
   const float l_col = sum_xor32(sum_xor16(l_run));
   __syncthreads();
-  float* const om = reinterpret_cast<float*>(vbuf);  // [wave][16][D]
+  float* const om = reinterpret_cast<float*>(vbuf);  // [wave][16][kMergeRow]
   if (G == 0) {
     ml[wave * kDRows + c16] = m_run;
     ml[(kWaves + wave) * kDRows + c16] = l_col;
   }
+  if (c16 < rows) {
 #pragma unroll
-  for (int dt = 0; dt < kDimTiles; ++dt)
-    *reinterpret_cast<floatx4*>(om + (wave * kDRows + c16) * D + 16 * dt + 4 * G) = acc[dt];
+    for (int dt = 0; dt < kDimTiles; ++dt)
+      *reinterpret_cast<floatx4*>(om + (wave * kDRows + c16) * kMergeRow + 16 * dt + 4 * G) = acc[dt];
+  }
   __syncthreads();
   for (int idx = threadIdx.x; idx < rows * (D / 4); idx += 64 * kWaves) {
     const int r = idx / (D / 4), d = 4 * (idx - r * (D / 4));
@@ -591,7 +610,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 4 : D == 128 ? 3 : 2) void m
     for (int w = 0; w < kWaves; ++w) {
       const float f = __builtin_amdgcn_exp2f(mw[w] - m_use);
       L += ml[(kWaves + w) * kDRows + r] * f;
-      const floatx4 o = *reinterpret_cast<const floatx4*>(om + (w * kDRows + r) * D + d);
+      const floatx4 o = *reinterpret_cast<const floatx4*>(om + (w * kDRows + r) * kMergeRow + d);
 #pragma unroll
       for (int i = 0; i < 4; ++i) O[i] += o[i] * f;
     }
@@ -705,7 +724,7 @@ int check_decode(const fa_mxfp4_decode_args* a) {
   FA_CHECK_ARG(a->dtype == 0 || a->dtype == 1, "dtype %d is not 0 (fp16) or 1 (bf16)", a->dtype);
   FA_CHECK_ARG(a->num_splits >= 1 && a->num_splits <= 65535 && a->split_tokens >= 1 &&
                    (a->num_splits == 1 || a->split_tokens % kDTile == 0) &&
-                   static_cast<int64_t>(a->num_splits - 1) * a->split_tokens <= INT32_MAX,
+                   static_cast<int64_t>(a->num_splits - 1) * a->split_tokens <= (1 << 30),
                "num_splits %d of %d tokens invalid", a->num_splits, a->split_tokens);
   FA_CHECK_ARG(a->num_splits == 1 || (a->o_part && a->lse_part),
                "num_splits %d > 1 needs o_part and lse_part", a->num_splits);
