@@ -402,29 +402,41 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 4 : D == 128 ? 3 : 2) void m
     ScaleBytes ks[2], vs[2];
     int keys[kBlocks];  // keys of each block, from its first token on (uniform)
   };
-  auto issue = [&](Tile& x, int i) {  // i: tile of the batch
+  auto base_of = [&](unsigned int (&at)[2], int l) -> unsigned long long {
+    return (static_cast<unsigned long long>(lane_of(at[1], l)) << 32) | lane_of(at[0], l);
+  };
+  // Seen afresh, a lane offset stays 32 bits beside a scalar base: hoisted as 64 bits it costs an
+  // addition per load and twice the registers.
+  auto afresh = [](unsigned int v) -> unsigned int {
+    asm volatile("" : "+v"(v));
+    return v;
+  };
+  auto issue_k = [&](Tile& x, int i) {  // i: tile of the batch
 #pragma unroll
-    for (int j = 0; j < kBlocks; ++j) {
-      const int l = kBlocks * i + j;
-      const unsigned long long c =
-          (static_cast<unsigned long long>(lane_of(at_c[1], l)) << 32) | lane_of(at_c[0], l);
-      const unsigned long long sc =
-          (static_cast<unsigned long long>(lane_of(at_s[1], l)) << 32) | lane_of(at_s[0], l);
-      x.keys[j] = __builtin_amdgcn_readlane(at_keys, l);
-      const FA_GLOBAL unsigned char *const kcp = kc + c, *const vcp = vc + c;
-      const FA_GLOBAL unsigned char *const ksp = ks + sc, *const vsp = vs + sc;
-#pragma unroll
-      for (int h = j; h < 2; h += kBlocks) {
-        // Seen afresh, a lane offset stays 32 bits beside a scalar base: hoisted as 64 bits it
-        // costs an addition per load and twice the registers.
-        unsigned int co = code_lane[h], so = scale_lane[h];
-        asm volatile("" : "+v"(co), "+v"(so));
-        x.k[h] = __builtin_nontemporal_load((const FA_GLOBAL Words*)(kcp + co));
-        x.v[h] = __builtin_nontemporal_load((const FA_GLOBAL Words*)(vcp + co));
-        x.ks[h] = *(const FA_GLOBAL ScaleBytes*)(ksp + so);
-        x.vs[h] = *(const FA_GLOBAL ScaleBytes*)(vsp + so);
-      }
+    for (int h = 0; h < 2; ++h) {
+      const int l = kBlocks * i + (kSmallBlocks ? h : 0);
+      const FA_GLOBAL unsigned char *const c = kc + base_of(at_c, l), *const sc = ks + base_of(at_s, l);
+      x.k[h] = __builtin_nontemporal_load((const FA_GLOBAL Words*)(c + afresh(code_lane[h])));
+      x.ks[h] = *(const FA_GLOBAL ScaleBytes*)(sc + afresh(scale_lane[h]));
     }
+  };
+  auto issue_v = [&](Tile& x, int i) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int l = kBlocks * i + (kSmallBlocks ? h : 0);
+      const FA_GLOBAL unsigned char *const c = vc + base_of(at_c, l), *const sc = vs + base_of(at_s, l);
+      x.v[h] = __builtin_nontemporal_load((const FA_GLOBAL Words*)(c + afresh(code_lane[h])));
+      x.vs[h] = *(const FA_GLOBAL ScaleBytes*)(sc + afresh(scale_lane[h]));
+    }
+  };
+  auto keys_of = [&](Tile& x, int i) {
+#pragma unroll
+    for (int j = 0; j < kBlocks; ++j) x.keys[j] = __builtin_amdgcn_readlane(at_keys, kBlocks * i + j);
+  };
+  auto issue = [&](Tile& x, int i) {
+    keys_of(x, i);
+    issue_k(x, i);
+    issue_v(x, i);
   };
   // the scale of word kk of a lane, from its scale bytes
   auto word_scale = [&](ScaleBytes bytes, int kk) -> float {
@@ -468,6 +480,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 4 : D == 128 ? 3 : 2) void m
         s[h] = mfma_16x16x32(codes8<T>(x.k[h][kk], word_scale(x.ks[h], kk)), qf[kk], s[h]);
       __builtin_amdgcn_sched_barrier(0);
     }
+    constexpr int kAhead = kTwoTiles ? 2 : 1;
+    if constexpr (!kTwoTiles) {
+      if (more) issue_k(x, i + kAhead);
+    }
     ScaleBytes vse[2] = {x.vs[0], x.vs[1]};
     if (!whole) {
       // a masked key's weight is 0, which does not hide a NaN: its scales become the smallest
@@ -482,7 +498,14 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 4 : D == 128 ? 3 : 2) void m
             codes8<T>(x.v[h][kk], word_scale(vse[h], kk));
       __builtin_amdgcn_sched_barrier(0);
     }
-    if (more) issue(x, i + (kTwoTiles ? 2 : 1));
+    if constexpr (kTwoTiles) {
+      if (more) issue(x, i + kAhead);
+    } else {
+      if (more) {
+        keys_of(x, i + kAhead);
+        issue_v(x, i + kAhead);
+      }
+    }
     __builtin_amdgcn_sched_barrier(0);
     // softmax down the column: keys 16h + 4G + i of the tile
     if (!whole) {
@@ -659,23 +682,26 @@ int launch_decode(const fa_mxfp4_decode_args* a, hipStream_t stream) {
 }
 
 // Splits of `groups` (sequence, KV head, block of heads) triples of up to max_len keys: the cheapest
-// by a model of the launch.  A work-group takes a step of 128 keys in kStep us by itself; k of them
-// on a CU share its memory bandwidth, from two on, and the sequences of a batch are taken to be
-// half as long as the longest on average; a further work-group on a CU costs 1.4 us, the merge
-// 3.5 us and a little per split.  Measured at 32 heads of 8 KV heads, D = 128: one step 0.72 us
-// with one work-group per CU, 1.48 with two, 2.96 with four; 1,024 work-groups of one key 9.0 us a
-// call, 256 of them 4.7.
+// by a model of the launch, in us.  By itself a work-group takes `step` for 128 keys; together they
+// take the time of their bytes, contexts being three quarters of the longest on average, and then
+// half of the last one's steps (a quarter where a CU has two or more unsplit ones, which fill each
+// other's ends); past the first on a CU a work-group costs 1.0 for its start and end, the merge 3.5
+// and a little per split.  Measured (32 heads of 8 KV heads, D = 128): a step 0.68
+// us with one work-group per CU, 1.48 with two; 1,024 work-groups of one key 7.0 a call, 256 of
+// them 3.9.  A call in 1 / 2 / 4 / 8 splits: 64 ragged contexts of up to 8,192 keys 78.5 / 67.2 /
+// 68.1 / 74.9 (64 x 8,192 101 / 107 / 107 / 116), 16 of up to 4,096 27.0 / 19.2 / 16.4 / 15.2.
 int choose_splits(int64_t groups, int d, int64_t max_len, int64_t cus) {
-  const double step = d == 64 ? 0.5 : d == 128 ? 0.72 : 1.26;
-  const double shared = 0.74 * d / 128;
+  const double step = d == 64 ? 0.49 : d == 128 ? 0.68 : 1.2;
+  const double per_cu = static_cast<double>(groups) / static_cast<double>(cus);
+  const double bytes = 0.74 * d / 128 * per_cu * static_cast<double>(max_len) / 128 * 0.75;
   double best = 0;
   int pick = 1;
   for (int s : {1, 2, 3, 4, 5, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128}) {
     if (s > 1 && max_len < 128 * static_cast<int64_t>(s)) break;
-    const double k = static_cast<double>(groups * s) / static_cast<double>(cus);
-    const double steps = static_cast<double>((max_len + 128 * s - 1) / (128 * s));
-    const double t = (k * shared / 2 > step ? k * shared / 2 : step) * steps +
-                     1.4 * (k > 1 ? k - 1 : 0) + (s > 1 ? 3.5 + 0.03 * s : 0);
+    const double alone = step * static_cast<double>((max_len + 128 * s - 1) / (128 * s));
+    const double k = per_cu * s, shared = bytes + alone * (per_cu < 2 ? 0.5 : 0.25);
+    const double t = (alone > shared ? alone : shared) + (k > 1 ? k - 1 : 0) +
+                     (s > 1 ? 3.5 + 0.03 * s : 0);
     if (s == 1 || t < best) {
       best = t;
       pick = s;
