@@ -105,10 +105,12 @@ __device__ inline Item find_in_order(const fa_varlen_args& a, int group, int ite
 // The same with the items ordered by the keys that they walk, the longest first, so that a launch
 // of several work-groups per CU ends with short ones (up to 62 sequences, a lane each).  In units
 // of about a row block's positions, block j of a causal sequence costs low + j, low from its
-// prefix, and a block of a full one low; how many blocks cost c or more is a sum over the
-// sequences, so the item's cost is found by bisection, and its sequence by a scan of those that
-// have a block of that cost.  This takes 1 us longer than going in order.
-__device__ inline Item find_by_cost(const fa_varlen_args& a, int group, int item) {
+// prefix, and a block of a full one low.  How many blocks cost c or more is a sum over the
+// sequences; 64 values of c are summed at once, a lane each (the sequences come from LDS, `table`:
+// 512 bytes of the wave's own), and the item is among the blocks of the largest with more than `item`.
+// By bisection, a sum over the lanes per value, it took 4,900 cycles at 16 sequences, so 3,900 (2,200
+// in order).
+__device__ inline Item find_by_cost(const fa_varlen_args& a, int group, int item, int* table) {
   const int lane = threadIdx.x & 63;
   const Seq x = seq_of(a, lane);
   const int shift = 31 - __builtin_clz(max(kLRows / group, 1));  // a power of two of positions
@@ -119,31 +121,35 @@ __device__ inline Item find_by_cost(const fa_varlen_args& a, int group, int item
   auto costing = [&](int c) -> int {           // this lane's blocks that cost c or more
     return rises ? min(max(end - c, 0), blocks) : low >= c ? blocks : 0;
   };
-  auto total = [&](int c) -> int {
-    return __builtin_amdgcn_readlane(wave_incl_scan(costing(c)), 63);
-  };
-  if (item >= total(0)) return Item{0, 0, 0, 0, -1};
-  int lo = 0;  // total(lo) > item >= total(hi)
-  int hi = __builtin_amdgcn_readlane(wave_incl_max(blocks > 0 ? end : 0), 63);
-  int above = 0;  // total(hi)
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    const int n = total(mid);
-    if (n > item) {
-      lo = mid;
+  table[2 * lane] = end;
+  table[2 * lane + 1] = lane < a.num_seqs ? blocks : 0;
+  const int all = __builtin_amdgcn_readlane(wave_incl_scan(blocks), 63);
+  const int top = __builtin_amdgcn_readlane(wave_incl_max(blocks > 0 ? end : 0), 63);
+  if (item >= all) return Item{0, 0, 0, 0, -1};
+  // costs in at most 64 steps: a step's blocks go in any order
+  const int stride = cdiv(top, 64);
+  const int c = (lane + 1) * stride;
+  int sum = 0;
+  for (int s = 0; s < a.num_seqs; s += 4) {  // lanes past the last sequence hold no block
+    const int4 p = *reinterpret_cast<const int4*>(table + 2 * s);
+    const int4 q = *reinterpret_cast<const int4*>(table + 2 * s + 4);
+    if (a.causal) {
+      sum += min(max(p.x - c, 0), p.y) + min(max(p.z - c, 0), p.w);
+      sum += min(max(q.x - c, 0), q.y) + min(max(q.z - c, 0), q.w);
     } else {
-      hi = mid;
-      above = n;
+      sum += (p.x > c ? p.y : 0) + (p.z > c ? p.w : 0) + (q.x > c ? q.y : 0) + (q.z > c ? q.w : 0);
     }
   }
-  const int rank = item - above;  // among the blocks that cost lo
-  const int here = costing(lo) - costing(hi);
+  const int k = __builtin_popcountll(__ballot(sum > item));  // sums fall with c
+  const int lo = k * stride;                                 // the item costs lo .. lo + stride - 1
+  const int rank = item - (k < 64 ? __builtin_amdgcn_readlane(sum, k) : 0);
+  const int here = costing(lo) - costing(lo + stride);
   const int upto = wave_incl_scan(here);
   const int l = __builtin_ctzll(__ballot(upto > rank));
   const int before = __builtin_amdgcn_readlane(upto - here, l);
   const int from = __builtin_amdgcn_readlane(low, l);
   const bool up = __builtin_amdgcn_readlane(static_cast<int>(rises), l) != 0;
-  return item_of(x, l, group, up ? lo - from : rank - before);
+  return item_of(x, l, group, (up ? max(lo - from, 0) : 0) + rank - before);
 }
 
 template <typename T, int D>
@@ -169,8 +175,10 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
   const int group = a.h_q / a.h_kv;
   const int hk = blockIdx.x % a.h_kv;
   const int item = blockIdx.x / a.h_kv;
-  const Item it = by_cost ? find_by_cost(a, group, item) : find_in_order(a, group, item);
+  const Item it = by_cost ? find_by_cost(a, group, item, reinterpret_cast<int*>(bufs + 512 * wave_id()))
+                          : find_in_order(a, group, item);
   if (it.block < 0) return;  // uniform
+  barrier();  // the tables are read: the buffers are free
   const int split = blockIdx.y;
   const int m = it.rows / group;
 
@@ -232,17 +240,18 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
   const int left = min(it.rows - row0, kLRows);  // the work-group's rows
   const int pos0 = row0 / group, rem0 = row0 - pos0 * group;
   const float group_inv = __builtin_amdgcn_rcpf(static_cast<float>(group));
-  auto pos_of = [&](int r) -> int {
+  auto pos_of = [&](int r) -> int {  // counted from pos0
     const int x = rem0 + r;
     int q = static_cast<int>(static_cast<float>(x) * group_inv);
     q += x - q * group >= group ? 1 : 0;
     q -= x - q * group < 0 ? 1 : 0;
-    return pos0 + q;
+    return q;
   };
-  auto head_of = [&](int r, int pos) -> int { return rem0 + r - (pos - pos0) * group; };
+  auto head_of = [&](int r, int pos) -> int { return rem0 + r - pos * group; };
   // keys visible to a position: [0, n - m + 1 + position) causal, all otherwise
-  auto limit_of = [&](int pos) -> int { return a.causal ? min(it.n - m + 1 + pos, t1) : t1; };
-  const int wg_min = limit_of(pos0);
+  const int first_lim = it.n - m + 1 + pos0;
+  auto limit_of = [&](int pos) -> int { return a.causal ? min(first_lim + pos, t1) : t1; };
+  const int wg_min = limit_of(0);
   const int wg_lim = limit_of(pos_of(left - 1));
   const int ntiles = wg_lim > t0 ? cdiv(wg_lim - t0, kTok) : 0;
   const int wrow0 = kLWaveRows * wave;
@@ -256,10 +265,14 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
   // Q^T operand: row c32, dims 16kk + 8g..+7
   T8 qf[kKSteps];
   {
-    const T* const qrow = static_cast<const T*>(a.q) + (it.q0 + mm) * a.q_stride_t +
-                          (hk * group + jj) * a.q_stride_h + 8 * g;
+    // a uniform base and 32-bit row offsets (host check), as for the output below
+    const T* const qbase = static_cast<const T*>(a.q) + (it.q0 + pos0) * a.q_stride_t +
+                           hk * group * a.q_stride_h;
+    const unsigned int off = mm * static_cast<unsigned int>(a.q_stride_t) +
+                             jj * static_cast<unsigned int>(a.q_stride_h) + 8 * g;
 #pragma unroll
-    for (int kk = 0; kk < kKSteps; ++kk) qf[kk] = *reinterpret_cast<const T8*>(qrow + 16 * kk);
+    for (int kk = 0; kk < kKSteps; ++kk)
+      qf[kk] = *reinterpret_cast<const T8*>(qbase + off + 16 * kk);
   }
 
   floatx16 acc[kDimTiles];
@@ -437,7 +450,7 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
   const float inv = some ? 1.f / l : 0.f;
   const float lse = some ? (mref + log2f(l)) * kLn2 : ninf;
   const int h = hk * group + jj;
-  const long long orow = static_cast<long long>(h) * a.total_q + it.q0 + mm;
+  const long long orow = static_cast<long long>(h) * a.total_q + it.q0 + pos0 + mm;
   const bool mine = wrow0 + c32 < left;
   if (a.num_splits > 1) {
     if (mine) {
@@ -459,6 +472,8 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
   }
   if (mine && g == 0 && a.lse) a.lse[orow] = lse;
   // whole output rows through LDS (the wave's own 32 rows): 16 bytes per lane and store
+  T* const obase = static_cast<T*>(a.out) + (it.q0 + pos0) * a.o_stride_t +
+                   hk * group * a.o_stride_h;
   unsigned char* const st = bufs + wave * kLWaveRows * kRowB;
 #pragma unroll
   for (int dt = 0; dt < kDimTiles; ++dt)
@@ -479,8 +494,9 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
     const T8 v = *reinterpret_cast<const T8*>(st + r * kRowB + 16 * (cslot ^ (r & 7)));
     if (rr < left) {
       const int m2 = pos_of(rr), j2 = head_of(rr, m2);
-      *reinterpret_cast<T8*>(static_cast<T*>(a.out) + (it.q0 + m2) * a.o_stride_t +
-                             (hk * group + j2) * a.o_stride_h + 8 * cslot) = v;
+      const unsigned int off = m2 * static_cast<unsigned int>(a.o_stride_t) +
+                               j2 * static_cast<unsigned int>(a.o_stride_h) + 8 * cslot;
+      *reinterpret_cast<T8*>(obase + off) = v;
     }
   }
 }
@@ -530,6 +546,12 @@ int check_varlen(const fa_varlen_args* a) {
   FA_CHECK_ARG(a->k_stride_t >= 0 && a->v_stride_t >= 0 && a->k_stride_t < (1ll << 23) &&
                    a->v_stride_t < (1ll << 23),
                "k / v token strides must be in [0, 2^23)");
+  // and inside a row block
+  const long long group = a->h_q / a->h_kv;
+  FA_CHECK_ARG(a->q_stride_t >= 0 && a->o_stride_t >= 0 && a->q_stride_t < (1ll << 23) &&
+                   a->o_stride_t < (1ll << 23) && a->q_stride_h >= 0 && a->o_stride_h >= 0 &&
+                   group * a->q_stride_h < (1ll << 29) && group * a->o_stride_h < (1ll << 29),
+               "q / out token strides must be in [0, 2^23), a group's heads within 2^29 elements");
   FA_CHECK_ARG(static_cast<long long>(a->total_q) * (a->h_q / a->h_kv) < (1ll << 30) &&
                    row_blocks(a) * a->h_kv < (1ll << 30),
                "too many query rows or row blocks");

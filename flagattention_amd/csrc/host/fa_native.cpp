@@ -679,7 +679,9 @@ PyObject* varlen(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     return none();
   constexpr int64_t kMaxStride = int64_t{1} << 23;
   if (q->stride(2) != 1 || k->stride(2) != 1 || v->stride(2) != 1 || !rows16(*q, 2) ||
-      !rows16(*k, 2) || !rows16(*v, 2) || k->stride(0) >= kMaxStride || v->stride(0) >= kMaxStride)
+      !rows16(*k, 2) || !rows16(*v, 2) || k->stride(0) >= kMaxStride || v->stride(0) >= kMaxStride ||
+      q->stride(0) >= kMaxStride || h_q * d >= kMaxStride ||
+      h_q / h_kv * q->stride(1) >= (int64_t{1} << 29))
     return none();
   if (cq->scalar_type() != at::kInt || cq->dim() != 1 || cq->size(0) < 1 || !cq->is_contiguous() ||
       ck->scalar_type() != at::kInt || !ck->sizes().equals(cq->sizes()) || !ck->is_contiguous())

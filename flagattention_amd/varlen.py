@@ -76,6 +76,7 @@ def flash_attention_varlen(
     _require(d in HEAD_DIMS, f"head dim {d} not in {HEAD_DIMS}")
     _require(h_kv >= 1 and h_q >= 1 and h_q % h_kv == 0,
              "number of heads in q must be a multiple of that in k & v")
+    _require(h_q * d < 1 << 23, "too many heads")
     code = _dtype_code(q.dtype)
     _require(k.dtype == q.dtype and v.dtype == q.dtype, "q, k, v dtypes differ")
     _require(cu_seqlens_q.dtype == torch.int32 and cu_seqlens_q.dim() == 1
@@ -97,7 +98,9 @@ def flash_attention_varlen(
              "all tensors must be CUDA (HIP) tensors on one device")
     q, k, v = (t if t.stride(-1) == 1 and _aligned(t, (0, 1)) else t.contiguous()
                for t in (q, k, v))
-    k, v = (t if 0 <= t.stride(0) < 1 << 23 else t.contiguous() for t in (k, v))
+    # 32-bit offsets inside a tile of keys and inside a block of rows (and its heads)
+    q, k, v = (t if t.stride(0) < 1 << 23 and h_q // h_kv * t.stride(1) < 1 << 29 else t.contiguous()
+               for t in (q, k, v))
     device = q.device
     o = torch.empty((total_q, h_q, d), dtype=q.dtype, device=device)
     lse = (torch.empty((h_q, total_q), dtype=torch.float32, device=device)
