@@ -684,22 +684,28 @@ int launch_decode(const fa_mxfp4_decode_args* a, hipStream_t stream) {
 // Splits of `groups` (sequence, KV head, block of heads) triples of up to max_len keys: the cheapest
 // by a model of the launch, in us.  By itself a work-group takes `step` for 128 keys; together they
 // take the time of their bytes, contexts being three quarters of the longest on average, and then
-// half of the last one's steps (a quarter where a CU has two or more unsplit ones, which fill each
+// some of the last one's steps (fewer where a CU has two or more unsplit ones, which fill each
 // other's ends); past the first on a CU a work-group costs 1.0 for its start and end, the merge 3.5
-// and a little per split.  Measured (32 heads of 8 KV heads, D = 128): a step 0.68
-// us with one work-group per CU, 1.48 with two; 1,024 work-groups of one key 7.0 a call, 256 of
-// them 3.9.  A call in 1 / 2 / 4 / 8 splits: 64 ragged contexts of up to 8,192 keys 78.5 / 67.2 /
-// 68.1 / 74.9 (64 x 8,192 101 / 107 / 107 / 116), 16 of up to 4,096 27.0 / 19.2 / 16.4 / 15.2.
+// and a little per split.  CUs hold a whole number of work-groups: the count per CU is taken halfway
+// to the next whole one.  Measured: 1,024 work-groups of one key take 7.0 a call, 256 of them 3.9; a
+// call in 1 / 2 / 3 / 4 / 5 / 8 splits at D = 128, 8 KV heads: 32 ragged contexts of up to 4,096 keys
+// 26.9 / 23.8 / 22.4 / 21.4 / 19.5 / 23.4, 64 x 8,192 95.7 / 103.5 / 104.4 / 105.8 / 108.9 / 116; at
+// D = 256, 4 KV heads, 32 of up to 3,000 33.0 / 23.0 / 28.8 / 24.5 / 22.2 / 26.2.  The constants are a
+// fit to 33 such calls in up to 48 splits each (D 64 .. 256, 1 .. 1,024 triples, 800 .. 131,001 keys):
+// the pick takes 4% longer than the best count on average and 12% at most; for 12 other calls 5% and
+// 23% (40 x 2,000 keys, D = 256).
 int choose_splits(int64_t groups, int d, int64_t max_len, int64_t cus) {
-  const double step = d == 64 ? 0.49 : d == 128 ? 0.68 : 1.2;
+  const double step = d == 64 ? 0.46 : d == 128 ? 0.89 : 0.87;
   const double per_cu = static_cast<double>(groups) / static_cast<double>(cus);
-  const double bytes = 0.74 * d / 128 * per_cu * static_cast<double>(max_len) / 128 * 0.75;
+  const double bytes = 0.48 * d / 128 * per_cu * static_cast<double>(max_len) / 128 * 0.75;
   double best = 0;
   int pick = 1;
-  for (int s : {1, 2, 3, 4, 5, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128}) {
+  for (int s : {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20, 24, 32, 48, 64, 96, 128}) {
     if (s > 1 && max_len < 128 * static_cast<int64_t>(s)) break;
     const double alone = step * static_cast<double>((max_len + 128 * s - 1) / (128 * s));
-    const double k = per_cu * s, shared = bytes + alone * (per_cu < 2 ? 0.5 : 0.25);
+    const double even = per_cu * s, whole = static_cast<double>((groups * s + cus - 1) / cus);
+    const double k = even + 0.51 * (whole - even);
+    const double shared = bytes * (k > 1 ? k / even : 1) + alone * (per_cu < 2 ? 0.44 : 0.19);
     const double t = (alone > shared ? alone : shared) + (k > 1 ? k - 1 : 0) +
                      (s > 1 ? 3.5 + 0.03 * s : 0);
     if (s == 1 || t < best) {
