@@ -152,6 +152,179 @@ __device__ inline Item find_by_cost(const fa_varlen_args& a, int group, int item
   return item_of(x, l, group, (up ? max(lo - from, 0) : 0) + rank - before);
 }
 
+// One 32-row tile's softmax state and operands (lane % 32 = row, g = lane / 32).
+template <typename T, int D>
+struct RowState {
+  typedef typename PVec<T>::v8 T8;
+  T8 qf[D / 16];         // Q^T operand: dims 16kk + 8g..+7
+  floatx16 acc[D / 32];  // O^T: dim 32dt + 8(i / 4) + 4g + i % 4
+  float mref, lsum;      // reference and sum of the weights, base 2
+};
+
+// The lane's parts of the LDS reads.
+template <int D>
+struct LaneReads {
+  static constexpr int C = D / 8;
+  static constexpr int kRowB = 2 * D;
+  static constexpr int kVBases = D / 32 < 4 ? D / 32 : 4;  // fv < 8: dt + 4 is 256 bytes on
+  int k;
+  int v[kVBases];
+  __device__ inline explicit LaneReads(int lane) {
+    const int g = lane >> 5, c32 = lane & 31;
+    k = c32 * kRowB + 16 * (g ^ fk<C>(c32));  // chunk 2kk + g: xor 32 kk
+    const int h16 = lane >> 4, e = (lane & 15) >> 2, qd = lane & 3;
+    const int vtok = 4 * g + e;  // token within 8
+#pragma unroll
+    for (int dt = 0; dt < kVBases; ++dt)
+      v[dt] = vtok * kRowB + 32 * ((2 * dt + (h16 & 1)) ^ fv<C>(vtok)) + 16 * (qd >> 1) +
+              8 * (qd & 1);
+  }
+};
+
+// Weights of 32 kSub keys at kb for the 32 rows: scores, mask, running maximum, exponentials.  A
+// masked tile's first `sees` keys (from the lane's own, 4g) are seen by the lane's row.
+template <typename T, int D, int kSub>
+__device__ inline void weigh(RowState<T, D>& r, const unsigned char* kb, const LaneReads<D>& at,
+                             bool masked, int sees, bool prescale, float prescale_by,
+                             float scale_log2, typename PVec<T>::v8 (&pb)[2 * kSub]) {
+  typedef typename PVec<T>::v8 T8;
+  constexpr int kKSteps = D / 16;
+  const float ninf = -__builtin_inff();
+      // K operands one k-step ahead of their MFMAs (the fences keep them there)
+      floatx16 s[kSub];
+      T8 ka[2][kSub];
+      auto k_read = [&](int kk, int tt) -> T8 {
+        return *reinterpret_cast<const T8*>(kb + 32 * tt * 2 * D + (at.k ^ (32 * kk)));
+      };
+  #pragma unroll
+      for (int tt = 0; tt < kSub; ++tt) {
+        s[tt] = floatx16{};
+        ka[0][tt] = k_read(0, tt);
+      }
+  #pragma unroll
+      for (int kk = 0; kk < kKSteps; ++kk) {
+        if (kk + 1 < kKSteps) {
+  #pragma unroll
+          for (int tt = 0; tt < kSub; ++tt) ka[(kk + 1) & 1][tt] = k_read(kk + 1, tt);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+  #pragma unroll
+        for (int tt = 0; tt < kSub; ++tt) s[tt] = mfma_32x32x16(ka[kk & 1][tt], r.qf[kk], s[tt]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (prescale) {
+  #pragma unroll
+        for (int tt = 0; tt < kSub; ++tt)
+  #pragma unroll
+          for (int i = 0; i < 16; ++i) s[tt][i] *= prescale_by;
+      }
+          if (masked) {
+      #pragma unroll
+        for (int tt = 0; tt < kSub; ++tt)
+  #pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int j = 32 * tt + 8 * (i >> 2) + (i & 3);  // + 4g: the key of s[tt][i]
+            s[tt][i] = j < sees ? s[tt][i] : ninf;
+          }
+      }
+      float mx = s[0][0];
+  #pragma unroll
+      for (int tt = 0; tt < kSub; ++tt)
+  #pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[tt][i]);
+      mx = max_xor32(mx) * scale_log2;
+      // The reference stays while no row's maximum is more than kLag above it: P then reaches
+      // 2^kLag, which rounds no worse, and the accumulators are left alone.
+      if (__ballot(mx > r.mref + kLag || (r.mref == ninf && mx != ninf)) != 0ull) {  // uniform
+        const float m_new = fmaxf(r.mref, mx);
+        const float alpha = m_new == ninf ? 1.f : __builtin_amdgcn_exp2f(r.mref - m_new);
+        r.lsum *= alpha;
+        r.mref = m_new;
+  #pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+  #pragma unroll
+          for (int i = 0; i < 16; ++i) r.acc[dt][i] *= alpha;
+      }
+      const float nm = r.mref == ninf ? 0.f : -r.mref;
+      float c = scale_log2;
+      if (__ballot(fabsf(nm) > kFusedMax) != 0ull) {  // uniform
+  #pragma unroll
+        for (int tt = 0; tt < kSub; ++tt)
+  #pragma unroll
+          for (int i = 0; i < 16; ++i) s[tt][i] *= c;
+        c = 1.f;
+      }
+          float ps = 0.f;
+  #pragma unroll
+      for (int ss = 0; ss < 2 * kSub; ++ss)
+  #pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float p =
+              __builtin_amdgcn_exp2f(__builtin_fmaf(s[ss >> 1][8 * (ss & 1) + i], c, nm));
+          ps += p;
+          pb[ss][i] = static_cast<T>(p);
+        }
+      r.lsum += ps;
+}
+
+// acc += V^T P^T of the 32 kSub keys at vb.
+template <typename T, int D, int kSub>
+__device__ inline void add_values(RowState<T, D>& r, const unsigned char* vb,
+                                  const LaneReads<D>& at,
+                                  const typename PVec<T>::v8 (&pb)[2 * kSub]) {
+  typedef typename PVec<T>::v8 T8;
+  typedef typename PVec<T>::v4 T4;
+  constexpr int kRowB = 2 * D;
+#pragma unroll
+  for (int ss = 0; ss < 2 * kSub; ++ss)
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) {
+      const unsigned char* const p = vb + 16 * ss * kRowB + 256 * (dt >> 2) + at.v[dt & 3];
+      const T4 lo = lds_tr_read4<T>(p);
+      const T4 hi = lds_tr_read4<T>(p + 8 * kRowB);
+      const T8 va = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      r.acc[dt] = mfma_32x32x16(va, pb[ss], r.acc[dt]);
+    }
+}
+
+// Infinities and NaNs of the keys at vb go to the rows that see their key as they are.
+template <typename T, int D>
+__device__ inline void add_odd_values(RowState<T, D>& r, const unsigned char* vb, int g, int keys,
+                                      int sees) {
+  typedef typename PVec<T>::v4 T4;
+  for (int j = 0; j < keys; ++j) {
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // dims 32dt + 8i + 4g..+3: chunk 4dt + i
+        const T4 v4 = *reinterpret_cast<const T4*>(
+            vb + j * 2 * D + 16 * ((4 * dt + i) ^ (fv<D / 8>(j) << 1)) + 8 * g);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float f = static_cast<float>(v4[x]);
+          r.acc[dt][4 * i + x] += j < sees && !(fabsf(f) < __builtin_inff()) ? f : 0.f;
+        }
+      }
+  }
+}
+
+// Whether a lane's part of a copy (16 bytes) holds an infinity or a NaN: the largest bit pattern.
+template <typename T>
+__device__ inline bool is_odd(unsigned int best) {
+  constexpr unsigned int kInf = __is_same(T, __bf16) ? 0x7F80u : 0x7C00u;
+  return (best & 0xFFFFu) >= kInf || (best >> 16) >= kInf;
+}
+template <typename T>
+__device__ inline void clean16(unsigned char* at) {
+  typedef typename PVec<T>::v8 T8;
+  T8* const p = reinterpret_cast<T8*>(at);
+  T8 w = *p;
+#pragma unroll
+  for (int x = 0; x < 8; ++x)
+    w[x] = fabsf(static_cast<float>(w[x])) < __builtin_inff() ? w[x] : static_cast<T>(0.f);
+  *p = w;
+}
+
 template <typename T, int D>
 __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_args a,
                                                              const int by_cost) {
@@ -263,7 +436,7 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
   const int lim = limit_of(mm);
 
   // Q^T operand: row c32, dims 16kk + 8g..+7
-  T8 qf[kKSteps];
+  RowState<T, D> r;
   {
     // a uniform base and 32-bit row offsets (host check), as for the output below
     const T* const qbase = static_cast<const T*>(a.q) + (it.q0 + pos0) * a.q_stride_t +
@@ -272,40 +445,29 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
                              jj * static_cast<unsigned int>(a.q_stride_h) + 8 * g;
 #pragma unroll
     for (int kk = 0; kk < kKSteps; ++kk)
-      qf[kk] = *reinterpret_cast<const T8*>(qbase + off + 16 * kk);
+      r.qf[kk] = *reinterpret_cast<const T8*>(qbase + off + 16 * kk);
   }
 
-  floatx16 acc[kDimTiles];
 #pragma unroll
-  for (int dt = 0; dt < kDimTiles; ++dt) acc[dt] = floatx16{};
-  float mref = ninf, lsum = 0.f;
-
-  // lane offsets of the LDS reads
-  const int kbase = c32 * kRowB + 16 * (g ^ fk<C>(c32));  // chunk 2kk + g: xor 32 kk
-  const int h16 = lane >> 4, e = (lane & 15) >> 2, qd = lane & 3;
-  const int vtok = 4 * g + e;  // token within 8
-  constexpr int kVBases = kDimTiles < 4 ? kDimTiles : 4;  // fv < 8: dt + 4 is 256 bytes on
-  int vbase[kVBases];
-#pragma unroll
-  for (int dt = 0; dt < kVBases; ++dt)
-    vbase[dt] = vtok * kRowB + 32 * ((2 * dt + (h16 & 1)) ^ fv<C>(vtok)) + 16 * (qd >> 1) +
-                8 * (qd & 1);
+  for (int dt = 0; dt < kDimTiles; ++dt) r.acc[dt] = floatx16{};
+  r.mref = ninf;
+  r.lsum = 0.f;
+  const LaneReads<D> at(lane);
 
   for (int u = 0; u < ntiles; ++u) {
     const int buf = u & 1;
     const int start = t0 + kTok * u;
     wait_vmem<0>();  // this wave's copies of tile u (requested one step ago)
     // A weight of 0 does not hide an infinity or a NaN in V: 0 times either is NaN.  A tile that
-    // some row sees in part is looked through for them (each wave its own copies).
-    const bool part_seen = a.causal && start + kTok > wg_min;  // uniform
+    // some row sees in part (or that ends behind the last key) is looked through for them (each wave its own copies).
+    const bool part_seen = start + kTok > wg_min;  // uniform
     if (part_seen) {
       unsigned int best = 0u;
 #pragma unroll
       for (int i = 0; i < kCopies; ++i)
         fold_bits(best, *reinterpret_cast<const uintx4*>(bufs + (2 + buf) * kTileB +
                                                          (kCopies * wave + i) * 1024 + 16 * lane));
-      constexpr unsigned int kInf = __is_same(T, __bf16) ? 0x7F80u : 0x7C00u;
-      const bool any = __ballot((best & 0xFFFFu) >= kInf || (best >> 16) >= kInf) != 0ull;
+      const bool any = __ballot(is_odd<T>(best)) != 0ull;
       if (lane == 0) odd_v[buf][wave] = any;
     }
     barrier();  // everyone's copies; and everyone is done with tile u-1
@@ -315,15 +477,8 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
     auto clean_tile = [&] {
       barrier();
 #pragma unroll
-      for (int i = 0; i < kCopies; ++i) {
-        T8* const p = reinterpret_cast<T8*>(bufs + (2 + buf) * kTileB +
-                                            (kCopies * wave + i) * 1024 + 16 * lane);
-        T8 w = *p;
-#pragma unroll
-        for (int x = 0; x < 8; ++x)
-          w[x] = fabsf(static_cast<float>(w[x])) < __builtin_inff() ? w[x] : static_cast<T>(0.f);
-        *p = w;
-      }
+      for (int i = 0; i < kCopies; ++i)
+        clean16<T>(bufs + (2 + buf) * kTileB + (kCopies * wave + i) * 1024 + 16 * lane);
       barrier();
     };
     if (!wave_on || start >= wave_max) {  // uniform: no row of the wave sees a key here
@@ -333,122 +488,24 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
     const unsigned char* const kb = bufs + buf * kTileB;
     const unsigned char* const vb = bufs + (2 + buf) * kTileB;
 
-    // K operands one k-step ahead of their MFMAs (the fences keep them there)
-    floatx16 s[kSub];
-    T8 ka[2][kSub];
-    auto k_read = [&](int kk, int tt) -> T8 {
-      return *reinterpret_cast<const T8*>(kb + 32 * tt * kRowB + (kbase ^ (32 * kk)));
-    };
-#pragma unroll
-    for (int tt = 0; tt < kSub; ++tt) {
-      s[tt] = floatx16{};
-      ka[0][tt] = k_read(0, tt);
-    }
-#pragma unroll
-    for (int kk = 0; kk < kKSteps; ++kk) {
-      if (kk + 1 < kKSteps) {
-#pragma unroll
-        for (int tt = 0; tt < kSub; ++tt) ka[(kk + 1) & 1][tt] = k_read(kk + 1, tt);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int tt = 0; tt < kSub; ++tt) s[tt] = mfma_32x32x16(ka[kk & 1][tt], qf[kk], s[tt]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    if (prescale) {
-#pragma unroll
-      for (int tt = 0; tt < kSub; ++tt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[tt][i] *= a.scale * kLog2e;
-    }
-    const bool masked = start + kTok > wave_min;  // uniform: some row does not see the whole tile
-    if (masked) {
-      const int sees = lim - start - 4 * g;
-#pragma unroll
-      for (int tt = 0; tt < kSub; ++tt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int j = 32 * tt + 8 * (i >> 2) + (i & 3);  // + 4g: the key of s[tt][i]
-          s[tt][i] = j < sees ? s[tt][i] : ninf;
-        }
-    }
-    float mx = s[0][0];
-#pragma unroll
-    for (int tt = 0; tt < kSub; ++tt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[tt][i]);
-    mx = max_xor32(mx) * scale_log2;
-    // The reference stays while no row's maximum is more than kLag above it: P then reaches
-    // 2^kLag, which rounds no worse, and the accumulators are left alone.
-    if (__ballot(mx > mref + kLag || (mref == ninf && mx != ninf)) != 0ull) {  // uniform
-      const float m_new = fmaxf(mref, mx);
-      const float alpha = m_new == ninf ? 1.f : __builtin_amdgcn_exp2f(mref - m_new);
-      lsum *= alpha;
-      mref = m_new;
-#pragma unroll
-      for (int dt = 0; dt < kDimTiles; ++dt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[dt][i] *= alpha;
-    }
-    const float nm = mref == ninf ? 0.f : -mref;
-    float c = scale_log2;
-    if (__ballot(fabsf(nm) > kFusedMax) != 0ull) {  // uniform
-#pragma unroll
-      for (int tt = 0; tt < kSub; ++tt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[tt][i] *= c;
-      c = 1.f;
-    }
     T8 pb[2 * kSub];
-    float ps = 0.f;
-#pragma unroll
-    for (int ss = 0; ss < 2 * kSub; ++ss)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float p =
-            __builtin_amdgcn_exp2f(__builtin_fmaf(s[ss >> 1][8 * (ss & 1) + i], c, nm));
-        ps += p;
-        pb[ss][i] = static_cast<T>(p);
-      }
-    lsum += ps;
+    // masked: some row does not see the whole tile (uniform)
+    weigh<T, D, kSub>(r, kb, at, start + kTok > wave_min, lim - start - 4 * g, prescale,
+                      a.scale * kLog2e, scale_log2, pb);
     if (odd) {
-      // An infinity or a NaN goes to the rows that see its key as it is, and out of the tile.
-      for (int j = 0; j < kTok; ++j) {
-        const bool sees = start + j < lim;
-#pragma unroll
-        for (int dt = 0; dt < kDimTiles; ++dt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {  // dims 32dt + 8i + 4g..+3: chunk 4dt + i
-            const T4 v4 = *reinterpret_cast<const T4*>(
-                vb + j * kRowB + 16 * ((4 * dt + i) ^ (fv<C>(j) << 1)) + 8 * g);
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const float f = static_cast<float>(v4[x]);
-              acc[dt][4 * i + x] += sees && !(fabsf(f) < __builtin_inff()) ? f : 0.f;
-            }
-          }
-      }
+      add_odd_values<T, D>(r, vb, g, kTok, lim - start);
       clean_tile();
     }
-#pragma unroll
-    for (int ss = 0; ss < 2 * kSub; ++ss)
-#pragma unroll
-      for (int dt = 0; dt < kDimTiles; ++dt) {
-        const unsigned char* const p = vb + 16 * ss * kRowB + 256 * (dt >> 2) + vbase[dt & 3];
-        const T4 lo = lds_tr_read4<T>(p);
-        const T4 hi = lds_tr_read4<T>(p + 8 * kRowB);
-        const T8 va = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        acc[dt] = mfma_32x32x16(va, pb[ss], acc[dt]);
-      }
+    add_values<T, D, kSub>(r, vb, at, pb);
   }
   wait_vmem<0>();
   barrier();  // the tile buffers are free
   if (!wave_on) return;
 
-  const float l = sum_xor32(lsum);
+  const float l = sum_xor32(r.lsum);
   const bool some = !(l == 0.f);  // else no visible key: out 0, lse -inf (NaN sums stay NaN)
   const float inv = some ? 1.f / l : 0.f;
-  const float lse = some ? (mref + log2f(l)) * kLn2 : ninf;
+  const float lse = some ? (r.mref + log2f(l)) * kLn2 : ninf;
   const int h = hk * group + jj;
   const long long orow = static_cast<long long>(h) * a.total_q + it.q0 + pos0 + mm;
   const bool mine = wrow0 + c32 < left;
@@ -462,7 +519,7 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
         for (int i = 0; i < 4; ++i) {
           floatx4 w;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) w[x] = some ? acc[dt][4 * i + x] * inv : 0.f;
+          for (int x = 0; x < 4; ++x) w[x] = some ? r.acc[dt][4 * i + x] * inv : 0.f;
           *reinterpret_cast<floatx4*>(op + 32 * dt + 8 * i) = w;
         }
       // the merge takes the largest lse, which a NaN would not be
@@ -481,7 +538,7 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
     for (int i = 0; i < 4; ++i) {
       T4 w;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) w[x] = static_cast<T>(some ? acc[dt][4 * i + x] * inv : 0.f);
+      for (int x = 0; x < 4; ++x) w[x] = static_cast<T>(some ? r.acc[dt][4 * i + x] * inv : 0.f);
       *reinterpret_cast<T4*>(st + c32 * kRowB + 16 * ((4 * dt + i) ^ (c32 & 7)) + 8 * g) = w;
     }
   asm volatile("" ::: "memory");
@@ -489,9 +546,9 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
   asm volatile("" ::: "memory");
 #pragma unroll
   for (int i = 0; i < kLWaveRows * kRowB / 1024; ++i) {
-    const int r = i * kRowsPerCopy + crow;
-    const int rr = wrow0 + r;
-    const T8 v = *reinterpret_cast<const T8*>(st + r * kRowB + 16 * (cslot ^ (r & 7)));
+    const int sr = i * kRowsPerCopy + crow;
+    const int rr = wrow0 + sr;
+    const T8 v = *reinterpret_cast<const T8*>(st + sr * kRowB + 16 * (cslot ^ (sr & 7)));
     if (rr < left) {
       const int m2 = pos_of(rr), j2 = head_of(rr, m2);
       const unsigned int off = m2 * static_cast<unsigned int>(a.o_stride_t) +

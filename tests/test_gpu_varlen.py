@@ -137,6 +137,24 @@ def test_odd_values_reach_only_the_rows_that_see_them(d, dtype):
     assert torch.equal(torch.isnan(lse), torch.isnan(ref_lse))
 
 
+@pytest.mark.parametrize("d", varlen.HEAD_DIMS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_odd_values_of_the_last_key_without_a_mask(d, dtype):
+    """The rows past the end repeat the last key's: an infinity there stays one."""
+    need_gpu()
+    say(f"varlen odd last key d={d} {dtype}")
+    q, k, v, cq, ck = inputs([150, 60, 3], [150, 90, 333], 4, 2, d, dtype, seed=5)
+    v[149, 0, 3] = math.inf
+    v[149, 1, 4] = math.nan
+    v[239, 1, d - 1] = -math.inf
+    v[572, 0, 0] = math.inf
+    o, lse = call(q, k, v, cq, ck, False)
+    ref, ref_lse, a, ds = po.varlen(q, k, v, cq, ck, d ** -0.5, False)
+    assert bool(torch.isinf(ref).any())
+    assert_rows(o, ref, a, ds.t(), 333, 6.0)
+    assert torch.equal(torch.isnan(lse), torch.isnan(ref_lse))
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1e-3, 40.0])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_scales(scale, dtype):
