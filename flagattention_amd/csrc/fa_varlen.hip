@@ -25,6 +25,8 @@ constexpr int kLRows = kLWaves * kLWaveRows;
 // multiply-add does not round their product with the scale, which the reference is made of.
 constexpr float kFusedMax = 1024.f;
 constexpr float kLag = 6.f;
+// Keys past which a row block of one wave's rows has them dealt out to the waves.
+constexpr int kFewKeys = 128;
 
 // Largest |x| of packed 16-bit values as unsigned bit patterns, folded into best.
 __device__ inline void fold_bits(unsigned int& best, uintx4 w) {
@@ -116,7 +118,9 @@ __device__ inline Item find_by_cost(const fa_varlen_args& a, int group, int item
   const int shift = 31 - __builtin_clz(max(kLRows / group, 1));  // a power of two of positions
   const int blocks = cdiv(x.m * group, kLRows);
   const bool rises = a.causal && lane < a.num_seqs;
-  const int low = rises ? (max(x.n - x.m, 0) >> shift) + 1 : cdiv(x.n, 1 << shift);
+  // (a block of one wave's rows walks its keys four times as fast)
+  const int fast = x.m * group <= kLWaveRows && x.n > kFewKeys ? shift + 2 : shift;
+  const int low = rises ? (max(x.n - x.m, 0) >> fast) + 1 : cdiv(x.n, 1 << fast);
   const int end = low + (rises ? blocks : 1);  // past the highest cost
   auto costing = [&](int c) -> int {           // this lane's blocks that cost c or more
     return rises ? min(max(end - c, 0), blocks) : low >= c ? blocks : 0;
@@ -325,6 +329,89 @@ __device__ inline void clean16(unsigned char* at) {
   *p = w;
 }
 
+// Copies of 32 rows of K (or V) from position `start` on into dst; rows past t1 repeat the last one.
+template <int D, bool kValues>
+__device__ inline void copy32(const unsigned char* base, unsigned int row_b, int start, int t1,
+                              unsigned char* dst) {
+  constexpr int C = D / 8, kRowsPerCopy = 512 / D;
+  int lane = threadIdx.x & 63;
+  if (D == 256) asm volatile("" : "+v"(lane));  // offsets afresh: kept, they would be spilled
+  const int crow = lane / C, cslot = lane % C;
+  const unsigned char* const src = base + static_cast<long long>(start) * row_b;
+  const int last = t1 - 1 - start;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    const int r = i * kRowsPerCopy + crow;
+    const int from = last < 31 ? min(r, last) : r;
+    const unsigned int off = from * row_b + 16 * (cslot ^ (kValues ? fv<C>(r) << 1 : fk<C>(r)));
+    lds_dma16_off(src, off, (FA_LDS void*)(dst + 1024 * i));
+  }
+}
+
+// Nothing the compiler moves passes here.
+__device__ inline void fence() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+}
+
+// A row block of at most 32 rows (a batch's single tokens, the ends of prompts): its rows are every
+// wave's, and the keys are dealt out, 32 at a time and round-robin, each wave's through its own
+// quarter of the tile buffers without a barrier.  The next tile's K is on its way from the end of
+// this one's scores, its V from the end of its values; at head dim 256 the quarter holds one of them
+// at a time.  The wave's first copies are on their way already: K, and V where both fit.
+template <typename T, int D>
+__device__ inline void walk_few(RowState<T, D>& r, const LaneReads<D>& at, unsigned char* mine,
+                                const unsigned char* kp, unsigned int k_tb,
+                                const unsigned char* vp, unsigned int v_tb, int first, int t1,
+                                int end, int min_lim, int lim, bool prescale, float prescale_by,
+                                float scale_log2) {
+  constexpr int kCopies = D / 16;
+  constexpr bool kBoth = D <= 128;
+  const int lane = threadIdx.x & 63;
+  unsigned char* const vb = mine + (kBoth ? 64 * D : 0);
+  for (int start = first; start < end; start += 32 * kLWaves) {
+    const int next = start + 32 * kLWaves;
+    wait_vmem<kBoth ? kCopies : 0>();  // K
+    fence();
+    typename PVec<T>::v8 pb[2];
+    weigh<T, D, 1>(r, mine, at, start + 32 > min_lim, lim - start - 4 * (lane >> 5), prescale,
+                   prescale_by, scale_log2, pb);
+    fence();
+    wait_lds();  // K is read
+    if (!kBoth) copy32<D, true>(vp, v_tb, start, t1, vb);
+    if (kBoth && next < end) {
+      copy32<D, false>(kp, k_tb, next, t1, mine);
+      wait_vmem<kCopies>();  // V
+    } else {
+      wait_vmem<0>();
+    }
+    fence();
+    if (start + 32 > min_lim) {  // as in the kernel, a wave's own
+      unsigned int best = 0u;
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i)
+        fold_bits(best, *reinterpret_cast<const uintx4*>(vb + 1024 * i + 16 * lane));
+      if (__ballot(is_odd<T>(best)) != 0ull) {
+        add_odd_values<T, D>(r, vb, lane >> 5, 32, lim - start);
+        fence();
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) clean16<T>(vb + 1024 * i + 16 * lane);
+        fence();
+        wait_lds();
+      }
+    }
+    add_values<T, D, 1>(r, vb, at, pb);
+    fence();
+    wait_lds();  // V is read
+    if (next < end) {
+      if (kBoth)
+        copy32<D, true>(vp, v_tb, next, t1, vb);
+      else
+        copy32<D, false>(kp, k_tb, next, t1, mine);
+    }
+  }
+}
+
 template <typename T, int D>
 __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_args a,
                                                              const int by_cost) {
@@ -344,6 +431,7 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
   __shared__ __attribute__((aligned(16))) unsigned char bufs[4 * kTileB];
   static_assert(4 * kTileB >= kLRows * kRowB, "output staging fits the tile buffers");
   __shared__ int odd_v[2][kLWaves];  // [tile parity][wave]: see below
+  __shared__ float few_m[kLWaves][32], few_l[kLWaves][32];
 
   const int group = a.h_q / a.h_kv;
   const int hk = blockIdx.x % a.h_kv;
@@ -405,12 +493,24 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
     }
   };
 
-  if (t1 > t0) issue(0, 0);  // the first tile is on its way from here on
+  const int row0 = it.block * kLRows;
+  const int left = min(it.rows - row0, kLRows);  // the work-group's rows
+  // One wave's rows and several tiles of keys: the keys are dealt out to the waves.
+  const bool few = left <= kLWaveRows && t1 - t0 > kFewKeys;  // uniform
+  unsigned char* const quarter = bufs + wave * kTileB;
+  // the first tile is on its way from here on
+  if (few) {
+    const int first = t0 + 32 * wave;
+    if (first < t1) {
+      copy32<D, false>(kp, k_tb, first, t1, quarter);
+      if (D <= 128) copy32<D, true>(vp, v_tb, first, t1, quarter + 64 * D);
+    }
+  } else if (t1 > t0) {
+    issue(0, 0);
+  }
 
   // Position and query head of the work-group's row r, counted from its first: rows are few, so a
   // reciprocal and a correction divide them by the group.
-  const int row0 = it.block * kLRows;
-  const int left = min(it.rows - row0, kLRows);  // the work-group's rows
   const int pos0 = row0 / group, rem0 = row0 - pos0 * group;
   const float group_inv = __builtin_amdgcn_rcpf(static_cast<float>(group));
   auto pos_of = [&](int r) -> int {  // counted from pos0
@@ -427,7 +527,7 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
   const int wg_min = limit_of(0);
   const int wg_lim = limit_of(pos_of(left - 1));
   const int ntiles = wg_lim > t0 ? cdiv(wg_lim - t0, kTok) : 0;
-  const int wrow0 = kLWaveRows * wave;
+  const int wrow0 = few ? 0 : kLWaveRows * wave;
   const int wave_min = limit_of(pos_of(min(wrow0, left - 1)));
   const int wave_max = limit_of(pos_of(min(wrow0 + kLWaveRows, left) - 1));
   const bool wave_on = wrow0 < left;
@@ -453,6 +553,81 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
   r.mref = ninf;
   r.lsum = 0.f;
   const LaneReads<D> at(lane);
+
+  if (few) {  // uniform
+    walk_few<T, D>(r, at, quarter, kp, k_tb, vp, v_tb, t0 + 32 * wave, t1, wg_lim, wg_min, lim,
+                   prescale, a.scale * kLog2e, scale_log2);
+    wait_vmem<0>();  // a first tile that no row sees
+    const float l = sum_xor32(r.lsum);
+    if (g == 0) {
+      few_m[wave][c32] = r.mref;
+      few_l[wave][c32] = l;
+    }
+    barrier();
+    auto top_of = [&](int row) -> float {
+      return fmaxf(fmaxf(few_m[0][row], few_m[1][row]), fmaxf(few_m[2][row], few_m[3][row]));
+    };
+    auto part_of = [&](float ref, float top) -> float {
+      return ref == top ? 1.f : __builtin_amdgcn_exp2f(ref - top);
+    };
+    const float mul = part_of(r.mref, top_of(c32));
+    // 128 dims at a time: every wave's rows as fp32, 16-byte chunks in another order in each row
+    constexpr int kDims = D <= 128 ? D : 128, kChunks = kDims / 4;
+    static_assert(kLWaves * 32 * kDims * 4 <= 4 * kTileB, "the rows fit the tile buffers");
+    float* const rows = reinterpret_cast<float*>(bufs);
+#pragma unroll
+    for (int d0 = 0; d0 < D; d0 += kDims) {
+      if (d0 > 0) barrier();  // the ones before are read
+#pragma unroll
+      for (int dt = 0; dt < kDims / 32; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          floatx4 w;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) w[x] = r.acc[d0 / 32 + dt][4 * i + x] * mul;
+          const int chunk = (8 * dt + 2 * i + g) ^ (c32 & (kChunks - 1));
+          *reinterpret_cast<floatx4*>(rows + (32 * wave + c32) * kDims + 4 * chunk) = w;
+        }
+      barrier();
+#pragma unroll
+      for (int j = 0; j < 32 * kChunks / kLThreads; ++j) {
+        const int at_row = (threadIdx.x + kLThreads * j) / kChunks;
+        const int at_chunk = (threadIdx.x + kLThreads * j) % kChunks;
+        if (at_row >= left) break;
+        const float top = top_of(at_row);
+        float sum = 0.f;
+        floatx4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kLWaves; ++w) {
+          sum += few_l[w][at_row] * part_of(few_m[w][at_row], top);
+          o += *reinterpret_cast<const floatx4*>(
+              rows + (32 * w + at_row) * kDims + 4 * (at_chunk ^ (at_row & (kChunks - 1))));
+        }
+        const bool some = !(sum == 0.f);  // else no visible key: out 0, lse -inf
+        const float inv = some ? 1.f / sum : 0.f;
+        const float lse = some ? (top + log2f(sum)) * kLn2 : ninf;
+        const int pos = pos_of(at_row), j2 = head_of(at_row, pos);
+        const long long orow =
+            static_cast<long long>(hk * group + j2) * a.total_q + it.q0 + pos0 + pos;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[x] = some ? o[x] * inv : 0.f;
+        const bool heads_row = d0 == 0 && at_chunk == 0;  // one lane per row
+        if (a.num_splits > 1) {
+          const long long prow = orow * a.num_splits + split;
+          if (some) *reinterpret_cast<floatx4*>(a.o_part + prow * D + d0 + 4 * at_chunk) = o;
+          if (heads_row) a.lse_part[prow] = lse == lse ? lse : -ninf;
+        } else {
+          T4 w;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) w[x] = static_cast<T>(o[x]);
+          *reinterpret_cast<T4*>(static_cast<T*>(a.out) + (it.q0 + pos0 + pos) * a.o_stride_t +
+                                 (hk * group + j2) * a.o_stride_h + d0 + 4 * at_chunk) = w;
+          if (heads_row && a.lse) a.lse[orow] = lse;
+        }
+      }
+    }
+    return;
+  }
 
   for (int u = 0; u < ntiles; ++u) {
     const int buf = u & 1;
@@ -519,8 +694,8 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
         for (int i = 0; i < 4; ++i) {
           floatx4 w;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) w[x] = some ? r.acc[dt][4 * i + x] * inv : 0.f;
-          *reinterpret_cast<floatx4*>(op + 32 * dt + 8 * i) = w;
+          for (int x = 0; x < 4; ++x) w[x] = r.acc[dt][4 * i + x] * inv;
+          if (some) *reinterpret_cast<floatx4*>(op + 32 * dt + 8 * i) = w;
         }
       // the merge takes the largest lse, which a NaN would not be
       if (g == 0) a.lse_part[prow] = lse == lse ? lse : -ninf;
@@ -558,6 +733,68 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
   }
 }
 
+// Merge of the splits' partial rows: lse = logsumexp_s lse_s, out = sum_s exp(lse_s - lse) o_s, a
+// wave per row.  A split without a visible key holds lse -inf and no values; one with a NaN holds
+// lse +inf, whose weight is NaN.  The rows' bytes bound it: 23,500 rows of head dim 256 in 3 splits,
+// a third of them empty, YY us.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void merge_kernel(const fa_varlen_args a) {
+  typedef typename PVec<T>::v4 T4;
+  constexpr int kLanes = D / 4, kPar = 64 / kLanes;  // lanes per split, splits side by side
+  constexpr int kBatch = 4;
+  const long long row = static_cast<long long>(blockIdx.x) * 4 + wave_id();
+  if (row >= static_cast<long long>(a.h_q) * a.total_q) return;  // whole waves
+  const int lane = threadIdx.x & 63, sub = lane / kLanes, d4 = lane % kLanes;
+  const int S = a.num_splits;
+  const float ninf = -__builtin_inff();
+  const float* const lp = a.lse_part + row * S;
+  const float* const op = a.o_part + row * S * D + 4 * d4;
+  float m = ninf;
+  for (int s = lane; s < S; s += 64) m = fmaxf(m, lp[s]);
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+  float l = 0.f;
+  floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int base = 0; base < S; base += 64) {
+    const float mine = base + lane < S ? lp[base + lane] : ninf;
+    const float weight = mine == ninf ? 0.f : expf(mine - m);
+    l += weight;
+    const unsigned long long some = __ballot(mine != ninf);
+    for (int s0 = 0; s0 < 64 && base + s0 < S; s0 += kPar * kBatch) {
+      floatx4 o[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int s = s0 + kPar * i + sub;  // below 64
+        o[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+        if ((some >> s) & 1)
+          o[i] = *reinterpret_cast<const floatx4*>(op + static_cast<long long>(base + s) * D);
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) acc += __shfl(weight, s0 + kPar * i + sub) * o[i];
+    }
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    l += __shfl_xor(l, off);
+    if (off >= kLanes) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) acc[x] += __shfl_xor(acc[x], off);
+    }
+  }
+  const bool seen = !(l == 0.f);  // else no visible key: out 0, lse -inf (NaN stays NaN)
+  const float inv = seen ? 1.f / l : 0.f;
+  const int h = static_cast<int>(row / a.total_q);
+  const int pos = static_cast<int>(row - static_cast<long long>(h) * a.total_q);
+  if (sub == 0) {
+    T4 w;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) w[x] = static_cast<T>(acc[x] * inv);
+    *reinterpret_cast<T4*>(static_cast<T*>(a.out) + pos * a.o_stride_t + h * a.o_stride_h +
+                           4 * d4) = w;
+  }
+  if (lane == 0 && a.lse) a.lse[row] = seen ? m + logf(l) : ninf;
+}
+
 // Row blocks per KV head at most: each sequence, and the rows behind the last and before the
 // first, rounds up once.
 long long row_blocks(const fa_varlen_args* a) {
@@ -577,6 +814,17 @@ void launch_varlen(const fa_varlen_args* a, hipStream_t stream) {
     hipLaunchKernelGGL((varlen_kernel<T, 128>), grid, dim3(kLThreads), 0, stream, *a, by_cost);
   else
     hipLaunchKernelGGL((varlen_kernel<T, 256>), grid, dim3(kLThreads), 0, stream, *a, by_cost);
+}
+
+template <typename T>
+void launch_merge(const fa_varlen_args* a, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>((static_cast<long long>(a->h_q) * a->total_q + 3) / 4));
+  if (a->d == 64)
+    hipLaunchKernelGGL((merge_kernel<T, 64>), grid, dim3(256), 0, stream, *a);
+  else if (a->d == 128)
+    hipLaunchKernelGGL((merge_kernel<T, 128>), grid, dim3(256), 0, stream, *a);
+  else
+    hipLaunchKernelGGL((merge_kernel<T, 256>), grid, dim3(256), 0, stream, *a);
 }
 
 bool rows16(const void* p, int64_t s0, int64_t s1) {
@@ -617,10 +865,7 @@ int check_varlen(const fa_varlen_args* a) {
                "num_splits %d of %d tokens invalid", a->num_splits, a->split_tokens);
   FA_CHECK_ARG(a->num_splits == 1 || (a->o_part && a->lse_part),
                "num_splits %d > 1 needs o_part and lse_part", a->num_splits);
-  // the merge's own limit
-  FA_CHECK_ARG(a->num_splits == 1 ||
-                   a->h_kv * ((static_cast<long long>(a->h_q / a->h_kv) * a->total_q + 15) / 16) <=
-                       65535,
+  FA_CHECK_ARG(a->num_splits == 1 || static_cast<long long>(a->h_q) * a->total_q <= INT32_MAX,
                "too many query rows for splits");
   return FA_OK;
 }
@@ -646,21 +891,11 @@ extern "C" int fa_varlen_combine(const fa_varlen_args* a, void* stream) {
   const int rc = fa::check_varlen(a);
   if (rc != FA_OK) return rc;
   FA_CHECK_ARG(a->o_part && a->lse_part, "combine needs o_part and lse_part");
-  fa_gqa_decode_args g = {};  // one batch entry of total_q positions; reads the partial rows alone
-  g.q = g.k = g.v = a->q;
-  g.out = a->out;
-  g.o_stride_h = a->o_stride_h;
-  g.o_stride_m = a->o_stride_t;
-  g.lse = a->lse;
-  g.o_part = a->o_part;
-  g.lse_part = a->lse_part;
-  g.batch = 1;
-  g.h_q = a->h_q;
-  g.h_kv = a->h_kv;
-  g.m = a->total_q;
-  g.d = a->d;
-  g.num_splits = a->num_splits;
-  g.split_tokens = a->split_tokens;
-  g.dtype = a->dtype;
-  return fa_gqa_combine(&g, stream);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (a->dtype == 1)
+    fa::launch_merge<__bf16>(a, s);
+  else
+    fa::launch_merge<_Float16>(a, s);
+  FA_CHECK_HIP(hipGetLastError());
+  return FA_OK;
 }

@@ -155,6 +155,40 @@ def test_odd_values_of_the_last_key_without_a_mask(d, dtype):
     assert torch.equal(torch.isnan(lse), torch.isnan(ref_lse))
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("h,hk,d", [(4, 4, 64), (8, 2, 128), (7, 1, 128), (4, 2, 256), (32, 1, 64),
+                                    (33, 1, 128)])
+def test_few_rows_over_long_contexts(h, hk, d, dtype, causal):
+    """Single tokens and short tails whose rows fill one wave at most, next to a prompt: contexts
+    around the keys that four waves take at a time, and a tail of a longer prompt."""
+    need_gpu()
+    say(f"varlen few rows h={h} hk={hk} d={d} {dtype} causal={causal}")
+    per = max(32 // (h // hk), 1)
+    lens_q = [1, 1, per, 1, 2, 0, 1, 128 // (h // hk) + 1, 300]
+    lens_k = [129, 1000, 257, 3001, 160, 500, 128, 700, 310]
+    q, k, v, cq, ck = inputs(lens_q, lens_k, h, hk, d, dtype, seed=21)
+    check(q, k, v, cq, ck, causal)
+    check(q[:cq[5]], k[:ck[5]], v[:ck[5]], cq[:6], ck[:6], causal)  # in splits
+
+
+@pytest.mark.parametrize("splits", [False, True])
+@pytest.mark.parametrize("d", varlen.HEAD_DIMS)
+def test_few_rows_with_odd_values(d, splits):
+    need_gpu()
+    say(f"varlen few rows, odd values d={d} splits={splits}")
+    seqs = 10 if splits else 70
+    q, k, v, cq, ck = inputs([5] * seqs, [390] * seqs, 4 * 4, 4, d, torch.float16, seed=22)
+    for s, (where, x) in enumerate(((389, math.nan), (387, math.inf), (388, -math.inf), (10, math.inf),
+                                    (386, math.nan))):
+        v[ck[s] + where, s % 4, 3 + s] = x
+    k[ck[5] + 388, 1, 5] = math.nan
+    o, lse = call(q, k, v, cq, ck, True)
+    ref, ref_lse, a, ds = po.varlen(q, k, v, cq, ck, d ** -0.5, True)
+    assert_rows(o, ref, a, ds.t(), 390, 6.0)
+    assert torch.equal(torch.isnan(lse), torch.isnan(ref_lse))
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1e-3, 40.0])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_scales(scale, dtype):
