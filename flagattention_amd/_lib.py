@@ -215,6 +215,9 @@ SIGNATURES = {
     "fa_mla_decode_noalloc": (
         ctypes.c_int, [ctypes.POINTER(DecodeArgs), ctypes.c_int32, ctypes.c_void_p]),
     "fa_varlen_args_size": (ctypes.c_int64, []),
+    "fa_varlen_plan": (
+        ctypes.c_int,
+        [ctypes.POINTER(VarlenArgs), ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]),
     "fa_varlen_attention": (ctypes.c_int, [ctypes.POINTER(VarlenArgs), ctypes.c_void_p]),
     "fa_varlen_combine": (ctypes.c_int, [ctypes.POINTER(VarlenArgs), ctypes.c_void_p]),
     "fa_mxfp4_cache_size": (ctypes.c_int64, []),

@@ -9,6 +9,8 @@
 // Per tile of 64 keys (32 at head dim 256) and wave, all MFMA 32x32x16, fp32 accumulation:
 //   S^T[keys, 32 rows] = K Q^T, softmax down the columns (lane % 32 = row), O^T[D, 32 rows] +=
 //   V^T P^T with P^T the lane's own scores (the k order only has to agree between the operands).
+#include <algorithm>
+
 #include "fa_common.h"
 #include "fa_rows_tile.h"
 #include "fa_wave.h"
@@ -25,6 +27,7 @@ constexpr int kLRows = kLWaves * kLWaveRows;
 // multiply-add does not round their product with the scale, which the reference is made of.
 constexpr float kFusedMax = 1024.f;
 constexpr float kLag = 6.f;
+constexpr int kCus = 256;  // the order of work-groups counts on these
 // Keys past which a row block of one wave's rows has them dealt out to the waves.
 constexpr int kFewKeys = 128;
 
@@ -112,7 +115,8 @@ __device__ inline Item find_in_order(const fa_varlen_args& a, int group, int ite
 // 512 bytes of the wave's own), and the item is among the blocks of the largest with more than `item`.
 // By bisection, a sum over the lanes per value, it took 4,900 cycles at 16 sequences, so 3,900 (2,200
 // in order).
-__device__ inline Item find_by_cost(const fa_varlen_args& a, int group, int item, int* table) {
+__device__ inline Item find_by_cost(const fa_varlen_args& a, int group, int item, int round,
+                                    int* table) {
   const int lane = threadIdx.x & 63;
   const Seq x = seq_of(a, lane);
   const int shift = 31 - __builtin_clz(max(kLRows / group, 1));  // a power of two of positions
@@ -130,6 +134,9 @@ __device__ inline Item find_by_cost(const fa_varlen_args& a, int group, int item
   const int all = __builtin_amdgcn_readlane(wave_incl_scan(blocks), 63);
   const int top = __builtin_amdgcn_readlane(wave_incl_max(blocks > 0 ? end : 0), 63);
   if (item >= all) return Item{0, 0, 0, 0, -1};
+  // the second round from its far end: a CU's first two work-groups then sum to about the same
+  // (2,048 tokens behind 4,096 keys, 512 work-groups: 189 -> 182 us)
+  if (item >= round && item < 2 * round) item = round + min(2 * round, all) - 1 - item;
   // costs in at most 64 steps: a step's blocks go in any order
   const int stride = cdiv(top, 64);
   const int c = (lane + 1) * stride;
@@ -358,7 +365,9 @@ __device__ inline void fence() {
 // wave's, and the keys are dealt out, 32 at a time and round-robin, each wave's through its own
 // quarter of the tile buffers without a barrier.  The next tile's K is on its way from the end of
 // this one's scores, its V from the end of its values; at head dim 256 the quarter holds one of them
-// at a time.  The wave's first copies are on their way already: K, and V where both fit.
+// at a time.  The wave's first copies are on their way already: K, and V where both fit.  Bound by
+// the keys' bytes: 32 single tokens over up to 7,218 keys (head dim 64, 8 KV heads, 190 MB) 98 us with
+// one wave at work on every tile of 64, 57 so, 43 with four work-groups per CU.
 template <typename T, int D>
 __device__ inline void walk_few(RowState<T, D>& r, const LaneReads<D>& at, unsigned char* mine,
                                 const unsigned char* kp, unsigned int k_tb,
@@ -414,7 +423,7 @@ __device__ inline void walk_few(RowState<T, D>& r, const LaneReads<D>& at, unsig
 
 template <typename T, int D>
 __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_args a,
-                                                             const int by_cost) {
+                                                             const int round) {
   typedef typename PVec<T>::v8 T8;
   typedef typename PVec<T>::v4 T4;
   constexpr int C = D / 8;
@@ -436,8 +445,9 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
   const int group = a.h_q / a.h_kv;
   const int hk = blockIdx.x % a.h_kv;
   const int item = blockIdx.x / a.h_kv;
-  const Item it = by_cost ? find_by_cost(a, group, item, reinterpret_cast<int*>(bufs + 512 * wave_id()))
-                          : find_in_order(a, group, item);
+  const Item it =
+      round > 0 ? find_by_cost(a, group, item, round, reinterpret_cast<int*>(bufs + 512 * wave_id()))
+                : find_in_order(a, group, item);
   if (it.block < 0) return;  // uniform
   barrier();  // the tables are read: the buffers are free
   const int split = blockIdx.y;
@@ -735,8 +745,7 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
 
 // Merge of the splits' partial rows: lse = logsumexp_s lse_s, out = sum_s exp(lse_s - lse) o_s, a
 // wave per row.  A split without a visible key holds lse -inf and no values; one with a NaN holds
-// lse +inf, whose weight is NaN.  The rows' bytes bound it: 23,500 rows of head dim 256 in 3 splits,
-// a third of them empty, YY us.
+// lse +inf, whose weight is NaN.  Bound by the bytes of the partial rows.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void merge_kernel(const fa_varlen_args a) {
   typedef typename PVec<T>::v4 T4;
@@ -806,14 +815,15 @@ void launch_varlen(const fa_varlen_args* a, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(row_blocks(a) * a->h_kv),
                   static_cast<unsigned>(a->num_splits));
   // More work-groups than run at once (2 per CU; 3 at head dim 64): the longest go first.  Under
-  // that their order is all the same and finding it costs 2 us.
-  const int by_cost = a->num_seqs + 2 <= 64 && grid.x * grid.y > (a->d == 64 ? 768u : 512u);
+  // that their order is all the same and finding it costs a little more than finding the next.
+  const bool by_cost = a->num_seqs + 2 <= 64 && grid.x * grid.y > (a->d == 64 ? 768u : 512u);
+  const int round = by_cost ? std::max(kCus / a->h_kv, 1) : 0;  // items that start at once
   if (a->d == 64)
-    hipLaunchKernelGGL((varlen_kernel<T, 64>), grid, dim3(kLThreads), 0, stream, *a, by_cost);
+    hipLaunchKernelGGL((varlen_kernel<T, 64>), grid, dim3(kLThreads), 0, stream, *a, round);
   else if (a->d == 128)
-    hipLaunchKernelGGL((varlen_kernel<T, 128>), grid, dim3(kLThreads), 0, stream, *a, by_cost);
+    hipLaunchKernelGGL((varlen_kernel<T, 128>), grid, dim3(kLThreads), 0, stream, *a, round);
   else
-    hipLaunchKernelGGL((varlen_kernel<T, 256>), grid, dim3(kLThreads), 0, stream, *a, by_cost);
+    hipLaunchKernelGGL((varlen_kernel<T, 256>), grid, dim3(kLThreads), 0, stream, *a, round);
 }
 
 template <typename T>
@@ -825,6 +835,47 @@ void launch_merge(const fa_varlen_args* a, hipStream_t stream) {
     hipLaunchKernelGGL((merge_kernel<T, 128>), grid, dim3(256), 0, stream, *a);
   else
     hipLaunchKernelGGL((merge_kernel<T, 256>), grid, dim3(256), 0, stream, *a);
+}
+
+// Splits along the keys: the cheapest by a model of the launch, in us.  A work-group takes `step`
+// for a tile of keys by itself, and `shared` times as many as a CU has (two at least once the grid
+// comes near the CUs, for the dispatcher then doubles some up); the merge costs 3.5 and the partial
+// rows written and read at 4 TB/s, of which a causal batch leaves some empty.  Measured / model, 8 KV
+// heads, group 4, D = 128: 256 tokens behind 8,192 keys in 1 / 2 / 4 / 8 / 12 splits 168 / 96 / 77 /
+// 57 / 61 against 170 / 95 / 76 / 56 / 63, 700 tokens 20.9 / 33.4 / 32.2 in 1 / 2 / 4 against 19 / 25 /
+// 34 (two splits per CU whatever their rows took 32.3), D = 256, 4 KV heads, 1,200 tokens 57 / 49 / 48 /
+// 51 in 1 / 2 / 3 / 4 against 58 / 54 / 48 / 51.  Blocks of few rows are bound by their keys' bytes
+// and want four work-groups per CU also where every CU has one: 32 tokens over up to 7,218 keys
+// 103 / 82 / 83 / 92 in 1 / 4 / 8 / 16, but 64 over up to 2,000 37 / 41 in 1 / 2.
+int choose_splits(const fa_varlen_args* a, int64_t max_q, int64_t max_k, int64_t cus) {
+  const int64_t group = a->h_q / a->h_kv;
+  const int64_t blocks =
+      a->h_kv * std::max<int64_t>({std::min(a->num_seqs, a->total_q),
+                                   (a->total_q * group + kLRows - 1) / kLRows, 1});
+  const bool few = max_q * group <= kLWaveRows;
+  int64_t pick = 1;
+  if (blocks < cus) {
+    const int keys = a->d == 256 ? 32 : 64;  // of a tile
+    const int64_t tiles = (max_k + keys - 1) / keys;
+    const double step = few ? (a->d == 64 ? 0.33 : 0.65) : a->d == 64 ? 0.87 : a->d == 128 ? 1.25 : 1.4;
+    const double shared = few ? (a->d == 64 ? 0.28 : 0.55) : a->d == 64 ? 0.47 : a->d == 128 ? 0.9 : 0.95;
+    const double full = a->causal ? 1 - 0.5 * a->total_q / std::max(a->total_k, a->total_q) : 1;
+    const double part = full * a->h_q * a->total_q * a->d * 8.0 / 4e6;
+    double best = 0;
+    for (int64_t s : {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20, 24, 32, 48, 64, 96, 128}) {
+      if (s > 1 && tiles < 2 * s) break;
+      const double per_cu = static_cast<double>(blocks * s) / static_cast<double>(cus);
+      const double load = few || per_cu <= 0.7 ? per_cu : std::max(per_cu, 2.0);
+      const double t = static_cast<double>((tiles + s - 1) / s) * std::max(step, shared * load) +
+                       (s > 1 ? 3.5 + 0.06 * s + part * s : 0);
+      if (s == 1 || t < best) {
+        best = t;
+        pick = s;
+      }
+    }
+  }
+  if (few) pick = std::max(pick, std::min((4 * cus + blocks - 1) / blocks, max_k / 1024));
+  return static_cast<int>(std::min<int64_t>(std::max<int64_t>(pick, 1), 128));
 }
 
 bool rows16(const void* p, int64_t s0, int64_t s1) {
@@ -874,6 +925,22 @@ int check_varlen(const fa_varlen_args* a) {
 }  // namespace fa
 
 extern "C" int64_t fa_varlen_args_size(void) { return static_cast<int64_t>(sizeof(fa_varlen_args)); }
+
+extern "C" int fa_varlen_plan(fa_varlen_args* a, int32_t max_q, int32_t max_k, int32_t cu_count) {
+  FA_CHECK_ARG(a != nullptr, "args is NULL");
+  FA_CHECK_ARG(a->num_seqs >= 0 && a->total_q >= 1 && a->total_k >= 0 && a->h_q >= 1 &&
+                   a->h_kv >= 1 && a->h_q % a->h_kv == 0 && a->d >= 1 && max_q >= 0 && max_k >= 0 &&
+                   cu_count >= 1,
+               "num_seqs %d / total_q %d / total_k %d / h_q %d / h_kv %d / max_q %d / max_k %d / "
+               "cu_count %d invalid",
+               a->num_seqs, a->total_q, a->total_k, a->h_q, a->h_kv, max_q, max_k, cu_count);
+  const int64_t longest = std::min(max_k, a->total_k);
+  const int64_t s = fa::choose_splits(a, max_q, longest, cu_count);
+  const int64_t each = ((longest + s - 1) / s + 63) / 64 * 64;  // whole tiles
+  a->split_tokens = static_cast<int32_t>(std::max<int64_t>(std::min<int64_t>(each, INT32_MAX - 63), 64));
+  a->num_splits = s == 1 ? 1 : static_cast<int32_t>((longest + a->split_tokens - 1) / a->split_tokens);
+  return FA_OK;
+}
 
 extern "C" int fa_varlen_attention(const fa_varlen_args* a, void* stream) {
   const int rc = fa::check_varlen(a);

@@ -637,24 +637,6 @@ PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // ---- packed prompts (varlen.py) and the 4-bit cache (mxfp4.py) ----
 bool packed_dim(int64_t d) { return d == 64 || d == 128 || d == 256; }
 
-// Split count of packed prompts: varlen.choose_splits.
-int64_t varlen_split_count(int64_t total_q, int64_t num_seqs, int64_t group, int64_t h_kv,
-                           int64_t max_k, int64_t cus) {
-  const int64_t blocks = h_kv * std::max<int64_t>({std::min(num_seqs, total_q),
-                                                   cdiv(total_q * group, kPrefillRowsPerWg), 1});
-  if (blocks >= cus || max_k <= kMinSplitTokens) return 1;
-  return std::min(cdiv(2 * cus, blocks), cdiv(max_k, kMinSplitTokens));
-}
-
-// varlen_splits(total_q, num_seqs, group, h_kv, max_k, cus), for the comparison with varlen.py.
-PyObject* varlen_splits(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  int64_t x[6];
-  if (nargs != 6) return none();
-  for (int i = 0; i < 6; ++i)
-    if (!to_int(args[i], &x[i]) || x[i] < 1) return none();
-  return PyLong_FromLongLong(varlen_split_count(x[0], x[1], x[2], x[3], x[4], x[5]));
-}
-
 // varlen(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal, sm_scale,
 //        want_lse): (o, lse) or o
 PyObject* varlen(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -691,8 +673,7 @@ PyObject* varlen(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (t->device() != device) return none();
   const int cus = cu_count(device.index());
   if (cus == 0) return none();
-  const int64_t num_seqs = cq->size(0) - 1, longest = std::min(max_k, total_k);
-  const int64_t s = varlen_split_count(total_q, num_seqs, h_q / h_kv, h_kv, longest, cus);
+  const int64_t num_seqs = cq->size(0) - 1;
   at::Tensor out, lse;
   {
     NoGil nogil;
@@ -722,11 +703,12 @@ PyObject* varlen(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     a.h_q = static_cast<int32_t>(h_q);
     a.h_kv = static_cast<int32_t>(h_kv);
     a.d = static_cast<int32_t>(d);
-    a.num_splits = static_cast<int32_t>(s);
-    a.split_tokens = s > 1 ? static_cast<int32_t>(whole_tiles(cdiv(longest, s))) : 1;
     a.scale = static_cast<float>(scale);
     a.causal = causal;
     a.dtype = q->scalar_type() == at::kBFloat16;
+    check(fa_varlen_plan(&a, static_cast<int32_t>(std::min(max_q, total_q)),
+                         static_cast<int32_t>(std::min(max_k, total_k)), cus));
+    const int64_t s = a.num_splits;
     if (s > 1) {
       const int64_t n = h_q * total_q * s;
       part = make({n * (d + 1)}, at::kFloat, device);
@@ -938,7 +920,7 @@ PyObject* mxfp4_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
    nullptr}
 PyMethodDef g_methods[] = {FA_METHOD(mla_metadata), FA_METHOD(mla_decode),   FA_METHOD(paged),
                            FA_METHOD(contiguous),   FA_METHOD(topk_indices), FA_METHOD(cache_write),
-                           FA_METHOD(split_counts), FA_METHOD(varlen),   FA_METHOD(varlen_splits),
+                           FA_METHOD(split_counts), FA_METHOD(varlen),
                            FA_METHOD(mxfp4_write),  FA_METHOD(mxfp4_gather),
                            FA_METHOD(mxfp4_decode), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, g_methods};

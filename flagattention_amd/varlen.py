@@ -19,22 +19,9 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .gqa import _aligned, _cu_count, _dtype_code, _require, whole_tiles
+from .gqa import _aligned, _cu_count, _dtype_code, _require
 
 HEAD_DIMS = (64, 128, 256)
-ROWS_PER_WG = 128
-MIN_SPLIT_TOKENS = 256
-
-
-def choose_splits(total_q: int, num_seqs: int, group: int, h_kv: int, max_k: int,
-                  cu_count: int) -> int:
-    """Split-KV count: none when the row blocks (at least one per sequence with tokens) give
-    every CU a work-group, else enough for about two work-groups per CU, each at least
-    MIN_SPLIT_TOKENS keys long (csrc/host/fa_native.cpp has the same rule)."""
-    blocks = h_kv * max(min(num_seqs, total_q), -(-total_q * group // ROWS_PER_WG), 1)
-    if blocks >= cu_count or max_k <= MIN_SPLIT_TOKENS:
-        return 1
-    return min(-(-2 * cu_count // blocks), -(-max_k // MIN_SPLIT_TOKENS))
 
 
 def flash_attention_varlen(
@@ -106,9 +93,6 @@ def flash_attention_varlen(
     lse = (torch.empty((h_q, total_q), dtype=torch.float32, device=device)
            if return_log_normalizer else None)
     if total_q > 0:
-        s = choose_splits(total_q, num_seqs, h_q // h_kv, h_kv, min(max_seqlen_k, total_k),
-                          _cu_count(device))
-        split_tokens = whole_tiles(-(-min(max_seqlen_k, total_k) // s)) if s > 1 else 1
         args = _lib.VarlenArgs(
             q=q.data_ptr(), q_stride_t=q.stride(0), q_stride_h=q.stride(1), k=k.data_ptr(),
             v=v.data_ptr(), k_stride_t=k.stride(0), k_stride_h=k.stride(1),
@@ -117,9 +101,12 @@ def flash_attention_varlen(
             out=o.data_ptr(), o_stride_t=o.stride(0), o_stride_h=o.stride(1),
             lse=None if lse is None else lse.data_ptr(), o_part=None, lse_part=None,
             num_seqs=num_seqs, total_q=total_q, total_k=total_k, h_q=h_q, h_kv=h_kv, d=d,
-            num_splits=s, split_tokens=split_tokens, scale=float(sm_scale),
+            num_splits=1, split_tokens=1, scale=float(sm_scale),
             causal=int(bool(causal)), dtype=code)
         lib = _lib.load()
+        _lib.check(lib.fa_varlen_plan(ctypes.byref(args), min(max_seqlen_q, total_q),
+                                      min(max_seqlen_k, total_k), _cu_count(device)))
+        s = args.num_splits
         with torch.cuda.device(device):
             stream = torch.cuda.current_stream(device).cuda_stream
             if s > 1:

@@ -22,8 +22,8 @@ extern "C" {
  * keys are rows cu_seqlens_k[s] .. cu_seqlens_k[s + 1] - 1 of k and v.  Starts are taken as clipped
  * to [0, total] and lengths as at least 0, so no list makes a call read or write past its tensors.
  * Rows of q that belong to no sequence (behind the last one, or before the first) get out = 0,
- * lse = -inf, as rows without a visible key do.  fp16 or bf16; element strides; last dimensions contiguous, rows
- * 16-byte aligned.  Head dims 64, 128, 256.
+ * lse = -inf, as rows without a visible key do.  fp16 or bf16; element strides; last dimensions
+ * contiguous, rows 16-byte aligned.  Head dims 64, 128, 256.
  */
 typedef struct fa_varlen_args {
   const void* q; /* [total_q][h_q][d] */
@@ -49,6 +49,12 @@ typedef struct fa_varlen_args {
 
 /* sizeof(fa_varlen_args) as compiled into the library. */
 int64_t fa_varlen_args_size(void);
+
+/*
+ * Fills in num_splits and split_tokens, from the totals, heads, head dim and causal of args, for
+ * sequences of up to max_q tokens and max_k keys on a device of cu_count compute units.
+ */
+int fa_varlen_plan(fa_varlen_args* args, int32_t max_q, int32_t max_k, int32_t cu_count);
 
 /*
  * Attention of every packed row: with num_splits == 1 writes out (and lse if given), otherwise

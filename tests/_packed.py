@@ -13,7 +13,11 @@ u is half a step of the output type (bf16 2^-8, fp16 2^-11).  Against the formul
 * fp32 sums over n keys, exponentials, the split weights and the division: (n + 64) 2^-24 a, the
   n for partial sums that are each rounded.
 """
+import ctypes
+
 import torch
+
+from flagattention_amd import _lib
 
 HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 TINY = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25}  # half of the smallest step
@@ -43,3 +47,11 @@ def assert_lse(lse, ref, ds, n, d):
     tol = (d + 8) * 2.0 ** -24 * ds + (n + 64) * 2.0 ** -24 + 2.0 ** -21 * ref.abs()
     err = (lse.double() - ref).abs()
     assert bool((err <= tol)[fin].all()), f"lse off by {float(err[fin].max()):.3e}"
+
+
+def varlen_splits(total_q, total_k, seqs, h, hk, d, causal, max_q, max_k, cus):
+    """(splits, tokens of each) that flash_attention_varlen takes."""
+    args = _lib.VarlenArgs(num_seqs=seqs, total_q=total_q, total_k=total_k, h_q=h, h_kv=hk, d=d,
+                           causal=int(causal))
+    _lib.check(_lib.load().fa_varlen_plan(ctypes.byref(args), max_q, max_k, cus))
+    return args.num_splits, args.split_tokens

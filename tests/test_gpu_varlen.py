@@ -9,7 +9,7 @@ import flag_attn
 from flagattention_amd import varlen
 from oracle import packed_oracle as po
 from tests._helpers import DEV, need_gpu, say
-from tests._packed import assert_lse, assert_rows
+from tests._packed import assert_lse, assert_rows, varlen_splits
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.float16, torch.bfloat16]
@@ -85,7 +85,8 @@ def test_split_keys(lens_q, lens_k, d, causal):
     need_gpu()
     say(f"varlen splits {lens_q} {lens_k} d={d} causal={causal}")
     cu = torch.cuda.get_device_properties(0).multi_processor_count
-    assert varlen.choose_splits(sum(lens_q), len(lens_q), 2, 2, max(lens_k), cu) > 1
+    assert varlen_splits(sum(lens_q), sum(lens_k), len(lens_q), 4, 2, d, causal, max(lens_q),
+                         max(lens_k), cu)[0] > 1
     check(*inputs(lens_q, lens_k, 4, 2, d, torch.bfloat16, seed=9), causal)
 
 

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import flag_attn
-from flagattention_amd import _lib, varlen
+from flagattention_amd import _lib
 from tests._helpers import DEV
 from tests.test_native_host import _both, _same
 
@@ -20,18 +20,6 @@ def test_calls_without_gpu_tensors_are_left_to_python():
     assert fast.mxfp4_gather(*c, cu.view(1, 2), cu, 4, True) is None
     assert fast.mxfp4_decode(q, *c, cu, cu.view(1, 2), 1.0, 4, 0) is None
     assert fast.mxfp4_decode(*[None] * 10) is None
-
-
-def test_split_rule_is_the_python_one():
-    fast = _lib.native()
-    for cus in (64, 256, 304):
-        for total in (1, 2, 16, 31, 32, 33, 100, 511, 1024, 5000):
-            for seqs in (1, 2, 7, 64, 300):
-                for group in (1, 4, 7, 128, 129):
-                    for hk in (1, 8, 40):
-                        for n in (1, 255, 256, 257, 511, 512, 513, 4097, 100000):
-                            assert fast.varlen_splits(total, seqs, group, hk, n, cus) == \
-                                varlen.choose_splits(total, seqs, group, hk, n, cus)
 
 
 @pytest.mark.gpu

@@ -9,6 +9,7 @@ import torch
 import flag_attn
 from flagattention_amd import ArgumentError, _lib, mxfp4, varlen
 from oracle import packed_oracle as po
+from tests._packed import varlen_splits
 
 
 def _varlen(dtype=torch.float16):
@@ -182,11 +183,21 @@ def test_oracle_formats():
 
 
 def test_split_rule():
-    assert varlen.choose_splits(1, 1, 4, 8, 100, 256) == 1
-    assert varlen.choose_splits(100000, 4, 4, 8, 100000, 256) == 1
-    for total, seqs, group, hk, n in ((1, 1, 1, 1, 10000), (64, 1, 8, 2, 300), (5, 4, 4, 1, 70000)):
-        s = varlen.choose_splits(total, seqs, group, hk, n, 256)
-        blocks = hk * max(min(seqs, total), -(-total * group // varlen.ROWS_PER_WG))
-        assert 1 < s <= -(-n // varlen.MIN_SPLIT_TOKENS) and s * blocks < 3 * 256
-        assert hk * -(-group * total // 16) <= 65535  # the merge's limit
+    """The splits of packed prompts: none for one tile of keys or where the rows fill the CUs; they
+    cover the keys, each with some."""
+    for d in varlen.HEAD_DIMS:
+        assert varlen_splits(1, 60, 1, 32, 8, d, True, 1, 60, 256)[0] == 1
+        assert varlen_splits(100000, 100000, 4, 32, 8, d, True, 50000, 50000, 256)[0] == 1
+        assert varlen_splits(5, 0, 1, 4, 4, d, True, 5, 0, 256)[0] == 1
+        for total, seqs, h, hk, n in ((1, 1, 1, 1, 10000), (64, 1, 16, 2, 3000), (5, 4, 4, 1, 70000),
+                                      (1, 1, 1, 1, 2 ** 31 - 1), (1, 1, 64, 1, 2 ** 31 - 100)):
+            for causal in (True, False):
+                s, each = varlen_splits(total, n, seqs, h, hk, d, causal, total, n, 256)
+                assert 1 < s <= 128 and each % 64 == 0 and (s - 1) * each < n <= s * each
+    for total in (1, 31, 500, 5000):
+        for seqs in (1, 2, 64, 300):
+            for h, hk in ((1, 1), (32, 8), (40, 40), (128, 1)):
+                for n in (1, 64, 65, 127, 129, 513, 4097, 100000):
+                    s, each = varlen_splits(total, n * seqs, seqs, h, hk, 128, True, total, n, 256)
+                    assert s == 1 or (s - 1) * each < n <= s * each
     assert mxfp4.HEAD_DIMS == varlen.HEAD_DIMS == (64, 128, 256)
