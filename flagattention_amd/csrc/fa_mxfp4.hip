@@ -240,6 +240,8 @@ __global__ __launch_bounds__(kWThreads) void mxfp4_gather_kernel(
   }
 }
 
+constexpr int kMaxTokens = 1 << 28;  // a grid holds less than 2^32 lanes per dimension
+
 // Tokens per work-group of the two: fewer where they would not give every CU work.
 int tokens_per_group(int64_t tokens) {
   int t = kWTokens;
@@ -794,6 +796,7 @@ extern "C" int fa_mxfp4_cache_write(const fa_mxfp4_cache* cache, const void* key
                "key / value rows must be 16-byte aligned");
   FA_CHECK_ARG(static_cast<int64_t>(num_tokens) * cache->h_kv <= INT32_MAX,
                "num_tokens %d x h_kv %d is 2^31 or more", num_tokens, cache->h_kv);
+  FA_CHECK_ARG(num_tokens < fa::kMaxTokens, "num_tokens %d is 2^28 or more", num_tokens);
   const int tokens = fa::tokens_per_group(num_tokens);
   const dim3 grid(static_cast<unsigned>(fa::cdiv(num_tokens, tokens)), 2);
   const hipStream_t s = static_cast<hipStream_t>(stream);
@@ -826,6 +829,7 @@ extern "C" int fa_mxfp4_gather(const fa_mxfp4_cache* cache, const int32_t* block
   FA_CHECK_ARG(fa::aligned(k_out, 16) && fa::aligned(v_out, 16), "outputs must be 16-byte aligned");
   FA_CHECK_ARG(static_cast<int64_t>(total) * cache->h_kv <= INT32_MAX,
                "total %d x h_kv %d is 2^31 or more", total, cache->h_kv);
+  FA_CHECK_ARG(total < fa::kMaxTokens, "total %d is 2^28 or more", total);
   const int tokens = fa::tokens_per_group(total);
   const dim3 grid(static_cast<unsigned>(fa::cdiv(total, tokens)), 2);
   const hipStream_t s = static_cast<hipStream_t>(stream);

@@ -909,14 +909,14 @@ int check_varlen(const fa_varlen_args* a) {
                    group * a->q_stride_h < (1ll << 29) && group * a->o_stride_h < (1ll << 29),
                "q / out token strides must be in [0, 2^23), a group's heads within 2^29 elements");
   FA_CHECK_ARG(static_cast<long long>(a->total_q) * (a->h_q / a->h_kv) < (1ll << 30) &&
-                   row_blocks(a) * a->h_kv < (1ll << 30),
-               "too many query rows or row blocks");
+                   row_blocks(a) * a->h_kv < (1ll << 24),
+               "too many query rows or row blocks");  // a grid holds less than 2^32 lanes
   FA_CHECK_ARG(a->num_splits >= 1 && a->num_splits <= 65535 && a->split_tokens >= 1 &&
                    static_cast<int64_t>(a->num_splits - 1) * a->split_tokens <= INT32_MAX,
                "num_splits %d of %d tokens invalid", a->num_splits, a->split_tokens);
   FA_CHECK_ARG(a->num_splits == 1 || (a->o_part && a->lse_part),
                "num_splits %d > 1 needs o_part and lse_part", a->num_splits);
-  FA_CHECK_ARG(a->num_splits == 1 || static_cast<long long>(a->h_q) * a->total_q <= INT32_MAX,
+  FA_CHECK_ARG(a->num_splits == 1 || static_cast<long long>(a->h_q) * a->total_q < (1 << 26),
                "too many query rows for splits");
   return FA_OK;
 }

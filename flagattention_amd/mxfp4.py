@@ -106,7 +106,7 @@ def cache_kv_mxfp4(
     _require(slot_mapping.dim() == 1 and slot_mapping.shape[0] == t
              and slot_mapping.dtype in (torch.int32, torch.int64),
              "slot_mapping must be int32 / int64 [num_tokens]")
-    _require(t * h_kv < 1 << 31, "too many tokens")
+    _require(t * h_kv < 1 << 31 and t < 1 << 28, "too many tokens")
     _require(all(x.is_cuda and x.device == key.device for x in (key, value, slot_mapping)),
              "all tensors must be CUDA (HIP) tensors on one device")
     if t == 0:
@@ -159,7 +159,7 @@ def gather_kv_mxfp4(
              and block_tables.shape[0] == num_seqs and block_tables.stride(1) == 1,
              "block_tables must be int32 [num_seqs, max_num_blocks_per_seq]")
     _require(isinstance(total_tokens, int) and total_tokens >= 0, "total_tokens must be an int >= 0")
-    _require(total_tokens * h_kv < 1 << 31, "too many tokens")
+    _require(total_tokens * h_kv < 1 << 31 and total_tokens < 1 << 28, "too many tokens")
     _require(all(x.is_cuda and x.device == device for x in (block_tables, cu_seqlens)),
              "all tensors must be CUDA (HIP) tensors on one device")
     k = torch.empty((total_tokens, h_kv, d), dtype=dtype, device=device)

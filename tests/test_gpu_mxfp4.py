@@ -84,7 +84,7 @@ def test_write_odd_values_and_layouts(dtype):
     assert bool(torch.isnan(k[:32]).all()) and bool(torch.isfinite(k[32:]).all())
     odd = torch.zeros((40, hk, d + 1), dtype=dtype, device=DEV)
     odd[..., 1:] = x.to(DEV)
-    again = [y.to(DEV).contiguous() for y in before[0:0]] or [y[:, 1::2].contiguous() for y in before]
+    again = [y[:, 1::2].contiguous() for y in before]
     flag_attn.cache_kv_mxfp4(odd[..., 1:], odd[..., 1:], *again, slots.long().to(DEV)[::1])
     assert all(torch.equal(y.cpu(), w) for y, w in zip(again, want))
     flag_attn.cache_kv_mxfp4(odd[:0, :, 1:], odd[:0, :, 1:], *again, slots[:0].to(DEV))
@@ -355,3 +355,51 @@ def test_serving_run():
         got = out.clone()
         torch.randn(4096, device=DEV).sum().item()
         assert torch.equal(got, check_decode(q, cache, [n + 1 for n in lens], bt, max_len=512))
+
+
+def test_replays_and_other_streams():
+    """Two captured graphs with their own splits' workspaces and a write and read back, replayed in
+    turn on changed inputs, against the same calls on another stream."""
+    need_gpu()
+    say("mxfp4 graphs")
+    d, hk, block = 128, 2, 32
+    cache = new_cache(200, hk, block, d, seed=9)
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    bt = torch.randperm(200, generator=torch.Generator().manual_seed(3)).int().view(2, 100).to(DEV)
+    lens = torch.tensor([3000, 1701], dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, 40, 140], dtype=torch.int32, device=DEV)
+    q = [queries(2, 8, d, torch.float16, seed=6), queries(2, 16, d, torch.float16, seed=7)]
+    kv = queries(60, hk, d, torch.float16, seed=8)
+    slots = torch.arange(64, 124, device=DEV)
+
+    def calls(x):
+        flag_attn.cache_kv_mxfp4(kv, kv, *cache, slots)
+        return (flag_attn.paged_attention_mxfp4(x, *cache, lens, bt, 0.1, 3200),
+                *flag_attn.gather_kv_mxfp4(*cache, bt, cu, 150, torch.float16))
+
+    for x in q:
+        calls(x)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for x in q:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(calls(x))
+        graphs.append(g)
+    stream = torch.cuda.Stream()
+    for rep in range(3):
+        for t in (*q, kv):
+            t.copy_(torch.randn(t.shape, generator=gen, device=DEV))
+        slots.copy_(torch.randperm(6400, device=DEV)[:60])
+        lens.copy_(torch.tensor([3200 - 7 * rep, 1 + 33 * rep], dtype=torch.int32))
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        got = [[t.clone() for t in o] for o in outs]
+        torch.randn(4096, device=DEV).sum().item()
+        with torch.cuda.stream(stream):
+            want = [calls(x) for x in q]
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(g, w)), rep
+        check_decode(q[0], cache, lens.tolist(), bt.cpu(), scale=0.1, max_len=3200)

@@ -127,7 +127,10 @@ def test_struct_mirrors_and_c_abi_refusals():
                          (dict(k=4104), b"aligned"), (dict(o_stride_h=60), b"aligned"),
                          (dict(k_stride_t=1 << 23), b"token strides"),
                          (dict(v_stride_t=-64), b"token strides"),
-                         (dict(total_q=1 << 30), b"too many"), (dict(num_splits=0), b"num_splits"),
+                         (dict(total_q=1 << 30), b"too many"),
+                         (dict(num_seqs=1 << 24), b"too many"),
+                         (dict(total_q=1 << 25, num_splits=2, o_part=4096, lse_part=4096),
+                          b"too many"), (dict(num_splits=0), b"num_splits"),
                          (dict(num_splits=2), b"o_part"),
                          (dict(num_splits=9, split_tokens=1 << 29), b"num_splits")):
         refused(lib.fa_varlen_attention(ctypes.byref(_lib.VarlenArgs(**{**good, **change})), None), text)
@@ -153,6 +156,8 @@ def test_struct_mirrors_and_c_abi_refusals():
                                      None), b"aligned")
     refused(lib.fa_mxfp4_cache_write(ctypes.byref(ok), 4096, 128, 64, 4096, 128, 64, 4096, 1, 1 << 30, 0,
                                      None), b"2^31")
+    refused(lib.fa_mxfp4_gather(ctypes.byref(ok), 4096, 1, 1, 4096, 1, 1 << 28, 4096, 4096, 0, None),
+            b"2^28")
     refused(lib.fa_mxfp4_gather(ctypes.byref(ok), None, 1, 1, 4096, 1, 3, 4096, 4096, 0, None), b"NULL")
     decode = dict(cache=ok, q=4096, out=4096, block_table=4096, seqlens=4096, max_blocks_per_seq=1,
                   batch=1, h_q=4, num_splits=1, split_tokens=7, q_stride_b=256, q_stride_h=64)
