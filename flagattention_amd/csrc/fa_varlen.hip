@@ -640,6 +640,10 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
   }
 
   for (int u = 0; u < ntiles; ++u) {
+    // The accumulators as whole registers: without this each of their elements is copied in every
+    // step, for its uses behind the loop (6 x 8,192 at head dim 128: 779 -> 744 us).
+#pragma unroll
+    for (int dt = 0; dt < kDimTiles; ++dt) asm volatile("" : "+v"(r.acc[dt]));
     const int buf = u & 1;
     const int start = t0 + kTok * u;
     wait_vmem<0>();  // this wave's copies of tile u (requested one step ago)
