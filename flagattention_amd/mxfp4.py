@@ -141,7 +141,9 @@ def gather_kv_mxfp4(
     total_tokens  rows of the result (cu_seqlens[-1], or more: rows behind it are zeros, as are
                   those of blocks outside the cache)
 
-    Returns ``(key, value)``, each ``dtype`` (fp16 or bf16) ``[total_tokens, H_kv, D]``.
+    Returns ``(key, value)``, each ``dtype`` (fp16 or bf16) ``[total_tokens, H_kv, D]``, the cache's
+    values rounded to it: past fp16's range they are infinities (also what was written as more than
+    57344, whose code is 4 * 2^14; ``paged_attention_mxfp4`` takes those as they are).
     """
     fast = _lib.native() if dtype in (torch.float16, torch.bfloat16) else None
     if fast is not None:

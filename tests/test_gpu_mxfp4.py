@@ -117,6 +117,24 @@ def test_gather(block, d, dtype):
             assert torch.equal(got.cpu(), want.to(dtype))
 
 
+@pytest.mark.parametrize("byte", [0, 100, 103, 126, 140, 141, 142, 254, 255])
+def test_gather_rounds_to_the_type(byte):
+    """Scales at the ends: below fp16's range the values round to it, past it they are infinities."""
+    need_gpu()
+    say(f"mxfp4 gather scale {byte}")
+    cache = new_cache(1, 1, 16, 64, seed=byte)
+    cache[1].fill_(byte), cache[3].fill_(byte)
+    bt = torch.zeros((1, 1), dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, 16], dtype=torch.int32, device=DEV)
+    for dtype in DTYPES:
+        k, v = flag_attn.gather_kv_mxfp4(*cache, bt, cu, 16, dtype)
+        for got, codes, scales in ((k, cache[0], cache[1]), (v, cache[2], cache[3])):
+            want = po.values(codes, scales)[0].transpose(0, 1).to(dtype)
+            assert torch.equal(got.isnan(), want.isnan())
+            assert torch.equal(got.nan_to_num(1.0, math.inf, -math.inf),
+                               want.nan_to_num(1.0, math.inf, -math.inf))
+
+
 def test_gather_of_no_rows_and_late_starts():
     need_gpu()
     say("mxfp4 gather edges")
