@@ -6,6 +6,7 @@
 // two significant bits, and with a power of two as the scale the quotient x / scale is exact,
 // so a code depends on nothing but the value.
 #include "fa_common.h"
+#include "fa_divide.h"
 #include "fa_wave.h"
 #include "flagattention_amd_packed.h"
 
@@ -282,9 +283,15 @@ struct ScaleOf<256> {
 
 #define FA_GLOBAL __attribute__((address_space(1)))
 
+// What a launch works out once for its work-groups.
+struct DecodePlan {
+  int group, turn;          // query heads per KV head; sequences that a split starts on from the last
+  Divisor row_blocks, batch;  // blocks of heads per KV head; sequences
+};
+
 template <typename T, int D, bool kSmallBlocks>
 __global__ __launch_bounds__(64 * kWaves, D == 64 ? 4 : D == 128 ? 3 : 2) void mxfp4_decode_kernel(
-    const fa_mxfp4_decode_args a) {
+    const fa_mxfp4_decode_args a, const DecodePlan plan) {
   typedef typename FVec<T>::v8 T8;
   typedef typename FVec<T>::v4 T4;
   // Bytes per token row of the V tile: 32 more than its values, so that the 8 rows x 32 bytes of a
@@ -304,14 +311,13 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 4 : D == 128 ? 3 : 2) void m
   constexpr bool kTwoTiles = D <= 128;
 
   const fa_mxfp4_cache& cache = a.cache;
-  const int group = a.h_q / cache.h_kv;
-  const int n_rb = cdiv(group, kDRows);
-  const int hk = blockIdx.x / n_rb;
-  const int rb = blockIdx.x - hk * n_rb;
+  const int group = plan.group;
+  const int hk = divide(blockIdx.x, plan.row_blocks);
+  const int rb = blockIdx.x - hk * plan.row_blocks.by;
   const int split = blockIdx.z;
   // the splits of a long context start away from each other (see launch_decode_d)
-  const int turned = blockIdx.y + split * cdiv(a.batch, a.num_splits);
-  const int b = turned % a.batch;
+  const int turned = blockIdx.y + split * plan.turn;
+  const int b = turned - divide(turned, plan.batch) * a.batch;
   const int wave = wave_id();
   const int lane = threadIdx.x & 63;
   const int G = lane >> 4, c16 = lane & 15;
@@ -665,10 +671,13 @@ void launch_decode_d(const fa_mxfp4_decode_args* a, hipStream_t stream) {
   // late splits of ragged contexts are empty (with splits fastest, 8 of them, one XCD had all the
   // last ones: 33.7 us instead of 27.3 at 32 sequences of 97 .. 4,096 keys).
   const dim3 grid(a->cache.h_kv * cdiv(group, kDRows), a->batch, a->num_splits);
+  const DecodePlan plan{group, cdiv(a->batch, a->num_splits), divisor(cdiv(group, kDRows)),
+                        divisor(a->batch)};
   if (a->cache.block_size < kDTile)
-    hipLaunchKernelGGL((mxfp4_decode_kernel<T, D, true>), grid, dim3(64 * kWaves), 0, stream, *a);
+    hipLaunchKernelGGL((mxfp4_decode_kernel<T, D, true>), grid, dim3(64 * kWaves), 0, stream, *a, plan);
   else
-    hipLaunchKernelGGL((mxfp4_decode_kernel<T, D, false>), grid, dim3(64 * kWaves), 0, stream, *a);
+    hipLaunchKernelGGL((mxfp4_decode_kernel<T, D, false>), grid, dim3(64 * kWaves), 0, stream, *a,
+                       plan);
 }
 
 template <typename T>

@@ -20,6 +20,7 @@
 #include <algorithm>
 
 #include "fa_common.h"
+#include "fa_divide.h"
 #include "fa_rows_tile.h"
 #include "fa_wave.h"
 #include "flagattention_amd_packed.h"
@@ -49,8 +50,15 @@ __device__ inline void fold_bits(unsigned int& best, uintx4 w) {
                                                 __builtin_bit_cast(ushortx2, w[i] & 0x7FFF7FFFu)));
 }
 
+// What a launch works out once for its work-groups.
+struct Plan {
+  Divisor group, h_kv;
+  int shift;  // log2 of about a row block's positions
+  int round;  // items that start at once, if they are ordered by their cost, else 0
+};
+
 struct Item {
-  int q0, rows;  // first packed position, rows (positions x group) of the sequence
+  int q0, m;     // first packed position, positions of the sequence
   int k0, n;     // first packed key, keys
   int block;     // row block, -1: none left
 };
@@ -77,10 +85,10 @@ __device__ inline Seq seq_of(const fa_varlen_args& a, int s) {
   }
   return x;
 }
-__device__ inline Item item_of(const Seq& x, int l, int group, int block) {
+__device__ inline Item item_of(const Seq& x, int l, int block) {
   Item it;
   it.q0 = __builtin_amdgcn_readlane(x.q0, l);
-  it.rows = __builtin_amdgcn_readlane(x.m, l) * group;
+  it.m = __builtin_amdgcn_readlane(x.m, l);
   it.k0 = __builtin_amdgcn_readlane(x.k0, l);
   it.n = __builtin_amdgcn_readlane(x.n, l);
   it.block = block;
@@ -108,7 +116,7 @@ __device__ inline Item find_in_order(const fa_varlen_args& a, int group, int ite
     const unsigned long long past = __ballot(upto > item);
     if (past != 0ull) {
       const int l = __builtin_ctzll(past);
-      return item_of(x, l, group, __builtin_amdgcn_readlane(upto, l) - 1 - item);
+      return item_of(x, l, __builtin_amdgcn_readlane(upto, l) - 1 - item);
     }
     item -= __builtin_amdgcn_readlane(upto, 63);
   }
@@ -123,16 +131,16 @@ __device__ inline Item find_in_order(const fa_varlen_args& a, int group, int ite
 // 512 bytes of the wave's own), and the item is among the blocks of the largest with more than `item`.
 // By bisection, a sum over the lanes per value, it took 4,900 cycles at 16 sequences, so 3,900 (2,200
 // in order).
-__device__ inline Item find_by_cost(const fa_varlen_args& a, int group, int item, int round,
-                                    int* table) {
+__device__ inline Item find_by_cost(const fa_varlen_args& a, int group, int item, int shift,
+                                    int round, int* table) {
   const int lane = threadIdx.x & 63;
   const Seq x = seq_of(a, lane);
-  const int shift = 31 - __builtin_clz(max(kLRows / group, 1));  // a power of two of positions
   const int blocks = cdiv(x.m * group, kLRows);
   const bool rises = a.causal && lane < a.num_seqs;
   // (a block of one wave's rows walks its keys four times as fast)
   const int fast = x.m * group <= kLWaveRows && x.n > kFewKeys ? shift + 2 : shift;
-  const int low = rises ? (max(x.n - x.m, 0) >> fast) + 1 : cdiv(x.n, 1 << fast);
+  const int low = rises ? (max(x.n - x.m, 0) >> fast) + 1
+                        : static_cast<int>((static_cast<unsigned int>(x.n) + (1u << fast) - 1) >> fast);
   const int end = low + (rises ? blocks : 1);  // past the highest cost
   auto costing = [&](int c) -> int {           // this lane's blocks that cost c or more
     return rises ? min(max(end - c, 0), blocks) : low >= c ? blocks : 0;
@@ -168,7 +176,7 @@ __device__ inline Item find_by_cost(const fa_varlen_args& a, int group, int item
   const int before = __builtin_amdgcn_readlane(upto - here, l);
   const int from = __builtin_amdgcn_readlane(low, l);
   const bool up = __builtin_amdgcn_readlane(static_cast<int>(rises), l) != 0;
-  return item_of(x, l, group, (up ? max(lo - from, 0) : 0) + rank - before);
+  return item_of(x, l, (up ? max(lo - from, 0) : 0) + rank - before);
 }
 
 // One 32-row tile's softmax state and operands (lane % 32 = row, g = lane / 32).
@@ -431,7 +439,7 @@ __device__ inline void walk_few(RowState<T, D>& r, const LaneReads<D>& at, unsig
 
 template <typename T, int D>
 __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_args a,
-                                                             const int round) {
+                                                             const Plan plan) {
   typedef typename PVec<T>::v8 T8;
   typedef typename PVec<T>::v4 T4;
   constexpr int C = D / 8;
@@ -450,16 +458,16 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
   __shared__ int odd_v[2][kLWaves];  // [tile parity][wave]: see below
   __shared__ float few_m[kLWaves][32], few_l[kLWaves][32];
 
-  const int group = a.h_q / a.h_kv;
-  const int hk = blockIdx.x % a.h_kv;
-  const int item = blockIdx.x / a.h_kv;
-  const Item it =
-      round > 0 ? find_by_cost(a, group, item, round, reinterpret_cast<int*>(bufs + 512 * wave_id()))
-                : find_in_order(a, group, item);
+  const int group = static_cast<int>(plan.group.by);
+  const int item = divide(blockIdx.x, plan.h_kv);
+  const int hk = blockIdx.x - item * a.h_kv;
+  const Item it = plan.round > 0 ? find_by_cost(a, group, item, plan.shift, plan.round,
+                                                reinterpret_cast<int*>(bufs + 512 * wave_id()))
+                                 : find_in_order(a, group, item);
   if (it.block < 0) return;  // uniform
   barrier();  // the tables are read: the buffers are free
   const int split = blockIdx.y;
-  const int m = it.rows / group;
+  const int m = it.m;
 
   const int wave = wave_id();
   const int lane = threadIdx.x & 63;
@@ -512,7 +520,7 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
   };
 
   const int row0 = it.block * kLRows;
-  const int left = min(it.rows - row0, kLRows);  // the work-group's rows
+  const int left = min(m * group - row0, kLRows);  // the work-group's rows
   // One wave's rows and several tiles of keys: the keys are dealt out to the waves.
   const bool few = left <= kLWaveRows && t1 - t0 > kFewKeys;  // uniform
   unsigned char* const quarter = bufs + wave * kTileB;
@@ -529,7 +537,7 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
 
   // Position and query head of the work-group's row r, counted from its first: rows are few, so a
   // reciprocal and a correction divide them by the group.
-  const int pos0 = row0 / group, rem0 = row0 - pos0 * group;
+  const int pos0 = divide(row0, plan.group), rem0 = row0 - pos0 * group;
   const float group_inv = __builtin_amdgcn_rcpf(static_cast<float>(group));
   auto pos_of = [&](int r) -> int {  // counted from pos0
     const int x = rem0 + r;
@@ -804,8 +812,8 @@ __global__ __launch_bounds__(256) void merge_kernel(const fa_varlen_args a) {
   }
   const bool seen = !(l == 0.f);  // else no visible key: out 0, lse -inf (NaN stays NaN)
   const float inv = seen ? 1.f / l : 0.f;
-  const int h = static_cast<int>(row / a.total_q);
-  const int pos = static_cast<int>(row - static_cast<long long>(h) * a.total_q);
+  const int h = static_cast<int>(row) / a.total_q;  // below 2^26 (host check)
+  const int pos = static_cast<int>(row) - h * a.total_q;
   if (sub == 0) {
     T4 w;
 #pragma unroll
@@ -829,13 +837,16 @@ void launch_varlen(const fa_varlen_args* a, hipStream_t stream) {
   // More work-groups than run at once (2 per CU; 3 at head dim 64): the longest go first.  Under
   // that their order is all the same and finding it costs a little more than finding the next.
   const bool by_cost = a->num_seqs + 2 <= 64 && grid.x * grid.y > (a->d == 64 ? 768u : 512u);
-  const int round = by_cost ? std::max(kCus / a->h_kv, 1) : 0;  // items that start at once
+  const int group = a->h_q / a->h_kv;
+  const Plan plan{divisor(group), divisor(a->h_kv),
+                  31 - __builtin_clz(static_cast<unsigned int>(std::max(kLRows / group, 1))),
+                  by_cost ? std::max(kCus / a->h_kv, 1) : 0};
   if (a->d == 64)
-    hipLaunchKernelGGL((varlen_kernel<T, 64>), grid, dim3(kLThreads), 0, stream, *a, round);
+    hipLaunchKernelGGL((varlen_kernel<T, 64>), grid, dim3(kLThreads), 0, stream, *a, plan);
   else if (a->d == 128)
-    hipLaunchKernelGGL((varlen_kernel<T, 128>), grid, dim3(kLThreads), 0, stream, *a, round);
+    hipLaunchKernelGGL((varlen_kernel<T, 128>), grid, dim3(kLThreads), 0, stream, *a, plan);
   else
-    hipLaunchKernelGGL((varlen_kernel<T, 256>), grid, dim3(kLThreads), 0, stream, *a, round);
+    hipLaunchKernelGGL((varlen_kernel<T, 256>), grid, dim3(kLThreads), 0, stream, *a, plan);
 }
 
 template <typename T>
