@@ -71,19 +71,13 @@ struct Seq {
   int q0, m, k0, n;
 };
 __device__ inline Seq seq_of(const fa_varlen_args& a, int s) {
-  Seq x{0, 0, 0, 0};
-  if (s < a.num_seqs) {
-    x.q0 = clip(a.cu_seqlens_q[s], a.total_q);
-    x.m = max(clip(a.cu_seqlens_q[s + 1], a.total_q) - x.q0, 0);
-    x.k0 = clip(a.cu_seqlens_k[s], a.total_k);
-    x.n = max(clip(a.cu_seqlens_k[s + 1], a.total_k) - x.k0, 0);
-  } else if (s == a.num_seqs) {
-    x.q0 = clip(a.cu_seqlens_q[s], a.total_q);
-    x.m = a.total_q - x.q0;
-  } else if (s == a.num_seqs + 1) {
-    x.m = clip(a.cu_seqlens_q[0], a.total_q);
-  }
-  return x;
+  // every lane loads, so that all of it is one trip to memory
+  const int first = s <= a.num_seqs ? s : 0, next = min(first + 1, a.num_seqs);
+  const int q0 = clip(a.cu_seqlens_q[first], a.total_q), q1 = clip(a.cu_seqlens_q[next], a.total_q);
+  const int k0 = clip(a.cu_seqlens_k[first], a.total_k), k1 = clip(a.cu_seqlens_k[next], a.total_k);
+  if (s < a.num_seqs) return Seq{q0, max(q1 - q0, 0), k0, max(k1 - k0, 0)};
+  if (s == a.num_seqs) return Seq{q0, a.total_q - q0, 0, 0};
+  return Seq{0, s == a.num_seqs + 1 ? q0 : 0, 0, 0};
 }
 __device__ inline Item item_of(const Seq& x, int l, int block) {
   Item it;
