@@ -12,8 +12,8 @@
 //
 // Two waves per SIMD (three at head dim 64): one's softmax fills the other's matrix instructions.
 // Long prompts are bound by power: 6 sequences of up to 8,192 tokens, 32 heads of 8 KV heads, D = 128,
-// take 745 us at 1.94 GHz, 1,005 TF (a product of 8,192^3 reaches 1,253), both pipes busy for 52% of the
-// cycles.  16 of up to 2,048 take 185 us, 740 TF, at 2.1 GHz: 3,400 work-groups of ten tiles on
+// take 712 .. 761 us at 1.94 GHz, 980 .. 1,050 TF (a product of 8,192^3 reaches 1,253), both pipes busy
+// for 52% of the cycles.  16 of up to 2,048 take 171 .. 185 us, 740 .. 800 TF, at 2.1 GHz: 3,400 work-groups of ten tiles on
 // average with their starts and ends.  64 rows per wave would halve the reads of LDS, but spill
 // (830 TF where these reach 1,045); a step whose QK runs beside the last one's softmax took 5%
 // fewer cycles and the same time.
@@ -123,8 +123,8 @@ __device__ inline Item find_in_order(const fa_varlen_args& a, int group, int ite
 // prefix, and a block of a full one low.  How many blocks cost c or more is a sum over the
 // sequences; 64 values of c are summed at once, a lane each (the sequences come from LDS, `table`:
 // 512 bytes of the wave's own), and the item is among the blocks of the largest with more than `item`.
-// By bisection, a sum over the lanes per value, it took 4,900 cycles at 16 sequences, so 3,900 (2,200
-// in order).
+// By bisection, a sum over the lanes per value, it took 1,000 cycles more at 16 sequences; in order
+// it takes 1,700 less.
 __device__ inline Item find_by_cost(const fa_varlen_args& a, int group, int item, int shift,
                                     int round, int* table) {
   const int lane = threadIdx.x & 63;
