@@ -196,6 +196,7 @@ def test_scales(scale, dtype):
     need_gpu()
     say(f"varlen scale {scale} {dtype}")
     check(*inputs([90, 33], [150, 33], 4, 2, 64, dtype, seed=6), True, scale=scale)
+    check(*inputs([1, 3, 16], [300, 1500, 129], 4, 2, 64, dtype, seed=6), True, scale=scale)
 
 
 def test_strided_inputs():
@@ -242,6 +243,21 @@ def test_many_sequences(seqs, causal):
     lens[seqs // 2] = 700
     keys = [n + int(x) for n, x in zip(lens, torch.randint(0, 30, (seqs,), generator=gen))]
     check(*inputs(lens, keys, 4, 1, 64, torch.bfloat16, seed=12, extra_q=130), causal)
+
+
+def test_few_rows_strided_and_alone():
+    """Short row blocks of fused and transposed tensors, and one row of one head over keys that end
+    at, before and behind what the waves take in turn."""
+    need_gpu()
+    say("varlen few rows, strides")
+    gen = torch.Generator(device=DEV).manual_seed(31)
+    fused = torch.randn((1200, 8, 128), generator=gen, device=DEV).bfloat16()
+    by_head = torch.randn((8, 1200, 128), generator=gen, device=DEV).bfloat16().transpose(0, 1)
+    for x in (fused, by_head):
+        check(x[:6, :4], x[:, 4:6], x[:, 6:], [0, 1, 6], [0, 700, 1200], True)
+    for n in (129, 159, 160, 161, 255, 256, 257, 288, 512):
+        for d in varlen.HEAD_DIMS:
+            check(*inputs([1], [n], 1, 1, d, torch.float16, seed=n), n % 2 == 0)
 
 
 def test_offsets_past_32_bits():
