@@ -35,7 +35,22 @@ constexpr int kLRows = kLWaves * kLWaveRows;
 // Past this reference (log2 units) the scores are scaled in a pass of their own: a fused
 // multiply-add does not round their product with the scale, which the reference is made of.
 constexpr float kFusedMax = 1024.f;
-constexpr float kLag = 6.f;  // log2 units, see weigh
+// P is relative to a reference per row, which moves where some row's maximum is more than kLag (log2
+// units) past its last place; in bf16 it then goes kAbove over the maximum, so that P reaches
+// 2^(kLag - kAbove) at most.  The sums of 2^10 keys of such a weight and the largest finite V stay
+// within fp32, those of 2^16 of equal weights (a reference at the maximum made an infinity of a single
+// such V whose weight was past 1).  P ends at 2^-126, so weights below 2^-104 of the largest are 0.
+// fp16 keeps 0: its P would lose bits below 2^-14, and its V is below 2^16.
+//
+// Between moves the accumulators are left alone, but the largest P is then no power of two, whose
+// rounding to 16 bits would cost nothing.  Following every new maximum instead (kLag = 0): bf16 error
+// against 64 bits at 300 / 512 / 2,048 / 6,144 keys 2.07 / 2.10 / 2.10 / 2.20e-3 where this has 2.17 /
+// 2.20 / 2.29 / 2.33e-3, fp16 2.58 .. 2.75e-4 where this has 2.71 .. 2.91e-4; 6 x 8,192 tokens take 763
+// instead of 733 us, 16 x 2,048 179 instead of 170, unmasked ones at head dim 256 120 instead of 110.5.
+// kLag = 2: 2.14 .. 2.28e-3, 743, 174 and 116 us.
+constexpr float kLag = 6.f;
+template <typename T>
+constexpr float kAbove = __is_same(T, __bf16) ? 16.f : 0.f;
 constexpr int kCus = 256;  // the order of work-groups counts on these
 // Keys past which a row block of one wave's rows has them dealt out to the waves: 32 each.
 constexpr int kFewKeys = 128;
@@ -254,10 +269,8 @@ __device__ inline void weigh(RowState<T, D>& r, const unsigned char* kb, const L
   #pragma unroll
         for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[tt][i]);
       mx = max_xor32(mx) * scale_log2;
-      // The reference stays while no row's maximum is more than kLag above it: P then reaches
-      // 2^kLag, which rounds no worse, and the accumulators are left alone.
-      if (__ballot(mx > r.mref + kLag || (r.mref == ninf && mx != ninf)) != 0ull) {  // uniform
-        const float m_new = fmaxf(r.mref, mx);
+      if (__ballot(mx > r.mref + (kLag - kAbove<T>)) != 0ull) {  // uniform
+        const float m_new = fmaxf(r.mref, mx + kAbove<T>);
         const float alpha = m_new == ninf ? 1.f : __builtin_amdgcn_exp2f(r.mref - m_new);
         r.lsum *= alpha;
         r.mref = m_new;

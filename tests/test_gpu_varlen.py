@@ -190,6 +190,43 @@ def test_few_rows_with_odd_values(d, splits):
     assert torch.equal(torch.isnan(lse), torch.isnan(ref_lse))
 
 
+# one prompt and a chunk; short tails over dealt-out keys; few rows over keys in splits
+SHAPES = [([200, 70], [200, 330]), ([5] * 40, [390] * 40), ([3, 1], [2111, 700])]
+
+
+@pytest.mark.parametrize("lens_q,lens_k", SHAPES)
+@pytest.mark.parametrize("d", varlen.HEAD_DIMS)
+def test_huge_values(lens_q, lens_k, d):
+    """The largest finite bf16 values at single keys of any weight: the sums of a row stay within fp32
+    where its result does."""
+    need_gpu()
+    say(f"varlen huge values {lens_q[:2]} d={d}")
+    top = torch.finfo(torch.bfloat16).max
+    for causal in (True, False):
+        q, k, v, cq, ck = inputs(lens_q, lens_k, 8, 2, d, torch.bfloat16, seed=d)
+        for at in ck[:-1]:
+            v[at + 50, 0], v[at + 7, 1] = -top, top
+        check(q, k, v, cq, ck, causal)
+
+
+def check_many_huge_values(lens_q, lens_k, d):
+    for causal in (True, False):
+        q, k, v, cq, ck = inputs(lens_q, lens_k, 8, 2, d, torch.bfloat16, seed=d)
+        v.fill_(2.0 ** 127)  # off by no more than a weight's rounding: below 2^128
+        check(q, k, v, cq, ck, causal)
+        v.fill_(torch.finfo(torch.bfloat16).max)
+        check(torch.zeros_like(q), k, v, cq, ck, causal)  # equal weights, all exact
+
+
+@pytest.mark.parametrize("lens_q,lens_k", [([5] * 40, [390] * 40), ([300] * 60, [300] * 60)])
+@pytest.mark.parametrize("d", varlen.HEAD_DIMS)
+def test_many_huge_values(lens_q, lens_k, d):
+    """The same at every key (nothing is split here)."""
+    need_gpu()
+    say(f"varlen many huge values {lens_q[:2]} d={d}")
+    check_many_huge_values(lens_q, lens_k, d)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1e-3, 40.0])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_scales(scale, dtype):
