@@ -35,7 +35,7 @@ constexpr int kLRows = kLWaves * kLWaveRows;
 // Past this reference (log2 units) the scores are scaled in a pass of their own: a fused
 // multiply-add does not round their product with the scale, which the reference is made of.
 constexpr float kFusedMax = 1024.f;
-// P is relative to a reference per row, which moves where some row's maximum is more than kLag (log2
+// P is relative to a reference per row, which moves where the row's maximum is more than kLag (log2
 // units) past its last place; in bf16 it then goes kAbove over the maximum, so that P reaches
 // 2^(kLag - kAbove) at most.  The sums of 2^10 keys of such a weight and the largest finite V stay
 // within fp32, those of 2^16 of equal weights (a reference at the maximum made an infinity of a single
@@ -269,9 +269,11 @@ __device__ inline void weigh(RowState<T, D>& r, const unsigned char* kb, const L
   #pragma unroll
         for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[tt][i]);
       mx = max_xor32(mx) * scale_log2;
-      if (__ballot(mx > r.mref + (kLag - kAbove<T>)) != 0ull) {  // uniform
-        const float m_new = fmaxf(r.mref, mx + kAbove<T>);
-        const float alpha = m_new == ninf ? 1.f : __builtin_amdgcn_exp2f(r.mref - m_new);
+      // only the rows that are up move: a row's result does not depend on those beside it
+      const bool up = mx > r.mref + (kLag - kAbove<T>);
+      if (__ballot(up) != 0ull) {  // uniform
+        const float m_new = up ? mx + kAbove<T> : r.mref;
+        const float alpha = up ? __builtin_amdgcn_exp2f(r.mref - m_new) : 1.f;
         r.lsum *= alpha;
         r.mref = m_new;
   #pragma unroll
@@ -281,12 +283,14 @@ __device__ inline void weigh(RowState<T, D>& r, const unsigned char* kb, const L
       }
       const float nm = r.mref == ninf ? 0.f : -r.mref;
       float c = scale_log2;
-      if (__ballot(fabsf(nm) > kFusedMax) != 0ull) {  // uniform
+      const bool far = fabsf(nm) > kFusedMax;
+      if (__ballot(far) != 0ull) {  // uniform
+        const float by = far ? c : 1.f;
   #pragma unroll
         for (int tt = 0; tt < kSub; ++tt)
   #pragma unroll
-          for (int i = 0; i < 16; ++i) s[tt][i] *= c;
-        c = 1.f;
+          for (int i = 0; i < 16; ++i) s[tt][i] *= by;
+        c = far ? 1.f : c;
       }
           float ps = 0.f;
   #pragma unroll

@@ -227,6 +227,24 @@ def test_many_huge_values(lens_q, lens_k, d):
     check_many_huge_values(lens_q, lens_k, d)
 
 
+@pytest.mark.parametrize("gain", [5.0, 4000.0])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens_q,lens_k", SHAPES)
+@pytest.mark.parametrize("d", varlen.HEAD_DIMS)
+def test_a_row_does_not_depend_on_its_neighbours(d, lens_q, lens_k, dtype, gain):
+    """One token's query grows: every other row keeps its bits."""
+    need_gpu()
+    say(f"varlen neighbours {lens_q[:2]} d={d} {dtype} gain={gain}")
+    q, k, v, cq, ck = inputs(lens_q, lens_k, 8, 2, d, dtype, seed=d)
+    o, lse = call(q, k, v, cq, ck, True)
+    for t, h in ((0, 0), (2, 5)):
+        other = q.clone()
+        other[t, h] *= gain
+        o2, l2 = call(other, k, v, cq, ck, True)
+        o2[t, h], l2[h, t] = o[t, h], lse[h, t]
+        assert torch.equal(o, o2) and torch.equal(lse, l2)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1e-3, 40.0])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_scales(scale, dtype):
