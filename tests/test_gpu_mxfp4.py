@@ -270,6 +270,42 @@ def test_decode_range_of_values(dtype):
         check_decode(queries(1, 4, 64, dtype), cache, [64], torch.arange(4, dtype=torch.int32)[None])
 
 
+def huge_case(d):
+    """(cache, contexts, table, queries) for values of up to 1.5 * 2^127."""
+    bt = torch.randperm(100, generator=torch.Generator().manual_seed(6)).int()
+    return (new_cache(100, 2, 16, d, seed=3), [700, 33, 200],
+            torch.stack([bt[:44], bt[44:88], bt[56:100]]), queries(3, 16, d, torch.bfloat16, seed=d))
+
+
+@pytest.mark.parametrize("splits", [1, 5])
+@pytest.mark.parametrize("d", DIMS)
+def test_decode_huge_values(d, splits):
+    """One key's values of up to 1.5 * 2^127, of any weight: the sums of a row stay within fp32 where
+    its result does."""
+    need_gpu()
+    say(f"mxfp4 decode huge values d={d} splits={splits}")
+    cache, lens, bt, q = huge_case(d)
+    for i, at in enumerate((300, 31, 64)):
+        cache[3][bt[i, at // 16], :, at % 16] = 252
+    check_decode(q, cache, lens, bt, splits=splits)
+
+
+def check_many_huge_values(d, splits):
+    cache, lens, bt, q = huge_case(d)
+    cache[3].fill_(252)
+    check_decode(q, cache, lens, bt, splits=splits)
+    cache[2].fill_(0x77)  # 6 * 2^125 everywhere, of equal weights
+    check_decode(torch.zeros_like(q), cache, lens, bt, splits=splits)
+
+
+@pytest.mark.parametrize("d", DIMS)
+def test_decode_many_huge_values(d):
+    """The same at every key."""
+    need_gpu()
+    say(f"mxfp4 decode many huge values d={d}")
+    check_many_huge_values(d, 1)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.2, 30.0])
 def test_decode_scales_and_layouts(scale):
     """Any finite scale; queries and caches as slices of larger tensors, repeated blocks."""
