@@ -39,7 +39,7 @@ constexpr float kFusedMax = 1024.f;
 // units) past its last place; in bf16 it then goes kAbove over the maximum, so that P reaches
 // 2^(kLag - kAbove) at most.  The sums of 2^10 keys of such a weight and the largest finite V stay
 // within fp32, those of 2^16 of equal weights (a reference at the maximum made an infinity of a single
-// such V whose weight was past 1).  P ends at 2^-126, so weights below 2^-104 of the largest are 0.
+// such V whose weight was past 1).  P ends at 2^-126, so weights below 2^-110 of the largest are 0.
 // fp16 keeps 0: its P would lose bits below 2^-14, and its V is below 2^16.
 //
 // Between moves the accumulators are left alone, but the largest P is then no power of two, whose
