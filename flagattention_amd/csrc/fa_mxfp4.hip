@@ -265,7 +265,7 @@ int tokens_per_group(int64_t tokens) {
 constexpr int kWaves = 4;
 constexpr int kDTile = 32;
 constexpr int kDRows = 16;
-// P is relative to a reference per row, which moves where some row's maximum is more than kLag (log2
+// P is relative to a reference per row, which moves where the row's maximum is more than kLag (log2
 // units) past its last place.  From the first bf16 tile with a scale byte of kHuge on (values of
 // 6 * 2^97 and more) it lies kAbove over the maximum: P reaches 2^(kLag - kAbove) at most, and the sums
 // of 2^10 keys of such a weight and the largest V stay within fp32, those of 2^16 of equal weights (a
@@ -553,9 +553,11 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 4 : D == 128 ? 3 : 2) void m
       for (int i = 0; i < 4; ++i) tmax = fmaxf(tmax, s[h][i]);
     tmax = max_xor32(max_xor16(tmax)) * scale_log2;
     const float up_by = huge ? kAbove : above;  // uniform
-    if (__ballot(tmax + up_by > m_run + kLag) != 0ull || up_by != above) {  // uniform
-      const float m_new = fmaxf(m_run - above, tmax) + up_by;
-      const float alpha = m_new == ninf ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+    const bool up = tmax + up_by > m_run + kLag || up_by != above;
+    if (__ballot(up) != 0ull) {  // uniform
+      // only the rows that are up move: a row's result does not depend on those beside it
+      const float m_new = up ? fmaxf(m_run - above, tmax) + up_by : m_run;
+      const float alpha = !up || m_new == ninf ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
       above = up_by;
       l_run *= alpha;
@@ -567,12 +569,14 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 4 : D == 128 ? 3 : 2) void m
     const float nm = m_run == ninf ? 0.f : -m_run;
     float c = scale_log2;
     // a fused multiply-add does not round the product that a large reference is made of
-    if (__ballot(fabsf(nm) > 1024.f) != 0ull) {  // uniform
+    const bool far = fabsf(nm) > 1024.f;
+    if (__ballot(far) != 0ull) {  // uniform
+      const float by = far ? c : 1.f;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[h][i] *= c;
-      c = 1.f;
+        for (int i = 0; i < 4; ++i) s[h][i] *= by;
+      c = far ? 1.f : c;
     }
     float psum = 0.f;
     T8 pb;

@@ -306,6 +306,26 @@ def test_decode_many_huge_values(d):
     check_many_huge_values(d, 1)
 
 
+@pytest.mark.parametrize("gain", [5.0, 4000.0])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", DIMS)
+def test_decode_rows_do_not_depend_on_their_neighbours(d, dtype, gain):
+    """One head's query grows: every other head keeps its bits."""
+    need_gpu()
+    say(f"mxfp4 decode neighbours d={d} {dtype} gain={gain}")
+    cache = new_cache(60, 2, 32, d, seed=3)
+    bt = torch.randperm(60, generator=torch.Generator().manual_seed(6)).int().view(2, 30)
+    q = queries(2, 16, d, dtype, seed=d)
+    for splits in (1, 3):
+        o = run_decode(q, cache, [900, 451], bt, splits=splits)
+        for h in (0, 13):
+            other = q.clone()
+            other[0, h] *= gain
+            o2 = run_decode(other, cache, [900, 451], bt, splits=splits)
+            o2[0, h] = o[0, h]
+            assert torch.equal(o, o2)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.2, 30.0])
 def test_decode_scales_and_layouts(scale):
     """Any finite scale; queries and caches as slices of larger tensors, repeated blocks."""
