@@ -241,7 +241,7 @@ __global__ __launch_bounds__(kWThreads) void mxfp4_gather_kernel(
   }
 }
 
-constexpr int kMaxTokens = 1 << 28;  // a grid holds less than 2^32 lanes per dimension
+constexpr int kMaxTokens = (1 << 28) - kWTokens;  // a grid holds less than 2^32 lanes per dimension
 
 // Tokens per work-group of the two: fewer where they would not give every CU work.
 int tokens_per_group(int64_t tokens) {
@@ -797,6 +797,9 @@ int check_decode(const fa_mxfp4_decode_args* a) {
                "num_splits %d of %d tokens invalid", a->num_splits, a->split_tokens);
   FA_CHECK_ARG(a->num_splits == 1 || (a->o_part && a->lse_part),
                "num_splits %d > 1 needs o_part and lse_part", a->num_splits);
+  // the merge takes up to a work-group of 256 lanes for a row
+  FA_CHECK_ARG(a->num_splits == 1 || static_cast<int64_t>(a->batch) * a->h_q < (1 << 24),
+               "batch %d x h_q %d is 2^24 or more, too many rows for splits", a->batch, a->h_q);
   FA_CHECK_ARG(a->q && a->out && a->block_table && a->seqlens && a->max_blocks_per_seq >= 1,
                "NULL q / out / block_table / seqlens or no block per sequence");
   FA_CHECK_ARG(aligned(a->q, 16) && a->q_stride_b % 8 == 0 && a->q_stride_h % 8 == 0,
@@ -831,7 +834,7 @@ extern "C" int fa_mxfp4_cache_write(const fa_mxfp4_cache* cache, const void* key
                "key / value rows must be 16-byte aligned");
   FA_CHECK_ARG(static_cast<int64_t>(num_tokens) * cache->h_kv <= INT32_MAX,
                "num_tokens %d x h_kv %d is 2^31 or more", num_tokens, cache->h_kv);
-  FA_CHECK_ARG(num_tokens < fa::kMaxTokens, "num_tokens %d is 2^28 or more", num_tokens);
+  FA_CHECK_ARG(num_tokens <= fa::kMaxTokens, "num_tokens %d is more than 2^28 - 16", num_tokens);
   const int tokens = fa::tokens_per_group(num_tokens);
   const dim3 grid(static_cast<unsigned>(fa::cdiv(num_tokens, tokens)), 2);
   const hipStream_t s = static_cast<hipStream_t>(stream);
@@ -864,7 +867,8 @@ extern "C" int fa_mxfp4_gather(const fa_mxfp4_cache* cache, const int32_t* block
   FA_CHECK_ARG(fa::aligned(k_out, 16) && fa::aligned(v_out, 16), "outputs must be 16-byte aligned");
   FA_CHECK_ARG(static_cast<int64_t>(total) * cache->h_kv <= INT32_MAX,
                "total %d x h_kv %d is 2^31 or more", total, cache->h_kv);
-  FA_CHECK_ARG(total < fa::kMaxTokens, "total %d is 2^28 or more", total);
+  FA_CHECK_ARG(total <= fa::kMaxTokens, "total %d is more than 2^28 - 16", total);
+  FA_CHECK_ARG(num_seqs <= fa::kMaxTokens, "num_seqs %d is more than 2^28 - 16", num_seqs);
   const int tokens = fa::tokens_per_group(total);
   const dim3 grid(static_cast<unsigned>(fa::cdiv(total, tokens)), 2);
   const hipStream_t s = static_cast<hipStream_t>(stream);

@@ -817,7 +817,7 @@ __global__ __launch_bounds__(256) void merge_kernel(const fa_varlen_args a) {
   }
   const bool seen = !(l == 0.f);  // else no visible key: out 0, lse -inf (NaN stays NaN)
   const float inv = seen ? 1.f / l : 0.f;
-  const int h = static_cast<int>(row) / a.total_q;  // below 2^26 (host check)
+  const int h = static_cast<int>(row) / a.total_q;  // at most 2^26 - 4 (host check)
   const int pos = static_cast<int>(row) - h * a.total_q;
   if (sub == 0) {
     T4 w;
@@ -944,7 +944,7 @@ int check_varlen(const fa_varlen_args* a) {
                "num_splits %d of %d tokens invalid", a->num_splits, a->split_tokens);
   FA_CHECK_ARG(a->num_splits == 1 || (a->o_part && a->lse_part),
                "num_splits %d > 1 needs o_part and lse_part", a->num_splits);
-  FA_CHECK_ARG(a->num_splits == 1 || static_cast<long long>(a->h_q) * a->total_q < (1 << 26),
+  FA_CHECK_ARG(a->num_splits == 1 || static_cast<long long>(a->h_q) * a->total_q <= (1 << 26) - 4,
                "too many query rows for splits");
   return FA_OK;
 }

@@ -171,6 +171,41 @@ def test_struct_mirrors_and_c_abi_refusals():
     refused(lib.fa_mxfp4_combine(ctypes.byref(_lib.Mxfp4DecodeArgs(**decode)), None), b"o_part")
 
 
+def test_grids_of_2_32_lanes_are_refused():
+    """The largest sizes under each limit, one past it: a launch of 2^24 work-groups of 256 lanes has
+    one lane too many for its counters."""
+    lib = _lib.load()
+
+    def refused(rc, text):
+        assert rc == -1 and text in lib.fa_last_error(), (rc, lib.fa_last_error())
+
+    cache = _lib.Mxfp4Cache(k_codes=4096, k_scales=4096, v_codes=4096, v_scales=4096, code_stride_0=512,
+                            code_stride_h=512, code_stride_t=32, scale_stride_0=32, scale_stride_h=32,
+                            scale_stride_t=2, num_blocks=4, block_size=16, h_kv=1, d=64)
+    for n in ((1 << 28) - 15, (1 << 28) - 1):
+        refused(lib.fa_mxfp4_cache_write(ctypes.byref(cache), 4096, 64, 64, 4096, 64, 64, 4096, 1, n, 0,
+                                         None), b"2^28 - 16")
+        refused(lib.fa_mxfp4_gather(ctypes.byref(cache), 4096, 1, 1, 4096, 1, n, 4096, 4096, 0, None),
+                b"2^28 - 16")
+        refused(lib.fa_mxfp4_gather(ctypes.byref(cache), 4096, 1, 1, 4096, n, 1, 4096, 4096, 0, None),
+                b"2^28 - 16")
+    varlen_args = dict(q=4096, k=4096, v=4096, out=4096, cu_seqlens_q=4096, cu_seqlens_k=4096,
+                       num_seqs=1, total_k=4, h_q=1, h_kv=1, d=64, num_splits=2, split_tokens=64,
+                       q_stride_t=64, q_stride_h=64, k_stride_t=64, k_stride_h=64, v_stride_t=64,
+                       v_stride_h=64, o_stride_t=64, o_stride_h=64, o_part=4096, lse_part=4096)
+    for n in ((1 << 26) - 3, (1 << 26) - 1):
+        args = _lib.VarlenArgs(**varlen_args, total_q=n)
+        refused(lib.fa_varlen_attention(ctypes.byref(args), None), b"too many query rows")
+        refused(lib.fa_varlen_combine(ctypes.byref(args), None), b"too many query rows")
+    for batch, h_q in ((1 << 14, 1 << 10), (4097, 4096)):
+        args = _lib.Mxfp4DecodeArgs(cache=cache, q=4096, out=4096, block_table=4096, seqlens=4096,
+                                    max_blocks_per_seq=1, batch=batch, h_q=h_q, num_splits=2,
+                                    split_tokens=32, q_stride_b=64, q_stride_h=64, o_part=4096,
+                                    lse_part=4096)
+        refused(lib.fa_mxfp4_decode(ctypes.byref(args), None), b"too many rows for splits")
+        refused(lib.fa_mxfp4_combine(ctypes.byref(args), None), b"too many rows for splits")
+
+
 def test_oracle_formats():
     """The oracle's writer keeps what a code can say exactly, and is never off by more than half of
     the widest step, which is the scale itself."""
