@@ -914,6 +914,8 @@ int check_varlen(const fa_varlen_args* a) {
   FA_CHECK_ARG(a != nullptr, "args is NULL");
   FA_CHECK_ARG(a->num_seqs >= 0 && a->total_q >= 1 && a->total_k >= 0,
                "num_seqs %d / total_q %d / total_k %d invalid", a->num_seqs, a->total_q, a->total_k);
+  // positions of the tile after the last one stay in 32 bits
+  FA_CHECK_ARG(a->total_k <= INT32_MAX - 256, "total_k %d is more than 2^31 - 257", a->total_k);
   FA_CHECK_ARG(a->h_q >= 1 && a->h_kv >= 1 && a->h_q % a->h_kv == 0,
                "h_q %d is not a multiple of h_kv %d", a->h_q, a->h_kv);
   FA_CHECK_ARG(a->d == 64 || a->d == 128 || a->d == 256, "head dim %d not in {64, 128, 256}", a->d);

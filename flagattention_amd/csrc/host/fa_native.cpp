@@ -657,7 +657,7 @@ PyObject* varlen(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (total_q < 1 || total_k < 1 || !packed_dim(d) || k->size(2) != d || h_kv < 1 || h_q < 1 ||
       h_q % h_kv != 0 || !gqa_dtype(*q) || k->scalar_type() != q->scalar_type() ||
       v->scalar_type() != q->scalar_type() || !std::isfinite(scale) ||
-      total_q * (h_q / h_kv) >= (int64_t{1} << 30) || total_k >= (int64_t{1} << 31))
+      total_q * (h_q / h_kv) >= (int64_t{1} << 30) || total_k > INT32_MAX - 256)
     return none();
   constexpr int64_t kMaxStride = int64_t{1} << 23;
   if (q->stride(2) != 1 || k->stride(2) != 1 || v->stride(2) != 1 || !rows16(*q, 2) ||

@@ -76,7 +76,8 @@ def flash_attention_varlen(
     _require(isinstance(max_seqlen_q, int) and isinstance(max_seqlen_k, int)
              and max_seqlen_q >= 0 and max_seqlen_k >= 0,
              "max_seqlen_q and max_seqlen_k must be ints >= 0")
-    _require(total_q * (h_q // h_kv) < 1 << 30 and total_k < 1 << 31, "too many tokens")
+    _require(total_q * (h_q // h_kv) < 1 << 30 and total_k <= (1 << 31) - 257,
+             "too many tokens")
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(d)
     _require(math.isfinite(sm_scale), "sm_scale must be finite")

@@ -206,6 +206,21 @@ def test_grids_of_2_32_lanes_are_refused():
         refused(lib.fa_mxfp4_combine(ctypes.byref(args), None), b"too many rows for splits")
 
 
+@pytest.mark.parametrize("n", [2 ** 31 - 256, 2 ** 31 - 1])
+def test_key_positions_stay_in_32_bits(n):
+    """Packed keys may be one row seen many times (stride 0), so their count is bounded by its own
+    check, not by memory: the walk over them adds up to 128 to the last position."""
+    args = _lib.VarlenArgs(q=4096, k=4096, v=4096, out=4096, cu_seqlens_q=4096, cu_seqlens_k=4096,
+                           num_seqs=1, total_q=1, total_k=n, h_q=1, h_kv=1, d=64, num_splits=1,
+                           split_tokens=1, q_stride_t=64, q_stride_h=64, o_stride_t=64, o_stride_h=64)
+    lib = _lib.load()
+    assert lib.fa_varlen_attention(ctypes.byref(args), None) == -1 and b"total_k" in lib.fa_last_error()
+    a = _varlen()
+    a.update({x: a[x][:1].expand(n, 2, 64) for x in "kv"})
+    with pytest.raises(ArgumentError, match="too many tokens"):
+        flag_attn.flash_attention_varlen(**a)
+
+
 def test_oracle_formats():
     """The oracle's writer keeps what a code can say exactly, and is never off by more than half of
     the widest step, which is the scale itself."""
