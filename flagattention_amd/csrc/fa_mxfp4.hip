@@ -7,6 +7,7 @@
 // so a code depends on nothing but the value.
 #include "fa_common.h"
 #include "fa_divide.h"
+#include "fa_merge.h"
 #include "fa_wave.h"
 #include "flagattention_amd_packed.h"
 
@@ -913,20 +914,16 @@ extern "C" int fa_mxfp4_combine(const fa_mxfp4_decode_args* a, void* stream) {
   const int rc = fa::check_decode(a);
   if (rc != FA_OK) return rc;
   FA_CHECK_ARG(a->o_part && a->lse_part, "combine needs o_part and lse_part");
-  fa_gqa_decode_args g = {};  // the merge reads the partial rows alone
-  g.q = g.k = g.v = a->q;
-  g.out = a->out;
-  g.o_stride_b = a->o_stride_b;
-  g.o_stride_h = a->o_stride_h;
-  g.o_part = a->o_part;
-  g.lse_part = a->lse_part;
-  g.batch = a->batch;
-  g.h_q = a->h_q;
-  g.h_kv = a->cache.h_kv;
-  g.m = 1;
-  g.d = a->cache.d;
-  g.num_splits = a->num_splits;
-  g.split_tokens = a->split_tokens;
-  g.dtype = a->dtype;
-  return fa_gqa_combine(&g, stream);
+  FA_CHECK_ARG(static_cast<int64_t>(a->batch) * a->h_q < (1 << 24),
+               "batch %d x h_q %d is 2^24 or more, too many rows for splits", a->batch, a->h_q);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const fa::MergeArgs m{a->o_part, a->lse_part, a->out, nullptr, a->o_stride_b, a->o_stride_h,
+                        static_cast<int>(static_cast<int64_t>(a->batch) * a->h_q), a->h_q,
+                        a->num_splits};
+  if (a->dtype == 1)
+    fa::launch_merge<__bf16>(m, a->cache.d, s);
+  else
+    fa::launch_merge<_Float16>(m, a->cache.d, s);
+  FA_CHECK_HIP(hipGetLastError());
+  return FA_OK;
 }

@@ -21,6 +21,7 @@
 
 #include "fa_common.h"
 #include "fa_divide.h"
+#include "fa_merge.h"
 #include "fa_rows_tile.h"
 #include "fa_wave.h"
 #include "flagattention_amd_packed.h"
@@ -768,67 +769,6 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
     }
 }
 
-// Merge of the splits' partial rows: lse = logsumexp_s lse_s, out = sum_s exp(lse_s - lse) o_s, a
-// wave per row.  A split without a visible key holds lse -inf and no values; one with a NaN holds
-// lse +inf, whose weight is NaN.  Bound by the bytes of the partial rows.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void merge_kernel(const fa_varlen_args a) {
-  typedef typename PVec<T>::v4 T4;
-  constexpr int kLanes = D / 4, kPar = 64 / kLanes;  // lanes per split, splits side by side
-  constexpr int kBatch = 4;
-  const long long row = static_cast<long long>(blockIdx.x) * 4 + wave_id();
-  if (row >= static_cast<long long>(a.h_q) * a.total_q) return;  // whole waves
-  const int lane = threadIdx.x & 63, sub = lane / kLanes, d4 = lane % kLanes;
-  const int S = a.num_splits;
-  const float ninf = -__builtin_inff();
-  const float* const lp = a.lse_part + row * S;
-  const float* const op = a.o_part + row * S * D + 4 * d4;
-  float m = ninf;
-  for (int s = lane; s < S; s += 64) m = fmaxf(m, lp[s]);
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
-  float l = 0.f;
-  floatx4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int base = 0; base < S; base += 64) {
-    const float mine = base + lane < S ? lp[base + lane] : ninf;
-    const float weight = mine == ninf ? 0.f : expf(mine - m);
-    l += weight;
-    const unsigned long long some = __ballot(mine != ninf);
-    for (int s0 = 0; s0 < 64 && base + s0 < S; s0 += kPar * kBatch) {
-      floatx4 o[kBatch];
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int s = s0 + kPar * i + sub;  // below 64
-        o[i] = floatx4{0.f, 0.f, 0.f, 0.f};
-        if ((some >> s) & 1)
-          o[i] = *reinterpret_cast<const floatx4*>(op + static_cast<long long>(base + s) * D);
-      }
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) acc += __shfl(weight, s0 + kPar * i + sub) * o[i];
-    }
-  }
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) {
-    l += __shfl_xor(l, off);
-    if (off >= kLanes) {
-#pragma unroll
-      for (int x = 0; x < 4; ++x) acc[x] += __shfl_xor(acc[x], off);
-    }
-  }
-  const bool seen = !(l == 0.f);  // else no visible key: out 0, lse -inf (NaN stays NaN)
-  const float inv = seen ? 1.f / l : 0.f;
-  const int h = static_cast<int>(row) / a.total_q;  // at most 2^26 - 4 (host check)
-  const int pos = static_cast<int>(row) - h * a.total_q;
-  if (sub == 0) {
-    T4 w;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) w[x] = static_cast<T>(acc[x] * inv);
-    *reinterpret_cast<T4*>(static_cast<T*>(a.out) + pos * a.o_stride_t + h * a.o_stride_h +
-                           4 * d4) = w;
-  }
-  if (lane == 0 && a.lse) a.lse[row] = seen ? m + logf(l) : ninf;
-}
-
 // Row blocks per KV head at most: each sequence, and the rows behind the last and before the
 // first, rounds up once.
 long long row_blocks(const fa_varlen_args* a) {
@@ -852,17 +792,6 @@ void launch_varlen(const fa_varlen_args* a, hipStream_t stream) {
     hipLaunchKernelGGL((varlen_kernel<T, 128>), grid, dim3(kLThreads), 0, stream, *a, plan);
   else
     hipLaunchKernelGGL((varlen_kernel<T, 256>), grid, dim3(kLThreads), 0, stream, *a, plan);
-}
-
-template <typename T>
-void launch_merge(const fa_varlen_args* a, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>((static_cast<long long>(a->h_q) * a->total_q + 3) / 4));
-  if (a->d == 64)
-    hipLaunchKernelGGL((merge_kernel<T, 64>), grid, dim3(256), 0, stream, *a);
-  else if (a->d == 128)
-    hipLaunchKernelGGL((merge_kernel<T, 128>), grid, dim3(256), 0, stream, *a);
-  else
-    hipLaunchKernelGGL((merge_kernel<T, 256>), grid, dim3(256), 0, stream, *a);
 }
 
 // Splits along the keys: the cheapest by a model of the launch, in us.  A work-group takes `step`
@@ -946,7 +875,8 @@ int check_varlen(const fa_varlen_args* a) {
                "num_splits %d of %d tokens invalid", a->num_splits, a->split_tokens);
   FA_CHECK_ARG(a->num_splits == 1 || (a->o_part && a->lse_part),
                "num_splits %d > 1 needs o_part and lse_part", a->num_splits);
-  FA_CHECK_ARG(a->num_splits == 1 || static_cast<long long>(a->h_q) * a->total_q <= (1 << 26) - 4,
+  FA_CHECK_ARG(a->num_splits == 1 ||
+                   static_cast<long long>(a->h_q) * a->total_q <= max_merge_rows(a->num_splits),
                "too many query rows for splits");
   return FA_OK;
 }
@@ -988,11 +918,16 @@ extern "C" int fa_varlen_combine(const fa_varlen_args* a, void* stream) {
   const int rc = fa::check_varlen(a);
   if (rc != FA_OK) return rc;
   FA_CHECK_ARG(a->o_part && a->lse_part, "combine needs o_part and lse_part");
+  FA_CHECK_ARG(static_cast<int64_t>(a->h_q) * a->total_q <= fa::max_merge_rows(a->num_splits),
+               "too many query rows for splits");
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  const fa::MergeArgs m{a->o_part, a->lse_part, a->out, a->lse, a->o_stride_h, a->o_stride_t,
+                        static_cast<int>(static_cast<int64_t>(a->h_q) * a->total_q), a->total_q,
+                        a->num_splits};
   if (a->dtype == 1)
-    fa::launch_merge<__bf16>(a, s);
+    fa::launch_merge<__bf16>(m, a->d, s);
   else
-    fa::launch_merge<_Float16>(a, s);
+    fa::launch_merge<_Float16>(m, a->d, s);
   FA_CHECK_HIP(hipGetLastError());
   return FA_OK;
 }

@@ -306,6 +306,15 @@ def test_decode_many_huge_values(d):
     check_many_huge_values(d, 1)
 
 
+@pytest.mark.parametrize("splits", [5, 40])
+@pytest.mark.parametrize("d", DIMS)
+def test_decode_many_huge_values_in_splits(d, splits):
+    """The same where the keys are split: the merge's sums stay within fp32 too."""
+    need_gpu()
+    say(f"mxfp4 decode many huge values d={d} splits={splits}")
+    check_many_huge_values(d, splits)
+
+
 @pytest.mark.parametrize("gain", [5.0, 4000.0])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("d", DIMS)

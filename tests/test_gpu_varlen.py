@@ -90,6 +90,18 @@ def test_split_keys(lens_q, lens_k, d, causal):
     check(*inputs(lens_q, lens_k, 4, 2, d, torch.bfloat16, seed=9), causal)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d", varlen.HEAD_DIMS)
+def test_split_keys_of_many_rows(d, causal):
+    """More rows than the merge requests ahead, many without a key in the later splits."""
+    need_gpu()
+    say(f"varlen splits of many rows d={d} causal={causal}")
+    cu = torch.cuda.get_device_properties(0).multi_processor_count
+    assert varlen_splits(1110, 2500, 2, 8, 1, d, causal, 1100, 2490, cu)[0] > 1
+    q, k, v, cq, ck = inputs([10, 1100], [10, 2490], 8, 1, d, torch.float16, seed=13)
+    check(q, k, v, cq, ck, causal)
+
+
 @pytest.mark.parametrize("max_k", [1, 700, 5000])
 def test_length_bounds_do_not_choose_the_result(max_k):
     need_gpu()
@@ -224,6 +236,16 @@ def test_many_huge_values(lens_q, lens_k, d):
     """The same at every key (nothing is split here)."""
     need_gpu()
     say(f"varlen many huge values {lens_q[:2]} d={d}")
+    check_many_huge_values(lens_q, lens_k, d)
+
+
+@pytest.mark.parametrize("lens_q,lens_k", [SHAPES[0], SHAPES[2], ([1], [70000])])
+@pytest.mark.parametrize("d", varlen.HEAD_DIMS)
+def test_many_huge_values_in_splits(lens_q, lens_k, d):
+    """The same where the keys are split, but for some of the first: the merge's sums stay within fp32
+    too."""
+    need_gpu()
+    say(f"varlen many huge values {lens_q[:2]} d={d} in splits")
     check_many_huge_values(lens_q, lens_k, d)
 
 
