@@ -84,11 +84,12 @@ def flash_attention_varlen(
     _require(all(t.is_cuda and t.device == q.device for t in (q, k, v, cu_seqlens_q,
                                                               cu_seqlens_k)),
              "all tensors must be CUDA (HIP) tensors on one device")
-    q, k, v = (t if t.stride(-1) == 1 and _aligned(t, (0, 1)) else t.contiguous()
-               for t in (q, k, v))
-    # 32-bit offsets inside a tile of keys and inside a block of rows (and its heads)
-    q, k, v = (t if t.stride(0) < 1 << 23 and h_q // h_kv * t.stride(1) < 1 << 29 else t.contiguous()
-               for t in (q, k, v))
+    # rows that the kernel cannot read as they lie are copied: past 32-bit offsets inside a tile of
+    # keys and inside a block of rows (and its heads), or not 16-byte aligned (`contiguous` would keep
+    # a misaligned base, and any stride of a dimension of one)
+    q, k, v = (t if t.stride(2) == 1 and _aligned(t, (0, 1)) and t.stride(0) < 1 << 23
+               and h_q // h_kv * t.stride(1) < 1 << 29
+               else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
     device = q.device
     o = torch.empty((total_q, h_q, d), dtype=q.dtype, device=device)
     lse = (torch.empty((h_q, total_q), dtype=torch.float32, device=device)

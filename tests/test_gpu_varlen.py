@@ -296,6 +296,34 @@ def test_strided_inputs():
     check(fused[:, :4].half(), one, wide, cu, cu, True)
 
 
+def off_base(t):
+    """t's values in a contiguous tensor whose base is not 16-byte aligned."""
+    out = torch.empty(t.numel() + 1, dtype=t.dtype, device=DEV)[1:].view(t.shape)
+    assert out.is_contiguous() and out.data_ptr() % 16 == 2
+    return out.copy_(t)
+
+
+@pytest.mark.parametrize("d", varlen.HEAD_DIMS)
+def test_contiguous_rows_off_the_alignment(d):
+    """A misaligned base, and strides of dimensions of one that no row needs: the same result."""
+    need_gpu()
+    say(f"varlen off the alignment d={d}")
+    q, k, v, cq, ck = inputs([70, 1], [70, 300], 4, 2, d, torch.bfloat16, seed=3)
+    want = check(q, k, v, cq, ck, True)
+    for args in ((off_base(q), k, v), (q, off_base(k), v), (q, k, off_base(v)),
+                 (off_base(q), off_base(k), off_base(v))):
+        assert all(torch.equal(x, y) for x, y in zip(call(*args, cq, ck, True), want))
+    one = inputs([1], [1], 1, 1, d, torch.float16, seed=4)
+    want = check(*one, False)
+    for strides in ((132, d, 1), (d, 132, 1), (1 << 24, 1 << 30, 1)):
+        views = [t.as_strided((1, 1, d), strides) for t in one[:3]]
+        assert all(torch.equal(x, y) for x, y in zip(call(*views, *one[3:], False), want))
+    q, k, v, cq, ck = inputs([1], [1], 4, 2, d, torch.float16, seed=5)
+    want = check(q, k, v, cq, ck, False)
+    views = [t.as_strided(t.shape, (1 << 24, d, 1)) for t in (q, k, v)]
+    assert all(torch.equal(x, y) for x, y in zip(call(*views, cq, ck, False), want))
+
+
 def test_equals_the_rectangular_operator_where_both_apply():
     """Sequences of one length: the same rows as flash_attention, within both tolerances."""
     need_gpu()
