@@ -111,8 +111,9 @@ def cache_kv_mxfp4(
              "all tensors must be CUDA (HIP) tensors on one device")
     if t == 0:
         return
-    key, value = (x if x.stride(2) == 1 and _aligned(x, (0, 1)) else x.contiguous()
-                  for x in (key, value))
+    # not 16-byte aligned rows are copied (`contiguous` would keep a misaligned base)
+    key, value = (x if x.stride(2) == 1 and _aligned(x, (0, 1))
+                  else x.clone(memory_format=torch.contiguous_format) for x in (key, value))
     slots = slot_mapping.contiguous()
     args = _cache_args(key_cache, key_scales, value_cache, value_scales)
     lib = _lib.load()

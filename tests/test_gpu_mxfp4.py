@@ -91,6 +91,34 @@ def test_write_odd_values_and_layouts(dtype):
     assert all(torch.equal(y.cpu(), w) for y, w in zip(again, want))
 
 
+@pytest.mark.parametrize("t,hk", [(20, 2), (1, 2), (1, 1)])
+@pytest.mark.parametrize("d", DIMS)
+def test_write_contiguous_rows_off_the_alignment(d, t, hk):
+    """A misaligned base, and strides of dimensions of one that no row needs."""
+    need_gpu()
+    say(f"mxfp4 write off the alignment d={d} t={t} hk={hk}")
+    x = queries(t, hk, d, torch.bfloat16, seed=d)
+    slots = torch.arange(5, 5 + t, device=DEV)
+
+    def written(k, v):
+        cache = new_cache(2, hk, 16, d)
+        flag_attn.cache_kv_mxfp4(k, v, *cache, slots)
+        return cache
+
+    want = new_cache(2, hk, 16, d)
+    want = [*po.write(want[0], want[1], x, slots), *po.write(want[2], want[3], x, slots)]
+    off = torch.empty(x.numel() + 1, dtype=x.dtype, device=DEV)[1:].view(x.shape).copy_(x)
+    assert off.is_contiguous() and off.data_ptr() % 16 == 2
+    views = [off]
+    if t == 1:
+        views.append(x.as_strided(x.shape, (x.numel() + 3, d, 1)))
+    if t == hk == 1:
+        views.append(x.as_strided(x.shape, (d, d + 3, 1)))
+    for y in views:
+        for k, v in ((y, x), (x, y), (y, y)):
+            assert all(torch.equal(a, b) for a, b in zip(written(k, v), want))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("d", DIMS)
 @pytest.mark.parametrize("block", [16, 32, 128])
