@@ -27,7 +27,7 @@ HEAD_DIMS = (64, 128, 256)
 GROUP = 32
 
 
-def _check_cache(key_cache, key_scales, value_cache, value_scales, device):
+def _check_cache(key_cache, key_scales, value_cache, value_scales):
     """(num_blocks, h_kv, block_size, d) of a cache."""
     _require(key_cache.dim() == 4 and value_cache.shape == key_cache.shape,
              "key_cache / value_cache must be [num_blocks, num_kv_heads, block_size, head_size / 2]")
@@ -56,9 +56,12 @@ def _check_cache(key_cache, key_scales, value_cache, value_scales, device):
              f"{scale_align}-byte aligned")
     _require(key_cache.stride(2) < 1 << 27 and key_scales.stride(2) < 1 << 27,
              "the cache's rows are too far apart")
-    _require(all(t.is_cuda and t.device == device for t in tensors),
-             "all tensors must be CUDA (HIP) tensors on one device")
     return num_blocks, h_kv, block_size, d
+
+
+def _check_device(*tensors):
+    _require(all(t.is_cuda and t.device == tensors[0].device for t in tensors),
+             "all tensors must be CUDA (HIP) tensors on one device")
 
 
 def _cache_args(key_cache, key_scales, value_cache, value_scales) -> "_lib.Mxfp4Cache":
@@ -100,15 +103,14 @@ def cache_kv_mxfp4(
              "key / value must be [num_tokens, num_kv_heads, head_size]")
     code = _dtype_code(key.dtype)
     _require(value.dtype == key.dtype, "key / value dtypes differ")
-    _, h_kv, _, d = _check_cache(key_cache, key_scales, value_cache, value_scales, key.device)
+    _, h_kv, _, d = _check_cache(key_cache, key_scales, value_cache, value_scales)
     t = key.shape[0]
     _require(tuple(key.shape[1:]) == (h_kv, d), "key / value heads or head size differ from the cache's")
     _require(slot_mapping.dim() == 1 and slot_mapping.shape[0] == t
              and slot_mapping.dtype in (torch.int32, torch.int64),
              "slot_mapping must be int32 / int64 [num_tokens]")
     _require(t * h_kv < 1 << 31 and t < 1 << 28, "too many tokens")
-    _require(all(x.is_cuda and x.device == key.device for x in (key, value, slot_mapping)),
-             "all tensors must be CUDA (HIP) tensors on one device")
+    _check_device(key, value, key_cache, key_scales, value_cache, value_scales, slot_mapping)
     if t == 0:
         return
     # not 16-byte aligned rows are copied (`contiguous` would keep a misaligned base)
@@ -154,7 +156,7 @@ def gather_kv_mxfp4(
             return done
     code = _dtype_code(dtype)
     device = key_cache.device
-    _, h_kv, _, d = _check_cache(key_cache, key_scales, value_cache, value_scales, device)
+    _, h_kv, _, d = _check_cache(key_cache, key_scales, value_cache, value_scales)
     _require(cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.shape[0] >= 1
              and cu_seqlens.is_contiguous(), "cu_seqlens must be contiguous int32 [num_seqs + 1]")
     num_seqs = cu_seqlens.shape[0] - 1
@@ -163,8 +165,7 @@ def gather_kv_mxfp4(
              "block_tables must be int32 [num_seqs, max_num_blocks_per_seq]")
     _require(isinstance(total_tokens, int) and total_tokens >= 0, "total_tokens must be an int >= 0")
     _require(total_tokens * h_kv < 1 << 31 and total_tokens < 1 << 28, "too many tokens")
-    _require(all(x.is_cuda and x.device == device for x in (block_tables, cu_seqlens)),
-             "all tensors must be CUDA (HIP) tensors on one device")
+    _check_device(key_cache, key_scales, value_cache, value_scales, block_tables, cu_seqlens)
     k = torch.empty((total_tokens, h_kv, d), dtype=dtype, device=device)
     v = torch.empty_like(k)
     if total_tokens > 0:
@@ -212,7 +213,7 @@ def paged_attention_mxfp4(
     num_seqs, h_q, d = query.shape
     code = _dtype_code(query.dtype)
     device = query.device
-    _, h_kv, _, d_k = _check_cache(key_cache, key_scales, value_cache, value_scales, device)
+    _, h_kv, _, d_k = _check_cache(key_cache, key_scales, value_cache, value_scales)
     _require(d == d_k, f"query head_size {d} != cache head_size {d_k}")
     _require(h_q >= 1 and h_q % h_kv == 0, "num_heads must be a multiple of num_kv_heads")
     _require(query.stride(2) == 1 and _aligned(query, (0, 1)), "query rows must be 16-byte aligned")
@@ -224,8 +225,7 @@ def paged_attention_mxfp4(
     _require(num_splits >= 0, "num_splits must be >= 0")
     _require(1 <= max_context_len <= 1 << 30, "max_context_len must be in [1, 2^30]")
     _require(math.isfinite(attn_scale), "attn_scale must be finite")
-    _require(all(t.is_cuda and t.device == device for t in (query, context_lens, block_tables)),
-             "all tensors must be CUDA (HIP) tensors on one device")
+    _check_device(query, key_cache, key_scales, value_cache, value_scales, context_lens, block_tables)
     out = torch.empty((num_seqs, h_q, d), dtype=query.dtype, device=device)
     if num_seqs == 0:
         return out

@@ -107,6 +107,88 @@ def test_write_rejects(kw, msg):
         flag_attn.cache_kv_mxfp4(**args)
 
 
+def _write_args(**kw):
+    return {**dict(key=torch.zeros((3, 2, 64)).half(), value=torch.zeros((3, 2, 64)).half(), **_cache(),
+                   slot_mapping=torch.zeros(3, dtype=torch.int64)), **kw}
+
+
+def _half(*shape):
+    return torch.zeros(shape, dtype=torch.float16)
+
+
+def _i32(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(key=_half(3, 4, 64), value=_half(3, 4, 64)), "heads or head size differ"),
+    (dict(key=_half(3, 2, 128), value=_half(3, 2, 128)), "heads or head size differ"),
+    (dict(slot_mapping=torch.zeros(2, dtype=torch.int64)), "slot_mapping must be"),
+    (dict(slot_mapping=torch.zeros(4, dtype=torch.int32)), "slot_mapping must be"),
+    (dict(slot_mapping=torch.zeros((3, 1), dtype=torch.int32)), "slot_mapping must be"),
+    (dict(slot_mapping=torch.zeros(3)), "slot_mapping must be"),
+    (dict(slot_mapping=torch.zeros(3, dtype=torch.int16)), "slot_mapping must be"),
+    (dict(), "CUDA"),  # valid, but CPU tensors
+])
+def test_write_names_its_own_fault(kw, msg):
+    with pytest.raises(ArgumentError, match=msg):
+        flag_attn.cache_kv_mxfp4(**_write_args(**kw))
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(dtype=torch.float32), "float16 / bfloat16"),
+    (dict(cu_seqlens=torch.zeros(3, dtype=torch.int64)), "cu_seqlens must be"),
+    (dict(cu_seqlens=_i32(3, 1)), "cu_seqlens must be"),
+    (dict(cu_seqlens=_i32(0)), "cu_seqlens must be"),
+    (dict(cu_seqlens=_i32(6)[::2]), "cu_seqlens must be"),
+    (dict(block_tables=torch.zeros((2, 4), dtype=torch.int64)), "block_tables must be"),
+    (dict(block_tables=_i32(8)), "block_tables must be"),
+    (dict(block_tables=_i32(3, 4)), "block_tables must be"),
+    (dict(block_tables=_i32(1, 4)), "block_tables must be"),
+    (dict(block_tables=_i32(4, 2).t()), "block_tables must be"),
+    (dict(total_tokens=-1), "total_tokens must be"),
+    (dict(total_tokens=5.0), "total_tokens must be"),
+    (dict(total_tokens=1 << 28), "too many tokens"),
+    (dict(), "CUDA"),
+])
+def test_gather_names_its_own_fault(kw, msg):
+    args = {**dict(**_cache(), block_tables=_i32(2, 4), cu_seqlens=_i32(3), total_tokens=5,
+                   dtype=torch.float16), **kw}
+    with pytest.raises(ArgumentError, match=msg):
+        flag_attn.gather_kv_mxfp4(**args)
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(query=_half(2, 64)), "query must be"),
+    (dict(query=torch.zeros((2, 4, 64))), "float16 / bfloat16"),
+    (dict(query=_half(2, 4, 128)), "head_size 128"),
+    (dict(query=_half(2, 3, 64)), "multiple"),
+    (dict(query=_half(2, 0, 64)), "multiple"),
+    (dict(query=_half(2, 4, 65)[..., 1:]), "16-byte aligned"),
+    (dict(query=_half(513)[1:].view(2, 4, 64)), "16-byte aligned"),
+    (dict(query=_half(2, 64, 4).transpose(1, 2)), "16-byte aligned"),
+    (dict(context_lens=_i32(3)), "context_lens must be"),
+    (dict(context_lens=_i32(2, 1)), "context_lens must be"),
+    (dict(context_lens=_i32(4)[::2]), "context_lens must be"),
+    (dict(context_lens=torch.zeros(2, dtype=torch.int64)), "context_lens must be"),
+    (dict(block_tables=_i32(3, 4)), "block_tables must be"),
+    (dict(block_tables=_i32(8)), "block_tables must be"),
+    (dict(block_tables=torch.zeros((2, 4), dtype=torch.int64)), "block_tables must be"),
+    (dict(block_tables=_i32(4, 2).t()), "block_tables must be"),
+    (dict(num_splits=-1), "num_splits must be"),
+    (dict(max_context_len=0), "max_context_len must be"),
+    (dict(max_context_len=(1 << 30) + 1), "max_context_len must be"),
+    (dict(attn_scale=math.nan), "attn_scale must be"),
+    (dict(attn_scale=-math.inf), "attn_scale must be"),
+    (dict(), "CUDA"),
+])
+def test_decode_names_its_own_fault(kw, msg):
+    args = {**dict(query=_half(2, 4, 64), **_cache(), context_lens=_i32(2), block_tables=_i32(2, 4),
+                   attn_scale=0.125, max_context_len=64), **kw}
+    with pytest.raises(ArgumentError, match=msg):
+        flag_attn.paged_attention_mxfp4(**args)
+
+
 def test_struct_mirrors_and_c_abi_refusals():
     lib = _lib.load()
     for name, mirror in (("fa_varlen_args", _lib.VarlenArgs), ("fa_mxfp4_cache", _lib.Mxfp4Cache),
