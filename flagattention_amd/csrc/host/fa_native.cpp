@@ -636,6 +636,7 @@ PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 // ---- packed prompts (varlen.py) and the 4-bit cache (mxfp4.py) ----
 bool packed_dim(int64_t d) { return d == 64 || d == 128 || d == 256; }
+constexpr int64_t kMaxCacheTokens = (int64_t{1} << 28) - 16;  // mxfp4.MAX_TOKENS
 
 // varlen(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal, sm_scale,
 //        want_lse): (o, lse) or o
@@ -674,6 +675,7 @@ PyObject* varlen(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int cus = cu_count(device.index());
   if (cus == 0) return none();
   const int64_t num_seqs = cq->size(0) - 1;
+  if ((total_q * (h_q / h_kv) / 128 + num_seqs + 2) * h_kv >= (int64_t{1} << 24)) return none();
   at::Tensor out, lse;
   {
     NoGil nogil;
@@ -783,7 +785,7 @@ PyObject* mxfp4_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       v->scalar_type() != k->scalar_type() || !mxfp4_cache_of(args + 2, t, &c))
     return none();
   const int64_t n = k->size(0);
-  if (n < 1 || k->size(1) != c.h_kv || k->size(2) != c.d || n * c.h_kv > INT32_MAX ||
+  if (n < 1 || k->size(1) != c.h_kv || k->size(2) != c.d || n * c.h_kv > INT32_MAX || n > kMaxCacheTokens ||
       k->stride(2) != 1 || v->stride(2) != 1 || !rows16(*k, 2) || !rows16(*v, 2) ||
       (slots->scalar_type() != at::kLong && slots->scalar_type() != at::kInt) ||
       slots->dim() != 1 || slots->size(0) != n || !slots->is_contiguous())
@@ -816,8 +818,8 @@ PyObject* mxfp4_gather(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     return none();
   if (cu->scalar_type() != at::kInt || cu->dim() != 1 || cu->size(0) < 2 || !cu->is_contiguous() ||
       bt->scalar_type() != at::kInt || bt->dim() != 2 || bt->size(0) != cu->size(0) - 1 ||
-      bt->size(1) < 1 || bt->stride(1) != 1 || total < 1 || total > INT32_MAX ||
-      total * c.h_kv > INT32_MAX)
+      bt->size(1) < 1 || bt->stride(1) != 1 || total < 1 || total > kMaxCacheTokens ||
+      total * c.h_kv > INT32_MAX || bt->size(0) > kMaxCacheTokens)
     return none();
   const c10::Device device = t[0]->device();
   if (bt->device() != device || cu->device() != device) return none();
@@ -862,7 +864,9 @@ PyObject* mxfp4_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       bt->scalar_type() != at::kInt || bt->dim() != 2 || bt->size(0) != seqs || bt->size(1) < 1 ||
       bt->stride(1) != 1)
     return none();
-  if (num_splits < 0 || max_len < 1 || max_len > (1 << 30) || !std::isfinite(scale)) return none();
+  if (num_splits < 0 || max_len < 1 || max_len > (1 << 30) || !std::isfinite(scale) ||
+      seqs > 65535 || h_kv * cdiv(h_q / h_kv, 16) > 65535)
+    return none();
   const c10::Device device = q->device();
   for (const at::Tensor* x : {lens, bt, t[0]})
     if (x->device() != device) return none();
@@ -870,7 +874,7 @@ PyObject* mxfp4_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   a.split_tokens = 1;
   if (num_splits == 0) {
     const int cus = cu_count(device.index());
-    if (cus == 0 || seqs > INT32_MAX || h_q > INT32_MAX) return none();
+    if (cus == 0) return none();
     check(fa_mxfp4_decode_plan(static_cast<int32_t>(seqs), static_cast<int32_t>(h_q), a.cache.h_kv,
                                a.cache.d, static_cast<int32_t>(max_len), cus, &a));
   } else if (num_splits > 1) {
@@ -881,6 +885,7 @@ PyObject* mxfp4_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     a.num_splits = static_cast<int32_t>(cdiv(max_len, split_tokens));
   }
   const int64_t s = a.num_splits;
+  if (s > 1 && seqs * h_q >= (1 << 24)) return none();
   at::Tensor out;
   {
     NoGil nogil;

@@ -25,6 +25,8 @@ from .gqa import TILE_TOKENS, _aligned, _cu_count, _dtype_code, _next_pow2, _req
 
 HEAD_DIMS = (64, 128, 256)
 GROUP = 32
+# a launch has fewer than 2^24 work-groups, of up to 16 tokens in the writer and the reader
+MAX_TOKENS = (1 << 28) - 16
 
 
 def _check_cache(key_cache, key_scales, value_cache, value_scales):
@@ -40,8 +42,9 @@ def _check_cache(key_cache, key_scales, value_cache, value_scales):
              "head_size / 32]")
     tensors = (key_cache, key_scales, value_cache, value_scales)
     _require(all(t.dtype == torch.uint8 for t in tensors), "the cache must be uint8")
-    _require(num_blocks >= 1 and 1 <= h_kv <= 65535, "the cache is empty or has too many heads")
-    _require(block_size >= 16 and block_size & (block_size - 1) == 0,
+    _require(1 <= num_blocks < 1 << 31 and 1 <= h_kv <= 65535,
+             "the cache is empty or has too many blocks or heads")
+    _require(16 <= block_size < 1 << 31 and block_size & (block_size - 1) == 0,
              "block_size must be a power of two of at least 16")
     _require(value_cache.stride() == key_cache.stride()
              and value_scales.stride() == key_scales.stride(),
@@ -109,7 +112,7 @@ def cache_kv_mxfp4(
     _require(slot_mapping.dim() == 1 and slot_mapping.shape[0] == t
              and slot_mapping.dtype in (torch.int32, torch.int64),
              "slot_mapping must be int32 / int64 [num_tokens]")
-    _require(t * h_kv < 1 << 31 and t < 1 << 28, "too many tokens")
+    _require(t * h_kv < 1 << 31 and t <= MAX_TOKENS, "too many tokens")
     _check_device(key, value, key_cache, key_scales, value_cache, value_scales, slot_mapping)
     if t == 0:
         return
@@ -164,7 +167,8 @@ def gather_kv_mxfp4(
              and block_tables.shape[0] == num_seqs and block_tables.stride(1) == 1,
              "block_tables must be int32 [num_seqs, max_num_blocks_per_seq]")
     _require(isinstance(total_tokens, int) and total_tokens >= 0, "total_tokens must be an int >= 0")
-    _require(total_tokens * h_kv < 1 << 31 and total_tokens < 1 << 28, "too many tokens")
+    _require(total_tokens * h_kv < 1 << 31 and total_tokens <= MAX_TOKENS, "too many tokens")
+    _require(num_seqs <= MAX_TOKENS, "too many sequences")
     _check_device(key_cache, key_scales, value_cache, value_scales, block_tables, cu_seqlens)
     k = torch.empty((total_tokens, h_kv, d), dtype=dtype, device=device)
     v = torch.empty_like(k)
@@ -222,6 +226,8 @@ def paged_attention_mxfp4(
     _require(block_tables.dtype == torch.int32 and block_tables.dim() == 2
              and block_tables.shape[0] == num_seqs and block_tables.stride(1) == 1,
              "block_tables must be int32 [num_seqs, max_num_blocks_per_seq]")
+    _require(num_seqs <= 65535 and h_kv * -(-(h_q // h_kv) // 16) <= 65535,
+             "too many sequences or heads")
     _require(num_splits >= 0, "num_splits must be >= 0")
     _require(1 <= max_context_len <= 1 << 30, "max_context_len must be in [1, 2^30]")
     _require(math.isfinite(attn_scale), "attn_scale must be finite")
@@ -247,6 +253,7 @@ def paged_attention_mxfp4(
         args.split_tokens = max(TILE_TOKENS, _next_pow2(-(-max_context_len // num_splits)))
         args.num_splits = -(-max_context_len // args.split_tokens)
     s = args.num_splits
+    _require(s == 1 or num_seqs * h_q < 1 << 24, "too many query rows for splits")
     with torch.cuda.device(device):
         stream = torch.cuda.current_stream(device).cuda_stream
         if s > 1:

@@ -78,6 +78,10 @@ def flash_attention_varlen(
              "max_seqlen_q and max_seqlen_k must be ints >= 0")
     _require(total_q * (h_q // h_kv) < 1 << 30 and total_k <= (1 << 31) - 257,
              "too many tokens")
+    # the work-groups of a launch, 128 rows of a KV head each: every sequence, and the rows of none,
+    # round up once
+    _require((total_q * (h_q // h_kv) // 128 + num_seqs + 2) * h_kv < 1 << 24,
+             "too many query rows or sequences")
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(d)
     _require(math.isfinite(sm_scale), "sm_scale must be finite")

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import flag_attn
-from flagattention_amd import _lib
+from flagattention_amd import ArgumentError, _lib
 from tests._helpers import DEV
 from tests.test_native_host import _both, _same
 
@@ -83,3 +83,38 @@ def test_mxfp4_matches_python_path(monkeypatch, d, block, dtype):
     assert fast.mxfp4_decode(q, *c, lens, bt, d ** -0.5, 12 * block, -1) is None
     assert fast.mxfp4_decode(q.float(), *c, lens, bt, d ** -0.5, 12 * block, 0) is None
     assert fast.mxfp4_decode(q, *c[:3], c[3].half(), lens, bt, d ** -0.5, 12 * block, 0) is None
+
+
+@pytest.mark.gpu
+def test_sizes_past_a_launch_are_left_to_python():
+    """And raise argument errors there.  (Large tensors are one row seen many times.)"""
+    fast = _lib.native()
+
+    def half(*shape):
+        return torch.zeros((1,) * (len(shape) - 1) + shape[-1:], device=DEV).half().expand(shape)
+
+    def i32(*shape):
+        return torch.zeros(shape, dtype=torch.int32, device=DEV)
+
+    def cache(hk):
+        return [torch.zeros((4, 1, 16, n), dtype=torch.uint8, device=DEV).expand(4, hk, 16, n)
+                for n in (32, 2, 32, 2)]
+
+    q = half((1 << 29) - 1, 1, 64)
+    args = (q, q[:8], q[:8], i32(1 << 24), i32(1 << 24), 4, 4, True, None, False)
+    assert fast.varlen(*args) is None
+    with pytest.raises(ArgumentError):
+        flag_attn.flash_attention_varlen(*args[:9])
+    n = (1 << 28) - 15
+    slots = i32(n)
+    assert fast.mxfp4_write(half(n, 1, 64), half(n, 1, 64), *cache(1), slots) is None
+    with pytest.raises(ArgumentError):
+        flag_attn.cache_kv_mxfp4(half(n, 1, 64), half(n, 1, 64), *cache(1), slots)
+    assert fast.mxfp4_gather(*cache(1), i32(2, 4), i32(3), n, True) is None
+    with pytest.raises(ArgumentError):
+        flag_attn.gather_kv_mxfp4(*cache(1), i32(2, 4), i32(3), n, torch.float16)
+    for seqs, h_q, hk, splits in ((65536, 1, 1, 0), (1, 65535 * 17, 65535, 0), (4097, 4096, 1, 2)):
+        args = (half(seqs, h_q, 64), *cache(hk), i32(seqs), i32(seqs, 1), 1.0, 1000, splits)
+        assert fast.mxfp4_decode(*args) is None
+        with pytest.raises(ArgumentError):
+            flag_attn.paged_attention_mxfp4(*args)

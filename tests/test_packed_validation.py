@@ -189,6 +189,34 @@ def test_decode_names_its_own_fault(kw, msg):
         flag_attn.paged_attention_mxfp4(**args)
 
 
+def test_sizes_past_a_launch_are_argument_errors():
+    """What the library refuses for its size is an argument error before that.  (Large tensors are one
+    row seen many times.)"""
+    a = _varlen()
+    a["q"] = a["q"][:1].expand((1 << 29) - 1, 4, 64)
+    a["cu_seqlens_q"] = a["cu_seqlens_k"] = _i32(1 << 24)
+    with pytest.raises(ArgumentError, match="too many query rows or sequences"):
+        flag_attn.flash_attention_varlen(**a)
+    a = _varlen()
+    a.update({x: _half(1, 1, 64).expand(1 << 18, 1 << 14, 64) for x in "qkv"})
+    with pytest.raises(ArgumentError, match="too many query rows or sequences"):
+        flag_attn.flash_attention_varlen(**a)
+    n = (1 << 28) - 15
+    c = _cache(hk=1)
+    kv = _half(1, 1, 64).expand(n, 1, 64)
+    with pytest.raises(ArgumentError, match="too many tokens"):
+        flag_attn.cache_kv_mxfp4(kv, kv, **c, slot_mapping=_i32(1).expand(n))
+    with pytest.raises(ArgumentError, match="too many tokens"):
+        flag_attn.gather_kv_mxfp4(**c, block_tables=_i32(2, 4), cu_seqlens=_i32(3), total_tokens=n,
+                                  dtype=torch.float16)
+    for seqs, h_q, hk in ((65536, 1, 1), (1, 65535 * 17, 65535)):
+        c = {x: t.expand(4, hk, *t.shape[2:]) for x, t in _cache(hk=1).items()}
+        with pytest.raises(ArgumentError, match="too many sequences or heads"):
+            flag_attn.paged_attention_mxfp4(_half(1, 1, 64).expand(seqs, h_q, 64), **c,
+                                            context_lens=_i32(seqs), block_tables=_i32(seqs, 1),
+                                            attn_scale=1.0, max_context_len=1000)
+
+
 def test_struct_mirrors_and_c_abi_refusals():
     lib = _lib.load()
     for name, mirror in (("fa_varlen_args", _lib.VarlenArgs), ("fa_mxfp4_cache", _lib.Mxfp4Cache),
