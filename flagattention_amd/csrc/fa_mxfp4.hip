@@ -863,8 +863,10 @@ extern "C" int fa_mxfp4_gather(const fa_mxfp4_cache* cache, const int32_t* block
   FA_CHECK_ARG(total >= 0 && num_seqs >= 0, "total %d / num_seqs %d < 0", total, num_seqs);
   FA_CHECK_ARG(dtype == 0 || dtype == 1, "dtype %d is not 0 (fp16) or 1 (bf16)", dtype);
   if (total == 0) return FA_OK;
-  FA_CHECK_ARG(cu_seqlens && k_out && v_out && (num_seqs == 0 || block_table), "NULL pointer");
   FA_CHECK_ARG(max_blocks_per_seq >= 0, "max_blocks_per_seq %d < 0", max_blocks_per_seq);
+  FA_CHECK_ARG(cu_seqlens && k_out && v_out &&
+                   (num_seqs == 0 || max_blocks_per_seq == 0 || block_table),
+               "NULL pointer");
   FA_CHECK_ARG(fa::aligned(k_out, 16) && fa::aligned(v_out, 16), "outputs must be 16-byte aligned");
   FA_CHECK_ARG(static_cast<int64_t>(total) * cache->h_kv <= INT32_MAX,
                "total %d x h_kv %d is 2^31 or more", total, cache->h_kv);

@@ -180,6 +180,18 @@ def test_gather_of_no_rows_and_late_starts():
     assert bool((k == 0).all()) and bool((v == 0).all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gather_without_blocks_is_zeros(dtype):
+    """A table without a column, as paged_attention_mxfp4 takes it: every token lies behind its end."""
+    need_gpu()
+    say(f"mxfp4 gather without blocks {dtype}")
+    cache = new_cache(3, 2, 16, 128)
+    bt = torch.zeros((2, 0), dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, 4, 9], dtype=torch.int32, device=DEV)
+    for x in flag_attn.gather_kv_mxfp4(*cache, bt, cu, 12, dtype):
+        assert x.shape == (12, 2, 128) and x.dtype == dtype and bool((x == 0).all())
+
+
 def run_decode(q, cache, lens, bt, scale=None, max_len=None, splits=0):
     d = q.shape[-1]
     ld = torch.tensor(lens, dtype=torch.int32, device=DEV)
