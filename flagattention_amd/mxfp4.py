@@ -49,8 +49,7 @@ def _check_cache(key_cache, key_scales, value_cache, value_scales):
     _require(value_cache.stride() == key_cache.stride()
              and value_scales.stride() == key_scales.stride(),
              "the V cache must have the same strides as the K cache")
-    _require(key_cache.stride(3) == 1 and (key_scales.stride(3) == 1 or d == GROUP),
-             "head dims must be contiguous")
+    _require(key_cache.stride(3) == 1 and key_scales.stride(3) == 1, "head dims must be contiguous")
     code_align, scale_align = min(16, d // 8), max(1, d // 128)
     _require(all(t.data_ptr() % n == 0 and all(t.stride(i) % n == 0 for i in range(3))
                  for t, n in ((key_cache, code_align), (value_cache, code_align),

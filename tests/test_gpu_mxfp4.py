@@ -163,6 +163,25 @@ def test_gather_rounds_to_the_type(byte):
                                want.nan_to_num(1.0, math.inf, -math.inf))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", DIMS)
+def test_gather_every_code_and_scale(d, dtype):
+    """Every byte of two codes under every scale byte, a block for each of those."""
+    need_gpu()
+    say(f"mxfp4 gather every code d={d} {dtype}")
+    codes = torch.arange(256, device=DEV).to(torch.uint8).repeat(256 * d // 32)
+    cache = [codes.view(256, 1, 16, d // 2), None, codes.flip(0).view(256, 1, 16, d // 2), None]
+    cache[1] = torch.arange(256, device=DEV).to(torch.uint8).view(256, 1, 1, 1).repeat(1, 1, 16, d // 32)
+    cache[3] = cache[1].clone()
+    bt = torch.arange(256, dtype=torch.int32, device=DEV)[None]
+    cu = torch.tensor([0, 4096], dtype=torch.int32, device=DEV)
+    for got, c, s in zip(flag_attn.gather_kv_mxfp4(*cache, bt, cu, 4096, dtype), cache[::2], cache[1::2]):
+        want = po.values(c, s).transpose(1, 2).flatten(0, 1).to(dtype)
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.isinf(), want.isinf())
+        assert torch.equal(got.nan_to_num(1.0), want.nan_to_num(1.0))
+
+
 def test_gather_of_no_rows_and_late_starts():
     need_gpu()
     say("mxfp4 gather edges")
