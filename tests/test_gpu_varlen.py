@@ -1,6 +1,7 @@
 """Prompt attention over packed sequences (flag_attn.flash_attention_varlen) against the formula
 in 64 bits, with tolerances made of the roundings it makes (tests/_packed.py)."""
 import math
+import random
 
 import pytest
 import torch
@@ -348,6 +349,52 @@ def test_many_sequences(seqs, causal):
     lens[seqs // 2] = 700
     keys = [n + int(x) for n, x in zip(lens, torch.randint(0, 30, (seqs,), generator=gen))]
     check(*inputs(lens, keys, 4, 1, 64, torch.bfloat16, seed=12, extra_q=130), causal)
+
+
+def mixed_lengths(seqs, tokens, seed):
+    """(new tokens, keys) of sequences with that many tokens in all, about: some empty, single tokens
+    over short and long contexts, chunks behind a prefix, more tokens than keys, whole prompts."""
+    gen = random.Random(seed)
+    kinds = [gen.choice("eostcmpppp") for _ in range(seqs)]
+    weights = [gen.uniform(0.2, 2.0) if x in "cmp" else 0.0 for x in kinds]
+    out = []
+    for kind, w in zip(kinds, weights):
+        m = max(1, round(tokens * w / max(sum(weights), 1e-9)))
+        out.append({"e": (0, 40), "o": (1, gen.randrange(1, 128)), "s": (1, gen.randrange(129, 900)),
+                    "t": (2, 0), "c": (m, m + gen.randrange(1, 700)), "m": (m, m - m // 3),
+                    "p": (m, m)}[kind])
+    return [m for m, _ in out], [n for _, n in out]
+
+
+# (h, hk, new tokens, keys): 8 KV heads, more than three rounds of work-groups; one KV head, the same;
+# 8 KV heads, the last work-group in the second round; more KV heads than work-groups in a round; as
+# many sequences as are ordered by their cost, and one more
+ORDERS = [(32, 8, *mixed_lengths(21, 4000, 1)), (8, 1, *mixed_lengths(9, 13100, 2)),
+          (32, 8, [58, 0, 0] * 20, [99, 40, 0] * 20), (300, 300, [137, 0], [150, 9]),
+          (16, 4, *mixed_lengths(62, 5100, 3)), (16, 4, *mixed_lengths(63, 5100, 4))]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d", varlen.HEAD_DIMS)
+@pytest.mark.parametrize("case", range(len(ORDERS)))
+def test_order_of_work_groups(case, d, causal):
+    """Launches of more work-groups than run at once, which take the row blocks in another order (up to
+    62 sequences): every row is written once, rows before, behind and between the sequences' too."""
+    need_gpu()
+    h, hk, lens, keys = ORDERS[case]
+    seqs = len(lens)
+    say(f"varlen order h={h} hk={hk} d={d} seqs={seqs} causal={causal}")
+    q, k, v, cq, ck = inputs(lens, keys, h, hk, d, torch.bfloat16, seed=d, extra_q=150)
+    cq = [c + 60 for c in cq]
+    cu = torch.cuda.get_device_properties(0).multi_processor_count
+    assert varlen_splits(q.shape[0], k.shape[0], seqs, h, hk, d, causal, max(lens), max(keys), cu)[0] == 1
+    blocks = sum(-(-m * (h // hk) // 128) for m in (*lens, 60, 90))
+    rounds = blocks / max(256 // hk, 1)
+    assert 1 < rounds < 2 if case == 2 else rounds > 3
+    assert (q.shape[0] * (h // hk) // 128 + seqs + 2) * hk > 768
+    old = [torch.full_like(q, math.nan), torch.full((h, q.shape[0]), math.nan, device=DEV)]
+    del old  # what the outputs' memory most likely holds
+    check(q, k, v, cq, ck, causal)
 
 
 def test_few_rows_strided_and_alone():
