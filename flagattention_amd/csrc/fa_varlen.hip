@@ -227,83 +227,82 @@ __device__ inline void weigh(RowState<T, D>& r, const unsigned char* kb, const L
   typedef typename PVec<T>::v8 T8;
   constexpr int kKSteps = D / 16;
   const float ninf = -__builtin_inff();
-      // K operands one k-step ahead of their MFMAs (the fences keep them there)
-      floatx16 s[kSub];
-      T8 ka[2][kSub];
-      auto k_read = [&](int kk, int tt) -> T8 {
-        return *reinterpret_cast<const T8*>(kb + 32 * tt * 2 * D + (at.k ^ (32 * kk)));
-      };
-  #pragma unroll
-      for (int tt = 0; tt < kSub; ++tt) {
-        s[tt] = floatx16{};
-        ka[0][tt] = k_read(0, tt);
+  // K operands one k-step ahead of their MFMAs (the fences keep them there)
+  floatx16 s[kSub];
+  T8 ka[2][kSub];
+  auto k_read = [&](int kk, int tt) -> T8 {
+    return *reinterpret_cast<const T8*>(kb + 32 * tt * 2 * D + (at.k ^ (32 * kk)));
+  };
+#pragma unroll
+  for (int tt = 0; tt < kSub; ++tt) {
+    s[tt] = floatx16{};
+    ka[0][tt] = k_read(0, tt);
+  }
+#pragma unroll
+  for (int kk = 0; kk < kKSteps; ++kk) {
+    if (kk + 1 < kKSteps) {
+#pragma unroll
+      for (int tt = 0; tt < kSub; ++tt) ka[(kk + 1) & 1][tt] = k_read(kk + 1, tt);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int tt = 0; tt < kSub; ++tt) s[tt] = mfma_32x32x16(ka[kk & 1][tt], r.qf[kk], s[tt]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  if (prescale) {
+#pragma unroll
+    for (int tt = 0; tt < kSub; ++tt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[tt][i] *= prescale_by;
+  }
+  if (masked) {
+#pragma unroll
+    for (int tt = 0; tt < kSub; ++tt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int j = 32 * tt + 8 * (i >> 2) + (i & 3);  // + 4g: the key of s[tt][i]
+        s[tt][i] = j < sees ? s[tt][i] : ninf;
       }
-  #pragma unroll
-      for (int kk = 0; kk < kKSteps; ++kk) {
-        if (kk + 1 < kKSteps) {
-  #pragma unroll
-          for (int tt = 0; tt < kSub; ++tt) ka[(kk + 1) & 1][tt] = k_read(kk + 1, tt);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-  #pragma unroll
-        for (int tt = 0; tt < kSub; ++tt) s[tt] = mfma_32x32x16(ka[kk & 1][tt], r.qf[kk], s[tt]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      if (prescale) {
-  #pragma unroll
-        for (int tt = 0; tt < kSub; ++tt)
-  #pragma unroll
-          for (int i = 0; i < 16; ++i) s[tt][i] *= prescale_by;
-      }
-          if (masked) {
-      #pragma unroll
-        for (int tt = 0; tt < kSub; ++tt)
-  #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int j = 32 * tt + 8 * (i >> 2) + (i & 3);  // + 4g: the key of s[tt][i]
-            s[tt][i] = j < sees ? s[tt][i] : ninf;
-          }
-      }
-      float mx = s[0][0];
-  #pragma unroll
-      for (int tt = 0; tt < kSub; ++tt)
-  #pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[tt][i]);
-      mx = max_xor32(mx) * scale_log2;
-      // only the rows that are up move: a row's result does not depend on those beside it
-      const bool up = mx > r.mref + (kLag - kAbove<T>);
-      if (__ballot(up) != 0ull) {  // uniform
-        const float m_new = up ? mx + kAbove<T> : r.mref;
-        const float alpha = up ? __builtin_amdgcn_exp2f(r.mref - m_new) : 1.f;
-        r.lsum *= alpha;
-        r.mref = m_new;
-  #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt)
-  #pragma unroll
-          for (int i = 0; i < 16; ++i) r.acc[dt][i] *= alpha;
-      }
-      const float nm = r.mref == ninf ? 0.f : -r.mref;
-      float c = scale_log2;
-      const bool far = fabsf(nm) > kFusedMax;
-      if (__ballot(far) != 0ull) {  // uniform
-        const float by = far ? c : 1.f;
-  #pragma unroll
-        for (int tt = 0; tt < kSub; ++tt)
-  #pragma unroll
-          for (int i = 0; i < 16; ++i) s[tt][i] *= by;
-        c = far ? 1.f : c;
-      }
-          float ps = 0.f;
-  #pragma unroll
-      for (int ss = 0; ss < 2 * kSub; ++ss)
-  #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float p =
-              __builtin_amdgcn_exp2f(__builtin_fmaf(s[ss >> 1][8 * (ss & 1) + i], c, nm));
-          ps += p;
-          pb[ss][i] = static_cast<T>(p);
-        }
-      r.lsum += ps;
+  }
+  float mx = s[0][0];
+#pragma unroll
+  for (int tt = 0; tt < kSub; ++tt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[tt][i]);
+  mx = max_xor32(mx) * scale_log2;
+  // only the rows that are up move: a row's result does not depend on those beside it
+  const bool up = mx > r.mref + (kLag - kAbove<T>);
+  if (__ballot(up) != 0ull) {  // uniform
+    const float m_new = up ? mx + kAbove<T> : r.mref;
+    const float alpha = up ? __builtin_amdgcn_exp2f(r.mref - m_new) : 1.f;
+    r.lsum *= alpha;
+    r.mref = m_new;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) r.acc[dt][i] *= alpha;
+  }
+  const float nm = r.mref == ninf ? 0.f : -r.mref;
+  float c = scale_log2;
+  const bool far = fabsf(nm) > kFusedMax;
+  if (__ballot(far) != 0ull) {  // uniform
+    const float by = far ? c : 1.f;
+#pragma unroll
+    for (int tt = 0; tt < kSub; ++tt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[tt][i] *= by;
+    c = far ? 1.f : c;
+  }
+  float ps = 0.f;
+#pragma unroll
+  for (int ss = 0; ss < 2 * kSub; ++ss)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ss >> 1][8 * (ss & 1) + i], c, nm));
+      ps += p;
+      pb[ss][i] = static_cast<T>(p);
+    }
+  r.lsum += ps;
 }
 
 // acc += V^T P^T of the 32 kSub keys at vb.

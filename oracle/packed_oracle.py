@@ -14,7 +14,7 @@ MAGNITUDES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
 
 def attend(q, k, v, scale, causal):
-    """One head of one sequence: q [m, D], k, v [n, D] -> (o, lse, a, ds, vmax, pmin).
+    """One head of one sequence: q [m, D], k, v [n, D] -> (o, lse, a, ds).
 
     a: sum of p |v| per output; ds: scale * max over the visible keys of sum |q| |k|, per row.
     A row without a visible key gets o = 0, lse = -inf.  A value of V at a key that a row does not
