@@ -8,31 +8,18 @@
 #include "fa_common.h"
 #include "fa_divide.h"
 #include "fa_merge.h"
+#include "fa_rows_tile.h"
 #include "fa_wave.h"
 #include "flagattention_amd_packed.h"
 
 namespace fa {
 namespace {
 
-template <typename T>
-struct FVec {
-  typedef T v8 __attribute__((ext_vector_type(8)));
-  typedef T v4 __attribute__((ext_vector_type(4)));
-  typedef T v2 __attribute__((ext_vector_type(2)));
-};
-
-__device__ inline floatx4 mfma_16x16x32(FVec<__bf16>::v8 a, FVec<__bf16>::v8 b, floatx4 c) {
+__device__ inline floatx4 mfma_16x16x32(PVec<__bf16>::v8 a, PVec<__bf16>::v8 b, floatx4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
-__device__ inline floatx4 mfma_16x16x32(FVec<_Float16>::v8 a, FVec<_Float16>::v8 b, floatx4 c) {
+__device__ inline floatx4 mfma_16x16x32(PVec<_Float16>::v8 a, PVec<_Float16>::v8 b, floatx4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-
-template <typename T>
-__device__ inline typename FVec<T>::v4 lds_tr4(const unsigned char* p) {
-  typedef short shortx4 __attribute__((ext_vector_type(4)));
-  const shortx4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FA_LDS shortx4*)(p));
-  return __builtin_bit_cast(typename FVec<T>::v4, v);
 }
 
 // The scale 2^(byte - 127) as the conversions take it: they read the exponent bits alone, 0 as
@@ -40,7 +27,7 @@ __device__ inline typename FVec<T>::v4 lds_tr4(const unsigned char* p) {
 __device__ inline float scale_of(unsigned int byte) { return __uint_as_float(byte << 23); }
 
 template <typename T, int kByte>
-__device__ inline typename FVec<T>::v2 codes2(unsigned int w, float scale) {
+__device__ inline typename PVec<T>::v2 codes2(unsigned int w, float scale) {
   if constexpr (__is_same(T, __bf16))
     return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, kByte);
   else
@@ -48,7 +35,7 @@ __device__ inline typename FVec<T>::v2 codes2(unsigned int w, float scale) {
 }
 // The eight values of a word of codes.
 template <typename T>
-__device__ inline typename FVec<T>::v8 codes8(unsigned int w, float scale) {
+__device__ inline typename PVec<T>::v8 codes8(unsigned int w, float scale) {
   const auto a = codes2<T, 0>(w, scale), b = codes2<T, 1>(w, scale);
   const auto c = codes2<T, 2>(w, scale), d = codes2<T, 3>(w, scale);
   const auto lo = __builtin_shufflevector(a, b, 0, 1, 2, 3);
@@ -56,7 +43,7 @@ __device__ inline typename FVec<T>::v8 codes8(unsigned int w, float scale) {
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 template <typename T, int kByte>
-__device__ inline unsigned int to_codes2(unsigned int old, typename FVec<T>::v2 x, float scale) {
+__device__ inline unsigned int to_codes2(unsigned int old, typename PVec<T>::v2 x, float scale) {
   if constexpr (__is_same(T, __bf16))
     return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(old, x, scale, kByte);
   else
@@ -109,7 +96,7 @@ __global__ __launch_bounds__(kWThreads) void mxfp4_write_kernel(
     const fa_mxfp4_cache cache, const T* __restrict__ key, long long key_st, long long key_sh,
     const T* __restrict__ value, long long value_st, long long value_sh, const void* slots,
     int slots64, int num_tokens, int tokens) {
-  typedef typename FVec<T>::v8 T8;
+  typedef typename PVec<T>::v8 T8;
   constexpr int kItems = 4;  // requested before the first is stored
   __shared__ RowSlots rows;
   const bool is_v = blockIdx.y != 0;
@@ -183,7 +170,7 @@ __global__ __launch_bounds__(kWThreads) void mxfp4_gather_kernel(
     const fa_mxfp4_cache cache, const int32_t* __restrict__ block_table, long long bt_stride,
     int max_blocks, const int32_t* __restrict__ cu, int num_seqs, int total, int tokens,
     T* __restrict__ k_out, T* __restrict__ v_out) {
-  typedef typename FVec<T>::v8 T8;
+  typedef typename PVec<T>::v8 T8;
   constexpr int kItems = 4;
   __shared__ RowSlots rows;
   const bool is_v = blockIdx.y != 0;
@@ -309,8 +296,8 @@ struct DecodePlan {
 template <typename T, int D, bool kSmallBlocks>
 __global__ __launch_bounds__(64 * kWaves, D == 64 ? 4 : D == 128 ? 3 : 2) void mxfp4_decode_kernel(
     const fa_mxfp4_decode_args a, const DecodePlan plan) {
-  typedef typename FVec<T>::v8 T8;
-  typedef typename FVec<T>::v4 T4;
+  typedef typename PVec<T>::v8 T8;
+  typedef typename PVec<T>::v4 T4;
   // Bytes per token row of the V tile: 32 more than its values, so that the 8 rows x 32 bytes of a
   // transposing read's half wave, and the 8 x 16 of a write's, lie in different banks.
   constexpr int kRowB = 2 * D + 32;
@@ -594,8 +581,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 4 : D == 128 ? 3 : 2) void m
     const unsigned char* const vr = vb + (4 * G + (c16 >> 2)) * kRowB + 8 * (c16 & 3);
 #pragma unroll
     for (int dt = 0; dt < kDimTiles; ++dt) {
-      const T4 lo = lds_tr4<T>(vr + 32 * dt);
-      const T4 hi = lds_tr4<T>(vr + 16 * kRowB + 32 * dt);
+      const T4 lo = lds_tr_read4<T>(vr + 32 * dt);
+      const T4 hi = lds_tr_read4<T>(vr + 16 * kRowB + 32 * dt);
       const T8 va = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
       acc[dt] = mfma_16x16x32(va, pb, acc[dt]);
       if (dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);

@@ -1,5 +1,6 @@
-// Tile helpers of the many-row attention kernels (fa_prefill.hip, fa_varlen.hip): vector types,
-// MFMA wrappers, transposing reads, offset copies into LDS and the swizzles of K and V rows.
+// Tile helpers of the many-row attention kernels (fa_prefill.hip, fa_varlen.hip) and of 4-bit decode
+// (fa_mxfp4.hip): vector types, MFMA wrappers, transposing reads, offset copies into LDS and the
+// swizzles of K and V rows.
 #pragma once
 
 #include "fa_common.h"
@@ -11,6 +12,7 @@ template <typename T>
 struct PVec {
   typedef T v8 __attribute__((ext_vector_type(8)));
   typedef T v4 __attribute__((ext_vector_type(4)));
+  typedef T v2 __attribute__((ext_vector_type(2)));
 };
 
 __device__ inline floatx16 mfma_32x32x16(PVec<__bf16>::v8 a, PVec<__bf16>::v8 b, floatx16 c) {
