@@ -858,7 +858,8 @@ extern "C" int fa_mxfp4_gather(const fa_mxfp4_cache* cache, const int32_t* block
   FA_CHECK_ARG(static_cast<int64_t>(total) * cache->h_kv <= INT32_MAX,
                "total %d x h_kv %d is 2^31 or more", total, cache->h_kv);
   FA_CHECK_ARG(total <= fa::kMaxTokens, "total %d is more than 2^28 - 16", total);
-  FA_CHECK_ARG(num_seqs <= fa::kMaxTokens, "num_seqs %d is more than 2^28 - 16", num_seqs);
+  // every wave goes through the starts
+  FA_CHECK_ARG(num_seqs <= 65535, "num_seqs %d is more than 65535, too many sequences", num_seqs);
   const int tokens = fa::tokens_per_group(total);
   const dim3 grid(static_cast<unsigned>(fa::cdiv(total, tokens)), 2);
   const hipStream_t s = static_cast<hipStream_t>(stream);

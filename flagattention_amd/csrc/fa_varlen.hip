@@ -866,6 +866,9 @@ int check_varlen(const fa_varlen_args* a) {
                    a->o_stride_t < (1ll << 23) && a->q_stride_h >= 0 && a->o_stride_h >= 0 &&
                    group * a->q_stride_h < (1ll << 29) && group * a->o_stride_h < (1ll << 29),
                "q / out token strides must be in [0, 2^23), a group's heads within 2^29 elements");
+  // every work-group goes through the starts, and each sequence may have one
+  FA_CHECK_ARG(a->num_seqs <= 65535, "num_seqs %d is more than 65535, too many sequences",
+               a->num_seqs);
   FA_CHECK_ARG(static_cast<long long>(a->total_q) * (a->h_q / a->h_kv) < (1ll << 30) &&
                    row_blocks(a) * a->h_kv < (1ll << 24),
                "too many query rows or row blocks");  // a grid holds less than 2^32 lanes

@@ -675,7 +675,7 @@ PyObject* varlen(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int cus = cu_count(device.index());
   if (cus == 0) return none();
   const int64_t num_seqs = cq->size(0) - 1;
-  if ((total_q * (h_q / h_kv) / 128 + num_seqs + 2) * h_kv >= (int64_t{1} << 24)) return none();
+  if (num_seqs > 65535 || (total_q * (h_q / h_kv) / 128 + num_seqs + 2) * h_kv >= (int64_t{1} << 24)) return none();
   at::Tensor out, lse;
   {
     NoGil nogil;
@@ -819,7 +819,7 @@ PyObject* mxfp4_gather(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (cu->scalar_type() != at::kInt || cu->dim() != 1 || cu->size(0) < 2 || !cu->is_contiguous() ||
       bt->scalar_type() != at::kInt || bt->dim() != 2 || bt->size(0) != cu->size(0) - 1 ||
       bt->size(1) < 1 || bt->stride(1) != 1 || total < 1 || total > kMaxCacheTokens ||
-      total * c.h_kv > INT32_MAX || bt->size(0) > kMaxCacheTokens)
+      total * c.h_kv > INT32_MAX || bt->size(0) > 65535)
     return none();
   const c10::Device device = t[0]->device();
   if (bt->device() != device || cu->device() != device) return none();

@@ -142,7 +142,8 @@ def gather_kv_mxfp4(
     """Read contexts back from the 4-bit cache as packed rows.
 
     block_tables  int32 [num_seqs, max_num_blocks_per_seq], as in ``paged_attention``
-    cu_seqlens    int32 [num_seqs + 1]: row cu_seqlens[s] + j of the result is token j of sequence s
+    cu_seqlens    int32 [num_seqs + 1], up to 65535 sequences: row cu_seqlens[s] + j of the result
+                  is token j of sequence s
     total_tokens  rows of the result (cu_seqlens[-1], or more: rows behind it are zeros, as are
                   those of blocks outside the cache)
 
@@ -167,7 +168,7 @@ def gather_kv_mxfp4(
              "block_tables must be int32 [num_seqs, max_num_blocks_per_seq]")
     _require(isinstance(total_tokens, int) and total_tokens >= 0, "total_tokens must be an int >= 0")
     _require(total_tokens * h_kv < 1 << 31 and total_tokens <= MAX_TOKENS, "too many tokens")
-    _require(num_seqs <= MAX_TOKENS, "too many sequences")
+    _require(num_seqs <= 65535, "too many sequences")
     _check_device(key_cache, key_scales, value_cache, value_scales, block_tables, cu_seqlens)
     k = torch.empty((total_tokens, h_kv, d), dtype=dtype, device=device)
     v = torch.empty_like(k)

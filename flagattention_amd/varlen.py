@@ -39,8 +39,9 @@ def flash_attention_varlen(
     """Attention of packed sequences (grouped heads, fp16 or bf16, head dim 64, 128 or 256).
 
     q             [total_q, H, D]; k, v [total_k, H_kv, D], H a multiple of H_kv
-    cu_seqlens_q  int32 [num_seqs + 1]: rows cu_seqlens_q[s] .. cu_seqlens_q[s + 1] - 1 of q are
-                  the tokens of sequence s; cu_seqlens_k likewise for the keys
+    cu_seqlens_q  int32 [num_seqs + 1], up to 65535 sequences: rows cu_seqlens_q[s] ..
+                  cu_seqlens_q[s + 1] - 1 of q are the tokens of sequence s; cu_seqlens_k likewise
+                  for the keys
     max_seqlen_q, max_seqlen_k
                   upper bounds of the lengths; they choose the launch, not the result
     causal        token i of m sees keys <= n - m + i of its n
@@ -80,8 +81,8 @@ def flash_attention_varlen(
              "too many tokens")
     # the work-groups of a launch, 128 rows of a KV head each: every sequence, and the rows of none,
     # round up once
-    _require((total_q * (h_q // h_kv) // 128 + num_seqs + 2) * h_kv < 1 << 24,
-             "too many query rows or sequences")
+    _require(num_seqs <= 65535 and (total_q * (h_q // h_kv) // 128 + num_seqs + 2)
+             * h_kv < 1 << 24, "too many query rows or sequences")
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(d)
     _require(math.isfinite(sm_scale), "sm_scale must be finite")

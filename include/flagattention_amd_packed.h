@@ -38,7 +38,8 @@ typedef struct fa_varlen_args {
   float* lse;      /* optional fp32 [h_q][total_q] (natural log) */
   float* o_part;   /* split workspace fp32 [h_q][total_q][num_splits][d] */
   float* lse_part; /* fp32 [h_q][total_q][num_splits] */
-  int32_t num_seqs, total_q, total_k, h_q, h_kv, d;
+  int32_t num_seqs; /* at most 65535 */
+  int32_t total_q, total_k, h_q, h_kv, d;
   /* split s covers keys [s * split_tokens, (s + 1) * split_tokens) of every sequence, the last
    * one the keys behind it too */
   int32_t num_splits, split_tokens;
@@ -106,7 +107,7 @@ int fa_mxfp4_cache_write(const fa_mxfp4_cache* cache, const void* key, int64_t k
 /*
  * Read back: row cu_seqlens[s] + j of k_out and v_out ([total][h_kv][d] contiguous, fp16 or bf16)
  * is token j of sequence s, row j % block_size of block block_table[s][j / block_size].  Rows that
- * belong to no sequence and rows of blocks outside the cache are zeros.
+ * belong to no sequence and rows of blocks outside the cache are zeros.  At most 65535 sequences.
  */
 int fa_mxfp4_gather(const fa_mxfp4_cache* cache, const int32_t* block_table, int64_t bt_stride_b,
                     int32_t max_blocks_per_seq, const int32_t* cu_seqlens, int32_t num_seqs,

@@ -297,8 +297,6 @@ def test_grids_of_2_32_lanes_are_refused():
                                          None), b"2^28 - 16")
         refused(lib.fa_mxfp4_gather(ctypes.byref(cache), 4096, 1, 1, 4096, 1, n, 4096, 4096, 0, None),
                 b"2^28 - 16")
-        refused(lib.fa_mxfp4_gather(ctypes.byref(cache), 4096, 1, 1, 4096, n, 1, 4096, 4096, 0, None),
-                b"2^28 - 16")
     varlen_args = dict(q=4096, k=4096, v=4096, out=4096, cu_seqlens_q=4096, cu_seqlens_k=4096,
                        num_seqs=1, total_k=4, h_q=1, h_kv=1, d=64, num_splits=2, split_tokens=64,
                        q_stride_t=64, q_stride_h=64, k_stride_t=64, k_stride_h=64, v_stride_t=64,
@@ -329,6 +327,31 @@ def test_key_positions_stay_in_32_bits(n):
     a.update({x: a[x][:1].expand(n, 2, 64) for x in "kv"})
     with pytest.raises(ArgumentError, match="too many tokens"):
         flag_attn.flash_attention_varlen(**a)
+
+
+def test_counts_of_sequences_that_a_launch_would_not_end_with_are_refused():
+    """A wave finds its sequence by going through all starts, so that the work grows with the square of
+    their number: as many sequences as one decode call takes."""
+    lib = _lib.load()
+    args = dict(q=4096, k=4096, v=4096, out=4096, cu_seqlens_q=4096, cu_seqlens_k=4096, total_q=4,
+                total_k=4, h_q=1, h_kv=1, d=64, num_splits=1, split_tokens=1, q_stride_t=64,
+                q_stride_h=64, k_stride_t=64, k_stride_h=64, v_stride_t=64, v_stride_h=64,
+                o_stride_t=64, o_stride_h=64)
+    cache = _lib.Mxfp4Cache(k_codes=4096, k_scales=4096, v_codes=4096, v_scales=4096, code_stride_0=512,
+                            code_stride_h=512, code_stride_t=32, scale_stride_0=32, scale_stride_h=32,
+                            scale_stride_t=2, num_blocks=4, block_size=16, h_kv=1, d=64)
+    for n in (65536, 1 << 23):
+        assert lib.fa_varlen_attention(ctypes.byref(_lib.VarlenArgs(num_seqs=n, **args)), None) == -1
+        assert b"too many sequences" in lib.fa_last_error()
+        assert lib.fa_mxfp4_gather(ctypes.byref(cache), 4096, 1, 1, 4096, n, 1, 4096, 4096, 0, None) == -1
+        assert b"too many sequences" in lib.fa_last_error()
+    a = _varlen()
+    a["cu_seqlens_q"] = a["cu_seqlens_k"] = _i32(65537)
+    with pytest.raises(ArgumentError, match="too many query rows or sequences"):
+        flag_attn.flash_attention_varlen(**a)
+    with pytest.raises(ArgumentError, match="too many sequences"):
+        flag_attn.gather_kv_mxfp4(**_cache(), block_tables=_i32(65536, 1), cu_seqlens=_i32(65537),
+                                  total_tokens=5, dtype=torch.float16)
 
 
 def test_oracle_formats():
