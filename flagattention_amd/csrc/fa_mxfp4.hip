@@ -264,8 +264,8 @@ constexpr int kDRows = 16;
 // rounding to 16 bits would cost nothing.  Following every new maximum instead (kLag = 0): bf16 error
 // against 64 bits at 512 / 4,096 keys 2.03 / 2.03e-3 where this has 2.23 / 2.26e-3, fp16 2.51 / 2.52e-4
 // where this has 2.77 / 2.81e-4; 32 ragged contexts of up to 4,096 keys take 21.2 instead of 20.7 us, 32
-// of up to 3,000 at head dim 256 24.5 instead of 24.1 (23.8 without a look at the scales), long ones the
-// same.  kLag = 2: 2.15e-3, 20.9 us.
+// of up to 3,000 at head dim 256 24.5 instead of 24.1 (23.8 without a look at the scales; the merge of
+// today takes 0.2 off each), long ones the same.  kLag = 2: 2.15e-3, 20.9 us.
 constexpr float kLag = 6.f;
 constexpr float kAbove = 16.f;
 constexpr unsigned int kHuge = 224;

@@ -12,8 +12,8 @@
 //
 // Two waves per SIMD (three at head dim 64): one's softmax fills the other's matrix instructions.
 // Long prompts are bound by power: 6 sequences of up to 8,192 tokens, 32 heads of 8 KV heads, D = 128,
-// take 712 .. 761 us at 1.94 GHz, 980 .. 1,050 TF (a product of 8,192^3 reaches 1,253), both pipes busy
-// for 52% of the cycles.  16 of up to 2,048 take 171 .. 185 us, 740 .. 800 TF, at 2.1 GHz: 3,400 work-groups of ten tiles on
+// take 712 .. 778 us at 1.94 GHz, 960 .. 1,050 TF (a product of 8,192^3 reaches 1,253), both pipes busy
+// for 52% of the cycles.  16 of up to 2,048 take 170 .. 189 us, 725 .. 805 TF, at 2.1 GHz: 3,400 work-groups of ten tiles on
 // average with their starts and ends.  64 rows per wave would halve the reads of LDS, but spill
 // (830 TF where these reach 1,045); a step whose QK runs beside the last one's softmax took 5%
 // fewer cycles and the same time.

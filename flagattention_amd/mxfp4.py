@@ -149,7 +149,8 @@ def gather_kv_mxfp4(
 
     Returns ``(key, value)``, each ``dtype`` (fp16 or bf16) ``[total_tokens, H_kv, D]``, the cache's
     values rounded to it: past fp16's range they are infinities (also what was written as more than
-    57344, whose code is 4 * 2^14; ``paged_attention_mxfp4`` takes those as they are).
+    57344, whose code is 4 * 2^14; ``paged_attention_mxfp4`` takes those as they are).  So are, here and
+    there, those past bf16's (written as more than 1.75 * 2^127).
     """
     fast = _lib.native() if dtype in (torch.float16, torch.bfloat16) else None
     if fast is not None:
@@ -202,6 +203,11 @@ def paged_attention_mxfp4(
                   j of sequence s is row ``j % block_size`` of block
                   ``block_tables[s, j // block_size]``; a block outside the cache reads as masked
                   keys
+    max_context_len
+                  a bound of the lengths.  It chooses the launch, not the result, and is worth
+                  keeping close: past it nothing is split any further, and under a loose one short
+                  contexts lie in one split (20.7 us at the bound, 21.6 at twice that, 31.6 at 32 times
+                  it, for 32 ragged contexts of up to 4,096 keys)
     num_splits    0 picks the split count, 1 disables splitting, s > 1 uses partitions of
                   ``next_pow2(cdiv(max_context_len, s))`` tokens, at least 32
 

@@ -43,7 +43,10 @@ def flash_attention_varlen(
                   cu_seqlens_q[s + 1] - 1 of q are the tokens of sequence s; cu_seqlens_k likewise
                   for the keys
     max_seqlen_q, max_seqlen_k
-                  upper bounds of the lengths; they choose the launch, not the result
+                  upper bounds of the lengths; they choose the launch, not the result.  One split
+                  count holds for the whole launch, 1 where its rows fill the CUs: a single token of
+                  a very long context beside a large chunk is then one work-group's walk (131,072
+                  keys 1.46 ms, 0.11 in a call of its own)
     causal        token i of m sees keys <= n - m + i of its n
 
     Returns ``o`` shaped and typed like ``q``, with ``return_log_normalizer`` the pair ``(o, L)``,
