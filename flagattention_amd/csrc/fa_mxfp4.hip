@@ -253,20 +253,17 @@ int tokens_per_group(int64_t tokens) {
 constexpr int kWaves = 4;
 constexpr int kDTile = 32;
 constexpr int kDRows = 16;
-// P is relative to a reference per row, which moves where the row's maximum is more than kLag (log2
-// units) past its last place.  From the first bf16 tile with a scale byte of kHuge on (values of
-// 6 * 2^97 and more) it lies kAbove over the maximum: P reaches 2^(kLag - kAbove) at most, and the sums
-// of 2^10 keys of such a weight and the largest V stay within fp32, those of 2^16 of equal weights (a
-// single value near bf16's largest at a weight past 1 made an infinity).  P ends at 2^-126: weights
-// below 2^-126 of the largest are 0, with such values those below 2^-110.
+// P is relative to a row's running maximum.  From the first bf16 tile with a scale byte of kHuge on
+// (values of 6 * 2^97 and more) it is 2^-kAbove of that: the sums of 2^16 keys of the largest finite V
+// then stay within fp32.  P ends at 2^-126: weights below 2^-126 of the largest are 0, with such values
+// those below 2^-110.
 //
-// Between moves the accumulators are left alone, but the largest P is then no power of two, whose
-// rounding to 16 bits would cost nothing.  Following every new maximum instead (kLag = 0): bf16 error
-// against 64 bits at 512 / 4,096 keys 2.03 / 2.03e-3 where this has 2.23 / 2.26e-3, fp16 2.51 / 2.52e-4
-// where this has 2.77 / 2.81e-4; 32 ragged contexts of up to 4,096 keys take 21.2 instead of 20.7 us, 32
-// of up to 3,000 at head dim 256 24.5 instead of 24.1 (23.8 without a look at the scales; the merge of
-// today takes 0.2 off each), long ones the same.  kLag = 2: 2.15e-3, 20.9 us.
-constexpr float kLag = 6.f;
+// The largest P is a power of two, whose rounding to 16 bits costs nothing.  A reference that lags up to
+// 2^6 behind rescales less often, but its error against 64 bits was 2.23 / 2.26e-3 in bf16 at 512 /
+// 4,096 keys where this has 2.03 / 2.03e-3, 2.77 / 2.81e-4 in fp16 where this has 2.51 / 2.52e-4; 32 ragged
+// contexts of up to 4,096 keys took 20.7 us with it and take 21.2, 32 of up to 3,000 at head dim 256 24.1
+// and 24.5 (23.8 without a look at the scales either; the merge of today takes 0.2 off each), long ones
+// the same.
 constexpr float kAbove = 16.f;
 constexpr unsigned int kHuge = 224;
 
@@ -541,7 +538,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 4 : D == 128 ? 3 : 2) void m
       for (int i = 0; i < 4; ++i) tmax = fmaxf(tmax, s[h][i]);
     tmax = max_xor32(max_xor16(tmax)) * scale_log2;
     const float up_by = huge ? kAbove : above;  // uniform
-    const bool up = tmax + up_by > m_run + kLag || up_by != above;
+    const bool up = tmax + up_by > m_run || up_by != above;
     if (__ballot(up) != 0ull) {  // uniform
       // only the rows that are up move: a row's result does not depend on those beside it
       const float m_new = up ? fmaxf(m_run - above, tmax) + up_by : m_run;

@@ -46,6 +46,15 @@ def attend(q, k, v, scale, causal):
     return o, lse, a, mag.amax(-1)
 
 
+def attend_rest(q, k, v, scale):
+    """One head that sees every key: (o, rest, ds), rest the sum of p |v| but for each row's largest
+    weight."""
+    o, lse, a, ds = attend(q, k, v, scale, False)
+    s = (q.double() @ k.double().t()) * scale
+    top, at = s.max(-1)
+    return o, a - torch.exp(top - lse)[:, None] * v.double()[at].abs(), ds
+
+
 def varlen(q, k, v, cu_q, cu_k, scale, causal):
     """Packed attention: (o [total_q, H, D], lse [H, total_q], a like o, ds like lse)."""
     total, h, d = q.shape

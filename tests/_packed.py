@@ -40,6 +40,23 @@ def assert_rows(o, ref, a, ds, n, vmax):
         f"its tolerance, error {float(err[bad].max()):.3e}")
 
 
+def assert_largest_exact(o, ref, rest, ds, n, vmax, terms):
+    """As assert_rows, where the rounding of the largest weight costs nothing: rest like ref, the sum of
+    p |v| over the other keys, whose weights are each off by u p.  terms: the products of a score
+    that are not 0 (the others add nothing, exactly).  The largest weight's own exponent is off by 2^-20
+    at most (a reference below 2^5 is rounded by that), which P's rounding takes away, but not the
+    row's sum."""
+    u = HALF[o.dtype]
+    fp32 = (2 * (terms + 8) * 2.0 ** -24 * ds.unsqueeze(-1) + (n + 64) * 2.0 ** -24 + 2.0 ** -20)
+    tol = u * ref.abs() + TINY[o.dtype] + 1.01 * (u * rest + fp32 * (ref.abs() + 2 * rest))
+    if o.dtype == torch.float16:
+        tol = tol + 2.0 ** -25 * n * vmax
+    err = (o.double() - ref).abs()
+    assert bool((err <= tol).all()), (
+        f"{int((err > tol).sum())} of {err.numel()} outside: worst {float((err - tol).max()):.3e} past "
+        f"its tolerance, error {float(err[err > tol].max()):.3e}")
+
+
 def assert_lse(lse, ref, ds, n, d):
     """lse: the scores' error, and that of a sum of n terms and of a logarithm in fp32."""
     assert torch.equal(torch.isneginf(lse), torch.isneginf(ref)), "-inf in other places"

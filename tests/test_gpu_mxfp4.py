@@ -9,7 +9,7 @@ import torch
 import flag_attn
 from oracle import packed_oracle as po
 from tests._helpers import DEV, need_gpu, say
-from tests._packed import assert_rows
+from tests._packed import assert_largest_exact, assert_rows
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.float16, torch.bfloat16]
@@ -392,6 +392,33 @@ def test_decode_rows_do_not_depend_on_their_neighbours(d, dtype, gain):
             o2 = run_decode(other, cache, [900, 451], bt, splits=splits)
             o2[0, h] = o[0, h]
             assert torch.equal(o, o2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", DIMS)
+def test_decode_largest_weight_is_exact(d, dtype):
+    """Two keys that a wave meets one after the other, the second e^0.6 .. e^4 times as heavy, among
+    keys of next to no weight: the largest weight of a row is a power of two, whose rounding costs
+    nothing, so that the first key's alone does."""
+    need_gpu()
+    say(f"mxfp4 decode largest weight d={d} {dtype}")
+    k = torch.zeros((200, 2, d), dtype=dtype, device=DEV)
+    k[..., 0] = -24.0
+    k[3, :, 0], k[140, :, 0] = 2.0, 6.0  # tiles 0 and 4 of the first wave
+    cache = new_cache(16, 2, 16, d, seed=d)
+    v, _ = po.context(cache[2], cache[3], torch.arange(16), 200)
+    flag_attn.cache_kv_mxfp4(k, v.to(dtype), *cache, torch.arange(200, device=DEV))
+    bt = torch.arange(16, dtype=torch.int32)[None]
+    q = torch.zeros((1, 32, d), dtype=dtype, device=DEV)
+    q[..., 0] = torch.linspace(0.15, 1.0, 32, device=DEV).to(dtype)
+    out = run_decode(q, cache, [200], bt, scale=1.0, splits=1)[0]
+    ck, _ = po.context(cache[0], cache[1], bt[0], 200)
+    cv, _ = po.context(cache[2], cache[3], bt[0], 200)
+    assert torch.equal(ck, k.double())
+    for j in range(2):
+        r = slice(16 * j, 16 * j + 16)
+        ref, rest, ds = po.attend_rest(q[0, r], ck[:, j], cv[:, j], 1.0)
+        assert_largest_exact(out[r], ref, rest, ds, 200, 48.0, terms=1)
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.2, 30.0])
