@@ -261,9 +261,8 @@ constexpr int kDRows = 16;
 // The largest P is a power of two, whose rounding to 16 bits costs nothing.  A reference that lags up to
 // 2^6 behind rescales less often, but its error against 64 bits was 2.23 / 2.26e-3 in bf16 at 512 /
 // 4,096 keys where this has 2.03 / 2.03e-3, 2.77 / 2.81e-4 in fp16 where this has 2.51 / 2.52e-4; 32 ragged
-// contexts of up to 4,096 keys took 20.7 us with it and take 21.2, 32 of up to 3,000 at head dim 256 24.1
-// and 24.5 (23.8 without a look at the scales either; the merge of today takes 0.2 off each), long ones
-// the same.
+// contexts of up to 4,096 keys took 20.5 us with it and take 20.7, 32 of up to 3,000 at head dim 256 23.9
+// and 24.3 (0.3 less without a look at the scales), long ones the same.
 constexpr float kAbove = 16.f;
 constexpr unsigned int kHuge = 224;
 

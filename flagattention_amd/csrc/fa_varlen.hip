@@ -48,7 +48,7 @@ constexpr float kFusedMax = 1024.f;
 // against 64 bits at 300 / 512 / 2,048 / 6,144 keys 2.07 / 2.10 / 2.10 / 2.20e-3 where this has 2.17 /
 // 2.20 / 2.29 / 2.33e-3, fp16 2.58 .. 2.75e-4 where this has 2.71 .. 2.91e-4; 6 x 8,192 tokens take 763
 // instead of 733 us, 16 x 2,048 179 instead of 170, unmasked ones at head dim 256 120 instead of 110.5.
-// kLag = 2: 2.14 .. 2.28e-3, 743, 174 and 116 us.
+// kLag = 2: 2.14 .. 2.28e-3, 743, 174 and 116 us.  Blocks of few rows, bound by bytes, follow (kFollow).
 constexpr float kLag = 6.f;
 template <typename T>
 constexpr float kAbove = __is_same(T, __bf16) ? 16.f : 0.f;
@@ -220,7 +220,7 @@ struct LaneReads {
 
 // Weights of 32 kSub keys at kb for the 32 rows: scores, mask, running maximum, exponentials.  A
 // masked tile's first `sees` keys (from the lane's own, 4g) are seen by the lane's row.
-template <typename T, int D, int kSub>
+template <typename T, int D, int kSub, bool kFollow>
 __device__ inline void weigh(RowState<T, D>& r, const unsigned char* kb, const LaneReads<D>& at,
                              bool masked, int sees, bool prescale, float prescale_by,
                              float scale_log2, typename PVec<T>::v8 (&pb)[2 * kSub]) {
@@ -271,7 +271,7 @@ __device__ inline void weigh(RowState<T, D>& r, const unsigned char* kb, const L
     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[tt][i]);
   mx = max_xor32(mx) * scale_log2;
   // only the rows that are up move: a row's result does not depend on those beside it
-  const bool up = mx > r.mref + (kLag - kAbove<T>);
+  const bool up = mx > r.mref + ((kFollow ? 0.f : kLag) - kAbove<T>);
   if (__ballot(up) != 0ull) {  // uniform
     const float m_new = up ? mx + kAbove<T> : r.mref;
     const float alpha = up ? __builtin_amdgcn_exp2f(r.mref - m_new) : 1.f;
@@ -410,7 +410,7 @@ __device__ inline void walk_few(RowState<T, D>& r, const LaneReads<D>& at, unsig
     wait_vmem<kBoth ? kCopies : 0>();  // K
     fence();
     typename PVec<T>::v8 pb[2];
-    weigh<T, D, 1>(r, mine, at, start + 32 > min_lim, lim - start - 4 * (lane >> 5), prescale,
+    weigh<T, D, 1, true>(r, mine, at, start + 32 > min_lim, lim - start - 4 * (lane >> 5), prescale,
                    prescale_by, scale_log2, pb);
     fence();
     wait_lds();  // K is read
@@ -705,7 +705,7 @@ __global__ __launch_bounds__(kLThreads, 2) void varlen_kernel(const fa_varlen_ar
 
     T8 pb[2 * kSub];
     // masked: some row does not see the whole tile (uniform)
-    weigh<T, D, kSub>(r, kb, at, start + kTok > wave_min, lim - start - 4 * g, prescale,
+    weigh<T, D, kSub, false>(r, kb, at, start + kTok > wave_min, lim - start - 4 * g, prescale,
                       a.scale * kLog2e, scale_log2, pb);
     if (odd) {
       add_odd_values<T, D>(r, vb, g, kTok, lim - start);

@@ -10,7 +10,7 @@ import flag_attn
 from flagattention_amd import varlen
 from oracle import packed_oracle as po
 from tests._helpers import DEV, need_gpu, say
-from tests._packed import assert_lse, assert_rows, varlen_splits
+from tests._packed import assert_largest_exact, assert_lse, assert_rows, varlen_splits
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.float16, torch.bfloat16]
@@ -248,6 +248,29 @@ def test_many_huge_values_in_splits(lens_q, lens_k, d):
     need_gpu()
     say(f"varlen many huge values {lens_q[:2]} d={d} in splits")
     check_many_huge_values(lens_q, lens_k, d)
+
+
+@pytest.mark.parametrize("tokens", [1, 40])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", varlen.HEAD_DIMS)
+def test_largest_weight_of_few_rows_is_exact(d, dtype, tokens):
+    """Single tokens: two keys that a wave meets one after the other, the second e^0.6 .. e^4 times as
+    heavy, among keys of next to no weight: the largest weight of a row is a power of two, whose
+    rounding costs nothing, so that the first key's alone does."""
+    need_gpu()
+    say(f"varlen largest weight d={d} {dtype} tokens={tokens}")
+    n = 200
+    q, k, v, cq, ck = inputs([1] * tokens, [n] * tokens, 32, 2, d, dtype, seed=d)
+    q.zero_(), k.zero_()
+    k[..., 0] = -24.0
+    k[3::n, :, 0], k[140::n, :, 0] = 2.0, 6.0  # tiles 0 and 4 of the first wave
+    q[..., 0] = torch.linspace(0.15, 1.0, 32, device=DEV).to(dtype)
+    o, _ = call(q, k, v, cq, ck, True, scale=1.0)
+    for i in range(tokens):
+        for j in range(2):
+            r, ks = slice(16 * j, 16 * j + 16), slice(ck[i], ck[i + 1])
+            ref, rest, ds = po.attend_rest(q[i, r], k[ks, j], v[ks, j], 1.0)
+            assert_largest_exact(o[i, r], ref, rest, ds, n, 6.0, terms=1)
 
 
 @pytest.mark.parametrize("gain", [5.0, 4000.0])
