@@ -642,8 +642,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 4 : D == 128 ? 3 : 2) void m
       mw[w] = ml[w * kDRows + r];
       M = fmaxf(M, mw[w]);
     }
-    // no visible key: every weight and sum is 0; NaN sums stay NaN.  (bf16: four waves' sums of P below
-    // 1 each stay so together.)
+    // no visible key: every weight and sum is 0; NaN sums stay NaN.  In bf16 the waves' sums are taken at
+    // a quarter: each may be as large as fp32 holds (see kAbove).
     const float m_use = M == ninf ? 0.f : M + (kHalved ? 0.f : 2.f);
     float L = 0.f;
     floatx4 O = floatx4{};
