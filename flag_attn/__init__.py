@@ -16,7 +16,11 @@ exports the decode operators built for MI355X:
   path (no dropout, no total attention, no backward);
 * ``flash_attention_varlen`` -- prompt attention over packed sequences of different lengths;
 * ``cache_kv_mxfp4`` / ``gather_kv_mxfp4`` / ``paged_attention_mxfp4`` -- a paged K/V cache in
-  4 bits: its writer, its reader and one-token decode over it.
+  4 bits: its writer, its reader and one-token decode over it;
+* ``rotary_embedding`` / ``rotary_cache_kv`` -- q and k turned by their positions of one or several
+  axes, into new rows, in place, or (k, with v) into the paged cache of ``paged_attention``;
+* ``linear_attention_varlen`` / ``linear_attention_decode`` -- linear attention with a decay per
+  head: packed prompts and single tokens over states that stay in slots.
 
 Every operator runs in ``flagattention_amd/libflagattention_amd.so`` (hand-written HIP for
 gfx950); there is no Triton and no CPU fallback.  The reference's training-path operators
@@ -36,9 +40,14 @@ from flag_attn.varlen import attention as flash_attention_varlen  # noqa: F401
 from flag_attn.mxfp4 import attention as paged_attention_mxfp4  # noqa: F401
 from flag_attn.mxfp4 import cache_kv as cache_kv_mxfp4  # noqa: F401
 from flag_attn.mxfp4 import gather_kv as gather_kv_mxfp4  # noqa: F401
+from flag_attn.rotary import cache_kv as rotary_cache_kv  # noqa: F401
+from flag_attn.rotary import embedding as rotary_embedding  # noqa: F401
+from flag_attn.linear import attention as linear_attention_varlen  # noqa: F401
+from flag_attn.linear import decode as linear_attention_decode  # noqa: F401
 
 __all__ = ["get_mla_metadata", "flash_mla_with_kvcache", "concat_and_cache_mla", "topk_indices",
            "paged_attention",
            "flash_attention_split_kv", "flash_attention", "flash_attention_varlen",
-           "cache_kv_mxfp4", "gather_kv_mxfp4", "paged_attention_mxfp4"]
+           "cache_kv_mxfp4", "gather_kv_mxfp4", "paged_attention_mxfp4", "rotary_embedding",
+           "rotary_cache_kv", "linear_attention_varlen", "linear_attention_decode"]
 __version__ = "0.2.0"

@@ -180,6 +180,86 @@ class Mxfp4DecodeArgs(ctypes.Structure):
     ]
 
 
+class RotaryArgs(ctypes.Structure):
+    """Mirror of ``fa_rotary_args``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("q_stride_t", ctypes.c_int64),
+        ("q_stride_h", ctypes.c_int64),
+        ("k", ctypes.c_void_p),
+        ("k_stride_t", ctypes.c_int64),
+        ("k_stride_h", ctypes.c_int64),
+        ("q_out", ctypes.c_void_p),
+        ("q_out_stride_t", ctypes.c_int64),
+        ("q_out_stride_h", ctypes.c_int64),
+        ("k_out", ctypes.c_void_p),
+        ("k_out_stride_t", ctypes.c_int64),
+        ("k_out_stride_h", ctypes.c_int64),
+        ("v", ctypes.c_void_p),
+        ("v_stride_t", ctypes.c_int64),
+        ("v_stride_h", ctypes.c_int64),
+        ("key_cache", ctypes.c_void_p),
+        ("value_cache", ctypes.c_void_p),
+        ("kc_stride_0", ctypes.c_int64),
+        ("kc_stride_h", ctypes.c_int64),
+        ("kc_stride_t", ctypes.c_int64),
+        ("vc_stride_0", ctypes.c_int64),
+        ("vc_stride_h", ctypes.c_int64),
+        ("vc_stride_t", ctypes.c_int64),
+        ("num_blocks", ctypes.c_int64),
+        ("slots", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("pos_stride_a", ctypes.c_int64),
+        ("inv_freq", ctypes.c_void_p),
+        ("tokens", ctypes.c_int32),
+        ("h_q", ctypes.c_int32),
+        ("h_kv", ctypes.c_int32),
+        ("d", ctypes.c_int32),
+        ("pairs", ctypes.c_int32),
+        ("axes", ctypes.c_int32),
+        ("sections", ctypes.c_int32 * 4),
+        ("block_size", ctypes.c_int32),
+        ("mixed", ctypes.c_int32),
+        ("adjacent", ctypes.c_int32),
+        ("pos64", ctypes.c_int32),
+        ("slots64", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class LinearArgs(ctypes.Structure):
+    """Mirror of ``fa_linear_args``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("q_stride_t", ctypes.c_int64),
+        ("q_stride_h", ctypes.c_int64),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_stride_t", ctypes.c_int64),
+        ("k_stride_h", ctypes.c_int64),
+        ("v_stride_t", ctypes.c_int64),
+        ("v_stride_h", ctypes.c_int64),
+        ("log_decay", ctypes.c_void_p),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("state", ctypes.c_void_p),
+        ("state_stride_s", ctypes.c_int64),
+        ("state_stride_h", ctypes.c_int64),
+        ("state_indices", ctypes.c_void_p),
+        ("has_state", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("num_slots", ctypes.c_int32),
+        ("num_seqs", ctypes.c_int32),
+        ("total", ctypes.c_int32),
+        ("h_q", ctypes.c_int32),
+        ("h_kv", ctypes.c_int32),
+        ("d", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
 # name -> (restype, argtypes) for every symbol declared in the header
 SIGNATURES = {
     "fa_abi_version": (ctypes.c_int, []),
@@ -238,6 +318,11 @@ SIGNATURES = {
          ctypes.c_int32, ctypes.POINTER(Mxfp4DecodeArgs)]),
     "fa_mxfp4_decode": (ctypes.c_int, [ctypes.POINTER(Mxfp4DecodeArgs), ctypes.c_void_p]),
     "fa_mxfp4_combine": (ctypes.c_int, [ctypes.POINTER(Mxfp4DecodeArgs), ctypes.c_void_p]),
+    "fa_rotary_args_size": (ctypes.c_int64, []),
+    "fa_rotary": (ctypes.c_int, [ctypes.POINTER(RotaryArgs), ctypes.c_void_p]),
+    "fa_linear_args_size": (ctypes.c_int64, []),
+    "fa_linear_prompt": (ctypes.c_int, [ctypes.POINTER(LinearArgs), ctypes.c_void_p]),
+    "fa_linear_token": (ctypes.c_int, [ctypes.POINTER(LinearArgs), ctypes.c_void_p]),
 }
 
 _lock = threading.Lock()
@@ -266,7 +351,8 @@ def load() -> ctypes.CDLL:
             raise RuntimeError(f"flagattention_amd: library ABI {ver} != binding ABI {ABI_VERSION}")
         for name, mirror in (("fa_mla_decode_args", DecodeArgs), ("fa_gqa_decode_args", GqaArgs),
                              ("fa_varlen_args", VarlenArgs), ("fa_mxfp4_cache", Mxfp4Cache),
-                             ("fa_mxfp4_decode_args", Mxfp4DecodeArgs)):
+                             ("fa_mxfp4_decode_args", Mxfp4DecodeArgs),
+                             ("fa_rotary_args", RotaryArgs), ("fa_linear_args", LinearArgs)):
             size = getattr(lib, name + "_size")()
             if size != ctypes.sizeof(mirror):
                 raise RuntimeError(

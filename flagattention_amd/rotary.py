@@ -1,0 +1,207 @@
+"""Rotary positions: host side of the gfx950 HIP path.
+
+Pair i of a head -- dims ``i`` and ``i + R/2``, or ``2i`` and ``2i + 1`` -- turns by the angle
+``position * inv_freq[i]``; the first ``R = 2 * len(inv_freq)`` dims turn, the others stay.  A token
+has one position, or one on each of up to four axes (time, height, width of images and video): every
+pair takes one axis, by the ``sections``.
+
+``rotary_embedding`` turns q and k, for any of the attention operators here; ``rotary_cache_kv`` turns
+q and writes the turned k and v into the paged 16-bit cache that ``paged_attention`` reads.  Angles
+are worked out in 64 bits from the positions as they are, so there is no table and no last position.
+
+Work is queued on the current stream; argument errors raise ``ArgumentError`` before any launch.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Sequence, Tuple
+
+import torch
+
+from . import _lib
+from .gqa import _dtype_code, _require
+
+MAX_AXES = 4
+MAX_HEAD_DIM = 4096
+
+
+def _check_turn(tokens, d, positions, inv_freq, sections, mixed_sections):
+    """(pairs, sections) of a call."""
+    _require(inv_freq.dtype == torch.float32 and inv_freq.dim() == 1 and inv_freq.is_contiguous(),
+             "inv_freq must be contiguous float32 [pairs]")
+    pairs = inv_freq.shape[0]
+    _require(1 <= pairs and 2 * pairs <= d <= MAX_HEAD_DIM,
+             f"{pairs} pairs do not fit head dim {d} (at most {MAX_HEAD_DIM})")
+    _require(positions.dtype in (torch.int32, torch.int64), "positions must be int32 or int64")
+    if sections is None:
+        _require(positions.shape == (tokens,) and positions.is_contiguous(),
+                 "positions must be contiguous [num_tokens]")
+        _require(not mixed_sections, "mixed_sections needs sections")
+        return pairs, (pairs,)
+    sections = tuple(sections)
+    _require(1 <= len(sections) <= MAX_AXES
+             and all(isinstance(n, int) and n >= 0 for n in sections) and sum(sections) == pairs,
+             f"sections must be 1 to {MAX_AXES} ints >= 0 that sum to {pairs}")
+    _require(positions.shape == (len(sections), tokens)
+             and (tokens <= 1 or positions.stride(1) == 1),
+             "positions must be [len(sections), num_tokens], tokens contiguous")
+    if mixed_sections:
+        axes = len(sections)
+        _require(all(n == 0 or (n - 1) * axes + a < pairs for a, n in enumerate(sections) if a > 0),
+                 "sections do not fit when they are mixed")
+    return pairs, sections
+
+
+def _apart(x, row_dims) -> bool:
+    """Whether no two rows of x share an element: every dimension steps past the ones inside it."""
+    reach = x.shape[-1]
+    for stride, size in sorted((x.stride(i), x.shape[i]) for i in row_dims):
+        if size > 1:
+            if stride < reach:
+                return False
+            reach += (size - 1) * stride
+    return True
+
+
+def _one_device(*tensors):
+    _require(all(t.is_cuda and t.device == tensors[0].device for t in tensors),
+             "all tensors must be CUDA (HIP) tensors on one device")
+
+
+def _dense(x):
+    return x if x.stride(2) == 1 else x.contiguous()
+
+
+def _args(q, k, q_out, positions, inv_freq, sections, mixed_sections, adjacent_pairs, code):
+    return _lib.RotaryArgs(
+        q=q.data_ptr(), q_stride_t=q.stride(0), q_stride_h=q.stride(1), k=k.data_ptr(),
+        k_stride_t=k.stride(0), k_stride_h=k.stride(1), q_out=q_out.data_ptr(),
+        q_out_stride_t=q_out.stride(0), q_out_stride_h=q_out.stride(1),
+        positions=positions.data_ptr(),
+        pos_stride_a=positions.stride(0) if positions.dim() == 2 else 0,
+        inv_freq=inv_freq.data_ptr(), tokens=q.shape[0], h_q=q.shape[1], h_kv=k.shape[1],
+        d=q.shape[2], pairs=inv_freq.shape[0], axes=len(sections),
+        sections=(ctypes.c_int32 * MAX_AXES)(*sections), mixed=int(bool(mixed_sections)),
+        adjacent=int(bool(adjacent_pairs)), pos64=int(positions.dtype == torch.int64), dtype=code)
+
+
+def _check_heads(q, k):
+    _require(q.dim() == 3 and k.dim() == 3 and k.shape[0] == q.shape[0]
+             and k.shape[2] == q.shape[2], "q and k must be [num_tokens, heads, head_dim]")
+    _require(1 <= q.shape[1] <= 65535 and 1 <= k.shape[1] <= 65535, "no heads or too many")
+    code = _dtype_code(q.dtype)
+    _require(k.dtype == q.dtype, "q and k dtypes differ")
+    # a thread for at least a pair of four rows; what is taken 16 bytes at a time needs an eighth
+    _require(q.shape[0] * -(-(q.shape[1] + 2 * k.shape[1] + 3) // 4) * (q.shape[2] // 2 + 1)
+             < (1 << 31) - 1024, "too many tokens or heads")
+    return code
+
+
+def rotary_embedding(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    positions: torch.Tensor,
+    inv_freq: torch.Tensor,
+    sections: Optional[Sequence[int]] = None,
+    mixed_sections: bool = False,
+    adjacent_pairs: bool = False,
+    inplace: bool = False,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Turn q and k by their tokens' positions.
+
+    q          fp16 or bf16 [T, H, D]; k [T, H_kv, D]; any strides
+    positions  int32 / int64 [T], or with ``sections`` [len(sections), T]
+    inv_freq   fp32 [R/2], R <= D: the angle per position of each pair
+    sections   pairs of each axis, up to four, which sum to R/2: the first ``sections[0]`` pairs take
+               axis 0, the next ``sections[1]`` axis 1, ...; with ``mixed_sections`` pair i takes axis
+               ``i % axes`` as long as that axis has its number, and axis 0 from there on
+    adjacent_pairs
+               pairs are dims 2i and 2i + 1 instead of i and i + R/2
+    inplace    write into q and k themselves (their rows must not overlap)
+
+    Returns ``(q, k)``, turned.
+    """
+    code = _check_heads(q, k)
+    _, sections = _check_turn(q.shape[0], q.shape[2], positions, inv_freq, sections, mixed_sections)
+    if inplace:
+        _require(all(x.stride(2) == 1 and _apart(x, (0, 1)) for x in (q, k)),
+                 "q and k must have contiguous rows that do not overlap")
+    _one_device(q, k, positions, inv_freq)
+    if inplace:
+        q_out, k_out = q, k
+    else:
+        q, k = _dense(q), _dense(k)
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    if q.shape[0] > 0:
+        args = _args(q, k, q_out, positions, inv_freq, sections, mixed_sections, adjacent_pairs,
+                     code)
+        args.k_out, args.k_out_stride_t, args.k_out_stride_h = (k_out.data_ptr(), k_out.stride(0),
+                                                                k_out.stride(1))
+        lib = _lib.load()
+        with torch.cuda.device(q.device):
+            _lib.check(lib.fa_rotary(ctypes.byref(args),
+                                     torch.cuda.current_stream(q.device).cuda_stream))
+    return q_out, k_out
+
+
+def rotary_cache_kv(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    positions: torch.Tensor,
+    inv_freq: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    sections: Optional[Sequence[int]] = None,
+    mixed_sections: bool = False,
+    adjacent_pairs: bool = False,
+) -> torch.Tensor:
+    """Turn q and k by their tokens' positions, and write k and v into the paged cache (in place).
+
+    q, k, positions, inv_freq, sections, mixed_sections, adjacent_pairs
+                  as in ``rotary_embedding``; v [T, H_kv, D]
+    key_cache, value_cache
+                  [num_blocks, H_kv, block_size, D] of q's type, as in ``paged_attention``
+    slot_mapping  int32 / int64 [T]: block * block_size + row of each token; negative slots (padding
+                  tokens) and slots past the cache are skipped.  The slots of one call must differ:
+                  rows that two tokens write are undefined
+
+    Returns the turned ``q``, ready for ``paged_attention`` or, with the packed k and v of a prompt,
+    ``flash_attention_varlen``.
+    """
+    code = _check_heads(q, k)
+    _require(v.shape == k.shape and v.dtype == k.dtype, "k and v shapes or dtypes differ")
+    tokens, _, d = q.shape
+    _, sections = _check_turn(tokens, d, positions, inv_freq, sections, mixed_sections)
+    _require(key_cache.dim() == 4 and value_cache.shape == key_cache.shape
+             and key_cache.shape[1] == k.shape[1] and key_cache.shape[3] == d,
+             "key_cache / value_cache must be [num_blocks, num_kv_heads, block_size, head_size]")
+    _require(key_cache.dtype == q.dtype and value_cache.dtype == q.dtype,
+             "the cache's dtype differs from q's")
+    _require(1 <= key_cache.shape[0] < 1 << 31 and 1 <= key_cache.shape[2] < 1 << 31,
+             "the cache is empty or has too many blocks")
+    _require(all(c.stride(3) == 1 and _apart(c, (0, 1, 2)) for c in (key_cache, value_cache)),
+             "rows of the cache must be contiguous and not overlap")
+    _require(slot_mapping.dim() == 1 and slot_mapping.shape[0] == tokens
+             and slot_mapping.dtype in (torch.int32, torch.int64),
+             "slot_mapping must be int32 / int64 [num_tokens]")
+    _one_device(q, k, v, positions, inv_freq, key_cache, value_cache, slot_mapping)
+    q, k, v = _dense(q), _dense(k), _dense(v)
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if tokens > 0:
+        slots = slot_mapping.contiguous()
+        args = _args(q, k, q_out, positions, inv_freq, sections, mixed_sections, adjacent_pairs,
+                     code)
+        args.v, args.v_stride_t, args.v_stride_h = v.data_ptr(), v.stride(0), v.stride(1)
+        args.key_cache, args.value_cache = key_cache.data_ptr(), value_cache.data_ptr()
+        args.kc_stride_0, args.kc_stride_h, args.kc_stride_t = key_cache.stride()[:3]
+        args.vc_stride_0, args.vc_stride_h, args.vc_stride_t = value_cache.stride()[:3]
+        args.num_blocks, args.block_size = key_cache.shape[0], key_cache.shape[2]
+        args.slots, args.slots64 = slots.data_ptr(), int(slots.dtype == torch.int64)
+        lib = _lib.load()
+        with torch.cuda.device(q.device):
+            _lib.check(lib.fa_rotary(ctypes.byref(args),
+                                     torch.cuda.current_stream(q.device).cuda_stream))
+    return q_out
