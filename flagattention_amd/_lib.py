@@ -249,12 +249,14 @@ class LinearArgs(ctypes.Structure):
         ("state_indices", ctypes.c_void_p),
         ("has_state", ctypes.c_void_p),
         ("out", ctypes.c_void_p),
+        ("part", ctypes.c_void_p),
         ("num_slots", ctypes.c_int32),
         ("num_seqs", ctypes.c_int32),
         ("total", ctypes.c_int32),
         ("h_q", ctypes.c_int32),
         ("h_kv", ctypes.c_int32),
         ("d", ctypes.c_int32),
+        ("segment", ctypes.c_int32),
         ("scale", ctypes.c_float),
         ("dtype", ctypes.c_int32),
     ]
@@ -321,6 +323,8 @@ SIGNATURES = {
     "fa_rotary_args_size": (ctypes.c_int64, []),
     "fa_rotary": (ctypes.c_int, [ctypes.POINTER(RotaryArgs), ctypes.c_void_p]),
     "fa_linear_args_size": (ctypes.c_int64, []),
+    "fa_linear_plan": (
+        ctypes.c_int64, [ctypes.POINTER(LinearArgs), ctypes.c_int32, ctypes.c_int32]),
     "fa_linear_prompt": (ctypes.c_int, [ctypes.POINTER(LinearArgs), ctypes.c_void_p]),
     "fa_linear_token": (ctypes.c_int, [ctypes.POINTER(LinearArgs), ctypes.c_void_p]),
 }

@@ -23,6 +23,7 @@ __device__ inline Fall fall_of(float a, int n) {
   return Fall{n == 0 ? 0.f : slow ? expm1f(x) : expf(x), slow || n == 0};
 }
 
+int check_linear_shape(const fa_linear_args& a);
 int check_linear(const fa_linear_args& a);
 
 }  // namespace fa

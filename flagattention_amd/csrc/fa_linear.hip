@@ -16,9 +16,12 @@
 // Bound by q, k, v and out.  Inputs come three chunks deep into LDS.
 //
 // Rounding: scores, sums and states are fp32.  P and the state's copy are rounded to the input type to
-// meet V and Q, as the output is.  The weighted values that a state takes in are split in two such
-// numbers, whose rest is 2^-16: the state is an output in fp32.  fp16 operands are taken relative to a
+// meet V and Q, as the output is.  The weighted values that a state takes in are split in three bf16 or
+// two fp16 numbers, which hold 24 and 22 bits: the state is an output in fp32 (two bf16 numbers left
+// it 2e-6 from 64 bits, three 2e-7).  fp16 operands are taken relative to a
 // power of two of the largest, since states, scores and products of tiny inputs leave its range.
+#include <algorithm>
+
 #include "fa_common.h"
 #include "fa_divide.h"
 #include "fa_linear.h"
@@ -28,7 +31,7 @@
 
 namespace fa {
 
-int check_linear(const fa_linear_args& a) {
+int check_linear_shape(const fa_linear_args& a) {
   FA_CHECK_ARG(a.d == 64 || a.d == 128 || a.d == 256, "head dim %d is not 64, 128 or 256", a.d);
   FA_CHECK_ARG(a.dtype == 0 || a.dtype == 1, "dtype %d", a.dtype);
   FA_CHECK_ARG(a.h_kv >= 1 && a.h_q >= 1 && a.h_q % a.h_kv == 0,
@@ -36,6 +39,12 @@ int check_linear(const fa_linear_args& a) {
   FA_CHECK_ARG(static_cast<int64_t>(a.h_q) * a.d < 1 << 23, "too many heads");
   FA_CHECK_ARG(a.num_seqs >= 0 && a.num_seqs <= 65535 && a.total >= 0,
                "%d sequences, %d tokens out of range", a.num_seqs, a.total);
+  return FA_OK;
+}
+
+int check_linear(const fa_linear_args& a) {
+  const int rc = check_linear_shape(a);
+  if (rc != FA_OK) return rc;
   if (a.total > 0) {
     FA_CHECK_ARG(a.q && a.k && a.v && a.log_decay && a.out, "NULL pointer");
     for (const void* p : {a.q, a.k, a.v, static_cast<const void*>(a.out)})
@@ -77,11 +86,83 @@ __device__ inline void sync() {
   asm volatile("" ::: "memory");
 }
 
+// Largest |x| of packed 16-bit values as unsigned bit patterns, folded into best.
+__device__ inline void fold_bits(unsigned int& best, uintx4 w) {
+  typedef unsigned short ushortx2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    best = __builtin_bit_cast(
+        unsigned int, __builtin_elementwise_max(__builtin_bit_cast(ushortx2, best),
+                                                __builtin_bit_cast(ushortx2, w[i] & 0x7FFF7FFFu)));
+}
+// Whether an infinity or a NaN is among them.
+template <typename T>
+__device__ inline bool is_odd(unsigned int best) {
+  constexpr unsigned int kInf = __is_same(T, __bf16) ? 0x7F80u : 0x7C00u;
+  return (best & 0xFFFFu) >= kInf || (best >> 16) >= kInf;
+}
+
+// The upper 8 bits of a float's 24 as a float, and those of two as bf16.
+__device__ inline float upper_of(float x) {
+  return __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
+}
+__device__ inline unsigned int upper_halves(float x, float y) {
+  return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+}
+
 // Power of two above |x|, 0 for 0, infinities and NaN.
 __device__ inline int power_of(float x) { return __builtin_amdgcn_frexp_expf(x); }
 __device__ inline float times_power(float x, int e) { return __builtin_amdgcn_ldexpf(x, e); }
 
-template <typename T, int D>
+// A run of tokens that a work-group takes: a sequence, or a segment of one.
+struct Run {
+  int seq;       // -1: none
+  int part;      // segment of the sequence
+  int start, n;  // first packed token, tokens
+  bool last;     // of its sequence
+};
+
+// Run `index` of the launch.  With segments of L tokens those of sequence s have the indices
+// start_s / L + s and on: a sequence of n tokens has ceil(n / L) of them, and the next sequence's start
+// is at least that far on.  The sequence is the last one whose first index is not past `index`; a
+// wave looks at 64 at a time.
+__device__ inline Run find_run(const fa_linear_args& a, int index) {
+  Run run = {-1, 0, 0, 0, true};
+  int seq = index;
+  if (a.segment > 0) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, hi = a.num_seqs;
+    while (hi > lo + 1 || lo == 0) {
+      const int step = cdiv(hi - lo, 64);
+      const int s = lo + lane * step;
+      const bool before =
+          s < hi && min(max(a.cu_seqlens[s], 0), a.total) / a.segment + s <= index;
+      const int count = __popcll(__ballot(before));
+      if (count == 0) return run;  // in front of the first
+      lo += (count - 1) * step;
+      hi = min(lo + step, hi);
+      if (step == 1) break;
+    }
+    seq = uniform(lo);
+  }
+  if (seq >= a.num_seqs) return run;
+  const int start = min(max(sload(a.cu_seqlens + seq), 0), a.total);
+  const int n = min(max(sload(a.cu_seqlens + seq + 1), start), a.total) - start;
+  if (a.segment > 0) {
+    run.part = index - (start / a.segment + seq);
+    if (run.part < 0 || run.part > (n - 1) / a.segment) return run;  // (< 0: starts that fall)
+  }
+  if (n == 0) return run;
+  const int from = run.part * a.segment;
+  run.seq = seq;
+  run.start = start + from;
+  run.n = a.segment > 0 ? min(n - from, a.segment) : n;
+  run.last = from + run.n == n;
+  return run;
+}
+
+// kStates: only the states that segments make, each from zeros (the first from its sequence's).
+template <typename T, int D, bool kStates>
 __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a,
                                                           const Divisor h_kv) {
   typedef typename PVec<T>::v8 T8;
@@ -94,19 +175,23 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
   constexpr int kRowsPerCopy = 512 / D;
   constexpr int kKSteps = D / 16;
   constexpr int kTiles = D / 32;
+  constexpr int kTerms = kHalf ? 2 : 3;  // 22 and 24 bits
+  constexpr int kGroupSteps = D == 256 ? 2 : 4;  // of a product of rows, read at once
   static_assert(kCopies * kTiles * 1024 == kTileB, "whole copies per wave");
-  // [q, k, v][stage]
-  __shared__ __attribute__((aligned(16))) unsigned char bufs[3 * kStages * kTileB];
+  // [k, v, q][stage]
+  __shared__ __attribute__((aligned(16))) unsigned char bufs[(kStates ? 2 : 3) * kStages * kTileB];
+  // weights by the place m of a token before the chunk's last: scale e^{a (31 - m)}, 0 past 31 (tokens
+  // to come); and e^{a (31 - m)}, 1 past 31
+  __shared__ float seen[2 * kChunk], left_of[2 * kChunk];
 
   const int wave = wave_id();
   const int lane = threadIdx.x & 63;
   const int h = lane >> 5, c32 = lane & 31;
-  const int group = a.h_q / a.h_kv;
+  const int group = kStates ? 1 : a.h_q / a.h_kv;
 
-  // rows of no sequence: everybody takes a share of their 16 bytes
-  {
-    const int first = min(max(a.cu_seqlens[0], 0), a.total);
-    const int behind = max(first, min(max(a.cu_seqlens[a.num_seqs], 0), a.total));
+  if constexpr (!kStates) {  // rows of no sequence: everybody takes a share of their 16 bytes
+    const int first = min(max(sload(a.cu_seqlens), 0), a.total);
+    const int behind = max(first, min(max(sload(a.cu_seqlens + a.num_seqs), 0), a.total));
     const long long row16 = static_cast<long long>(a.h_q) * C;
     const long long head = first * row16, all = a.total * row16, tail = behind * row16;
     uintx4* const out16 = static_cast<uintx4*>(a.out);
@@ -116,30 +201,35 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
     for (long long i = tail + me; i < all; i += step) out16[i] = uintx4{0, 0, 0, 0};
   }
 
-  const int seq = divide(blockIdx.x, h_kv);
-  const int hk = blockIdx.x - seq * a.h_kv;
-  if (seq >= a.num_seqs) return;  // uniform
-  const int start = min(max(sload(a.cu_seqlens + seq), 0), a.total);
-  const int n = min(max(sload(a.cu_seqlens + seq + 1), start), a.total) - start;
-  if (n == 0) return;
+  const int index = divide(blockIdx.x, h_kv);
+  const int hk = blockIdx.x - index * a.h_kv;
+  const Run run = find_run(a, index);
+  if (run.seq < 0 || (kStates && run.last)) return;  // uniform
+  const int n = run.n;
   const float log_decay = sload(a.log_decay + hk);
-  float* state = nullptr;  // where the state stays
-  bool kept = false;
+  float* slot_state = nullptr;  // the sequence's
   if (a.state) {
-    const int slot = a.state_indices ? sload(a.state_indices + seq) : seq;
-    if (slot >= 0 && slot < a.num_slots) {
-      state = a.state + slot * a.state_stride_s + hk * a.state_stride_h;
-      kept = a.has_state == nullptr || a.has_state[seq] != 0;
-    }
+    const int slot = a.state_indices ? sload(a.state_indices + run.seq) : run.seq;
+    if (slot >= 0 && slot < a.num_slots)
+      slot_state = a.state + slot * a.state_stride_s + hk * a.state_stride_h;
   }
+  // where the run starts from, and where it leaves its state
+  const float* from_state = nullptr;
+  if (run.part > 0)
+    from_state = kStates ? nullptr
+                         : a.part + (static_cast<long long>(index - 1) * a.h_kv + hk) * (D * D);
+  else if (slot_state && (a.has_state == nullptr || a.has_state[run.seq] != 0))
+    from_state = slot_state;
+  float* const to_state = kStates ? a.part + (static_cast<long long>(index) * a.h_kv + hk) * (D * D)
+                                  : run.last ? slot_state : nullptr;
 
   const unsigned char* const qp =
       static_cast<const unsigned char*>(a.q) +
-      2 * (start * a.q_stride_t + static_cast<long long>(hk) * group * a.q_stride_h);
+      2 * (run.start * a.q_stride_t + static_cast<long long>(hk) * group * a.q_stride_h);
   const unsigned char* const kp = static_cast<const unsigned char*>(a.k) +
-                                  2 * (start * a.k_stride_t + hk * a.k_stride_h);
+                                  2 * (run.start * a.k_stride_t + hk * a.k_stride_h);
   const unsigned char* const vp = static_cast<const unsigned char*>(a.v) +
-                                  2 * (start * a.v_stride_t + hk * a.v_stride_h);
+                                  2 * (run.start * a.v_stride_t + hk * a.v_stride_h);
   const unsigned int q_tb = 2 * a.q_stride_t, k_tb = 2 * a.k_stride_t, v_tb = 2 * a.v_stride_t;
 
   // Items are (chunk, query head of the group), heads innermost; k and v come with the first head.
@@ -161,10 +251,11 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
   int next_item = 0, next_head = 0, next_chunk = 0, next_q = 0, next_kv = 0;
   auto fetch = [&]() {
     if (next_item >= items) return;
-    copy(qp + 2 * next_head * a.q_stride_h, q_tb, next_chunk * kChunk, tile(0, next_q));
+    if (!kStates)
+      copy(qp + 2 * next_head * a.q_stride_h, q_tb, next_chunk * kChunk, tile(2, next_q));
     if (next_head == 0) {
-      copy(kp, k_tb, next_chunk * kChunk, tile(1, next_kv));
-      copy(vp, v_tb, next_chunk * kChunk, tile(2, next_kv));
+      copy(kp, k_tb, next_chunk * kChunk, tile(0, next_kv));
+      copy(vp, v_tb, next_chunk * kChunk, tile(1, next_kv));
     }
     ++next_item;
     next_q = next_q == kStages - 1 ? 0 : next_q + 1;
@@ -180,28 +271,30 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
   // Row rho of a 32-row tile of the state (or of O^T) is dim 16 (rho / 16) + 8 ((rho / 4) % 2) +
   // 4 ((rho / 8) % 2) + rho % 4: accumulator register r of half h is then dim 16 (r / 8) + 8h + r % 8.
   const int pi = (c32 & 16) + 8 * ((c32 >> 2) & 1) + 4 * ((c32 >> 3) & 1) + (c32 & 3);
+  const int state_at = 8 * h * D + 32 * wave + pi;
   floatx16 s[kTiles];
-  {
-    const float* const from = state + 32 * wave + pi;
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t)
+  for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        s[t][r] = kept ? from[(32 * t + 16 * (r >> 3) + 8 * h + (r & 7)) * D] : 0.f;
-  }
+    for (int r = 0; r < 16; ++r)
+      s[t][r] = from_state ? from_state[state_at + (32 * t + 16 * (r >> 3) + (r & 7)) * D] : 0.f;
 
-  // Token of register r in P^T's rows, and of element r of the values' operands.
-  auto token = [&](int r) { return 8 * (r >> 2) + 4 * h + (r & 3); };
-  float wp[16], wv[16];
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int j = token(r);
-    wp[r] = j <= c32 ? a.scale * decay(log_decay, c32 - j) : 0.f;
-    wv[r] = decay(log_decay, kChunk - 1 - j);
+  if (threadIdx.x < 2 * kChunk) {
+    const int m = threadIdx.x;
+    const float e = decay(log_decay, max(kChunk - 1 - m, 0));
+    seen[m] = m < kChunk ? a.scale * e : 0.f;
+    left_of[m] = e;
   }
+  // The state is s times sigma = e^{a reset}, reset the tokens since s was last brought up: a product
+  // of a whole state only where sigma has fallen by 16 (or grown, for a > 0), and no rounding of a
+  // factor next to 1 at every chunk.
+  const float log2_decay = log_decay * kLog2e;
+  int reset = 0;
+  float sigma = 1.f;
   const float since = a.scale * decay(log_decay, c32 + 1);
-  Fall fall = fall_of(log_decay, kChunk);
 
+  // Token of register r in P^T's rows, and of element r of the values' operands, less 4h.
+  auto token = [&](int r) { return 8 * (r >> 2) + (r & 3); };
   const int row_at = c32 * kRowB + 16 * (h ^ swizzle<C>(c32));
   // transposed reads: lanes 4e + x of 16 point at 4 dims of token row e
   const int e = (lane & 15) >> 2, x4 = lane & 3, p16 = (lane >> 4) & 1;
@@ -217,14 +310,16 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
   int item = 0, q_stage = 0, kv_stage = 0;
   for (int chunk = 0; chunk < chunks; ++chunk) {
     const int left = min(n - chunk * kChunk, kChunk);
-    unsigned char* const kb = tile(1, kv_stage);
-    unsigned char* const vb = tile(2, kv_stage);
+    unsigned char* const kb = tile(0, kv_stage);
+    unsigned char* const vb = tile(1, kv_stage);
     T8 va[2];
     bool odd = false;
     for (int g = 0; g < group; ++g, ++item) {
       // all but what was issued after this item's copies: the next item's, and the last one's stores
       if (item + 1 < items && item > 0) {
-        if (g + 1 == group)
+        if (kStates)
+          wait_vmem<2 * kCopies>();
+        else if (g + 1 == group)
           wait_vmem<3 * kCopies + 2>();
         else
           wait_vmem<kCopies + 2>();
@@ -233,8 +328,6 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
       }
       sync();
       fetch();
-      const unsigned char* const qb = tile(0, q_stage);
-      q_stage = q_stage == kStages - 1 ? 0 : q_stage + 1;
       if (g == 0) {
         if (left < kChunk) {  // uniform: rows past the end become zeros
           for (int i = left * kRowB / 16 + threadIdx.x; i < kTileB / 16; i += 2 * D) {
@@ -244,17 +337,23 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
           sync();
         }
         // An infinity or a NaN in v would reach the tokens before its own through weights of 0.
-        bool is_odd = false;
+        unsigned int best = 0u;
 #pragma unroll
         for (int ss = 0; ss < 2; ++ss) {
           va[ss] = transposed(vb, wave, ss);
-#pragma unroll
-          for (int x = 0; x < 8; ++x)
-            is_odd |= !(fabsf(static_cast<float>(va[ss][x])) < __builtin_inff());
+          fold_bits(best, __builtin_bit_cast(uintx4, va[ss]));
         }
-        odd = __ballot(is_odd) != 0ull;
+        odd = __ballot(is_odd<T>(best)) != 0ull;  // uniform
+      }
+      if constexpr (kStates) continue;
+      // the state's copy is made afresh for every head: kept, its registers would be spilled
+      if constexpr (D == 256) {
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) asm volatile("" : "+v"(s[t]));
       }
 
+      const unsigned char* const qb = tile(2, q_stage);
+      q_stage = q_stage == kStages - 1 ? 0 : q_stage + 1;
       // scores and S^T Q^T: a step of Q meets both
       int s_power = 0, p_power = 0;
       if constexpr (kHalf) {
@@ -275,22 +374,47 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
         for (int m = 1; m < 64; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
         s_power = max(power_of(most), kLeastPower);
       }
+      // A group of steps is read while the last one is multiplied.
       floatx16 p = {}, o = {};
+      T8 qa[2][kGroupSteps], ka[2][kGroupSteps];
+      auto read = [&](int i) {
 #pragma unroll
-      for (int ks = 0; ks < kKSteps; ++ks) {
-        const T8 qa = *reinterpret_cast<const T8*>(qb + (row_at ^ (32 * ks)));
-        const T8 ka = *reinterpret_cast<const T8*>(kb + (row_at ^ (32 * ks)));
-        p = mfma_32x32x16(ka, qa, p);
-        T8 sa;
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const float f = s[ks >> 1][8 * (ks & 1) + x];
-          sa[x] = static_cast<T>(kHalf ? times_power(f, -s_power) : f);
+        for (int x = 0; x < kGroupSteps; ++x) {
+          const int at = row_at ^ (32 * (kGroupSteps * i + x));
+          ka[i & 1][x] = *reinterpret_cast<const T8*>(kb + at);
+          qa[i & 1][x] = *reinterpret_cast<const T8*>(qb + at);
         }
-        o = mfma_32x32x16(sa, qa, o);
-      }
+      };
+      read(0);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) p[r] = token(r) <= c32 ? p[r] * wp[r] : 0.f;
+      for (int i = 0; i < kKSteps / kGroupSteps; ++i) {
+        if (i + 1 < kKSteps / kGroupSteps) read(i + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int x = 0; x < kGroupSteps; ++x) {
+          const int ks = kGroupSteps * i + x;
+          p = mfma_32x32x16(ka[i & 1][x], qa[i & 1][x], p);
+          T8 sa;
+#pragma unroll
+          for (int y = 0; y < 8; ++y) {
+            const float f = s[ks >> 1][8 * (ks & 1) + y];
+            sa[y] = static_cast<T>(kHalf ? times_power(f, -s_power) : f);
+          }
+          o = mfma_32x32x16(sa, qa[i & 1][x], o);
+        }
+      }
+      // A score that is not finite would reach the tokens before its own through weights of 0.
+      floatx4 trace = {0.f, 0.f, 0.f, 0.f};
+      const float* const weight = seen + kChunk - 1 - c32 + 4 * h;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        p[r] *= weight[token(r)];
+        trace[r & 3] = __builtin_fmaf(p[r], 0.f, trace[r & 3]);
+      }
+      if (__ballot((trace[0] + trace[1]) + (trace[2] + trace[3]) != 0.f) != 0ull) {  // uniform
+#pragma unroll
+        for (int r = 0; r < 16; ++r) p[r] = token(r) + 4 * h <= c32 ? p[r] : 0.f;
+      }
       if constexpr (kHalf) {
         float top = 0.f;
 #pragma unroll
@@ -298,7 +422,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
         p_power = max(power_of(max_xor32(top)), kLeastPower);
       }
       // O^T, relative to 2^p_power
-      const float by = kHalf ? times_power(since, s_power - p_power) : since;
+      const float by = kHalf ? times_power(since * sigma, s_power - p_power) : since * sigma;
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[r] *= by;
 #pragma unroll
@@ -310,6 +434,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
           pb[x] = static_cast<T>(kHalf ? times_power(f, -p_power) : f);
         }
         if (odd) {  // uniform
+          asm volatile("" ::: "memory");
 #pragma unroll
           for (int x = 0; x < 8; ++x)
             v8[x] = fabsf(static_cast<float>(v8[x])) < __builtin_inff() ? v8[x]
@@ -325,7 +450,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
         for (int j = 0; j < left; ++j) {
           float w = 0.f;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) w = 8 * (r >> 2) + (r & 3) == (j & ~4) ? p[r] : w;
+          for (int r = 0; r < 16; ++r) w = token(r) == (j & ~4) ? p[r] : w;
           w = __shfl(w, c32 + 32 * ((j >> 2) & 1));
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
@@ -341,7 +466,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
       }
 
       T* const out = static_cast<T*>(a.out) +
-                     ((static_cast<long long>(start) + chunk * kChunk + c32) * a.h_q +
+                     ((static_cast<long long>(run.start) + chunk * kChunk + c32) * a.h_q +
                       hk * group + g) * D + 32 * wave + 8 * h;
       if (c32 < left) {
 #pragma unroll
@@ -353,85 +478,162 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
         }
       }
     }
-    if (chunk + 1 == chunks && state == nullptr) break;
+    if (chunk + 1 == chunks && to_state == nullptr) break;
 
-    if (left < kChunk) {
+    T8 kt[2][2];  // K^T of a tile of the state, the next one on its way
+    kt[0][0] = transposed(kb, 0, 0);
+    kt[0][1] = transposed(kb, 0, 1);
+    reset += left;
+    sigma = __builtin_amdgcn_exp2f(log2_decay * static_cast<float>(reset));
+    float against = __builtin_amdgcn_exp2f(-log2_decay * static_cast<float>(reset));  // 1 / sigma
+    if (!(sigma >= 0.0625f && sigma <= 16.f)) {  // uniform
 #pragma unroll
-      for (int r = 0; r < 16; ++r) wv[r] = decay(log_decay, max(left - 1 - token(r), 0));
-      fall = fall_of(log_decay, left);
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[t][r] *= sigma;
+      reset = 0;
+      sigma = against = 1.f;
     }
-    T8 hi[2], lo[2];
+    // the weighted values, each as a sum of kTerms numbers of the type
+    const float* const weight = left_of + kChunk - left + 4 * h;
+    T8 part[kTerms][2];
+    float f[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      f[r] = static_cast<float>(va[r >> 3][r & 7]) * (weight[token(r)] * against);
     int v_power = 0;
     if constexpr (kHalf) {
       float top = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        top = fmaxf(top, fabsf(static_cast<float>(va[r >> 3][r & 7]) * wv[r]));
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(f[r]));
       v_power = max(power_of(max_xor32(top)), -100);
     }
+    if constexpr (kHalf) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      float f = static_cast<float>(va[r >> 3][r & 7]) * wv[r];
-      if (kHalf) f = times_power(f, -v_power);
-      hi[r >> 3][r & 7] = static_cast<T>(f);
-      lo[r >> 3][r & 7] = static_cast<T>(f - static_cast<float>(hi[r >> 3][r & 7]));
+      for (int r = 0; r < 16; ++r) {
+        const float x = times_power(f[r], -v_power);
+        part[0][r >> 3][r & 7] = static_cast<T>(x);
+        part[1][r >> 3][r & 7] = static_cast<T>(x - static_cast<float>(part[0][r >> 3][r & 7]));
+      }
+    } else {  // the upper 8 bits, the next 8, the rest
+#pragma unroll
+      for (int ss = 0; ss < 2; ++ss) {
+        uintx4 upper, next, rest;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          float y = f[8 * ss + 2 * x], z = f[8 * ss + 2 * x + 1];
+          upper[x] = upper_halves(y, z);
+          y -= upper_of(y), z -= upper_of(z);
+          next[x] = upper_halves(y, z);
+          y -= upper_of(y), z -= upper_of(z);
+          rest[x] = upper_halves(y, z);
+        }
+        part[0][ss] = __builtin_bit_cast(T8, upper);
+        part[1][ss] = __builtin_bit_cast(T8, next);
+        part[2][ss] = __builtin_bit_cast(T8, rest);
+      }
     }
-    if (odd) {
+    if (odd) {  // what is not finite has no rest
+      asm volatile("" ::: "memory");  // a branch: it is rarely taken
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        if (!(fabsf(static_cast<float>(hi[r >> 3][r & 7])) < __builtin_inff()))
-          lo[r >> 3][r & 7] = static_cast<T>(0.f);
-    }
-    if (fall.slow) {  // uniform
+        if (!(fabsf(static_cast<float>(part[0][r >> 3][r & 7])) < __builtin_inff()))
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[t][r] = __builtin_fmaf(s[t][r], fall.by, s[t][r]);
-    } else {
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[t][r] *= fall.by;
+          for (int x = 1; x < kTerms; ++x) part[x][r >> 3][r & 7] = static_cast<T>(0.f);
     }
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
-      if constexpr (kHalf) {
-        floatx16 add = {};
+      if (t + 1 < kTiles) {
+        kt[(t + 1) & 1][0] = transposed(kb, t + 1, 0);
+        kt[(t + 1) & 1][1] = transposed(kb, t + 1, 1);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      floatx16 add = {};
 #pragma unroll
-        for (int ss = 0; ss < 2; ++ss) {
-          const T8 ka = transposed(kb, t, ss);
-          add = mfma_32x32x16(ka, hi[ss], add);
-          add = mfma_32x32x16(ka, lo[ss], add);
+      for (int ss = 0; ss < 2; ++ss) {
+#pragma unroll
+        for (int x = 0; x < kTerms; ++x) {
+          if (kHalf)
+            add = mfma_32x32x16(kt[t & 1][ss], part[x][ss], add);
+          else
+            s[t] = mfma_32x32x16(kt[t & 1][ss], part[x][ss], s[t]);
         }
+      }
+      if constexpr (kHalf) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[t][r] += times_power(add[r], v_power);
-      } else {
-#pragma unroll
-        for (int ss = 0; ss < 2; ++ss) {
-          const T8 ka = transposed(kb, t, ss);
-          s[t] = mfma_32x32x16(ka, hi[ss], s[t]);
-          s[t] = mfma_32x32x16(ka, lo[ss], s[t]);
-        }
       }
     }
     kv_stage = kv_stage == kStages - 1 ? 0 : kv_stage + 1;
   }
 
-  if (state != nullptr) {
-    float* const to = state + 32 * wave + pi;
+  if (to_state != nullptr) {
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        to[(32 * t + 16 * (r >> 3) + 8 * h + (r & 7)) * D] = s[t][r];
+        to_state[state_at + (32 * t + 16 * (r >> 3) + (r & 7)) * D] = s[t][r] * sigma;
   }
+}
+
+// The segments' states, each on top of the one before: part[i] += e^{a L} part[i - 1].
+template <int D>
+__global__ __launch_bounds__(256) void join_kernel(const fa_linear_args a, const Divisor h_kv) {
+  constexpr int kAhead = 8;
+  const int seq = divide(blockIdx.x, h_kv);
+  const int hk = blockIdx.x - seq * a.h_kv;
+  const int start = min(max(sload(a.cu_seqlens + seq), 0), a.total);
+  const int n = min(max(sload(a.cu_seqlens + seq + 1), start), a.total) - start;
+  const int states = n == 0 ? 0 : (n - 1) / a.segment;  // of all segments but the last
+  if (states < 2) return;
+  const long long step = static_cast<long long>(a.h_kv) * (D * D) / 4;
+  floatx4* at = reinterpret_cast<floatx4*>(a.part) +
+                (static_cast<long long>(start / a.segment + seq) * a.h_kv + hk) * (D * D / 4) +
+                blockIdx.y * 256 + threadIdx.x;
+  const float fall = decay(sload(a.log_decay + hk), a.segment);
+  floatx4 sum = *at;
+  for (int i = 1; i < states; i += kAhead) {
+    floatx4 next[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (i + j < states) next[j] = at[(j + 1) * step];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (i + j < states) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sum[x] = __builtin_fmaf(sum[x], fall, next[j][x]);
+        at[(j + 1) * step] = sum;
+      }
+    }
+    at += kAhead * step;
+  }
+}
+
+// Indices of runs in a launch (find_run).
+int runs_of(const fa_linear_args& a) {
+  const int seqs = a.num_seqs > 0 ? a.num_seqs : 1;  // rows of no sequence are there too
+  return a.segment > 0 ? a.total / a.segment + seqs : seqs;
+}
+
+// Tokens of a segment, 0 for whole sequences.
+int choose_segment(const fa_linear_args& a, int max_seqlen, int cus) {
+  const int resident = cus * (a.d == 64 ? 4 : a.d == 128 ? 2 : 1);  // work-groups at once
+  const int64_t each = static_cast<int64_t>(std::min(a.total, max_seqlen > 0 ? a.total : 0)) * a.h_kv / resident;
+  const int64_t segment = (std::max<int64_t>(each, 256) + kChunk - 1) / kChunk * kChunk;
+  if (max_seqlen <= 2 * segment) return 0;
+  return static_cast<int>(segment);
 }
 
 template <typename T, int D>
 void launch(const fa_linear_args& a, hipStream_t stream) {
-  const int seqs = a.num_seqs > 0 ? a.num_seqs : 1;  // rows of no sequence are there too
-  hipLaunchKernelGGL((linear_kernel<T, D>), dim3(static_cast<unsigned>(seqs * a.h_kv)), dim3(2 * D),
-                     0, stream, a, divisor(a.h_kv));
+  const dim3 grid(static_cast<unsigned>(runs_of(a) * a.h_kv));
+  const Divisor h_kv = divisor(a.h_kv);
+  if (a.segment > 0) {
+    hipLaunchKernelGGL((linear_kernel<T, D, true>), grid, dim3(2 * D), 0, stream, a, h_kv);
+    hipLaunchKernelGGL((join_kernel<D>), dim3(static_cast<unsigned>(a.num_seqs * a.h_kv), D * D / 1024),
+                       dim3(256), 0, stream, a, h_kv);
+  }
+  hipLaunchKernelGGL((linear_kernel<T, D, false>), grid, dim3(2 * D), 0, stream, a, h_kv);
 }
 
 }  // namespace
@@ -441,13 +643,28 @@ extern "C" int64_t fa_linear_args_size(void) {
   return static_cast<int64_t>(sizeof(fa_linear_args));
 }
 
+extern "C" int64_t fa_linear_plan(fa_linear_args* args, int32_t max_seqlen, int32_t cu_count) {
+  FA_CHECK_ARG(args != nullptr, "args is NULL");
+  fa_linear_args& a = *args;
+  const int rc = fa::check_linear_shape(a);
+  if (rc != FA_OK) return rc;
+  FA_CHECK_ARG(max_seqlen >= 0 && cu_count >= 1, "max_seqlen %d, %d CUs", max_seqlen, cu_count);
+  a.segment = fa::choose_segment(a, max_seqlen, cu_count);
+  return a.segment > 0 ? static_cast<int64_t>(fa::runs_of(a)) * a.h_kv * a.d * a.d : 0;
+}
+
 extern "C" int fa_linear_prompt(const fa_linear_args* args, void* stream) {
   FA_CHECK_ARG(args != nullptr, "args is NULL");
   const fa_linear_args& a = *args;
   const int rc = fa::check_linear(a);
   if (rc != FA_OK) return rc;
-  FA_CHECK_ARG(static_cast<int64_t>(a.num_seqs) * a.h_kv < 1 << 22, "too many sequences or heads");
+  FA_CHECK_ARG(a.segment >= 0 && a.segment % fa::kChunk == 0, "segments of %d tokens", a.segment);
+  FA_CHECK_ARG(a.segment == 0 || a.num_seqs == 0 ||
+                   (a.part && (reinterpret_cast<uintptr_t>(a.part) & 15) == 0),
+               "part is NULL or not 16-byte aligned");
   FA_CHECK_ARG(a.total <= INT32_MAX - 256, "too many tokens");
+  FA_CHECK_ARG((static_cast<int64_t>(a.segment > 0 ? a.total / a.segment : 0) + a.num_seqs) * a.h_kv <
+                   1 << 22, "too many sequences or heads");
   if (a.total == 0) return FA_OK;
   FA_CHECK_ARG(a.cu_seqlens != nullptr, "cu_seqlens is NULL");
   const hipStream_t s = static_cast<hipStream_t>(stream);

@@ -21,7 +21,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .gqa import _aligned, _dtype_code, _require
+from .gqa import _aligned, _cu_count, _dtype_code, _require
 
 HEAD_DIMS = (64, 128, 256)
 
@@ -91,8 +91,9 @@ def _args(q, k, v, log_decay, state, state_indices, out, num_seqs, scale, code):
         state_stride_s=0 if state is None else state.stride(0),
         state_stride_h=0 if state is None else state.stride(1),
         state_indices=None if state_indices is None else state_indices.data_ptr(), has_state=None,
-        out=out.data_ptr(), num_slots=0 if state is None else state.shape[0], num_seqs=num_seqs,
-        total=total, h_q=h_q, h_kv=k.shape[1], d=d, scale=scale, dtype=code)
+        out=out.data_ptr(), part=None, num_slots=0 if state is None else state.shape[0], num_seqs=num_seqs,
+        total=total, h_q=h_q, h_kv=k.shape[1], d=d, segment=0, scale=scale,
+        dtype=code)
 
 
 def _one_device(*tensors):
@@ -161,7 +162,11 @@ def linear_attention_varlen(
         args.cu_seqlens = cu_seqlens.data_ptr()
         args.has_state = None if has_state is None else has_state.data_ptr()
         lib = _lib.load()
+        floats = lib.fa_linear_plan(ctypes.byref(args), min(max_seqlen, total), _cu_count(q.device))
+        _lib.check(min(floats, 0))
         with torch.cuda.device(q.device):
+            part = torch.empty(floats, dtype=torch.float32, device=q.device) if floats > 0 else None
+            args.part = None if part is None else part.data_ptr()
             _lib.check(lib.fa_linear_prompt(ctypes.byref(args),
                                             torch.cuda.current_stream(q.device).cuda_stream))
     return o

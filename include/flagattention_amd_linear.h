@@ -82,13 +82,22 @@ typedef struct fa_linear_args {
   const int32_t* state_indices; /* [num_seqs] or NULL */
   const uint8_t* has_state;     /* [num_seqs] or NULL, fa_linear_prompt only */
   void* out; /* contiguous [total][h_q][d] */
+  float* part; /* workspace of fa_linear_plan's size, 16-byte aligned, where segment > 0 */
   int32_t num_slots, num_seqs, total, h_q, h_kv, d;
+  int32_t segment; /* fa_linear_prompt: tokens that a sequence is cut into, a multiple of 32, or 0 */
   float scale;
   int32_t dtype; /* 0 fp16, 1 bf16 */
 } fa_linear_args;
 
 /* sizeof(fa_linear_args) as compiled into the library. */
 int64_t fa_linear_args_size(void);
+
+/*
+ * Fills in segment, from the totals, heads and head dim of args, for sequences of up to max_seqlen
+ * tokens on a device of cu_count compute units.  Returns the floats that part has to hold (0: none),
+ * or a negative code.
+ */
+int64_t fa_linear_plan(fa_linear_args* args, int32_t max_seqlen, int32_t cu_count);
 
 /*
  * Packed sequences: rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 of q, k and v are sequence s's
