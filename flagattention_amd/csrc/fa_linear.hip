@@ -86,6 +86,14 @@ __device__ inline void sync() {
   asm volatile("" ::: "memory");
 }
 
+// 16 bytes per lane from base + off into LDS at `to`, lane after lane.
+__device__ inline void lds_dma16_at(const unsigned char* base, unsigned int off, unsigned int to) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(off), "s"(base), "s"(to)
+               : "memory", "m0");
+}
+
 // Largest |x| of packed 16-bit values as unsigned bit patterns, folded into best.
 __device__ inline void fold_bits(unsigned int& best, uintx4 w) {
   typedef unsigned short ushortx2 __attribute__((ext_vector_type(2)));
@@ -162,7 +170,8 @@ __device__ inline Run find_run(const fa_linear_args& a, int index) {
 }
 
 // kStates: only the states that segments make, each from zeros (the first from its sequence's).
-template <typename T, int D, bool kStates>
+// kOne: groups of one query head.
+template <typename T, int D, bool kStates, bool kOne>
 __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a,
                                                           const Divisor h_kv) {
   typedef typename PVec<T>::v8 T8;
@@ -177,9 +186,11 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
   constexpr int kTiles = D / 32;
   constexpr int kTerms = kHalf ? 2 : 3;  // 22 and 24 bits
   constexpr int kGroupSteps = D == 256 ? 2 : 4;  // of a product of rows, read at once
+  constexpr bool kEarly = kOne && D <= 128;  // values are split beside the scores' products
+  constexpr bool kKeepQ = D == 64;  // from the scores to S^T Q^T, else it is read twice
   static_assert(kCopies * kTiles * 1024 == kTileB, "whole copies per wave");
   // [k, v, q][stage]
-  __shared__ __attribute__((aligned(16))) unsigned char bufs[(kStates ? 2 : 3) * kStages * kTileB];
+  __shared__ __attribute__((aligned(1024))) unsigned char bufs[(kStates ? 2 : 3) * kStages * kTileB];
   // weights by the place m of a token before the chunk's last: scale e^{a (31 - m)}, 0 past 31 (tokens
   // to come); and e^{a (31 - m)}, 1 past 31
   __shared__ float seen[2 * kChunk], left_of[2 * kChunk];
@@ -187,7 +198,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
   const int wave = wave_id();
   const int lane = threadIdx.x & 63;
   const int h = lane >> 5, c32 = lane & 31;
-  const int group = kStates ? 1 : a.h_q / a.h_kv;
+  const int group = kStates || kOne ? 1 : a.h_q / a.h_kv;
 
   if constexpr (!kStates) {  // rows of no sequence: everybody takes a share of their 16 bytes
     const int first = min(max(sload(a.cu_seqlens), 0), a.total);
@@ -223,61 +234,79 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
   float* const to_state = kStates ? a.part + (static_cast<long long>(index) * a.h_kv + hk) * (D * D)
                                   : run.last ? slot_state : nullptr;
 
-  const unsigned char* const qp =
+  // Items are (chunk, query head of the group), heads innermost; k and v come with the first head.
+  // The next chunk's rows, and q's of its next head.
+  const unsigned char* k_next = static_cast<const unsigned char*>(a.k) +
+                                2 * (run.start * a.k_stride_t + hk * a.k_stride_h);
+  const unsigned char* v_next = static_cast<const unsigned char*>(a.v) +
+                                2 * (run.start * a.v_stride_t + hk * a.v_stride_h);
+  const unsigned char* q_next =
       static_cast<const unsigned char*>(a.q) +
       2 * (run.start * a.q_stride_t + static_cast<long long>(hk) * group * a.q_stride_h);
-  const unsigned char* const kp = static_cast<const unsigned char*>(a.k) +
-                                  2 * (run.start * a.k_stride_t + hk * a.k_stride_h);
-  const unsigned char* const vp = static_cast<const unsigned char*>(a.v) +
-                                  2 * (run.start * a.v_stride_t + hk * a.v_stride_h);
   const unsigned int q_tb = 2 * a.q_stride_t, k_tb = 2 * a.k_stride_t, v_tb = 2 * a.v_stride_t;
-
-  // Items are (chunk, query head of the group), heads innermost; k and v come with the first head.
-  const int chunks = cdiv(n, kChunk);
-  const int items = chunks * group;
-  const int crow = lane / C, cslot = lane % C;
-  auto copy = [&](const unsigned char* src, unsigned int row_b, int first, unsigned char* dst) {
-    const unsigned char* const from = src + static_cast<long long>(first) * row_b;
-    const int last = n - 1 - first;  // rows past the end repeat the last one
+  const long long q_hb = 2 * a.q_stride_h;
+  const long long q_step = static_cast<long long>(kChunk) * q_tb - (group - 1) * q_hb;
+  int copy_row[kCopies], copy_piece[kCopies];
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i) {
+    copy_row[i] = (kCopies * wave + i) * kRowsPerCopy + lane / C;
+    copy_piece[i] = 16 * ((lane % C) ^ swizzle<C>(copy_row[i]));
+  }
+  const unsigned int lds = uniform(static_cast<int>(reinterpret_cast<__SIZE_TYPE__>(
+                               (FA_LDS unsigned char*)bufs))) + kCopies * 1024 * wave;
+  // Rows past the end repeat the last one.  Offsets are worked out afresh: kept for three tensors they
+  // would be spilled, and a wait for one that comes back from memory waits for every copy.
+  auto copy = [&](const unsigned char* from, unsigned int row_b, int rows, unsigned int to) {
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
-      const int r = (kCopies * wave + i) * kRowsPerCopy + crow;
-      lds_dma16_off(from, min(r, last) * row_b + 16 * (cslot ^ swizzle<C>(r)),
-                    (FA_LDS void*)(dst + (kCopies * wave + i) * 1024));
+      int r = copy_row[i];
+      asm volatile("" : "+v"(r));
+      lds_dma16_at(from, __umul24(min(r, rows - 1), row_b) + copy_piece[i], to + 1024 * i);
     }
   };
-  auto tile = [&](int which, int stage) { return bufs + (which * kStages + stage) * kTileB; };
-  // the item to be fetched next
-  int next_item = 0, next_head = 0, next_chunk = 0, next_q = 0, next_kv = 0;
-  auto fetch = [&]() {
-    if (next_item >= items) return;
-    if (!kStates)
-      copy(qp + 2 * next_head * a.q_stride_h, q_tb, next_chunk * kChunk, tile(2, next_q));
-    if (next_head == 0) {
-      copy(kp, k_tb, next_chunk * kChunk, tile(0, next_kv));
-      copy(vp, v_tb, next_chunk * kChunk, tile(1, next_kv));
+  int to_come = n, next_head = 0;  // tokens from the next item's chunk on; its head
+  int next_q = 0, next_kv = 0;     // bytes of its stages
+  // Returns the copies that it issues.
+  auto fetch = [&]() -> int {
+    if (to_come <= 0) return 0;
+    int issued = 0;
+    if (!kStates) {
+      copy(q_next, q_tb, to_come, lds + 2 * kStages * kTileB + next_q);
+      next_q = next_q == (kStages - 1) * kTileB ? 0 : next_q + kTileB;
+      issued += kCopies;
     }
-    ++next_item;
-    next_q = next_q == kStages - 1 ? 0 : next_q + 1;
+    if (next_head == 0) {
+      copy(k_next, k_tb, to_come, lds + next_kv);
+      copy(v_next, v_tb, to_come, lds + kStages * kTileB + next_kv);
+      next_kv = next_kv == (kStages - 1) * kTileB ? 0 : next_kv + kTileB;
+      k_next += kChunk * static_cast<unsigned long long>(k_tb);
+      v_next += kChunk * static_cast<unsigned long long>(v_tb);
+      issued += 2 * kCopies;
+    }
     if (++next_head == group) {
       next_head = 0;
-      ++next_chunk;
-      next_kv = next_kv == kStages - 1 ? 0 : next_kv + 1;
+      to_come -= kChunk;
+      q_next += q_step;
+    } else {
+      q_next += q_hb;
     }
+    return issued;
   };
   fetch();
-  fetch();
+  int ahead = fetch();  // copies on their way after those of the item at hand
 
   // Row rho of a 32-row tile of the state (or of O^T) is dim 16 (rho / 16) + 8 ((rho / 4) % 2) +
   // 4 ((rho / 8) % 2) + rho % 4: accumulator register r of half h is then dim 16 (r / 8) + 8h + r % 8.
   const int pi = (c32 & 16) + 8 * ((c32 >> 2) & 1) + 4 * ((c32 >> 3) & 1) + (c32 & 3);
   const int state_at = 8 * h * D + 32 * wave + pi;
-  floatx16 s[kTiles];
+  floatx16 s[kTiles] = {};
+  if (from_state) {
 #pragma unroll
-  for (int t = 0; t < kTiles; ++t)
+    for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-      s[t][r] = from_state ? from_state[state_at + (32 * t + 16 * (r >> 3) + (r & 7)) * D] : 0.f;
+      for (int r = 0; r < 16; ++r)
+        s[t][r] = from_state[state_at + (32 * t + 16 * (r >> 3) + (r & 7)) * D];
+  }
 
   if (threadIdx.x < 2 * kChunk) {
     const int m = threadIdx.x;
@@ -290,7 +319,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
   // factor next to 1 at every chunk.
   const float log2_decay = log_decay * kLog2e;
   int reset = 0;
-  float sigma = 1.f;
+  float sigma = 1.f, sigma_then = 1.f;
   const float since = a.scale * decay(log_decay, c32 + 1);
 
   // Token of register r in P^T's rows, and of element r of the values' operands, less 4h.
@@ -301,251 +330,289 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
   const int tr_at = (4 * h + e) * kRowB + 16 * ((2 * p16 + (x4 & 1)) ^ swizzle<C>(4 * h + e)) +
                     8 * (x4 >> 1);
   // dims 32t .. 32t + 31 of tokens token(8 ss) .. token(8 ss + 7), transposed
-  auto transposed = [&](const unsigned char* from, int t, int ss) -> T8 {
-    const T4 lo = lds_tr_read4<T>(from + (tr_at ^ (64 * t)) + 16 * ss * kRowB);
-    const T4 hi = lds_tr_read4<T>(from + (tr_at ^ (64 * t) ^ 16) + (16 * ss + 8) * kRowB);
+  // (from: the tile's first byte plus tr_at)
+  auto transposed = [&](int from, int t, int ss) -> T8 {
+    const unsigned char* const p = bufs + 16 * ss * kRowB;
+    const T4 lo = lds_tr_read4<T>(p + (from ^ (64 * t)));
+    const T4 hi = lds_tr_read4<T>(p + 8 * kRowB + (from ^ (64 * t + 16)));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   };
 
-  int item = 0, q_stage = 0, kv_stage = 0;
-  for (int chunk = 0; chunk < chunks; ++chunk) {
-    const int left = min(n - chunk * kChunk, kChunk);
-    unsigned char* const kb = tile(0, kv_stage);
-    unsigned char* const vb = tile(1, kv_stage);
-    T8 va[2];
-    bool odd = false;
-    for (int g = 0; g < group; ++g, ++item) {
-      // all but what was issued after this item's copies: the next item's, and the last one's stores
-      if (item + 1 < items && item > 0) {
-        if (kStates)
-          wait_vmem<2 * kCopies>();
-        else if (g + 1 == group)
-          wait_vmem<3 * kCopies + 2>();
-        else
-          wait_vmem<kCopies + 2>();
-      } else {
-        wait_vmem<0>();
+  int q_stage = 0, kv_stage = 0, head = 0;
+  int left = n;  // tokens from this chunk on
+  bool first = true;
+  T8 va[2];
+  // bytes of a lane's first row of the output, then of the item's first
+  const unsigned int out_at = 2 * (c32 * static_cast<unsigned int>(a.h_q * D) + 32 * wave + 8 * h);
+  unsigned char* out = static_cast<unsigned char*>(a.out) +
+                       2 * (static_cast<long long>(run.start) * a.h_q + hk * group) * D;
+  while (true) {
+    // all but what was issued after this item's copies: the next item's, and the last one's stores
+    if (first || ahead == 0)
+      wait_vmem<0>();
+    else if (ahead == (kStates ? 2 : 3) * kCopies)
+      wait_vmem<(kStates ? 2 * kCopies : 3 * kCopies + 2)>();
+    else
+      wait_vmem<kCopies + 2>();
+    first = false;
+    sync();
+    ahead = fetch();
+    unsigned char* const kb = bufs + kv_stage;
+    unsigned char* const vb = bufs + kStages * kTileB + kv_stage;
+    const int taken = min(left, kChunk);
+    if (left < kChunk && head == 0) {  // uniform: rows past the end become zeros
+      for (int i = left * kRowB / 16 + threadIdx.x; i < kTileB / 16; i += 2 * D) {
+        reinterpret_cast<uintx4*>(kb)[i] = uintx4{0, 0, 0, 0};
+        reinterpret_cast<uintx4*>(vb)[i] = uintx4{0, 0, 0, 0};
       }
       sync();
-      fetch();
-      if (g == 0) {
-        if (left < kChunk) {  // uniform: rows past the end become zeros
-          for (int i = left * kRowB / 16 + threadIdx.x; i < kTileB / 16; i += 2 * D) {
-            reinterpret_cast<uintx4*>(kb)[i] = uintx4{0, 0, 0, 0};
-            reinterpret_cast<uintx4*>(vb)[i] = uintx4{0, 0, 0, 0};
-          }
-          sync();
-        }
-        // An infinity or a NaN in v would reach the tokens before its own through weights of 0.
-        unsigned int best = 0u;
-#pragma unroll
-        for (int ss = 0; ss < 2; ++ss) {
-          va[ss] = transposed(vb, wave, ss);
-          fold_bits(best, __builtin_bit_cast(uintx4, va[ss]));
-        }
-        odd = __ballot(is_odd<T>(best)) != 0ull;  // uniform
-      }
-      if constexpr (kStates) continue;
-      // the state's copy is made afresh for every head: kept, its registers would be spilled
-      if constexpr (D == 256) {
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) asm volatile("" : "+v"(s[t]));
-      }
-
-      const unsigned char* const qb = tile(2, q_stage);
-      q_stage = q_stage == kStages - 1 ? 0 : q_stage + 1;
-      // scores and S^T Q^T: a step of Q meets both
-      int s_power = 0, p_power = 0;
-      if constexpr (kHalf) {
-        float most = 0.f;
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(s[t][r]));
-        if (__ballot(most == __builtin_inff()) != 0ull) {  // uniform: of those that are finite
-          most = 0.f;
+    }
+    if (head == 0) {  // the state after this chunk is s times sigma_then
+      sigma_then = __builtin_amdgcn_exp2f(log2_decay * static_cast<float>(reset + taken));
+      if (!(sigma_then >= 0.0625f && sigma_then <= 16.f)) {  // uniform
+        if (reset > 0) {
 #pragma unroll
           for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              most = fabsf(s[t][r]) < __builtin_inff() ? fmaxf(most, fabsf(s[t][r])) : most;
+            for (int r = 0; r < 16; ++r) s[t][r] *= sigma;
+          reset = 0;
+          sigma = 1.f;
         }
-#pragma unroll
-        for (int m = 1; m < 64; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
-        s_power = max(power_of(most), kLeastPower);
+        sigma_then = __builtin_amdgcn_exp2f(log2_decay * static_cast<float>(taken));
       }
-      // A group of steps is read while the last one is multiplied.
-      floatx16 p = {}, o = {};
-      T8 qa[2][kGroupSteps], ka[2][kGroupSteps];
-      auto read = [&](int i) {
+    }
+    // A chunk whose own fall is past the range is taken into s before its values are.
+    const bool steep = !(sigma_then >= 0.0625f && sigma_then <= 16.f);  // uniform
+    // Addresses of this chunk, worked out afresh: kept, each of their many forms would be a register.
+    int k_row = kv_stage + row_at, k_tr = kv_stage + tr_at;
+    asm volatile("" : "+v"(k_row), "+v"(k_tr));
+    va[0] = transposed(kStages * kTileB + k_tr, wave, 0);
+    va[1] = transposed(kStages * kTileB + k_tr, wave, 1);
+
+    // The weighted values, each as a sum of kTerms numbers of the type (relative to 2^v_power).
+    T8 part[kTerms][2];
+    int v_power = 0;
+    auto split = [&]() {
+      const float* const weight = left_of + kChunk - taken + 4 * h;
+      const float against =
+          steep ? 1.f : __builtin_amdgcn_exp2f(-log2_decay * static_cast<float>(reset + taken));
+      float f[16];
 #pragma unroll
-        for (int x = 0; x < kGroupSteps; ++x) {
-          const int at = row_at ^ (32 * (kGroupSteps * i + x));
-          ka[i & 1][x] = *reinterpret_cast<const T8*>(kb + at);
-          qa[i & 1][x] = *reinterpret_cast<const T8*>(qb + at);
-        }
-      };
-      read(0);
-#pragma unroll
-      for (int i = 0; i < kKSteps / kGroupSteps; ++i) {
-        if (i + 1 < kKSteps / kGroupSteps) read(i + 1);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int x = 0; x < kGroupSteps; ++x) {
-          const int ks = kGroupSteps * i + x;
-          p = mfma_32x32x16(ka[i & 1][x], qa[i & 1][x], p);
-          T8 sa;
-#pragma unroll
-          for (int y = 0; y < 8; ++y) {
-            const float f = s[ks >> 1][8 * (ks & 1) + y];
-            sa[y] = static_cast<T>(kHalf ? times_power(f, -s_power) : f);
-          }
-          o = mfma_32x32x16(sa, qa[i & 1][x], o);
-        }
-      }
-      // A score that is not finite would reach the tokens before its own through weights of 0.
-      floatx4 trace = {0.f, 0.f, 0.f, 0.f};
-      const float* const weight = seen + kChunk - 1 - c32 + 4 * h;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        p[r] *= weight[token(r)];
-        trace[r & 3] = __builtin_fmaf(p[r], 0.f, trace[r & 3]);
-      }
-      if (__ballot((trace[0] + trace[1]) + (trace[2] + trace[3]) != 0.f) != 0ull) {  // uniform
-#pragma unroll
-        for (int r = 0; r < 16; ++r) p[r] = token(r) + 4 * h <= c32 ? p[r] : 0.f;
-      }
+      for (int r = 0; r < 16; ++r)
+        f[r] = static_cast<float>(va[r >> 3][r & 7]) * (weight[token(r)] * against);
       if constexpr (kHalf) {
         float top = 0.f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(p[r]));
-        p_power = max(power_of(max_xor32(top)), kLeastPower);
-      }
-      // O^T, relative to 2^p_power
-      const float by = kHalf ? times_power(since * sigma, s_power - p_power) : since * sigma;
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(f[r]));
+        v_power = max(power_of(max_xor32(top)), -100);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[r] *= by;
-#pragma unroll
-      for (int ss = 0; ss < 2; ++ss) {
-        T8 pb, v8 = va[ss];
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const float f = p[8 * ss + x];
-          pb[x] = static_cast<T>(kHalf ? times_power(f, -p_power) : f);
+        for (int r = 0; r < 16; ++r) {
+          const float x = times_power(f[r], -v_power);
+          part[0][r >> 3][r & 7] = static_cast<T>(x);
+          part[1][r >> 3][r & 7] = static_cast<T>(x - static_cast<float>(part[0][r >> 3][r & 7]));
         }
-        if (odd) {  // uniform
-          asm volatile("" ::: "memory");
+      } else {  // the upper 8 bits, the next 8, the rest
 #pragma unroll
-          for (int x = 0; x < 8; ++x)
-            v8[x] = fabsf(static_cast<float>(v8[x])) < __builtin_inff() ? v8[x]
-                                                                       : static_cast<T>(0.f);
+        for (int ss = 0; ss < 2; ++ss) {
+          uintx4 upper, next, rest;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            float y = f[8 * ss + 2 * x], z = f[8 * ss + 2 * x + 1];
+            upper[x] = upper_halves(y, z);
+            y -= upper_of(y), z -= upper_of(z);
+            next[x] = upper_halves(y, z);
+            y -= upper_of(y), z -= upper_of(z);
+            rest[x] = upper_halves(y, z);
+          }
+          part[0][ss] = __builtin_bit_cast(T8, upper);
+          part[1][ss] = __builtin_bit_cast(T8, next);
+          part[2][ss] = __builtin_bit_cast(T8, rest);
         }
-        o = mfma_32x32x16(v8, pb, o);
       }
-      if constexpr (kHalf) {
+    };
+
+    bool odd = false;  // something is not finite
+    floatx16 o = {};
+    if constexpr (kStates) {
+      unsigned int best = 0u;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[r] = times_power(o[r], p_power);
-      }
-      if (odd) {  // those values, for the tokens that see them
-        for (int j = 0; j < left; ++j) {
-          float w = 0.f;
+      for (int ss = 0; ss < 2; ++ss) fold_bits(best, __builtin_bit_cast(uintx4, va[ss]));
+      odd = __ballot(is_odd<T>(best)) != 0ull;
+    } else {
+      int q_row = 2 * kStages * kTileB + q_stage + row_at;
+      asm volatile("" : "+v"(q_row));
+      q_stage = q_stage == (kStages - 1) * kTileB ? 0 : q_stage + kTileB;
+      // O^T of the item.  kOdd: with weights of 0 for what is not finite and yet to come.
+      auto attend = [&](auto tag) {
+        constexpr bool kOdd = decltype(tag)::value != 0;
+        int s_power = 0, p_power = 0;
+        if constexpr (kHalf) {
+          float most = 0.f;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) w = token(r) == (j & ~4) ? p[r] : w;
-          w = __shfl(w, c32 + 32 * ((j >> 2) & 1));
+          for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const T8 v8 = *reinterpret_cast<const T8*>(
-                vb + j * kRowB + 16 * ((4 * wave + 2 * half + h) ^ swizzle<C>(j)));
+            for (int r = 0; r < 16; ++r) {
+              const float f = fabsf(s[t][r]);
+              most = kOdd && !(f < __builtin_inff()) ? most : fmaxf(most, f);
+            }
 #pragma unroll
-            for (int x = 0; x < 8; ++x) {
-              const float f = static_cast<float>(v8[x]);
-              o[8 * half + x] += j <= c32 && !(fabsf(f) < __builtin_inff()) ? w * f : 0.f;
+          for (int m = 1; m < 64; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
+          s_power = max(power_of(most), kLeastPower);
+        }
+        // A group of steps is read while the last one is multiplied.
+        floatx16 p = {};
+        T8 qa[kKeepQ ? kKSteps : 2 * kGroupSteps], ka[2 * kGroupSteps];
+        auto read = [&](int i, bool keys) {
+#pragma unroll
+          for (int x = kGroupSteps * i; x < kGroupSteps * (i + 1); ++x) {
+            if (keys)
+              ka[x % (2 * kGroupSteps)] = *reinterpret_cast<const T8*>(bufs + (k_row ^ (32 * x)));
+            if (keys || !kKeepQ)
+              qa[kKeepQ ? x : x % (2 * kGroupSteps)] =
+                  *reinterpret_cast<const T8*>(bufs + (q_row ^ (32 * x)));
+          }
+        };
+        read(0, true);
+#pragma unroll
+        for (int i = 0; i < kKSteps / kGroupSteps; ++i) {
+          if (i + 1 < kKSteps / kGroupSteps) read(i + 1, true);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int x = kGroupSteps * i; x < kGroupSteps * (i + 1); ++x)
+            p = mfma_32x32x16(ka[x % (2 * kGroupSteps)], qa[kKeepQ ? x : x % (2 * kGroupSteps)], p);
+        }
+        if (kEarly && !kOdd) split();  // beside those products
+        if (!kKeepQ) read(0, false);
+#pragma unroll
+        for (int i = 0; i < kKSteps / kGroupSteps; ++i) {
+          if (!kKeepQ && i + 1 < kKSteps / kGroupSteps) read(i + 1, false);
+          if (D == 256) __builtin_amdgcn_sched_barrier(0);  // few of s's copies at once
+#pragma unroll
+          for (int x = kGroupSteps * i; x < kGroupSteps * (i + 1); ++x) {
+            T8 sa;
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+              const float f = s[x >> 1][8 * (x & 1) + y];
+              sa[y] = static_cast<T>(kHalf ? times_power(f, -s_power) : f);
+            }
+            o = mfma_32x32x16(sa, qa[kKeepQ ? x : x % (2 * kGroupSteps)], o);
+          }
+        }
+        const float* const weight = seen + kChunk - 1 - c32 + 4 * h;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          p[r] *= weight[token(r)];
+          if (kOdd) p[r] = token(r) + 4 * h <= c32 ? p[r] : 0.f;
+        }
+        if constexpr (kHalf) {
+          float top = 0.f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(p[r]));
+          p_power = max(power_of(max_xor32(top)), kLeastPower);
+        }
+        // O^T, relative to 2^p_power
+        const float by = kHalf ? times_power(since * sigma, s_power - p_power) : since * sigma;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[r] *= by;
+#pragma unroll
+        for (int ss = 0; ss < 2; ++ss) {
+          T8 pb, v8 = va[ss];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const float f = p[8 * ss + x];
+            pb[x] = static_cast<T>(kHalf ? times_power(f, -p_power) : f);
+            if (kOdd)
+              v8[x] = fabsf(static_cast<float>(v8[x])) < __builtin_inff() ? v8[x]
+                                                                         : static_cast<T>(0.f);
+          }
+          o = mfma_32x32x16(v8, pb, o);
+        }
+        if constexpr (kHalf) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[r] = times_power(o[r], p_power);
+        }
+        if constexpr (kOdd) {  // those values, for the tokens that see them
+          for (int j = 0; j < taken; ++j) {
+            float w = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) w = token(r) == (j & ~4) ? p[r] : w;
+            w = __shfl(w, c32 + 32 * ((j >> 2) & 1));
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const T8 v8 = *reinterpret_cast<const T8*>(
+                  vb + j * kRowB + 16 * ((4 * wave + 2 * half + h) ^ swizzle<C>(j)));
+#pragma unroll
+              for (int x = 0; x < 8; ++x) {
+                const float f = static_cast<float>(v8[x]);
+                o[8 * half + x] += j <= c32 && !(fabsf(f) < __builtin_inff()) ? w * f : 0.f;
+              }
             }
           }
         }
+      };
+      attend(IntTag<0>{});
+      // An infinity or a NaN among the scores or in v reaches the tokens before its own, through
+      // weights of 0, and the outputs of its own: such a chunk is taken again.
+      floatx4 trace = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int r = 0; r < 16; ++r) trace[r & 3] = __builtin_fmaf(o[r], 0.f, trace[r & 3]);
+      odd = __ballot((trace[0] + trace[1]) + (trace[2] + trace[3]) != 0.f) != 0ull;  // uniform
+      if (odd) {
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) asm volatile("" : "+v"(s[t]));  // nothing is kept for it
+        o = floatx16{};
+        attend(IntTag<1>{});
       }
+    }
 
-      T* const out = static_cast<T*>(a.out) +
-                     ((static_cast<long long>(run.start) + chunk * kChunk + c32) * a.h_q +
-                      hk * group + g) * D + 32 * wave + 8 * h;
+    T8 kt[2][2];  // K^T of a tile of the state, the next one on its way
+    if (kStates || head + 1 == group) {
+      kt[0][0] = transposed(k_tr, 0, 0);
+      kt[0][1] = transposed(k_tr, 0, 1);
+    }
+    if constexpr (!kStates) {
       if (c32 < left) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           T8 y;
 #pragma unroll
           for (int x = 0; x < 8; ++x) y[x] = static_cast<T>(o[8 * half + x]);
-          *reinterpret_cast<T8*>(out + 16 * half) = y;
+          *reinterpret_cast<T8*>(out + out_at + 32 * half) = y;
         }
       }
+      out += 2 * D;
+      if (++head < group) continue;
+      head = 0;
+      out += 2 * D * (static_cast<long long>(kChunk) * a.h_q - group);
+      if (left <= kChunk && to_state == nullptr) break;
     }
-    if (chunk + 1 == chunks && to_state == nullptr) break;
 
-    T8 kt[2][2];  // K^T of a tile of the state, the next one on its way
-    kt[0][0] = transposed(kb, 0, 0);
-    kt[0][1] = transposed(kb, 0, 1);
-    reset += left;
-    sigma = __builtin_amdgcn_exp2f(log2_decay * static_cast<float>(reset));
-    float against = __builtin_amdgcn_exp2f(-log2_decay * static_cast<float>(reset));  // 1 / sigma
-    if (!(sigma >= 0.0625f && sigma <= 16.f)) {  // uniform
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[t][r] *= sigma;
-      reset = 0;
-      sigma = against = 1.f;
-    }
-    // the weighted values, each as a sum of kTerms numbers of the type
-    const float* const weight = left_of + kChunk - left + 4 * h;
-    T8 part[kTerms][2];
-    float f[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-      f[r] = static_cast<float>(va[r >> 3][r & 7]) * (weight[token(r)] * against);
-    int v_power = 0;
-    if constexpr (kHalf) {
-      float top = 0.f;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(f[r]));
-      v_power = max(power_of(max_xor32(top)), -100);
-    }
-    if constexpr (kHalf) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float x = times_power(f[r], -v_power);
-        part[0][r >> 3][r & 7] = static_cast<T>(x);
-        part[1][r >> 3][r & 7] = static_cast<T>(x - static_cast<float>(part[0][r >> 3][r & 7]));
-      }
-    } else {  // the upper 8 bits, the next 8, the rest
-#pragma unroll
-      for (int ss = 0; ss < 2; ++ss) {
-        uintx4 upper, next, rest;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          float y = f[8 * ss + 2 * x], z = f[8 * ss + 2 * x + 1];
-          upper[x] = upper_halves(y, z);
-          y -= upper_of(y), z -= upper_of(z);
-          next[x] = upper_halves(y, z);
-          y -= upper_of(y), z -= upper_of(z);
-          rest[x] = upper_halves(y, z);
-        }
-        part[0][ss] = __builtin_bit_cast(T8, upper);
-        part[1][ss] = __builtin_bit_cast(T8, next);
-        part[2][ss] = __builtin_bit_cast(T8, rest);
-      }
-    }
+    if (!kEarly) split();
     if (odd) {  // what is not finite has no rest
-      asm volatile("" ::: "memory");  // a branch: it is rarely taken
+      asm volatile("" ::: "memory");
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         if (!(fabsf(static_cast<float>(part[0][r >> 3][r & 7])) < __builtin_inff()))
 #pragma unroll
           for (int x = 1; x < kTerms; ++x) part[x][r >> 3][r & 7] = static_cast<T>(0.f);
     }
+    if (steep) {
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[t][r] *= sigma_then;
+      reset = 0;
+      sigma = 1.f;
+    } else {
+      reset += taken;
+      sigma = sigma_then;
+    }
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
       if (t + 1 < kTiles) {
-        kt[(t + 1) & 1][0] = transposed(kb, t + 1, 0);
-        kt[(t + 1) & 1][1] = transposed(kb, t + 1, 1);
+        kt[(t + 1) & 1][0] = transposed(k_tr, t + 1, 0);
+        kt[(t + 1) & 1][1] = transposed(k_tr, t + 1, 1);
       }
       __builtin_amdgcn_sched_barrier(0);
       floatx16 add = {};
@@ -564,7 +631,9 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
         for (int r = 0; r < 16; ++r) s[t][r] += times_power(add[r], v_power);
       }
     }
-    kv_stage = kv_stage == kStages - 1 ? 0 : kv_stage + 1;
+    kv_stage = kv_stage == (kStages - 1) * kTileB ? 0 : kv_stage + kTileB;
+    left -= kChunk;
+    if (left <= 0) break;
   }
 
   if (to_state != nullptr) {
@@ -629,11 +698,14 @@ void launch(const fa_linear_args& a, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(runs_of(a) * a.h_kv));
   const Divisor h_kv = divisor(a.h_kv);
   if (a.segment > 0) {
-    hipLaunchKernelGGL((linear_kernel<T, D, true>), grid, dim3(2 * D), 0, stream, a, h_kv);
+    hipLaunchKernelGGL((linear_kernel<T, D, true, false>), grid, dim3(2 * D), 0, stream, a, h_kv);
     hipLaunchKernelGGL((join_kernel<D>), dim3(static_cast<unsigned>(a.num_seqs * a.h_kv), D * D / 1024),
                        dim3(256), 0, stream, a, h_kv);
   }
-  hipLaunchKernelGGL((linear_kernel<T, D, false>), grid, dim3(2 * D), 0, stream, a, h_kv);
+  if (a.h_q == a.h_kv)
+    hipLaunchKernelGGL((linear_kernel<T, D, false, true>), grid, dim3(2 * D), 0, stream, a, h_kv);
+  else
+    hipLaunchKernelGGL((linear_kernel<T, D, false, false>), grid, dim3(2 * D), 0, stream, a, h_kv);
 }
 
 }  // namespace
