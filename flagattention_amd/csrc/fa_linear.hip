@@ -118,9 +118,23 @@ __device__ inline unsigned int upper_halves(float x, float y) {
   return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
 }
 
+// Largest of a wave's values.
+template <int kCtrl>
+__device__ inline float dpp_f32(float x) {
+  return __uint_as_float(static_cast<unsigned int>(__builtin_amdgcn_update_dpp(
+      0, static_cast<int>(__float_as_uint(x)), kCtrl, 0xF, 0xF, false)));
+}
+__device__ inline float wave_max(float x) {
+  x = fmaxf(x, dpp_f32<0xB1>(x));   // quad_perm [1, 0, 3, 2]
+  x = fmaxf(x, dpp_f32<0x4E>(x));   // quad_perm [2, 3, 0, 1]
+  x = fmaxf(x, dpp_f32<0x141>(x));  // row_half_mirror
+  x = fmaxf(x, dpp_f32<0x140>(x));  // row_mirror
+  return max_xor32(max_xor16(x));
+}
+
 // Power of two above |x|, 0 for 0, infinities and NaN.
 __device__ inline int power_of(float x) { return __builtin_amdgcn_frexp_expf(x); }
-__device__ inline float times_power(float x, int e) { return __builtin_amdgcn_ldexpf(x, e); }
+__device__ inline float two_to(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
 
 // A run of tokens that a work-group takes: a sequence, or a segment of one.
 struct Run {
@@ -224,25 +238,33 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
     if (slot >= 0 && slot < a.num_slots)
       slot_state = a.state + slot * a.state_stride_s + hk * a.state_stride_h;
   }
-  // where the run starts from, and where it leaves its state
+  // Where the run starts from, and where it leaves its state.  A sequence of several runs has the state
+  // that run p starts from in part, at its index: the last run may write the sequence's own while
+  // the first has not read it yet.
+  float* const part = a.part + (static_cast<long long>(index) * a.h_kv + hk) * (D * D);
+  const bool kept = slot_state && (a.has_state == nullptr || a.has_state[run.seq] != 0);
+  const bool alone = run.part == 0 && run.last;
   const float* from_state = nullptr;
-  if (run.part > 0)
-    from_state = kStates ? nullptr
-                         : a.part + (static_cast<long long>(index - 1) * a.h_kv + hk) * (D * D);
-  else if (slot_state && (a.has_state == nullptr || a.has_state[run.seq] != 0))
-    from_state = slot_state;
-  float* const to_state = kStates ? a.part + (static_cast<long long>(index) * a.h_kv + hk) * (D * D)
+  if (kStates || alone)
+    from_state = run.part == 0 && kept ? slot_state : nullptr;
+  else if (run.part > 0 || kept)
+    from_state = part;
+  float* const to_state = kStates ? part + static_cast<long long>(a.h_kv) * (D * D)
                                   : run.last ? slot_state : nullptr;
 
   // Items are (chunk, query head of the group), heads innermost; k and v come with the first head.
+  // States alone go through the chunks from the last one back: what they read last is what the next
+  // launch reads first.
+  const int chunks = cdiv(n, kChunk);
+  const int begin = run.start + (kStates ? (chunks - 1) * kChunk : 0);
   // The next chunk's rows, and q's of its next head.
   const unsigned char* k_next = static_cast<const unsigned char*>(a.k) +
-                                2 * (run.start * a.k_stride_t + hk * a.k_stride_h);
+                                2 * (begin * a.k_stride_t + hk * a.k_stride_h);
   const unsigned char* v_next = static_cast<const unsigned char*>(a.v) +
-                                2 * (run.start * a.v_stride_t + hk * a.v_stride_h);
+                                2 * (begin * a.v_stride_t + hk * a.v_stride_h);
   const unsigned char* q_next =
       static_cast<const unsigned char*>(a.q) +
-      2 * (run.start * a.q_stride_t + static_cast<long long>(hk) * group * a.q_stride_h);
+      2 * (begin * a.q_stride_t + static_cast<long long>(hk) * group * a.q_stride_h);
   const unsigned int q_tb = 2 * a.q_stride_t, k_tb = 2 * a.k_stride_t, v_tb = 2 * a.v_stride_t;
   const long long q_hb = 2 * a.q_stride_h;
   const long long q_step = static_cast<long long>(kChunk) * q_tb - (group - 1) * q_hb;
@@ -264,28 +286,32 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
       lds_dma16_at(from, __umul24(min(r, rows - 1), row_b) + copy_piece[i], to + 1024 * i);
     }
   };
-  int to_come = n, next_head = 0;  // tokens from the next item's chunk on; its head
+  auto rows_of = [&](int chunk) {  // chunk: from the run's first item on
+    return kStates ? (chunk == 0 ? n - (chunks - 1) * kChunk : kChunk) : n - chunk * kChunk;
+  };
+  int next_chunk = 0, next_head = 0;
   int next_q = 0, next_kv = 0;     // bytes of its stages
   // Returns the copies that it issues.
   auto fetch = [&]() -> int {
-    if (to_come <= 0) return 0;
+    if (next_chunk == chunks) return 0;
+    const int rows = rows_of(next_chunk);
     int issued = 0;
     if (!kStates) {
-      copy(q_next, q_tb, to_come, lds + 2 * kStages * kTileB + next_q);
+      copy(q_next, q_tb, rows, lds + 2 * kStages * kTileB + next_q);
       next_q = next_q == (kStages - 1) * kTileB ? 0 : next_q + kTileB;
       issued += kCopies;
     }
     if (next_head == 0) {
-      copy(k_next, k_tb, to_come, lds + next_kv);
-      copy(v_next, v_tb, to_come, lds + kStages * kTileB + next_kv);
+      copy(k_next, k_tb, rows, lds + next_kv);
+      copy(v_next, v_tb, rows, lds + kStages * kTileB + next_kv);
       next_kv = next_kv == (kStages - 1) * kTileB ? 0 : next_kv + kTileB;
-      k_next += kChunk * static_cast<unsigned long long>(k_tb);
-      v_next += kChunk * static_cast<unsigned long long>(v_tb);
+      k_next += (kStates ? -kChunk : kChunk) * static_cast<long long>(k_tb);
+      v_next += (kStates ? -kChunk : kChunk) * static_cast<long long>(v_tb);
       issued += 2 * kCopies;
     }
     if (++next_head == group) {
       next_head = 0;
-      to_come -= kChunk;
+      ++next_chunk;
       q_next += q_step;
     } else {
       q_next += q_hb;
@@ -307,6 +333,18 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
       for (int r = 0; r < 16; ++r)
         s[t][r] = from_state[state_at + (32 * t + 16 * (r >> 3) + (r & 7)) * D];
   }
+  if constexpr (kStates) {
+    if (from_state) {
+      const float fall = decay(log_decay, n);
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          part[state_at + (32 * t + 16 * (r >> 3) + (r & 7)) * D] = s[t][r];
+          s[t][r] *= fall;
+        }
+    }
+  }
 
   if (threadIdx.x < 2 * kChunk) {
     const int m = threadIdx.x;
@@ -320,6 +358,41 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
   const float log2_decay = log_decay * kLog2e;
   int reset = 0;
   float sigma = 1.f, sigma_then = 1.f;
+  // States alone have their weights counted to the run's end instead, and are never brought up.
+  int after = 0;
+
+  // fp16: s is kept times 2^-s_power, its largest at about 8 when it was last looked at: there is room
+  // for a growth by 2^12 (past it an output is not finite, and the chunk is taken again) and a fall
+  // by 2^17 (counted below) before its copies lose bits.
+  int s_power = 0, looked = -1;  // tokens since, -1: not yet
+  auto look = [&]() {
+    float most = 0.f;
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(s[t][r]));
+    if (__ballot(most == __builtin_inff()) != 0ull) {  // uniform: of those that are finite
+      most = 0.f;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          most = fabsf(s[t][r]) < __builtin_inff() ? fmaxf(most, fabsf(s[t][r])) : most;
+    }
+    // |s| 2^s_power is at most 2^128: both factors stay in range
+    most = wave_max(most);
+    const int by = uniform(most > 0.f ? max(power_of(most) - 3, -100 - s_power) : 0);
+    if (by < -2 || by > 2) {  // uniform
+      const float x = two_to(-by);
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[t][r] *= x;
+      s_power += by;
+    }
+    looked = 0;
+  };
+  if (kHalf && !kStates && from_state) look();
   const float since = a.scale * decay(log_decay, c32 + 1);
 
   // Token of register r in P^T's rows, and of element r of the values' operands, less 4h.
@@ -339,7 +412,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
   };
 
   int q_stage = 0, kv_stage = 0, head = 0;
-  int left = n;  // tokens from this chunk on
+  int chunk = 0;
   bool first = true;
   T8 va[2];
   // bytes of a lane's first row of the output, then of the item's first
@@ -359,15 +432,15 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
     ahead = fetch();
     unsigned char* const kb = bufs + kv_stage;
     unsigned char* const vb = bufs + kStages * kTileB + kv_stage;
-    const int taken = min(left, kChunk);
-    if (left < kChunk && head == 0) {  // uniform: rows past the end become zeros
-      for (int i = left * kRowB / 16 + threadIdx.x; i < kTileB / 16; i += 2 * D) {
+    const int taken = min(rows_of(chunk), kChunk);
+    if (taken < kChunk && head == 0) {  // uniform: rows past the end become zeros
+      for (int i = taken * kRowB / 16 + threadIdx.x; i < kTileB / 16; i += 2 * D) {
         reinterpret_cast<uintx4*>(kb)[i] = uintx4{0, 0, 0, 0};
         reinterpret_cast<uintx4*>(vb)[i] = uintx4{0, 0, 0, 0};
       }
       sync();
     }
-    if (head == 0) {  // the state after this chunk is s times sigma_then
+    if (!kStates && head == 0) {  // the state after this chunk is s times sigma_then
       sigma_then = __builtin_amdgcn_exp2f(log2_decay * static_cast<float>(reset + taken));
       if (!(sigma_then >= 0.0625f && sigma_then <= 16.f)) {  // uniform
         if (reset > 0) {
@@ -382,7 +455,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
       }
     }
     // A chunk whose own fall is past the range is taken into s before its values are.
-    const bool steep = !(sigma_then >= 0.0625f && sigma_then <= 16.f);  // uniform
+    const bool steep = !kStates && !(sigma_then >= 0.0625f && sigma_then <= 16.f);  // uniform
     // Addresses of this chunk, worked out afresh: kept, each of their many forms would be a register.
     int k_row = kv_stage + row_at, k_tr = kv_stage + tr_at;
     asm volatile("" : "+v"(k_row), "+v"(k_tr));
@@ -390,12 +463,14 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
     va[1] = transposed(kStages * kTileB + k_tr, wave, 1);
 
     // The weighted values, each as a sum of kTerms numbers of the type (relative to 2^v_power).
-    T8 part[kTerms][2];
+    T8 terms[kTerms][2];
     int v_power = 0;
     auto split = [&]() {
       const float* const weight = left_of + kChunk - taken + 4 * h;
-      const float against =
-          steep ? 1.f : __builtin_amdgcn_exp2f(-log2_decay * static_cast<float>(reset + taken));
+      float against = 1.f;
+      if (kStates ? after > 0 : !steep)
+        against = __builtin_amdgcn_exp2f(
+            log2_decay * static_cast<float>(kStates ? after : -(reset + taken)));
       float f[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r)
@@ -404,12 +479,13 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
         float top = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(f[r]));
-        v_power = max(power_of(max_xor32(top)), -100);
+        v_power = min(max(power_of(max_xor32(top)), -100), 100);
+        const float by = two_to(-v_power);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const float x = times_power(f[r], -v_power);
-          part[0][r >> 3][r & 7] = static_cast<T>(x);
-          part[1][r >> 3][r & 7] = static_cast<T>(x - static_cast<float>(part[0][r >> 3][r & 7]));
+          const float x = f[r] * by;
+          terms[0][r >> 3][r & 7] = static_cast<T>(x);
+          terms[1][r >> 3][r & 7] = static_cast<T>(x - static_cast<float>(terms[0][r >> 3][r & 7]));
         }
       } else {  // the upper 8 bits, the next 8, the rest
 #pragma unroll
@@ -424,9 +500,9 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
             y -= upper_of(y), z -= upper_of(z);
             rest[x] = upper_halves(y, z);
           }
-          part[0][ss] = __builtin_bit_cast(T8, upper);
-          part[1][ss] = __builtin_bit_cast(T8, next);
-          part[2][ss] = __builtin_bit_cast(T8, rest);
+          terms[0][ss] = __builtin_bit_cast(T8, upper);
+          terms[1][ss] = __builtin_bit_cast(T8, next);
+          terms[2][ss] = __builtin_bit_cast(T8, rest);
         }
       }
     };
@@ -445,20 +521,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
       // O^T of the item.  kOdd: with weights of 0 for what is not finite and yet to come.
       auto attend = [&](auto tag) {
         constexpr bool kOdd = decltype(tag)::value != 0;
-        int s_power = 0, p_power = 0;
-        if constexpr (kHalf) {
-          float most = 0.f;
-#pragma unroll
-          for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const float f = fabsf(s[t][r]);
-              most = kOdd && !(f < __builtin_inff()) ? most : fmaxf(most, f);
-            }
-#pragma unroll
-          for (int m = 1; m < 64; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
-          s_power = max(power_of(most), kLeastPower);
-        }
+        int p_power = 0;
         // A group of steps is read while the last one is multiplied.
         floatx16 p = {};
         T8 qa[kKeepQ ? kKSteps : 2 * kGroupSteps], ka[2 * kGroupSteps];
@@ -491,10 +554,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
           for (int x = kGroupSteps * i; x < kGroupSteps * (i + 1); ++x) {
             T8 sa;
 #pragma unroll
-            for (int y = 0; y < 8; ++y) {
-              const float f = s[x >> 1][8 * (x & 1) + y];
-              sa[y] = static_cast<T>(kHalf ? times_power(f, -s_power) : f);
-            }
+            for (int y = 0; y < 8; ++y) sa[y] = static_cast<T>(s[x >> 1][8 * (x & 1) + y]);
             o = mfma_32x32x16(sa, qa[kKeepQ ? x : x % (2 * kGroupSteps)], o);
           }
         }
@@ -508,10 +568,12 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
           float top = 0.f;
 #pragma unroll
           for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(p[r]));
-          p_power = max(power_of(max_xor32(top)), kLeastPower);
+          p_power = min(max(power_of(max_xor32(top)), kLeastPower), 100);
         }
         // O^T, relative to 2^p_power
-        const float by = kHalf ? times_power(since * sigma, s_power - p_power) : since * sigma;
+        const float by = kHalf ? __builtin_amdgcn_ldexpf(since * sigma, s_power - p_power)
+                               : since * sigma;
+        const float p_by = two_to(-p_power), p_back = two_to(p_power);
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[r] *= by;
 #pragma unroll
@@ -519,8 +581,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
           T8 pb, v8 = va[ss];
 #pragma unroll
           for (int x = 0; x < 8; ++x) {
-            const float f = p[8 * ss + x];
-            pb[x] = static_cast<T>(kHalf ? times_power(f, -p_power) : f);
+            pb[x] = static_cast<T>(kHalf ? p[8 * ss + x] * p_by : p[8 * ss + x]);
             if (kOdd)
               v8[x] = fabsf(static_cast<float>(v8[x])) < __builtin_inff() ? v8[x]
                                                                          : static_cast<T>(0.f);
@@ -529,7 +590,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
         }
         if constexpr (kHalf) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) o[r] = times_power(o[r], p_power);
+          for (int r = 0; r < 16; ++r) o[r] *= p_back;
         }
         if constexpr (kOdd) {  // those values, for the tokens that see them
           for (int j = 0; j < taken; ++j) {
@@ -561,6 +622,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
         asm volatile("" ::: "memory");
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) asm volatile("" : "+v"(s[t]));  // nothing is kept for it
+        if (kHalf) look();
         o = floatx16{};
         attend(IntTag<1>{});
       }
@@ -572,7 +634,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
       kt[0][1] = transposed(k_tr, 0, 1);
     }
     if constexpr (!kStates) {
-      if (c32 < left) {
+      if (c32 < taken) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           T8 y;
@@ -585,7 +647,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
       if (++head < group) continue;
       head = 0;
       out += 2 * D * (static_cast<long long>(kChunk) * a.h_q - group);
-      if (left <= kChunk && to_state == nullptr) break;
+      if (chunk + 1 == chunks && to_state == nullptr) break;
     }
 
     if (!kEarly) split();
@@ -593,9 +655,9 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
       asm volatile("" ::: "memory");
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        if (!(fabsf(static_cast<float>(part[0][r >> 3][r & 7])) < __builtin_inff()))
+        if (!(fabsf(static_cast<float>(terms[0][r >> 3][r & 7])) < __builtin_inff()))
 #pragma unroll
-          for (int x = 1; x < kTerms; ++x) part[x][r >> 3][r & 7] = static_cast<T>(0.f);
+          for (int x = 1; x < kTerms; ++x) terms[x][r >> 3][r & 7] = static_cast<T>(0.f);
     }
     if (steep) {
 #pragma unroll
@@ -608,6 +670,9 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
       reset += taken;
       sigma = sigma_then;
     }
+    after += taken;
+    // of the products in units of s
+    const float add_by = kHalf ? two_to(min(max(v_power - s_power, -126), 127)) : 1.f;
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
       if (t + 1 < kTiles) {
@@ -621,31 +686,36 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
 #pragma unroll
         for (int x = 0; x < kTerms; ++x) {
           if (kHalf)
-            add = mfma_32x32x16(kt[t & 1][ss], part[x][ss], add);
+            add = mfma_32x32x16(kt[t & 1][ss], terms[x][ss], add);
           else
-            s[t] = mfma_32x32x16(kt[t & 1][ss], part[x][ss], s[t]);
+            s[t] = mfma_32x32x16(kt[t & 1][ss], terms[x][ss], s[t]);
         }
       }
       if constexpr (kHalf) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[t][r] += times_power(add[r], v_power);
+        for (int r = 0; r < 16; ++r) s[t][r] = __builtin_fmaf(add[r], add_by, s[t][r]);
       }
     }
     kv_stage = kv_stage == (kStages - 1) * kTileB ? 0 : kv_stage + kTileB;
-    left -= kChunk;
-    if (left <= 0) break;
+    if (++chunk == chunks) break;
+    if constexpr (kHalf && !kStates) {
+      if (looked >= 0) looked += taken;
+      if (looked < 0 || !(log2_decay * static_cast<float>(looked) > -16.f)) look();  // uniform
+    }
   }
 
   if (to_state != nullptr) {
+    const float back = kHalf ? __builtin_amdgcn_ldexpf(sigma, s_power) : sigma;
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        to_state[state_at + (32 * t + 16 * (r >> 3) + (r & 7)) * D] = s[t][r] * sigma;
+        to_state[state_at + (32 * t + 16 * (r >> 3) + (r & 7)) * D] = s[t][r] * back;
   }
 }
 
-// The segments' states, each on top of the one before: part[i] += e^{a L} part[i - 1].
+// The states that segments start from, but for the first: each what its predecessor made on top of what
+// that one started from, part[i] += e^{a L} part[i - 1].
 template <int D>
 __global__ __launch_bounds__(256) void join_kernel(const fa_linear_args a, const Divisor h_kv) {
   constexpr int kAhead = 8;
@@ -653,11 +723,11 @@ __global__ __launch_bounds__(256) void join_kernel(const fa_linear_args a, const
   const int hk = blockIdx.x - seq * a.h_kv;
   const int start = min(max(sload(a.cu_seqlens + seq), 0), a.total);
   const int n = min(max(sload(a.cu_seqlens + seq + 1), start), a.total) - start;
-  const int states = n == 0 ? 0 : (n - 1) / a.segment;  // of all segments but the last
+  const int states = n == 0 ? 0 : (n - 1) / a.segment;  // those that the others start from
   if (states < 2) return;
   const long long step = static_cast<long long>(a.h_kv) * (D * D) / 4;
   floatx4* at = reinterpret_cast<floatx4*>(a.part) +
-                (static_cast<long long>(start / a.segment + seq) * a.h_kv + hk) * (D * D / 4) +
+                (static_cast<long long>(start / a.segment + seq + 1) * a.h_kv + hk) * (D * D / 4) +
                 blockIdx.y * 256 + threadIdx.x;
   const float fall = decay(sload(a.log_decay + hk), a.segment);
   floatx4 sum = *at;
