@@ -124,7 +124,7 @@ extern "C" int fa_linear_token(const fa_linear_args* args, void* stream) {
   FA_CHECK_ARG(a.total == a.num_seqs, "%d tokens of %d sequences", a.total, a.num_seqs);
   FA_CHECK_ARG(static_cast<int64_t>(a.num_seqs) * a.h_kv < 1 << 22, "too many sequences or heads");
   if (a.num_seqs == 0) return FA_OK;
-  FA_CHECK_ARG(a.state != nullptr || a.num_slots == 0, "state is NULL");
+  FA_CHECK_ARG(a.state != nullptr, "state is NULL");
   const hipStream_t s = static_cast<hipStream_t>(stream);
   a.dtype == 1 ? fa::launch_dim<fa::bf16>(a, s) : fa::launch_dim<_Float16>(a, s);
   FA_CHECK_HIP(hipGetLastError());

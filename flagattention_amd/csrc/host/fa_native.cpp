@@ -29,6 +29,7 @@
 #include <string>
 
 #include "flagattention_amd.h"
+#include "flagattention_amd_linear.h"
 #include "flagattention_amd_packed.h"
 
 namespace {
@@ -920,6 +921,314 @@ PyObject* mxfp4_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- rotary positions (rotary.py) ----
+// A turn's sections, positions and frequencies (rotary._check_turn), and the heads of q and k.
+bool rotary_of(const at::Tensor& q, const at::Tensor& k, PyObject* positions, PyObject* inv_freq,
+               PyObject* sections, PyObject* mixed, PyObject* adjacent, fa_rotary_args* a) {
+  const at::Tensor *pos = plain(positions), *freq = plain(inv_freq);
+  bool is_mixed, is_adjacent;
+  if (!pos || !freq || !to_bool(mixed, &is_mixed) || !to_bool(adjacent, &is_adjacent) ||
+      q.dim() != 3 || k.dim() != 3 || !gqa_dtype(q) || k.scalar_type() != q.scalar_type() ||
+      k.size(0) != q.size(0) || k.size(2) != q.size(2) || q.stride(2) != 1 || k.stride(2) != 1)
+    return false;
+  const int64_t tokens = q.size(0), h_q = q.size(1), h_kv = k.size(1), d = q.size(2);
+  if (tokens < 1 || tokens > INT32_MAX || h_q < 1 || h_q > 65535 || h_kv < 1 || h_kv > 65535 ||
+      d > 4096 || tokens * cdiv(h_q + 2 * h_kv, 4) * (d / 2 + 1) >= (int64_t{1} << 31) - 1024 ||
+      freq->scalar_type() != at::kFloat || freq->dim() != 1 || !freq->is_contiguous() ||
+      (pos->scalar_type() != at::kInt && pos->scalar_type() != at::kLong))
+    return false;
+  const int64_t pairs = freq->size(0);
+  if (pairs < 1 || 2 * pairs > d || pos->device() != q.device() || freq->device() != q.device() ||
+      k.device() != q.device())
+    return false;
+  if (sections == Py_None) {
+    if (is_mixed || pos->dim() != 1 || pos->size(0) != tokens || !pos->is_contiguous()) return false;
+    a->axes = 1;
+    a->sections[0] = static_cast<int32_t>(pairs);
+  } else {
+    if (!PyTuple_CheckExact(sections) && !PyList_CheckExact(sections)) return false;
+    const Py_ssize_t axes = PySequence_Fast_GET_SIZE(sections);
+    if (axes < 1 || axes > FA_ROTARY_MAX_AXES || pos->dim() != 2 || pos->size(0) != axes ||
+        pos->size(1) != tokens || (tokens > 1 && pos->stride(1) != 1))
+      return false;
+    int64_t sum = 0;
+    for (Py_ssize_t i = 0; i < axes; ++i) {
+      int64_t n;
+      if (!to_int(PySequence_Fast_GET_ITEM(sections, i), &n) || n < 0 || n > pairs) return false;
+      if (is_mixed && i > 0 && n > 0 && (n - 1) * axes + i >= pairs) return false;
+      a->sections[i] = static_cast<int32_t>(n);
+      sum += n;
+    }
+    if (sum != pairs) return false;
+    a->axes = static_cast<int32_t>(axes);
+    a->pos_stride_a = pos->stride(0);
+  }
+  a->q = q.data_ptr();
+  a->q_stride_t = q.stride(0);
+  a->q_stride_h = q.stride(1);
+  a->k = k.data_ptr();
+  a->k_stride_t = k.stride(0);
+  a->k_stride_h = k.stride(1);
+  a->positions = pos->data_ptr();
+  a->inv_freq = freq->data_ptr<float>();
+  a->tokens = static_cast<int32_t>(tokens);
+  a->h_q = static_cast<int32_t>(h_q);
+  a->h_kv = static_cast<int32_t>(h_kv);
+  a->d = static_cast<int32_t>(d);
+  a->pairs = static_cast<int32_t>(pairs);
+  a->mixed = is_mixed;
+  a->adjacent = is_adjacent;
+  a->pos64 = pos->scalar_type() == at::kLong;
+  a->dtype = q.scalar_type() == at::kBFloat16;
+  return true;
+}
+void rotary_out(fa_rotary_args* a, const at::Tensor& q) {
+  a->q_out = q.data_ptr();
+  a->q_out_stride_t = q.stride(0);
+  a->q_out_stride_h = q.stride(1);
+}
+// No two rows share an element (rotary._apart): the last dim is contiguous.
+bool rows_apart(const at::Tensor& t, int dims) {
+  int order[3] = {0, 1, 2};
+  std::sort(order, order + dims, [&](int x, int y) {
+    return t.stride(x) != t.stride(y) ? t.stride(x) < t.stride(y) : t.size(x) < t.size(y);
+  });
+  int64_t reach = t.size(dims);
+  for (int i = 0; i < dims; ++i) {
+    const int64_t size = t.size(order[i]), stride = t.stride(order[i]);
+    if (size <= 1) continue;
+    if (stride < reach) return false;
+    reach += (size - 1) * stride;
+  }
+  return true;
+}
+
+// rotary(q, k, positions, inv_freq, sections, mixed_sections, adjacent_pairs, inplace): (q, k)
+PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 8) return none();
+  const at::Tensor *q = plain(args[0]), *k = plain(args[1]);
+  bool inplace;
+  fa_rotary_args a = {};
+  if (!q || !k || !to_bool(args[7], &inplace) ||
+      !rotary_of(*q, *k, args[2], args[3], args[4], args[5], args[6], &a))
+    return none();
+  if (inplace && (!rows_apart(*q, 2) || !rows_apart(*k, 2))) return none();
+  const c10::Device device = q->device();
+  at::Tensor q_out, k_out;
+  {
+    NoGil nogil;
+    c10::DeviceGuard guard(device);
+    q_out = inplace ? *q : make(q->sizes(), q->scalar_type(), device);
+    k_out = inplace ? *k : make(k->sizes(), k->scalar_type(), device);
+    rotary_out(&a, q_out);
+    a.k_out = k_out.data_ptr();
+    a.k_out_stride_t = k_out.stride(0);
+    a.k_out_stride_h = k_out.stride(1);
+    check(fa_rotary(&a, stream_of(device)));
+  }
+  if (inplace) return PyTuple_Pack(2, args[0], args[1]);
+  PyObject* const x = THPVariable_Wrap(std::move(q_out));
+  PyObject* const y = THPVariable_Wrap(std::move(k_out));
+  PyObject* const both = x && y ? PyTuple_Pack(2, x, y) : nullptr;
+  Py_XDECREF(x);
+  Py_XDECREF(y);
+  return both;
+  END_HANDLE_TH_ERRORS
+}
+
+// rotary_cache(q, k, v, positions, inv_freq, key_cache, value_cache, slot_mapping, sections,
+//              mixed_sections, adjacent_pairs): q
+PyObject* rotary_cache(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 11) return none();
+  const at::Tensor *q = plain(args[0]), *k = plain(args[1]), *v = plain(args[2]),
+                   *kc = plain(args[5]), *vc = plain(args[6]), *slots = plain(args[7]);
+  fa_rotary_args a = {};
+  if (!q || !k || !v || !kc || !vc || !slots ||
+      !rotary_of(*q, *k, args[3], args[4], args[8], args[9], args[10], &a))
+    return none();
+  if (!v->sizes().equals(k->sizes()) || v->scalar_type() != k->scalar_type() || v->stride(2) != 1 ||
+      kc->dim() != 4 || !vc->sizes().equals(kc->sizes()) || kc->size(1) != a.h_kv ||
+      kc->size(3) != a.d || kc->scalar_type() != q->scalar_type() ||
+      vc->scalar_type() != q->scalar_type() || kc->size(0) < 1 || kc->size(0) > INT32_MAX ||
+      kc->size(2) < 1 || kc->size(2) > INT32_MAX || kc->stride(3) != 1 || vc->stride(3) != 1 ||
+      !rows_apart(*kc, 3) || !rows_apart(*vc, 3))
+    return none();
+  if ((slots->scalar_type() != at::kInt && slots->scalar_type() != at::kLong) || slots->dim() != 1 ||
+      slots->size(0) != a.tokens || !slots->is_contiguous())
+    return none();
+  const c10::Device device = q->device();
+  for (const at::Tensor* t : {v, kc, vc, slots})
+    if (t->device() != device) return none();
+  at::Tensor q_out;
+  {
+    NoGil nogil;
+    c10::DeviceGuard guard(device);
+    q_out = make(q->sizes(), q->scalar_type(), device);
+    rotary_out(&a, q_out);
+    a.v = v->data_ptr();
+    a.v_stride_t = v->stride(0);
+    a.v_stride_h = v->stride(1);
+    a.key_cache = kc->data_ptr();
+    a.value_cache = vc->data_ptr();
+    a.kc_stride_0 = kc->stride(0);
+    a.kc_stride_h = kc->stride(1);
+    a.kc_stride_t = kc->stride(2);
+    a.vc_stride_0 = vc->stride(0);
+    a.vc_stride_h = vc->stride(1);
+    a.vc_stride_t = vc->stride(2);
+    a.num_blocks = kc->size(0);
+    a.block_size = static_cast<int32_t>(kc->size(2));
+    a.slots = slots->data_ptr();
+    a.slots64 = slots->scalar_type() == at::kLong;
+    check(fa_rotary(&a, stream_of(device)));
+  }
+  return THPVariable_Wrap(std::move(q_out));
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- linear attention (linear.py) ----
+// Rows, decays and states of a call (linear._check_rows, _check_decay, _check_state), or false.
+// state and indices may be Py_None where `optional`.
+bool linear_of(PyObject* const* args, PyObject* state, PyObject* indices, PyObject* scale,
+               bool optional, int64_t num_seqs, fa_linear_args* a, const at::Tensor** q_out) {
+  const at::Tensor *q = plain(args[0]), *k = plain(args[1]), *v = plain(args[2]),
+                   *decay = plain(args[3]);
+  if (!q || !k || !v || !decay || q->dim() != 3 || k->dim() != 3 || !v->sizes().equals(k->sizes()))
+    return false;
+  const int64_t total = q->size(0), h_q = q->size(1), d = q->size(2), h_kv = k->size(1);
+  if (num_seqs < 0) num_seqs = total;  // a token each
+  double sm_scale = 1.0 / std::sqrt(static_cast<double>(d));
+  if (scale != Py_None && !to_double(scale, &sm_scale)) return false;
+  if (total < 1 || total > INT32_MAX - 256 || k->size(0) != total || k->size(2) != d ||
+      !packed_dim(d) || h_kv < 1 || h_q < 1 || h_q % h_kv != 0 || h_q * d >= (int64_t{1} << 23) ||
+      !gqa_dtype(*q) || k->scalar_type() != q->scalar_type() || v->scalar_type() != q->scalar_type() ||
+      !std::isfinite(sm_scale) || num_seqs > 65535 || num_seqs * h_kv >= (int64_t{1} << 22))
+    return false;
+  constexpr int64_t kMaxStride = int64_t{1} << 23;
+  for (const at::Tensor* t : {q, k, v})
+    if (t->stride(2) != 1 || !rows16(*t, 2) || t->stride(0) >= kMaxStride ||
+        t->device() != q->device())
+      return false;
+  if (decay->scalar_type() != at::kFloat || decay->dim() != 1 || decay->size(0) != h_kv ||
+      !decay->is_contiguous() || decay->device() != q->device())
+    return false;
+  if (state == Py_None) {
+    if (!optional || indices != Py_None) return false;
+  } else {
+    const at::Tensor* s = plain(state);
+    if (!s || s->scalar_type() != at::kFloat || s->dim() != 4 || s->size(1) != h_kv ||
+        s->size(2) != d || s->size(3) != d || s->stride(3) != 1 || s->stride(2) != d ||
+        s->stride(0) % 4 != 0 || s->stride(1) % 4 != 0 || !aligned16(*s) || s->size(0) < 1 ||
+        s->size(0) > INT32_MAX || s->device() != q->device())
+      return false;
+    int in = 0, over = 1;  // dims by stride
+    if (s->stride(1) < s->stride(0) || (s->stride(1) == s->stride(0) && s->size(1) < s->size(0)))
+      std::swap(in, over);
+    const int64_t n_in = s->size(in), n_over = s->size(over);
+    if ((n_in > 1 && s->stride(in) < d * d) ||
+        (n_over > 1 && s->stride(over) < d * d + (n_in - 1) * s->stride(in)))
+      return false;
+    a->state = s->data_ptr<float>();
+    a->state_stride_s = s->stride(0);
+    a->state_stride_h = s->stride(1);
+    a->num_slots = static_cast<int32_t>(s->size(0));
+    if (indices == Py_None) {
+      if (s->size(0) < num_seqs) return false;
+    } else {
+      const at::Tensor* ids = plain(indices);
+      if (!ids || ids->scalar_type() != at::kInt || ids->dim() != 1 || ids->size(0) != num_seqs ||
+          !ids->is_contiguous() || ids->device() != q->device())
+        return false;
+      a->state_indices = ids->data_ptr<int32_t>();
+    }
+  }
+  a->q = q->data_ptr();
+  a->q_stride_t = q->stride(0);
+  a->q_stride_h = q->stride(1);
+  a->k = k->data_ptr();
+  a->v = v->data_ptr();
+  a->k_stride_t = k->stride(0);
+  a->k_stride_h = k->stride(1);
+  a->v_stride_t = v->stride(0);
+  a->v_stride_h = v->stride(1);
+  a->log_decay = decay->data_ptr<float>();
+  a->num_seqs = static_cast<int32_t>(num_seqs);
+  a->total = static_cast<int32_t>(total);
+  a->h_q = static_cast<int32_t>(h_q);
+  a->h_kv = static_cast<int32_t>(h_kv);
+  a->d = static_cast<int32_t>(d);
+  a->scale = static_cast<float>(sm_scale);
+  a->dtype = q->scalar_type() == at::kBFloat16;
+  *q_out = q;
+  return true;
+}
+
+// linear_varlen(q, k, v, log_decay, cu_seqlens, max_seqlen, state, state_indices, has_state, sm_scale): o
+PyObject* linear_varlen(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 10) return none();
+  const at::Tensor *cu = plain(args[4]), *q;
+  int64_t most;
+  fa_linear_args a = {};
+  if (!cu || !to_int(args[5], &most) || most < 0 || cu->scalar_type() != at::kInt ||
+      cu->dim() != 1 || cu->size(0) < 1 || !cu->is_contiguous() ||
+      !linear_of(args, args[6], args[7], args[9], true, cu->size(0) - 1, &a, &q) ||
+      cu->device() != q->device())
+    return none();
+  a.cu_seqlens = cu->data_ptr<int32_t>();
+  if (args[8] != Py_None) {
+    const at::Tensor* has = plain(args[8]);
+    if (!has || !a.state || (has->scalar_type() != at::kBool && has->scalar_type() != at::kByte) ||
+        has->dim() != 1 || has->size(0) != a.num_seqs || !has->is_contiguous() ||
+        has->device() != q->device())
+      return none();
+    a.has_state = static_cast<const uint8_t*>(has->data_ptr());
+  }
+  const c10::Device device = q->device();
+  const int cus = cu_count(device.index());
+  if (cus == 0) return none();
+  at::Tensor out;
+  {
+    NoGil nogil;
+    c10::DeviceGuard guard(device);
+    out = make(q->sizes(), q->scalar_type(), device);
+    a.out = out.data_ptr();
+    const int64_t floats =
+        fa_linear_plan(&a, static_cast<int32_t>(std::min<int64_t>(most, a.total)), cus);
+    check(static_cast<int>(std::min<int64_t>(floats, 0)));
+    at::Tensor part;
+    if (floats > 0) {
+      part = make({floats}, at::kFloat, device);
+      a.part = part.data_ptr<float>();
+    }
+    check(fa_linear_prompt(&a, stream_of(device)));
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// linear_decode(q, k, v, log_decay, state, state_indices, sm_scale): o
+PyObject* linear_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 7) return none();
+  const at::Tensor* q;
+  fa_linear_args a = {};
+  if (!linear_of(args, args[4], args[5], args[6], false, -1, &a, &q)) return none();
+  const c10::Device device = q->device();
+  at::Tensor out;
+  {
+    NoGil nogil;
+    c10::DeviceGuard guard(device);
+    out = make(q->sizes(), q->scalar_type(), device);
+    a.out = out.data_ptr();
+    check(fa_linear_token(&a, stream_of(device)));
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 #define FA_METHOD(name)                                                                     \
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, \
    nullptr}
@@ -927,7 +1236,8 @@ PyMethodDef g_methods[] = {FA_METHOD(mla_metadata), FA_METHOD(mla_decode),   FA_
                            FA_METHOD(contiguous),   FA_METHOD(topk_indices), FA_METHOD(cache_write),
                            FA_METHOD(split_counts), FA_METHOD(varlen),
                            FA_METHOD(mxfp4_write),  FA_METHOD(mxfp4_gather),
-                           FA_METHOD(mxfp4_decode), {nullptr, nullptr, 0, nullptr}};
+                           FA_METHOD(mxfp4_decode), FA_METHOD(rotary),     FA_METHOD(rotary_cache),
+                           FA_METHOD(linear_varlen), FA_METHOD(linear_decode), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, g_methods};
 
 }  // namespace

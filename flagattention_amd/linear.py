@@ -137,6 +137,12 @@ def linear_attention_varlen(
     outputs that it reaches and the state not finite (not always the infinity that the sums
     would have); tokens before it are not touched.
     """
+    fast = _lib.native()
+    if fast is not None:
+        o = fast.linear_varlen(q, k, v, log_decay, cu_seqlens, max_seqlen, state, state_indices,
+                               has_state, sm_scale)
+        if o is not None:
+            return o
     total, h_q, h_kv, d, code = _check_rows(q, k, v)
     _check_decay(log_decay, h_kv)
     _require(cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.shape[0] >= 1
@@ -192,6 +198,11 @@ def linear_attention_decode(
 
     Returns ``o`` shaped and typed like ``q``.
     """
+    fast = _lib.native()
+    if fast is not None:
+        o = fast.linear_decode(q, k, v, log_decay, state, state_indices, sm_scale)
+        if o is not None:
+            return o
     num_seqs, h_q, h_kv, d, code = _check_rows(q, k, v)
     _check_decay(log_decay, h_kv)
     _require(num_seqs <= 65535 and num_seqs * h_kv < 1 << 22, "too many sequences or heads")
@@ -199,6 +210,8 @@ def linear_attention_decode(
     scale = _scale(sm_scale, d)
     _one_device(q, k, v, log_decay, state, state_indices)
     q, k, v = _rows(q, k, v)
+    if state.shape[0] == 0:
+        return torch.zeros((num_seqs, h_q, d), dtype=q.dtype, device=q.device)
     o = torch.empty((num_seqs, h_q, d), dtype=q.dtype, device=q.device)
     if num_seqs > 0:
         args = _args(q, k, v, log_decay, state, state_indices, o, num_seqs, scale, code)

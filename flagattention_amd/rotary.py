@@ -121,6 +121,12 @@ def rotary_embedding(
 
     Returns ``(q, k)``, turned.
     """
+    fast = _lib.native()
+    if fast is not None:
+        both = fast.rotary(q, k, positions, inv_freq, sections, mixed_sections, adjacent_pairs,
+                           inplace)
+        if both is not None:
+            return both
     code = _check_heads(q, k)
     _, sections = _check_turn(q.shape[0], q.shape[2], positions, inv_freq, sections, mixed_sections)
     if inplace:
@@ -171,6 +177,12 @@ def rotary_cache_kv(
     Returns the turned ``q``, ready for ``paged_attention`` or, with the packed k and v of a prompt,
     ``flash_attention_varlen``.
     """
+    fast = _lib.native()
+    if fast is not None:
+        done = fast.rotary_cache(q, k, v, positions, inv_freq, key_cache, value_cache, slot_mapping,
+                                 sections, mixed_sections, adjacent_pairs)
+        if done is not None:
+            return done
     code = _check_heads(q, k)
     _require(v.shape == k.shape and v.dtype == k.dtype, "k and v shapes or dtypes differ")
     tokens, _, d = q.shape
