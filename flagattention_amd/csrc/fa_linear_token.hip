@@ -9,6 +9,7 @@
 #include "fa_common.h"
 #include "fa_divide.h"
 #include "fa_linear.h"
+#include "fa_wave.h"
 #include "flagattention_amd_linear.h"
 
 namespace fa {
@@ -16,6 +17,13 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kGroup = 8;  // query heads whose sums are taken at once
+
+// The value of the lane kBy places on, around a row of 16.
+template <int kBy>
+__device__ inline float ror16(float x) {
+  return __uint_as_float(static_cast<unsigned int>(__builtin_amdgcn_update_dpp(
+      0, static_cast<int>(__float_as_uint(x)), 0x120 + kBy, 0xF, 0xF, false)));
+}
 
 template <typename T, int D, int kCols>
 __global__ __launch_bounds__(kThreads) void linear_token_kernel(const fa_linear_args a,
@@ -25,7 +33,7 @@ __global__ __launch_bounds__(kThreads) void linear_token_kernel(const fa_linear_
   constexpr int kSteps = D / kRows;
   static_assert(kSteps >= 1 && kSteps * kRows == D, "whole steps");
   __shared__ float ks[D], qs[kGroup][D];
-  __shared__ float sums[4][kGroup][kCols];
+  __shared__ __attribute__((aligned(16))) float sums[4][kGroup][kCols];
 
   const int tid = threadIdx.x;
   const int b = divide(blockIdx.x, h_kv);
@@ -81,10 +89,11 @@ __global__ __launch_bounds__(kThreads) void linear_token_kernel(const fa_linear_
       }
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-#pragma unroll
-        for (int m = kLanes; m < 64; m *= 2) o[x] += __shfl_xor(o[x], m);
-        if ((tid & 63) < kLanes) sums[tid >> 6][g][col + x] = o[x];
+        if (kLanes <= 8) o[x] += ror16<8>(o[x]);
+        if (kLanes <= 16) o[x] = sum_xor16(o[x]);
+        o[x] = sum_xor32(o[x]);
       }
+      if ((tid & 63) < kLanes) *reinterpret_cast<floatx4*>(&sums[tid >> 6][g][col]) = o;
     }
     __syncthreads();
     for (int i = tid; i < heads * kCols; i += kThreads) {
@@ -103,14 +112,28 @@ void launch(const fa_linear_args& a, hipStream_t stream) {
                      stream, a, divisor(a.h_kv));
 }
 
-template <typename T>
+// Columns of a work-group.  With few of them the state's rows are cut finer, so that more of the card
+// loads them (89 sequences of 2 KV heads, D = 128: 8.1 us with 32, 8.3 with 64; one of 16, D = 256: 4.3
+// / 4.9; 16 of 32, D = 128: 12.1 / 12.4); with many, wider pieces of rows come faster (64 of 32, D =
+// 128: 59.4 / 57.7; 64 of 64, D = 64: 23.8 / 22.0).  16 columns are 16 and 25% slower in these.
+constexpr int kManyWgs = 2048;
+
+template <typename T, int D>
 void launch_dim(const fa_linear_args& a, hipStream_t stream) {
-  if (a.d == 64)
-    launch<T, 64, 64>(a, stream);
-  else if (a.d == 128)
-    launch<T, 128, 64>(a, stream);
+  if (static_cast<int64_t>(a.num_seqs) * a.h_kv * (D / 64) < kManyWgs)
+    launch<T, D, 32>(a, stream);
   else
-    launch<T, 256, 64>(a, stream);
+    launch<T, D, 64>(a, stream);
+}
+
+template <typename T>
+void launch_type(const fa_linear_args& a, hipStream_t stream) {
+  if (a.d == 64)
+    launch_dim<T, 64>(a, stream);
+  else if (a.d == 128)
+    launch_dim<T, 128>(a, stream);
+  else
+    launch_dim<T, 256>(a, stream);
 }
 
 }  // namespace
@@ -126,7 +149,7 @@ extern "C" int fa_linear_token(const fa_linear_args* args, void* stream) {
   if (a.num_seqs == 0) return FA_OK;
   FA_CHECK_ARG(a.state != nullptr, "state is NULL");
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  a.dtype == 1 ? fa::launch_dim<fa::bf16>(a, s) : fa::launch_dim<_Float16>(a, s);
+  a.dtype == 1 ? fa::launch_type<fa::bf16>(a, s) : fa::launch_type<_Float16>(a, s);
   FA_CHECK_HIP(hipGetLastError());
   return FA_OK;
 }

@@ -13,22 +13,23 @@ namespace fa {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kHeads = 4;  // rows that a thread takes at most
 
 struct RotaryPlan {
   Divisor units, chunks;  // units of a row; threads that share a token's rows
+  Divisor axes, block;    // block: where a slot fits 31 bits
+  bool small_slots;
   int rows;               // rows of a token: q's heads, k's, and with caches v's
-  long long threads;
+  int threads;
 };
 
-template <typename T, int kVec>
+template <typename T, int kVec, int kHeads, bool kAdjacent>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(const fa_rotary_args a,
                                                           const RotaryPlan plan) {
   typedef T Vec __attribute__((ext_vector_type(kVec)));
-  const long long id = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x;
+  const int id = blockIdx.x * kThreads + threadIdx.x;  // below 2^31 (host)
   if (id >= plan.threads) return;
-  const int of_block = divide(static_cast<int>(id), plan.units);  // below 2^31 (host)
-  const int unit = static_cast<int>(id) - of_block * static_cast<int>(plan.units.by);
+  const int of_block = divide(id, plan.units);
+  const int unit = id - of_block * static_cast<int>(plan.units.by);
   const int t = divide(of_block, plan.chunks);
   const int chunk = of_block - t * static_cast<int>(plan.chunks.by);
 
@@ -37,108 +38,138 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const fa_rotary_args a
   const bool turns = unit < turning;
   int first, second;
   if (turns) {
-    first = a.adjacent ? 2 * kVec * unit : kVec * unit;
-    second = first + (a.adjacent ? kVec : a.pairs);
+    first = kAdjacent ? 2 * kVec * unit : kVec * unit;
+    second = first + (kAdjacent ? kVec : a.pairs);
   } else {
     first = 2 * a.pairs + 2 * kVec * (unit - turning);
     second = first + kVec;
   }
   const bool both = second < a.d;
 
+  // where the rows come from and go to; every load is on its way before the first is used
+  const T* src[kHeads];
+  T* dst[kHeads];
+  bool turn[kHeads], write[kHeads];
+  long long k_at = 0, v_at = 0;
+  bool kept = true;
+  if (a.key_cache) {
+    const long long slot = a.slots64 ? static_cast<const long long*>(a.slots)[t]
+                                     : static_cast<const int*>(a.slots)[t];
+    kept = slot >= 0 && slot < a.num_blocks * a.block_size;
+    const long long block = !kept ? 0 : plan.small_slots ? divide(static_cast<int>(slot), plan.block)
+                                                         : slot / a.block_size;
+    const long long row = kept ? slot - block * a.block_size : 0;
+    k_at = block * a.kc_stride_0 + row * a.kc_stride_t;
+    v_at = block * a.vc_stride_0 + row * a.vc_stride_t;
+  }
+#pragma unroll
+  for (int n = 0; n < kHeads; ++n) {
+    const int row = chunk + n * static_cast<int>(plan.chunks.by);
+    write[n] = row < plan.rows;
+    turn[n] = turns;
+    if (row < a.h_q) {
+      src[n] = static_cast<const T*>(a.q) + t * a.q_stride_t + row * a.q_stride_h;
+      dst[n] = static_cast<T*>(a.q_out) + t * a.q_out_stride_t + row * a.q_out_stride_h;
+    } else if (row < a.h_q + a.h_kv) {
+      const int h = row - a.h_q;
+      src[n] = static_cast<const T*>(a.k) + t * a.k_stride_t + h * a.k_stride_h;
+      if (a.key_cache) {
+        dst[n] = static_cast<T*>(a.key_cache) + k_at + h * a.kc_stride_h;
+        write[n] = kept;
+      } else {
+        dst[n] = static_cast<T*>(a.k_out) + t * a.k_out_stride_t + h * a.k_out_stride_h;
+      }
+    } else {
+      const int h = row - a.h_q - a.h_kv;
+      src[n] = static_cast<const T*>(a.v) + t * a.v_stride_t + h * a.v_stride_h;
+      dst[n] = static_cast<T*>(a.value_cache) + v_at + h * a.vc_stride_h;
+      write[n] = write[n] && kept;
+      turn[n] = false;
+    }
+  }
+  Vec p[kHeads], q[kHeads];
+#pragma unroll
+  for (int n = 0; n < kHeads; ++n) {
+    if (!write[n]) continue;
+    p[n] = *reinterpret_cast<const Vec*>(src[n] + first);
+    if (both) q[n] = *reinterpret_cast<const Vec*>(src[n] + second);
+  }
+
   float c[kVec], s[kVec];
   if (turns) {
+    // every axis at once (past the last one, the last one again): one trip to memory
+    long long whole[FA_ROTARY_MAX_AXES];
+    if (a.pos64) {
+#pragma unroll
+      for (int n = 0; n < FA_ROTARY_MAX_AXES; ++n)
+        whole[n] = static_cast<const long long*>(a.positions)[min(n, a.axes - 1) * a.pos_stride_a + t];
+    } else {
+#pragma unroll
+      for (int n = 0; n < FA_ROTARY_MAX_AXES; ++n)
+        whole[n] = static_cast<const int*>(a.positions)[min(n, a.axes - 1) * a.pos_stride_a + t];
+    }
+    double at[FA_ROTARY_MAX_AXES];
+#pragma unroll
+    for (int n = 0; n < FA_ROTARY_MAX_AXES; ++n) at[n] = static_cast<double>(whole[n]);
+    // mixed: pair i is number `round` of axis `of`
+    int round = 0, of = 0;
+    if (a.mixed) {
+      round = divide(kVec * unit, plan.axes);
+      of = kVec * unit - round * a.axes;
+    }
 #pragma unroll
     for (int x = 0; x < kVec; ++x) {
       const int i = kVec * unit + x;
-      int axis = 0;
+      double pos = at[0];
       if (a.axes > 1) {
-        if (a.mixed) {
-          const int of = i % a.axes;
-          axis = i / a.axes < a.sections[of] ? of : 0;
-        } else {
-          int end = a.sections[0];
+        int end = a.sections[0];
 #pragma unroll
-          for (int n = 1; n < FA_ROTARY_MAX_AXES; ++n) {
-            axis = n < a.axes && i >= end ? n : axis;
-            end += a.sections[n];
-          }
+        for (int n = 1; n < FA_ROTARY_MAX_AXES; ++n) {
+          if (n >= a.axes) break;
+          const bool takes = a.mixed ? of == n && round < a.sections[n] : i >= end;
+          pos = takes ? at[n] : pos;
+          end += a.sections[n];
+        }
+        if (a.mixed && ++of == a.axes) {
+          of = 0;
+          ++round;
         }
       }
-      const long long at = axis * a.pos_stride_a + t;
-      const long long pos = a.pos64 ? static_cast<const long long*>(a.positions)[at]
-                                    : static_cast<const int*>(a.positions)[at];
       constexpr double kPerTurn = 0.15915494309189533577;  // 1 / (2 pi)
-      const double turn = static_cast<double>(pos) * static_cast<double>(a.inv_freq[i]) * kPerTurn;
-      const float part = static_cast<float>(turn - __builtin_rint(turn));
+      const double turned = pos * static_cast<double>(a.inv_freq[i]) * kPerTurn;
+      const float part = static_cast<float>(turned - __builtin_rint(turned));
       c[x] = __builtin_amdgcn_cosf(part);
       s[x] = __builtin_amdgcn_sinf(part);
     }
   }
 
-  long long slot = 0, block = 0, row_of = 0;
-  bool kept = true;
-  if (a.key_cache) {
-    slot = a.slots64 ? static_cast<const long long*>(a.slots)[t]
-                     : static_cast<const int*>(a.slots)[t];
-    kept = slot >= 0 && slot < a.num_blocks * a.block_size;
-    block = kept ? slot / a.block_size : 0;
-    row_of = kept ? slot - block * a.block_size : 0;
-  }
+#pragma unroll
   for (int n = 0; n < kHeads; ++n) {
-    const int row = chunk + n * static_cast<int>(plan.chunks.by);
-    if (row >= plan.rows) break;
-    const T* src;
-    T* dst;
-    bool turn = turns, write = true;
-    if (row < a.h_q) {
-      src = static_cast<const T*>(a.q) + t * a.q_stride_t + row * a.q_stride_h;
-      dst = static_cast<T*>(a.q_out) + t * a.q_out_stride_t + row * a.q_out_stride_h;
-    } else if (row < a.h_q + a.h_kv) {
-      const int h = row - a.h_q;
-      src = static_cast<const T*>(a.k) + t * a.k_stride_t + h * a.k_stride_h;
-      if (a.key_cache) {
-        dst = static_cast<T*>(a.key_cache) + block * a.kc_stride_0 + h * a.kc_stride_h +
-              row_of * a.kc_stride_t;
-        write = kept;
-      } else {
-        dst = static_cast<T*>(a.k_out) + t * a.k_out_stride_t + h * a.k_out_stride_h;
-      }
-    } else {
-      const int h = row - a.h_q - a.h_kv;
-      src = static_cast<const T*>(a.v) + t * a.v_stride_t + h * a.v_stride_h;
-      dst = static_cast<T*>(a.value_cache) + block * a.vc_stride_0 + h * a.vc_stride_h +
-            row_of * a.vc_stride_t;
-      write = kept;
-      turn = false;
-    }
-    if (!write) continue;
-    const Vec p = *reinterpret_cast<const Vec*>(src + first);
-    Vec q = p;
-    if (both) q = *reinterpret_cast<const Vec*>(src + second);
-    Vec y = p, z = q;
-    if (turn) {
-      if (a.adjacent) {
+    if (!write[n]) continue;
+    Vec y = p[n], z = q[n];
+    if (turn[n]) {
 #pragma unroll
-        for (int x = 0; x < kVec; ++x) {
-          // pair x of the unit is elements 2x, 2x + 1 of its 2 kVec
-          const float u = static_cast<float>(2 * x < kVec ? p[(2 * x) % kVec] : q[(2 * x) % kVec]);
-          const float w = static_cast<float>(2 * x + 1 < kVec ? p[(2 * x + 1) % kVec]
-                                                              : q[(2 * x + 1) % kVec]);
-          const T yu = static_cast<T>(u * c[x] - w * s[x]), yw = static_cast<T>(w * c[x] + u * s[x]);
-          if (2 * x < kVec) y[(2 * x) % kVec] = yu; else z[(2 * x) % kVec] = yu;
-          if (2 * x + 1 < kVec) y[(2 * x + 1) % kVec] = yw; else z[(2 * x + 1) % kVec] = yw;
-        }
-      } else {
-#pragma unroll
-        for (int x = 0; x < kVec; ++x) {
-          const float u = static_cast<float>(p[x]), w = static_cast<float>(q[x]);
-          y[x] = static_cast<T>(u * c[x] - w * s[x]);
-          z[x] = static_cast<T>(w * c[x] + u * s[x]);
+      for (int x = 0; x < kVec; ++x) {
+        // pair x of adjacent ones is elements 2x and 2x + 1 of the unit's 2 kVec
+        constexpr auto lower = [](int e) { return e < kVec; };
+        const int e = 2 * x;
+        const float u = static_cast<float>(!kAdjacent ? p[n][x] : lower(e) ? p[n][e % kVec]
+                                                                            : q[n][e % kVec]);
+        const float w = static_cast<float>(!kAdjacent      ? q[n][x]
+                                           : lower(e + 1) ? p[n][(e + 1) % kVec]
+                                                          : q[n][(e + 1) % kVec]);
+        const T yu = static_cast<T>(u * c[x] - w * s[x]), yw = static_cast<T>(w * c[x] + u * s[x]);
+        if (!kAdjacent) {
+          y[x] = yu;
+          z[x] = yw;
+        } else {
+          if (lower(e)) y[e % kVec] = yu; else z[e % kVec] = yu;
+          if (lower(e + 1)) y[(e + 1) % kVec] = yw; else z[(e + 1) % kVec] = yw;
         }
       }
     }
-    *reinterpret_cast<Vec*>(dst + first) = y;
-    if (both) *reinterpret_cast<Vec*>(dst + second) = z;
+    *reinterpret_cast<Vec*>(dst[n] + first) = y;
+    if (both) *reinterpret_cast<Vec*>(dst[n] + second) = z;
   }
 }
 
@@ -146,20 +177,38 @@ bool rows_of_16(const void* p, int64_t s0, int64_t s1) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s0 % 8 == 0 && s1 % 8 == 0;
 }
 
+// Rows of a thread: one while the launch leaves the card idle, four to share the sines then.  A thread's
+// rows come one after the other (three of 10 heads, D = 64: 4.8 us with four, 3.0 with one).
+constexpr int kFewThreads = 1 << 18;
+
+template <typename T, int kVec, int kHeads, bool kAdjacent>
+void launch_kernel(const fa_rotary_args& a, RotaryPlan plan, hipStream_t stream) {
+  const int chunks = cdiv(plan.rows, kHeads);
+  plan.chunks = divisor(chunks);
+  plan.threads = static_cast<int>(plan.units.by) * chunks * a.tokens;
+  hipLaunchKernelGGL((rotary_kernel<T, kVec, kHeads, kAdjacent>),
+                     dim3(static_cast<unsigned>(cdiv(plan.threads, kThreads))), dim3(kThreads), 0,
+                     stream, a, plan);
+}
+
 template <typename T, int kVec>
 void launch(const fa_rotary_args& a, hipStream_t stream) {
   RotaryPlan plan;
   // in place the dims that do not turn are there already
   const bool rest = a.key_cache || (a.h_q > 0 ? a.q != a.q_out : a.k != a.k_out);
-  const int units = a.pairs / kVec + (rest ? (a.d - 2 * a.pairs + 2 * kVec - 1) / (2 * kVec) : 0);
+  const int units = a.pairs / kVec + (rest ? cdiv(a.d - 2 * a.pairs, 2 * kVec) : 0);
   plan.rows = a.h_q + a.h_kv * (a.key_cache ? 2 : 1);
-  const int chunks = (plan.rows + kHeads - 1) / kHeads;
   plan.units = divisor(units);
-  plan.chunks = divisor(chunks);
-  plan.threads = static_cast<long long>(units) * chunks * a.tokens;
-  hipLaunchKernelGGL((rotary_kernel<T, kVec>),
-                     dim3(static_cast<unsigned>((plan.threads + kThreads - 1) / kThreads)),
-                     dim3(kThreads), 0, stream, a, plan);
+  plan.axes = divisor(a.axes);
+  plan.small_slots = a.key_cache && a.num_blocks * a.block_size <= INT32_MAX;
+  plan.block = divisor(plan.small_slots ? a.block_size : 1);
+  const bool few = static_cast<int64_t>(units) * plan.rows * a.tokens <= kFewThreads;
+  if (a.adjacent)
+    few ? launch_kernel<T, kVec, 1, true>(a, plan, stream)
+        : launch_kernel<T, kVec, 4, true>(a, plan, stream);
+  else
+    few ? launch_kernel<T, kVec, 1, false>(a, plan, stream)
+        : launch_kernel<T, kVec, 4, false>(a, plan, stream);
 }
 
 }  // namespace
@@ -204,7 +253,7 @@ extern "C" int fa_rotary(const fa_rotary_args* args, void* stream) {
   if (a.tokens == 0) return FA_OK;
   // a thread per unit and heads: ids of 31 bits
   FA_CHECK_ARG(static_cast<int64_t>(a.tokens) * (a.h_q + 2 * a.h_kv) * a.d < int64_t{1} << 40 &&
-                   static_cast<int64_t>(a.tokens) * ((a.h_q + 2 * a.h_kv + fa::kHeads - 1) / fa::kHeads) *
+                   static_cast<int64_t>(a.tokens) * ((a.h_q + 2 * a.h_kv + 3) / 4) *
                            (a.d / 2 + 1) < INT32_MAX - fa::kThreads,
                "too many tokens or heads");
   bool wide = a.pairs % 8 == 0 && a.d % 8 == 0;
