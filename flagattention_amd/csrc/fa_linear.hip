@@ -90,7 +90,7 @@ __device__ inline void sync() {
 __device__ inline void lds_dma16_at(const unsigned char* base, unsigned int off, unsigned int to) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                :
-               : "v"(off), "s"(base), "s"(to)
+               : "v"(off), "s"(base), "s"(uniform(static_cast<int>(to)))
                : "memory", "m0");
 }
 
@@ -184,9 +184,10 @@ __device__ inline Run find_run(const fa_linear_args& a, int index) {
 }
 
 // kStates: only the states that segments make, each from zeros (the first from its sequence's).
-// kOne: groups of one query head.
-template <typename T, int D, bool kStates, bool kOne>
-__global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a,
+// kOne: groups of one query head.  kSplit: heads that are attended at once, by D / 32 waves each, which
+// all keep the state.
+template <typename T, int D, bool kStates, bool kOne, int kSplit>
+__global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_linear_args a,
                                                           const Divisor h_kv) {
   typedef typename PVec<T>::v8 T8;
   typedef typename PVec<T>::v4 T4;
@@ -194,7 +195,9 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
   constexpr int C = D / 8;
   constexpr int kRowB = 2 * D;
   constexpr int kTileB = kChunk * kRowB;
-  constexpr int kCopies = 2;  // of 1 KiB a wave and tile
+  constexpr int kThreads = 2 * D * kSplit;
+  constexpr int kCopies = 2;               // of 1 KiB a wave, of its head's q tile
+  constexpr int kKvCopies = 4 / kSplit;    // of the k and v tiles
   constexpr int kRowsPerCopy = 512 / D;
   constexpr int kKSteps = D / 16;
   constexpr int kTiles = D / 32;
@@ -204,12 +207,13 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
   constexpr bool kKeepQ = D == 64;  // from the scores to S^T Q^T, else it is read twice
   static_assert(kCopies * kTiles * 1024 == kTileB, "whole copies per wave");
   // [k, v, q][stage]
-  __shared__ __attribute__((aligned(1024))) unsigned char bufs[(kStates ? 2 : 3) * kStages * kTileB];
+  __shared__ __attribute__((aligned(1024))) unsigned char bufs[(kStates ? 2 : 2 + kSplit) * kStages * kTileB];
   // weights by the place m of a token before the chunk's last: scale e^{a (31 - m)}, 0 past 31 (tokens
   // to come); and e^{a (31 - m)}, 1 past 31
   __shared__ float seen[2 * kChunk], left_of[2 * kChunk];
 
-  const int wave = wave_id();
+  const int wave = uniform(wave_id() % kTiles);     // 32 columns of the state
+  const int part_of = uniform(wave_id() / kTiles);  // of the heads at once
   const int lane = threadIdx.x & 63;
   const int h = lane >> 5, c32 = lane & 31;
   const int group = kStates || kOne ? 1 : a.h_q / a.h_kv;
@@ -220,8 +224,8 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
     const long long row16 = static_cast<long long>(a.h_q) * C;
     const long long head = first * row16, all = a.total * row16, tail = behind * row16;
     uintx4* const out16 = static_cast<uintx4*>(a.out);
-    const long long step = static_cast<long long>(gridDim.x) * (2 * D);
-    const long long me = static_cast<long long>(blockIdx.x) * (2 * D) + threadIdx.x;
+    const long long step = static_cast<long long>(gridDim.x) * kThreads;
+    const long long me = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x;
     for (long long i = me; i < head; i += step) out16[i] = uintx4{0, 0, 0, 0};
     for (long long i = tail + me; i < all; i += step) out16[i] = uintx4{0, 0, 0, 0};
   }
@@ -252,7 +256,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
   float* const to_state = kStates ? part + static_cast<long long>(a.h_kv) * (D * D)
                                   : run.last ? slot_state : nullptr;
 
-  // Items are (chunk, query head of the group), heads innermost; k and v come with the first head.
+  // Items are (chunk, kSplit query heads of the group), heads innermost; k and v come with the first.
   // States alone go through the chunks from the last one back: what they read last is what the next
   // launch reads first.
   const int chunks = cdiv(n, kChunk);
@@ -267,25 +271,23 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
       2 * (begin * a.q_stride_t + static_cast<long long>(hk) * group * a.q_stride_h);
   const unsigned int q_tb = 2 * a.q_stride_t, k_tb = 2 * a.k_stride_t, v_tb = 2 * a.v_stride_t;
   const long long q_hb = 2 * a.q_stride_h;
-  const long long q_step = static_cast<long long>(kChunk) * q_tb - (group - 1) * q_hb;
+  // A tile is 2 kTiles copies of 1 KiB; a wave's are number 2 wave and 2 wave + 1.
   int copy_row[kCopies], copy_piece[kCopies];
 #pragma unroll
   for (int i = 0; i < kCopies; ++i) {
     copy_row[i] = (kCopies * wave + i) * kRowsPerCopy + lane / C;
     copy_piece[i] = 16 * ((lane % C) ^ swizzle<C>(copy_row[i]));
   }
-  const unsigned int lds = uniform(static_cast<int>(reinterpret_cast<__SIZE_TYPE__>(
-                               (FA_LDS unsigned char*)bufs))) + kCopies * 1024 * wave;
   // Rows past the end repeat the last one.  Offsets are worked out afresh: kept for three tensors they
   // would be spilled, and a wait for one that comes back from memory waits for every copy.
-  auto copy = [&](const unsigned char* from, unsigned int row_b, int rows, unsigned int to) {
-#pragma unroll
-    for (int i = 0; i < kCopies; ++i) {
-      int r = copy_row[i];
-      asm volatile("" : "+v"(r));
-      lds_dma16_at(from, __umul24(min(r, rows - 1), row_b) + copy_piece[i], to + 1024 * i);
-    }
+  auto copy = [&](const unsigned char* from, unsigned int row_b, int rows, unsigned int to, int i) {
+    int r = copy_row[i];
+    asm volatile("" : "+v"(r));
+    lds_dma16_at(from, __umul24(min(r, rows - 1), row_b) + copy_piece[i],
+                 to + 1024 * (kCopies * wave + i));
   };
+  const unsigned int lds = uniform(static_cast<int>(
+      reinterpret_cast<__SIZE_TYPE__>((FA_LDS unsigned char*)bufs)));
   auto rows_of = [&](int chunk) {  // chunk: from the run's first item on
     return kStates ? (chunk == 0 ? n - (chunks - 1) * kChunk : kChunk) : n - chunk * kChunk;
   };
@@ -297,29 +299,44 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
     const int rows = rows_of(next_chunk);
     int issued = 0;
     if (!kStates) {
-      copy(q_next, q_tb, rows, lds + 2 * kStages * kTileB + next_q);
-      next_q = next_q == (kStages - 1) * kTileB ? 0 : next_q + kTileB;
+      const int mine = kSplit == 1 ? next_head : min(next_head + part_of, group - 1);
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i)
+        copy(q_next + mine * q_hb, q_tb, rows, lds + (2 * kStages + part_of) * kTileB + next_q, i);
+      next_q = next_q == (kStages - 1) * kSplit * kTileB ? 0 : next_q + kSplit * kTileB;
       issued += kCopies;
     }
     if (next_head == 0) {
-      copy(k_next, k_tb, rows, lds + next_kv);
-      copy(v_next, v_tb, rows, lds + kStages * kTileB + next_kv);
+      // the heads' waves share them: all of k and v, k or v, or half of one
+      const unsigned int to_k = lds + next_kv, to_v = to_k + kStages * kTileB;
+      if constexpr (kSplit == 1) {
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) copy(k_next, k_tb, rows, to_k, i);
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) copy(v_next, v_tb, rows, to_v, i);
+      } else {
+        const bool takes_v = part_of >= kSplit / 2;  // uniform
+        const unsigned char* const from = takes_v ? v_next : k_next;
+        const unsigned int row_b = takes_v ? v_tb : k_tb, to = takes_v ? to_v : to_k;
+        if (kSplit == 2 || part_of % 2 == 0) copy(from, row_b, rows, to, 0);
+        if (kSplit == 2 || part_of % 2 == 1) copy(from, row_b, rows, to, 1);
+      }
       next_kv = next_kv == (kStages - 1) * kTileB ? 0 : next_kv + kTileB;
       k_next += (kStates ? -kChunk : kChunk) * static_cast<long long>(k_tb);
       v_next += (kStates ? -kChunk : kChunk) * static_cast<long long>(v_tb);
-      issued += 2 * kCopies;
+      issued += kKvCopies;
     }
-    if (++next_head == group) {
+    next_head += kSplit;
+    if (next_head >= group) {
       next_head = 0;
       ++next_chunk;
-      q_next += q_step;
-    } else {
-      q_next += q_hb;
+      q_next += kChunk * static_cast<long long>(q_tb);
     }
     return issued;
   };
   fetch();
   int ahead = fetch();  // copies on their way after those of the item at hand
+  int stored = 0;       // stores of the last item
 
   // Row rho of a 32-row tile of the state (or of O^T) is dim 16 (rho / 16) + 8 ((rho / 4) % 2) +
   // 4 ((rho / 8) % 2) + rho % 4: accumulator register r of half h is then dim 16 (r / 8) + 8h + r % 8.
@@ -421,12 +438,17 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
                        2 * (static_cast<long long>(run.start) * a.h_q + hk * group) * D;
   while (true) {
     // all but what was issued after this item's copies: the next item's, and the last one's stores
-    if (first || ahead == 0)
-      wait_vmem<0>();
-    else if (ahead == (kStates ? 2 : 3) * kCopies)
-      wait_vmem<(kStates ? 2 * kCopies : 3 * kCopies + 2)>();
+    const int pending = first || ahead == 0 ? 0 : ahead + stored;
+    if (pending >= 8)
+      wait_vmem<8>();
+    else if (pending >= 6)
+      wait_vmem<6>();
+    else if (pending >= 4)
+      wait_vmem<4>();
+    else if (pending >= 2)
+      wait_vmem<2>();
     else
-      wait_vmem<kCopies + 2>();
+      wait_vmem<0>();
     first = false;
     sync();
     ahead = fetch();
@@ -434,7 +456,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
     unsigned char* const vb = bufs + kStages * kTileB + kv_stage;
     const int taken = min(rows_of(chunk), kChunk);
     if (taken < kChunk && head == 0) {  // uniform: rows past the end become zeros
-      for (int i = taken * kRowB / 16 + threadIdx.x; i < kTileB / 16; i += 2 * D) {
+      for (int i = taken * kRowB / 16 + threadIdx.x; i < kTileB / 16; i += kThreads) {
         reinterpret_cast<uintx4*>(kb)[i] = uintx4{0, 0, 0, 0};
         reinterpret_cast<uintx4*>(vb)[i] = uintx4{0, 0, 0, 0};
       }
@@ -507,6 +529,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
       }
     };
 
+    const bool mine = kSplit == 1 || head + part_of < group;  // uniform
     bool odd = false;  // something is not finite
     floatx16 o = {};
     if constexpr (kStates) {
@@ -515,9 +538,9 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
       for (int ss = 0; ss < 2; ++ss) fold_bits(best, __builtin_bit_cast(uintx4, va[ss]));
       odd = __ballot(is_odd<T>(best)) != 0ull;
     } else {
-      int q_row = 2 * kStages * kTileB + q_stage + row_at;
+      int q_row = (2 * kStages + part_of) * kTileB + q_stage + row_at;
       asm volatile("" : "+v"(q_row));
-      q_stage = q_stage == (kStages - 1) * kTileB ? 0 : q_stage + kTileB;
+      q_stage = q_stage == (kStages - 1) * kSplit * kTileB ? 0 : q_stage + kSplit * kTileB;
       // O^T of the item.  kOdd: with weights of 0 for what is not finite and yet to come.
       auto attend = [&](auto tag) {
         constexpr bool kOdd = decltype(tag)::value != 0;
@@ -611,7 +634,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
           }
         }
       };
-      attend(IntTag<0>{});
+      if (mine) attend(IntTag<0>{});
       // An infinity or a NaN among the scores or in v reaches the tokens before its own, through
       // weights of 0, and the outputs of its own: such a chunk is taken again.
       floatx4 trace = {0.f, 0.f, 0.f, 0.f};
@@ -629,24 +652,29 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
     }
 
     T8 kt[2][2];  // K^T of a tile of the state, the next one on its way
-    if (kStates || head + 1 == group) {
+    if (kStates || head + kSplit >= group) {
       kt[0][0] = transposed(k_tr, 0, 0);
       kt[0][1] = transposed(k_tr, 0, 1);
     }
     if constexpr (!kStates) {
-      if (c32 < taken) {
+      stored = 0;
+      if (mine) {
+        if (c32 < taken) {
+          unsigned char* const to = out + 2 * D * (head + part_of) + out_at;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          T8 y;
+          for (int half = 0; half < 2; ++half) {
+            T8 y;
 #pragma unroll
-          for (int x = 0; x < 8; ++x) y[x] = static_cast<T>(o[8 * half + x]);
-          *reinterpret_cast<T8*>(out + out_at + 32 * half) = y;
+            for (int x = 0; x < 8; ++x) y[x] = static_cast<T>(o[8 * half + x]);
+            *reinterpret_cast<T8*>(to + 32 * half) = y;
+          }
         }
+        stored = 2;
       }
-      out += 2 * D;
-      if (++head < group) continue;
+      head += kSplit;
+      if (head < group) continue;
       head = 0;
-      out += 2 * D * (static_cast<long long>(kChunk) * a.h_q - group);
+      out += 2 * D * static_cast<long long>(kChunk) * a.h_q;
       if (chunk + 1 == chunks && to_state == nullptr) break;
     }
 
@@ -704,6 +732,10 @@ __global__ __launch_bounds__(2 * D, 2) void linear_kernel(const fa_linear_args a
     }
   }
 
+  if (kSplit > 1) {  // the heads' waves read the state that those of the first write
+    sync();
+    if (part_of > 0) return;
+  }
   if (to_state != nullptr) {
     const float back = kHalf ? __builtin_amdgcn_ldexpf(sigma, s_power) : sigma;
 #pragma unroll
@@ -768,14 +800,20 @@ void launch(const fa_linear_args& a, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(runs_of(a) * a.h_kv));
   const Divisor h_kv = divisor(a.h_kv);
   if (a.segment > 0) {
-    hipLaunchKernelGGL((linear_kernel<T, D, true, false>), grid, dim3(2 * D), 0, stream, a, h_kv);
+    hipLaunchKernelGGL((linear_kernel<T, D, true, false, 1>), grid, dim3(2 * D), 0, stream, a, h_kv);
     hipLaunchKernelGGL((join_kernel<D>), dim3(static_cast<unsigned>(a.num_seqs * a.h_kv), D * D / 1024),
                        dim3(256), 0, stream, a, h_kv);
   }
+  constexpr int kWide = D == 64 ? 4 : D == 128 ? 2 : 1;
+  constexpr int kTwo = D == 256 ? 1 : 2;
   if (a.h_q == a.h_kv)
-    hipLaunchKernelGGL((linear_kernel<T, D, false, true>), grid, dim3(2 * D), 0, stream, a, h_kv);
+    hipLaunchKernelGGL((linear_kernel<T, D, false, true, 1>), grid, dim3(2 * D), 0, stream, a, h_kv);
+  else if (a.h_q == 2 * a.h_kv)
+    hipLaunchKernelGGL((linear_kernel<T, D, false, false, kTwo>), grid, dim3(2 * D * kTwo), 0, stream,
+                       a, h_kv);
   else
-    hipLaunchKernelGGL((linear_kernel<T, D, false, false>), grid, dim3(2 * D), 0, stream, a, h_kv);
+    hipLaunchKernelGGL((linear_kernel<T, D, false, false, kWide>), grid, dim3(2 * D * kWide), 0,
+                       stream, a, h_kv);
 }
 
 }  // namespace
