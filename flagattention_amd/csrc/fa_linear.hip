@@ -208,14 +208,15 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
   static_assert(kCopies * kTiles * 1024 == kTileB, "whole copies per wave");
   // [k, v, q][stage]
   __shared__ __attribute__((aligned(1024))) unsigned char bufs[(kStates ? 2 : 2 + kSplit) * kStages * kTileB];
-  // weights by the place m of a token before the chunk's last: scale e^{a (31 - m)}, 0 past 31 (tokens
-  // to come); and e^{a (31 - m)}, 1 past 31
-  __shared__ float seen[2 * kChunk], left_of[2 * kChunk];
+  // weights by the place m of a token before the chunk's last: at 1 + m scale e^{a (31 - m)}, 0 past 31
+  // (tokens to come); and e^{a (31 - m)}, 1 past 31
+  __shared__ float seen[1 + 2 * kChunk], left_of[2 * kChunk];
 
   const int wave = uniform(wave_id() % kTiles);     // 32 columns of the state
   const int part_of = uniform(wave_id() / kTiles);  // of the heads at once
-  const int lane = threadIdx.x & 63;
-  const int h = lane >> 5, c32 = lane & 31;
+  // At head dim 256 the state leaves few registers: what follows from the lane is worked out where it is
+  // used, and not kept (a wait for a register that comes back from memory waits for every copy too).
+  auto lane_id = [&]() -> int { return D == 256 ? fresh_lane() : threadIdx.x & 63; };
   const int group = kStates || kOne ? 1 : a.h_q / a.h_kv;
 
   if constexpr (!kStates) {  // rows of no sequence: everybody takes a share of their 16 bytes
@@ -271,19 +272,14 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
       2 * (begin * a.q_stride_t + static_cast<long long>(hk) * group * a.q_stride_h);
   const unsigned int q_tb = 2 * a.q_stride_t, k_tb = 2 * a.k_stride_t, v_tb = 2 * a.v_stride_t;
   const long long q_hb = 2 * a.q_stride_h;
-  // A tile is 2 kTiles copies of 1 KiB; a wave's are number 2 wave and 2 wave + 1.
-  int copy_row[kCopies], copy_piece[kCopies];
-#pragma unroll
-  for (int i = 0; i < kCopies; ++i) {
-    copy_row[i] = (kCopies * wave + i) * kRowsPerCopy + lane / C;
-    copy_piece[i] = 16 * ((lane % C) ^ swizzle<C>(copy_row[i]));
-  }
-  // Rows past the end repeat the last one.  Offsets are worked out afresh: kept for three tensors they
-  // would be spilled, and a wait for one that comes back from memory waits for every copy.
+  // A tile is 2 kTiles copies of 1 KiB; a wave's are number 2 wave and 2 wave + 1.  Rows past the end
+  // repeat the last one.
   auto copy = [&](const unsigned char* from, unsigned int row_b, int rows, unsigned int to, int i) {
-    int r = copy_row[i];
-    asm volatile("" : "+v"(r));
-    lds_dma16_at(from, __umul24(min(r, rows - 1), row_b) + copy_piece[i],
+    const int lane = lane_id();
+    int r = (kCopies * wave + i) * kRowsPerCopy + lane / C;
+    const int piece = 16 * ((lane % C) ^ swizzle<C>(r));
+    asm volatile("" : "+v"(r));  // no offsets are kept for three tensors
+    lds_dma16_at(from, __umul24(min(r, rows - 1), row_b) + piece,
                  to + 1024 * (kCopies * wave + i));
   };
   const unsigned int lds = uniform(static_cast<int>(
@@ -340,10 +336,14 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
 
   // Row rho of a 32-row tile of the state (or of O^T) is dim 16 (rho / 16) + 8 ((rho / 4) % 2) +
   // 4 ((rho / 8) % 2) + rho % 4: accumulator register r of half h is then dim 16 (r / 8) + 8h + r % 8.
-  const int pi = (c32 & 16) + 8 * ((c32 >> 2) & 1) + 4 * ((c32 >> 3) & 1) + (c32 & 3);
-  const int state_at = 8 * h * D + 32 * wave + pi;
+  auto state_place = [&]() -> int {
+    const int lane = lane_id(), c32 = lane & 31;
+    const int pi = (c32 & 16) + 8 * ((c32 >> 2) & 1) + 4 * ((c32 >> 3) & 1) + (c32 & 3);
+    return 8 * (lane >> 5) * D + 32 * wave + pi;
+  };
   floatx16 s[kTiles] = {};
   if (from_state) {
+    const int state_at = state_place();
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
@@ -352,6 +352,7 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
   }
   if constexpr (kStates) {
     if (from_state) {
+      const int state_at = state_place();
       const float fall = decay(log_decay, n);
 #pragma unroll
       for (int t = 0; t < kTiles; ++t)
@@ -366,7 +367,8 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
   if (threadIdx.x < 2 * kChunk) {
     const int m = threadIdx.x;
     const float e = decay(log_decay, max(kChunk - 1 - m, 0));
-    seen[m] = m < kChunk ? a.scale * e : 0.f;
+    seen[1 + m] = m < kChunk ? a.scale * e : 0.f;
+    if (m == 0) seen[0] = a.scale * decay(log_decay, kChunk);
     left_of[m] = e;
   }
   // The state is s times sigma = e^{a reset}, reset the tokens since s was last brought up: a product
@@ -410,15 +412,8 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
     looked = 0;
   };
   if (kHalf && !kStates && from_state) look();
-  const float since = a.scale * decay(log_decay, c32 + 1);
-
   // Token of register r in P^T's rows, and of element r of the values' operands, less 4h.
   auto token = [&](int r) { return 8 * (r >> 2) + (r & 3); };
-  const int row_at = c32 * kRowB + 16 * (h ^ swizzle<C>(c32));
-  // transposed reads: lanes 4e + x of 16 point at 4 dims of token row e
-  const int e = (lane & 15) >> 2, x4 = lane & 3, p16 = (lane >> 4) & 1;
-  const int tr_at = (4 * h + e) * kRowB + 16 * ((2 * p16 + (x4 & 1)) ^ swizzle<C>(4 * h + e)) +
-                    8 * (x4 >> 1);
   // dims 32t .. 32t + 31 of tokens token(8 ss) .. token(8 ss + 7), transposed
   // (from: the tile's first byte plus tr_at)
   auto transposed = [&](int from, int t, int ss) -> T8 {
@@ -432,8 +427,7 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
   int chunk = 0;
   bool first = true;
   T8 va[2];
-  // bytes of a lane's first row of the output, then of the item's first
-  const unsigned int out_at = 2 * (c32 * static_cast<unsigned int>(a.h_q * D) + 32 * wave + 8 * h);
+  // the chunk's first row of the output
   unsigned char* out = static_cast<unsigned char*>(a.out) +
                        2 * (static_cast<long long>(run.start) * a.h_q + hk * group) * D;
   while (true) {
@@ -479,6 +473,12 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
     // A chunk whose own fall is past the range is taken into s before its values are.
     const bool steep = !kStates && !(sigma_then >= 0.0625f && sigma_then <= 16.f);  // uniform
     // Addresses of this chunk, worked out afresh: kept, each of their many forms would be a register.
+    const int lane = lane_id(), h = lane >> 5, c32 = lane & 31;
+    const int row_at = c32 * kRowB + 16 * (h ^ swizzle<C>(c32));
+    // transposed reads: lanes 4e + x of 16 point at 4 dims of token row e
+    const int e = (lane & 15) >> 2, x4 = lane & 3, p16 = (lane >> 4) & 1;
+    const int tr_at = (4 * h + e) * kRowB +
+                      16 * ((2 * p16 + (x4 & 1)) ^ swizzle<C>(4 * h + e)) + 8 * (x4 >> 1);
     int k_row = kv_stage + row_at, k_tr = kv_stage + tr_at;
     asm volatile("" : "+v"(k_row), "+v"(k_tr));
     va[0] = transposed(kStages * kTileB + k_tr, wave, 0);
@@ -581,7 +581,8 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
             o = mfma_32x32x16(sa, qa[kKeepQ ? x : x % (2 * kGroupSteps)], o);
           }
         }
-        const float* const weight = seen + kChunk - 1 - c32 + 4 * h;
+        const float* const weight = seen + kChunk - c32 + 4 * h;
+        const float since = seen[kChunk - 1 - c32] * sigma;  // scale e^{a (i + 1)} of the state
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           p[r] *= weight[token(r)];
@@ -594,8 +595,7 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
           p_power = min(max(power_of(max_xor32(top)), kLeastPower), 100);
         }
         // O^T, relative to 2^p_power
-        const float by = kHalf ? __builtin_amdgcn_ldexpf(since * sigma, s_power - p_power)
-                               : since * sigma;
+        const float by = kHalf ? __builtin_amdgcn_ldexpf(since, s_power - p_power) : since;
         const float p_by = two_to(-p_power), p_back = two_to(p_power);
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[r] *= by;
@@ -660,7 +660,9 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
       stored = 0;
       if (mine) {
         if (c32 < taken) {
-          unsigned char* const to = out + 2 * D * (head + part_of) + out_at;
+          unsigned char* const to =
+              out + 2 * D * (head + part_of) +
+              2 * (c32 * static_cast<unsigned int>(a.h_q * D) + 32 * wave + 8 * h);
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             T8 y;
@@ -737,6 +739,7 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
     if (part_of > 0) return;
   }
   if (to_state != nullptr) {
+    const int state_at = state_place();
     const float back = kHalf ? __builtin_amdgcn_ldexpf(sigma, s_power) : sigma;
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
