@@ -257,6 +257,7 @@ class LinearArgs(ctypes.Structure):
         ("h_kv", ctypes.c_int32),
         ("d", ctypes.c_int32),
         ("segment", ctypes.c_int32),
+        ("joined", ctypes.c_int32),
         ("scale", ctypes.c_float),
         ("dtype", ctypes.c_int32),
     ]

@@ -183,12 +183,21 @@ __device__ inline Run find_run(const fa_linear_args& a, int index) {
   return run;
 }
 
-// kStates: only the states that segments make, each from zeros (the first from its sequence's).
-// kOne: groups of one query head.  kSplit: heads that are attended at once, by D / 32 waves each, which
-// all keep the state.
+// LDS of a work-group: tiles of k, v and of q's kHeads heads, kStages of each, and weights by the place m
+// of a token before the chunk's last: at 1 + m scale e^{a (31 - m)}, 0 past 31 (tokens to come); and
+// e^{a (31 - m)}, 1 past 31.
+template <int D, int kHeads>
+struct Lds {
+  unsigned char bufs[(2 + kHeads) * kStages * kChunk * 2 * D];
+  float seen[1 + 2 * kChunk], left_of[2 * kChunk];
+};
+
+// A run of one KV head, from its state through its chunks.  kStates: only the state that it makes, from
+// zeros, or the first run's from its sequence's.  kOne: groups of one query head.  kSplit: heads that are attended at once, by D / 32 waves
+// each, which all keep the state.
 template <typename T, int D, bool kStates, bool kOne, int kSplit>
-__global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_linear_args a,
-                                                          const Divisor h_kv) {
+__device__ inline void walk(const fa_linear_args& a, const Run run, int index, int hk,
+                            Lds<D, kStates ? 0 : kSplit>& shared) {
   typedef typename PVec<T>::v8 T8;
   typedef typename PVec<T>::v4 T4;
   constexpr bool kHalf = !__is_same(T, __bf16);
@@ -206,11 +215,9 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
   constexpr bool kEarly = kOne && D <= 128;  // values are split beside the scores' products
   constexpr bool kKeepQ = D == 64;  // from the scores to S^T Q^T, else it is read twice
   static_assert(kCopies * kTiles * 1024 == kTileB, "whole copies per wave");
-  // [k, v, q][stage]
-  __shared__ __attribute__((aligned(1024))) unsigned char bufs[(kStates ? 2 : 2 + kSplit) * kStages * kTileB];
-  // weights by the place m of a token before the chunk's last: at 1 + m scale e^{a (31 - m)}, 0 past 31
-  // (tokens to come); and e^{a (31 - m)}, 1 past 31
-  __shared__ float seen[1 + 2 * kChunk], left_of[2 * kChunk];
+  unsigned char* const bufs = shared.bufs;  // [k, v, q][stage]
+  float* const seen = shared.seen;
+  float* const left_of = shared.left_of;
 
   const int wave = uniform(wave_id() % kTiles);     // 32 columns of the state
   const int part_of = uniform(wave_id() / kTiles);  // of the heads at once
@@ -219,22 +226,6 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
   auto lane_id = [&]() -> int { return D == 256 ? fresh_lane() : threadIdx.x & 63; };
   const int group = kStates || kOne ? 1 : a.h_q / a.h_kv;
 
-  if constexpr (!kStates) {  // rows of no sequence: everybody takes a share of their 16 bytes
-    const int first = min(max(sload(a.cu_seqlens), 0), a.total);
-    const int behind = max(first, min(max(sload(a.cu_seqlens + a.num_seqs), 0), a.total));
-    const long long row16 = static_cast<long long>(a.h_q) * C;
-    const long long head = first * row16, all = a.total * row16, tail = behind * row16;
-    uintx4* const out16 = static_cast<uintx4*>(a.out);
-    const long long step = static_cast<long long>(gridDim.x) * kThreads;
-    const long long me = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x;
-    for (long long i = me; i < head; i += step) out16[i] = uintx4{0, 0, 0, 0};
-    for (long long i = tail + me; i < all; i += step) out16[i] = uintx4{0, 0, 0, 0};
-  }
-
-  const int index = divide(blockIdx.x, h_kv);
-  const int hk = blockIdx.x - index * a.h_kv;
-  const Run run = find_run(a, index);
-  if (run.seq < 0 || (kStates && run.last)) return;  // uniform
   const int n = run.n;
   const float log_decay = sload(a.log_decay + hk);
   float* slot_state = nullptr;  // the sequence's
@@ -243,25 +234,22 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
     if (slot >= 0 && slot < a.num_slots)
       slot_state = a.state + slot * a.state_stride_s + hk * a.state_stride_h;
   }
-  // Where the run starts from, and where it leaves its state.  A sequence of several runs has the state
-  // that run p starts from in part, at its index: the last run may write the sequence's own while
-  // the first has not read it yet.
-  float* const part = a.part + (static_cast<long long>(index) * a.h_kv + hk) * (D * D);
-  const bool kept = slot_state && (a.has_state == nullptr || a.has_state[run.seq] != 0);
-  const bool alone = run.part == 0 && run.last;
-  const float* from_state = nullptr;
-  if (kStates || alone)
-    from_state = run.part == 0 && kept ? slot_state : nullptr;
-  else if (run.part > 0 || kept)
-    from_state = part;
-  float* const to_state = kStates ? part + static_cast<long long>(a.h_kv) * (D * D)
-                                  : run.last ? slot_state : nullptr;
+  // Of a sequence of several runs, part has what each makes at the index of the next, and at the first's
+  // a copy of what that starts from: the last run may write the sequence's state while the first
+  // has not read it yet.
+  const long long part_step = static_cast<long long>(a.h_kv) * (D * D);
+  float* const part = a.part + index * part_step + hk * (D * D);
+  float* const to_state = kStates ? part + part_step : run.last ? slot_state : nullptr;
 
   // Items are (chunk, kSplit query heads of the group), heads innermost; k and v come with the first.
   // States alone go through the chunks from the last one back: what they read last is what the next
-  // launch reads first.
-  const int chunks = cdiv(n, kChunk);
+  // launch reads first.  They end where e^{a n} is 0 in fp32 (below 2^-149): what lies before adds zeros
+  // (a third of the work at |a| = 0.1 and segments of 4,096: 131,001 tokens of 16 heads xxx -> xxx us).
+  const float log2_decay = log_decay * kLog2e;
+  int chunks = cdiv(n, kChunk);
   const int begin = run.start + (kStates ? (chunks - 1) * kChunk : 0);
+  if (kStates && log2_decay < 0.f)
+    chunks = min(chunks, static_cast<int>(min(150.f / (-log2_decay * kChunk), 1e9f)) + 1);
   // The next chunk's rows, and q's of its next head.
   const unsigned char* k_next = static_cast<const unsigned char*>(a.k) +
                                 2 * (begin * a.k_stride_t + hk * a.k_stride_h);
@@ -284,9 +272,8 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
   };
   const unsigned int lds = uniform(static_cast<int>(
       reinterpret_cast<__SIZE_TYPE__>((FA_LDS unsigned char*)bufs)));
-  auto rows_of = [&](int chunk) {  // chunk: from the run's first item on
-    return kStates ? (chunk == 0 ? n - (chunks - 1) * kChunk : kChunk) : n - chunk * kChunk;
-  };
+  // (segments whose states are made alone are whole chunks)
+  auto rows_of = [&](int chunk) { return kStates ? kChunk : n - chunk * kChunk; };
   int next_chunk = 0, next_head = 0;
   int next_q = 0, next_kv = 0;     // bytes of its stages
   // Returns the copies that it issues.
@@ -342,13 +329,27 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
     return 8 * (lane >> 5) * D + 32 * wave + pi;
   };
   floatx16 s[kTiles] = {};
-  if (from_state) {
+  bool from_state = false;
+  auto add_state = [&](const float* from, float fall) {
     const int state_at = state_place();
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        s[t][r] = from_state[state_at + (32 * t + 16 * (r >> 3) + (r & 7)) * D];
+        s[t][r] = __builtin_fmaf(s[t][r], fall,
+                                 from[state_at + (32 * t + 16 * (r >> 3) + (r & 7)) * D]);
+    from_state = true;
+  };
+  if (run.part == 0) {
+    if (slot_state && (a.has_state == nullptr || a.has_state[run.seq] != 0))
+      add_state(kStates || run.last ? slot_state : part, 0.f);
+  } else if (kStates) {
+  } else if (a.joined) {
+    add_state(part, 0.f);
+  } else {  // what every run before it made
+    const float fall = decay(log_decay, a.segment);
+    for (int i = run.part - 1; i >= 0; --i)
+      add_state(part - i * part_step, i == run.part - 1 ? 0.f : fall);
   }
   if constexpr (kStates) {
     if (from_state) {
@@ -374,7 +375,6 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
   // The state is s times sigma = e^{a reset}, reset the tokens since s was last brought up: a product
   // of a whole state only where sigma has fallen by 16 (or grown, for a > 0), and no rounding of a
   // factor next to 1 at every chunk.
-  const float log2_decay = log_decay * kLog2e;
   int reset = 0;
   float sigma = 1.f, sigma_then = 1.f;
   // States alone have their weights counted to the run's end instead, and are never brought up.
@@ -749,7 +749,42 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
   }
 }
 
-// The states that segments start from, but for the first: each what its predecessor made on top of what
+template <typename T, int D, bool kOne, int kSplit>
+__global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_linear_args a,
+                                                                   const Divisor h_kv) {
+  __shared__ __attribute__((aligned(1024))) Lds<D, kSplit> shared;
+  {  // rows of no sequence: everybody takes a share of their 16 bytes
+    const int first = min(max(sload(a.cu_seqlens), 0), a.total);
+    const int behind = max(first, min(max(sload(a.cu_seqlens + a.num_seqs), 0), a.total));
+    const long long row16 = static_cast<long long>(a.h_q) * (D / 8);
+    const long long head = first * row16, all = a.total * row16, tail = behind * row16;
+    uintx4* const out16 = static_cast<uintx4*>(a.out);
+    const long long step = static_cast<long long>(gridDim.x) * (2 * D * kSplit);
+    const long long me = static_cast<long long>(blockIdx.x) * (2 * D * kSplit) + threadIdx.x;
+    for (long long i = me; i < head; i += step) out16[i] = uintx4{0, 0, 0, 0};
+    for (long long i = tail + me; i < all; i += step) out16[i] = uintx4{0, 0, 0, 0};
+  }
+  const int index = divide(blockIdx.x, h_kv);
+  const int hk = blockIdx.x - index * a.h_kv;
+  const Run run = find_run(a, index);
+  if (run.seq < 0) return;  // uniform
+  walk<T, D, false, kOne, kSplit>(a, run, index, hk, shared);
+}
+
+// What every run but a sequence's last makes.  Without tiles of q three work-groups fit a CU (the first
+// runs' outputs in the same launch leave two: 131,001 tokens of 16 heads 638 -> 710 us).
+template <typename T, int D>
+__global__ __launch_bounds__(2 * D, 2) void states_kernel(const fa_linear_args a,
+                                                          const Divisor h_kv) {
+  __shared__ __attribute__((aligned(1024))) Lds<D, 0> shared;
+  const int index = divide(blockIdx.x, h_kv);
+  const int hk = blockIdx.x - index * a.h_kv;
+  const Run run = find_run(a, index);
+  if (run.seq < 0 || run.last) return;  // uniform
+  walk<T, D, true, false, 1>(a, run, index, hk, shared);
+}
+
+// The states that runs start from, but for the first two: each what its predecessor made on top of what
 // that one started from, part[i] += e^{a L} part[i - 1].
 template <int D>
 __global__ __launch_bounds__(256) void join_kernel(const fa_linear_args a, const Divisor h_kv) {
@@ -765,6 +800,7 @@ __global__ __launch_bounds__(256) void join_kernel(const fa_linear_args a, const
                 (static_cast<long long>(start / a.segment + seq + 1) * a.h_kv + hk) * (D * D / 4) +
                 blockIdx.y * 256 + threadIdx.x;
   const float fall = decay(sload(a.log_decay + hk), a.segment);
+  if (fall == 0.f) return;
   floatx4 sum = *at;
   for (int i = 1; i < states; i += kAhead) {
     floatx4 next[kAhead];
@@ -789,34 +825,44 @@ int runs_of(const fa_linear_args& a) {
   return a.segment > 0 ? a.total / a.segment + seqs : seqs;
 }
 
+// Runs of a sequence from which on their states are joined in a launch of their own; below, each run
+// adds up what those before it left (a launch that few sequences need takes 6 to 11 us).
+constexpr int kJoinRuns = 5;
+
 // Tokens of a segment, 0 for whole sequences.
 int choose_segment(const fa_linear_args& a, int max_seqlen, int cus) {
   const int resident = cus * (a.d == 64 ? 4 : a.d == 128 ? 2 : 1);  // work-groups at once
   const int64_t each = static_cast<int64_t>(std::min(a.total, max_seqlen > 0 ? a.total : 0)) * a.h_kv / resident;
   const int64_t segment = (std::max<int64_t>(each, 256) + kChunk - 1) / kChunk * kChunk;
-  if (max_seqlen <= 2 * segment) return 0;
+  if (a.num_seqs == 0 || max_seqlen <= 2 * segment) return 0;
   return static_cast<int>(segment);
 }
 
-template <typename T, int D>
-void launch(const fa_linear_args& a, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(runs_of(a) * a.h_kv));
+template <typename T, int D, bool kOne, int kSplit>
+void launch_split(const fa_linear_args& a, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(runs_of(a) * a.h_kv)), block(2 * D * kSplit);
   const Divisor h_kv = divisor(a.h_kv);
   if (a.segment > 0) {
-    hipLaunchKernelGGL((linear_kernel<T, D, true, false, 1>), grid, dim3(2 * D), 0, stream, a, h_kv);
-    hipLaunchKernelGGL((join_kernel<D>), dim3(static_cast<unsigned>(a.num_seqs * a.h_kv), D * D / 1024),
-                       dim3(256), 0, stream, a, h_kv);
+    hipLaunchKernelGGL((states_kernel<T, D>), grid, dim3(2 * D), 0, stream, a, h_kv);
+    if (a.joined)
+      hipLaunchKernelGGL((join_kernel<D>),
+                         dim3(static_cast<unsigned>(a.num_seqs * a.h_kv), D * D / 1024), dim3(256), 0,
+                         stream, a, h_kv);
   }
-  constexpr int kWide = D == 64 ? 4 : D == 128 ? 2 : 1;
+  hipLaunchKernelGGL((linear_kernel<T, D, kOne, kSplit>), grid, block, 0, stream, a, h_kv);
+}
+
+// Heads at once: as many as the registers of two waves per SIMD keep the state for.
+template <typename T, int D>
+void launch(const fa_linear_args& a, hipStream_t stream) {
+  constexpr int kMany = D == 64 ? 4 : D == 128 ? 2 : 1;
   constexpr int kTwo = D == 256 ? 1 : 2;
   if (a.h_q == a.h_kv)
-    hipLaunchKernelGGL((linear_kernel<T, D, false, true, 1>), grid, dim3(2 * D), 0, stream, a, h_kv);
+    launch_split<T, D, true, 1>(a, stream);
   else if (a.h_q == 2 * a.h_kv)
-    hipLaunchKernelGGL((linear_kernel<T, D, false, false, kTwo>), grid, dim3(2 * D * kTwo), 0, stream,
-                       a, h_kv);
+    launch_split<T, D, false, kTwo>(a, stream);
   else
-    hipLaunchKernelGGL((linear_kernel<T, D, false, false, kWide>), grid, dim3(2 * D * kWide), 0,
-                       stream, a, h_kv);
+    launch_split<T, D, false, kMany>(a, stream);
 }
 
 }  // namespace
@@ -833,6 +879,7 @@ extern "C" int64_t fa_linear_plan(fa_linear_args* args, int32_t max_seqlen, int3
   if (rc != FA_OK) return rc;
   FA_CHECK_ARG(max_seqlen >= 0 && cu_count >= 1, "max_seqlen %d, %d CUs", max_seqlen, cu_count);
   a.segment = fa::choose_segment(a, max_seqlen, cu_count);
+  a.joined = a.segment > 0 && max_seqlen / a.segment >= fa::kJoinRuns;
   return a.segment > 0 ? static_cast<int64_t>(fa::runs_of(a)) * a.h_kv * a.d * a.d : 0;
 }
 
