@@ -258,6 +258,7 @@ class LinearArgs(ctypes.Structure):
         ("d", ctypes.c_int32),
         ("segment", ctypes.c_int32),
         ("joined", ctypes.c_int32),
+        ("sorted", ctypes.c_int32),
         ("scale", ctypes.c_float),
         ("dtype", ctypes.c_int32),
     ]

@@ -85,8 +85,9 @@ typedef struct fa_linear_args {
   float* part; /* workspace of fa_linear_plan's size, 16-byte aligned, where segment > 0 */
   int32_t num_slots, num_seqs, total, h_q, h_kv, d;
   /* fa_linear_prompt: tokens that a sequence is cut into, a multiple of 32, or 0; whether what the
-   * pieces start from is added up in a launch of its own */
-  int32_t segment, joined;
+   * pieces start from is added up in a launch of its own; whether the longest go first (up to 64
+   * sequences) */
+  int32_t segment, joined, sorted;
   float scale;
   int32_t dtype; /* 0 fp16, 1 bf16 */
 } fa_linear_args;
@@ -95,7 +96,7 @@ typedef struct fa_linear_args {
 int64_t fa_linear_args_size(void);
 
 /*
- * Fills in segment and joined, from the totals, heads and head dim of args, for sequences of up to max_seqlen
+ * Fills in segment, joined and sorted, from the totals, heads and head dim of args, for sequences of up to max_seqlen
  * tokens on a device of cu_count compute units.  Returns the floats that part has to hold (0: none),
  * or a negative code.
  */
