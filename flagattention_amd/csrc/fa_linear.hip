@@ -21,6 +21,7 @@
 // it 2e-6 from 64 bits, three 2e-7).  fp16 operands are taken relative to a
 // power of two of the largest, since states, scores and products of tiny inputs leave its range.
 #include <algorithm>
+#include <cmath>
 
 #include "fa_common.h"
 #include "fa_divide.h"
@@ -875,13 +876,65 @@ int runs_of(const fa_linear_args& a) {
 // adds up what those before it left (a launch that few sequences need takes 6 to 11 us).
 constexpr int kJoinRuns = 5;
 
-// Tokens of a segment, 0 for whole sequences.
+// Heads that a work-group attends at once: as many as the registers of two waves per SIMD keep the state
+// for (8 sequences of 1,024 tokens, 64 heads of 8, D = 128: 136 us with one, 97 with two; three of up to
+// 48, 8 heads of 2, D = 64: 10.8 with one, 8.1 with four).
+int heads_at_once(int group, int d) {
+  return group == 1 || d == 256 ? 1 : d == 128 || group == 2 ? 2 : 4;
+}
+
+// What a launch takes, in us, by segments of L tokens (0: whole sequences), from times of 36 shapes per
+// head dim (one sequence of 1,000 to 60 of up to 8,000, groups of 1 and 4 to 8; off by a tenth on average).  The
+// longest run's chunks or a slot's share of all, whichever is more; starts and ends of the work-groups;
+// the segments' states; no less than the bytes.
+struct Cost {
+  float chunk_one;          // a chunk, groups of one head
+  float item, chunk_group;  // heads at once, a chunk beside them
+  float chunk_state;        // a chunk of the states alone
+  float state;              // a segment's state, written, read and joined
+  float start;              // a work-group's start and end
+  int slots;                // work-groups per CU
+};
+double cost_of(const fa_linear_args& a, int segment, int max_seqlen, int cus) {
+  static const Cost kCost[3] = {{1.4f, 1.f, .9f, .42f, .01f, 5.2f, 4},
+                                {1.95f, 1.36f, .93f, .54f, .031f, 9.4f, 2},
+                                {4.4f, 1.95f, .7f, 2.8f, .11f, 23.f, 1}};
+  constexpr double kBytesPerUs = 5.1e6;
+  const Cost& c = kCost[a.d == 64 ? 0 : a.d == 128 ? 1 : 2];
+  const int group = a.h_q / a.h_kv, split = heads_at_once(group, a.d);
+  const double slots = cus * std::max(1, c.slots / split);
+  const double chunk = group == 1 ? c.chunk_one : cdiv(group, split) * c.item + c.chunk_group;
+  const double share = static_cast<double>(a.total) * a.h_kv / kChunk / slots;
+  double runs = a.num_seqs, longest = cdiv(max_seqlen, kChunk), each = chunk, states = 0.;
+  if (segment > 0) {
+    runs = static_cast<double>(a.total) / segment + .6 * a.num_seqs;
+    longest = segment / kChunk;
+    each += c.chunk_state;
+    states = runs * a.h_kv * c.state;
+  }
+  const double starts = c.start * std::ceil(runs * a.h_kv / slots) * (segment > 0 ? 1. : .5);
+  const double bytes = 4. * a.total * a.d * (a.h_q + a.h_kv * (segment > 0 ? 2. : 1.));
+  return (segment > 0 ? 8. : 3.) +
+         std::max(std::max(longest, share) * each + starts, bytes / kBytesPerUs) + states;
+}
+
+// Tokens of a segment, 0 for whole sequences: the cheapest of powers of two and of what gives every slot
+// one segment.
 int choose_segment(const fa_linear_args& a, int max_seqlen, int cus) {
-  const int resident = cus * (a.d == 64 ? 4 : a.d == 128 ? 2 : 1);  // work-groups at once
-  const int64_t each = static_cast<int64_t>(std::min(a.total, max_seqlen > 0 ? a.total : 0)) * a.h_kv / resident;
-  const int64_t segment = (std::max<int64_t>(each, 256) + kChunk - 1) / kChunk * kChunk;
-  if (a.num_seqs == 0 || max_seqlen <= 2 * segment) return 0;
-  return static_cast<int>(segment);
+  if (a.num_seqs == 0 || max_seqlen <= 2 * kChunk) return 0;
+  int best = 0;
+  double least = cost_of(a, 0, max_seqlen, cus);
+  auto consider = [&](int64_t segment) {
+    if (segment >= max_seqlen) return;
+    const double c = cost_of(a, static_cast<int>(segment), max_seqlen, cus);
+    if (c < least) least = c, best = static_cast<int>(segment);
+  };
+  for (int64_t segment = 2 * kChunk; segment <= 1 << 16; segment *= 2) consider(segment);
+  const int64_t slots = static_cast<int64_t>(cus) * (a.d == 64 ? 4 : a.d == 128 ? 2 : 1) /
+                        heads_at_once(a.h_q / a.h_kv, a.d);
+  const int64_t fit = static_cast<int64_t>(a.total) * a.h_kv / std::max<int64_t>(slots, 1);
+  consider(std::max<int64_t>((fit + kChunk - 1) / kChunk, 2) * kChunk);
+  return best;
 }
 
 template <typename T, int D, bool kOne, int kSplit>
@@ -898,17 +951,16 @@ void launch_split(const fa_linear_args& a, hipStream_t stream) {
   hipLaunchKernelGGL((linear_kernel<T, D, kOne, kSplit>), grid, block, 0, stream, a, h_kv);
 }
 
-// Heads at once: as many as the registers of two waves per SIMD keep the state for.
 template <typename T, int D>
 void launch(const fa_linear_args& a, hipStream_t stream) {
-  constexpr int kMany = D == 64 ? 4 : D == 128 ? 2 : 1;
-  constexpr int kTwo = D == 256 ? 1 : 2;
-  if (a.h_q == a.h_kv)
+  constexpr int kTwo = D == 256 ? 1 : 2, kMany = D == 64 ? 4 : kTwo;
+  const int group = a.h_q / a.h_kv;
+  if (group == 1)
     launch_split<T, D, true, 1>(a, stream);
-  else if (a.h_q == 2 * a.h_kv)
-    launch_split<T, D, false, kTwo>(a, stream);
-  else
+  else if (heads_at_once(group, D) == kMany)
     launch_split<T, D, false, kMany>(a, stream);
+  else
+    launch_split<T, D, false, kTwo>(a, stream);
 }
 
 }  // namespace
