@@ -699,7 +699,7 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
     }
 
     T8 kt[2][2];  // K^T of a tile of the state, the next one on its way
-    if (kStates || head + kSplit >= group) {
+    if (kStates || kOne) {
       kt[0][0] = transposed(k_tr, 0, 0);
       kt[0][1] = transposed(k_tr, 0, 1);
     }
@@ -727,6 +727,10 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
       if (chunk + 1 == chunks && to_state == nullptr) break;
     }
 
+    if (!(kStates || kOne)) {
+      kt[0][0] = transposed(k_tr, 0, 0);
+      kt[0][1] = transposed(k_tr, 0, 1);
+    }
     if (!kEarly) split();
     if (odd) {  // what is not finite has no rest
       asm volatile("" ::: "memory");
@@ -872,9 +876,10 @@ int runs_of(const fa_linear_args& a) {
   return a.segment > 0 ? a.total / a.segment + seqs : seqs;
 }
 
-// Runs of a sequence from which on their states are joined in a launch of their own; below, each run
-// adds up what those before it left (a launch that few sequences need takes 6 to 11 us).
-constexpr int kJoinRuns = 5;
+// Runs of a sequence from which on their states are joined in a launch of their own, which takes 6 to 24
+// us; below, each run adds up what those before it made, 3 us a state at head dim 128, 13 at 256
+// (8 prompts of up to 2,048 tokens, 16 KV heads, in segments of 416: 310 us so, 217 joined).
+int join_runs(int d) { return d == 256 ? 3 : 5; }
 
 // Heads that a work-group attends at once: as many as the registers of two waves per SIMD keep the state
 // for (8 sequences of 1,024 tokens, 64 heads of 8, D = 128: 136 us with one, 97 with two; three of up to
@@ -977,7 +982,7 @@ extern "C" int64_t fa_linear_plan(fa_linear_args* args, int32_t max_seqlen, int3
   if (rc != FA_OK) return rc;
   FA_CHECK_ARG(max_seqlen >= 0 && cu_count >= 1, "max_seqlen %d, %d CUs", max_seqlen, cu_count);
   a.segment = fa::choose_segment(a, max_seqlen, cu_count);
-  a.joined = a.segment > 0 && max_seqlen / a.segment >= fa::kJoinRuns;
+  a.joined = a.segment > 0 && fa::cdiv(max_seqlen, a.segment) >= fa::join_runs(a.d);
   a.sorted = a.num_seqs >= 2 && a.num_seqs <= 64 && max_seqlen > 4 * fa::kChunk;
   return a.segment > 0 ? static_cast<int64_t>(fa::runs_of(a)) * a.h_kv * a.d * a.d : 0;
 }
