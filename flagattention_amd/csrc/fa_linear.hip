@@ -144,7 +144,17 @@ struct Run {
   int place;     // of its state in the workspace
   int start, n;  // first packed token, tokens
   bool last;     // of its sequence
+  int slot;      // of the sequence's state, as given
+  bool has;      // whether it starts from it
 };
+
+// The slot and the has_state of sequence s, where there are states.
+__device__ inline int slot_of(const fa_linear_args& a, int s) {
+  return !a.state ? -1 : a.state_indices ? a.state_indices[s] : s;
+}
+__device__ inline bool has_of(const fa_linear_args& a, int s) {
+  return a.has_state == nullptr || a.has_state[s] != 0;
+}
 
 // Run `index` of the launch.  With segments of L tokens those of sequence s have the places start_s / L + s
 // and on: a sequence of n tokens has ceil(n / L) of them, and the next one's start is at least that
@@ -156,14 +166,17 @@ struct Run {
 // ones).  Otherwise in packed order, by their places; the sequence is the last one whose first place
 // is not past `index`, and a wave looks at 64 at a time.
 __device__ inline Run find_run(const fa_linear_args& a, int index) {
-  Run run = {-1, 0, 0, 0, 0, true};
+  Run run = {-1, 0, 0, 0, 0, true, -1, false};
   const int lane = threadIdx.x & 63;
   int seq, start, n;
   if (a.sorted) {
-    int start_of = 0, n_of = 0;
+    int start_of = 0, n_of = 0, slot = -1;
+    bool has = false;
     if (lane < a.num_seqs) {
       start_of = min(max(a.cu_seqlens[lane], 0), a.total);
       n_of = min(max(a.cu_seqlens[lane + 1], start_of), a.total) - start_of;
+      slot = slot_of(a, lane);
+      has = has_of(a, lane);
     }
     const int whole = a.segment > 0 ? n_of / a.segment : 0;
     const int rest = n_of - whole * a.segment;
@@ -192,6 +205,8 @@ __device__ inline Run find_run(const fa_linear_args& a, int index) {
     seq = uniform(__ffsll(found) - 1);
     start = __builtin_amdgcn_readlane(start_of, seq);
     n = __builtin_amdgcn_readlane(n_of, seq);
+    run.slot = __builtin_amdgcn_readlane(slot, seq);
+    run.has = __builtin_amdgcn_readlane(static_cast<int>(has), seq) != 0;
     const int mine = __builtin_amdgcn_readlane(whole, seq);
     run.part = index < wholes ? index - (__builtin_amdgcn_readlane(upto, seq) - mine) : mine;
     run.place = a.segment > 0 ? start / a.segment + seq + run.part : seq;
@@ -213,8 +228,13 @@ __device__ inline Run find_run(const fa_linear_args& a, int index) {
       seq = uniform(lo);
     }
     if (seq >= a.num_seqs) return run;
-    start = min(max(sload(a.cu_seqlens + seq), 0), a.total);
-    n = min(max(sload(a.cu_seqlens + seq + 1), start), a.total) - start;
+    const int begins = a.cu_seqlens[seq], ends = a.cu_seqlens[seq + 1];  // one trip to memory for all
+    const int slot = slot_of(a, seq);
+    const bool has = has_of(a, seq);
+    start = uniform(min(max(begins, 0), a.total));
+    n = uniform(min(max(ends, start), a.total) - start);
+    run.slot = uniform(slot);
+    run.has = uniform(static_cast<int>(has)) != 0;
     if (n == 0) return run;
     run.place = index;
     if (a.segment > 0) {
@@ -275,12 +295,11 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
 
   const int n = run.n;
   const float log_decay = sload(a.log_decay + hk);
-  float* slot_state = nullptr;  // the sequence's
-  if (a.state) {
-    const int slot = a.state_indices ? sload(a.state_indices + run.seq) : run.seq;
-    if (slot >= 0 && slot < a.num_slots)
-      slot_state = a.state + slot * a.state_stride_s + hk * a.state_stride_h;
-  }
+  float* const slot_state =  // the sequence's
+      run.slot >= 0 && run.slot < a.num_slots
+          ? a.state + run.slot * a.state_stride_s + hk * a.state_stride_h
+          : nullptr;
+
   // Of a sequence of several runs, part has what each makes at the place of the next, and at the first's
   // a copy of what that starts from: the last run may write the sequence's state while the first
   // has not read it yet.
@@ -388,7 +407,7 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
     from_state = true;
   };
   if (run.part == 0) {
-    if (slot_state && (a.has_state == nullptr || a.has_state[run.seq] != 0))
+    if (slot_state && run.has)
       add_state(kStates || run.last ? slot_state : part, 0.f);
   } else if (kStates) {
   } else if (a.joined) {
@@ -804,9 +823,13 @@ template <typename T, int D, bool kOne, int kSplit>
 __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_linear_args a,
                                                                    const Divisor h_kv) {
   __shared__ __attribute__((aligned(1024))) Lds<D, kSplit> shared;
+  const int begins = sload(a.cu_seqlens), ends = sload(a.cu_seqlens + a.num_seqs);
+  const int index = divide(blockIdx.x, h_kv);
+  const int hk = blockIdx.x - index * a.h_kv;
+  const Run run = find_run(a, index);
   {  // rows of no sequence: everybody takes a share of their 16 bytes
-    const int first = min(max(sload(a.cu_seqlens), 0), a.total);
-    const int behind = max(first, min(max(sload(a.cu_seqlens + a.num_seqs), 0), a.total));
+    const int first = min(max(begins, 0), a.total);
+    const int behind = max(first, min(max(ends, 0), a.total));
     const long long row16 = static_cast<long long>(a.h_q) * (D / 8);
     const long long head = first * row16, all = a.total * row16, tail = behind * row16;
     uintx4* const out16 = static_cast<uintx4*>(a.out);
@@ -815,9 +838,6 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
     for (long long i = me; i < head; i += step) out16[i] = uintx4{0, 0, 0, 0};
     for (long long i = tail + me; i < all; i += step) out16[i] = uintx4{0, 0, 0, 0};
   }
-  const int index = divide(blockIdx.x, h_kv);
-  const int hk = blockIdx.x - index * a.h_kv;
-  const Run run = find_run(a, index);
   if (run.seq < 0) return;  // uniform
   walk<T, D, false, kOne, kSplit>(a, run, hk, shared);
 }
