@@ -19,7 +19,8 @@
 // meet V and Q, as the output is.  The weighted values that a state takes in are split in three bf16 or
 // two fp16 numbers, which hold 24 and 22 bits: the state is an output in fp32 (two bf16 numbers left
 // it 2e-6 from 64 bits, three 2e-7).  fp16 operands are taken relative to a
-// power of two of the largest, since states, scores and products of tiny inputs leave its range.
+// power of two of the largest (a column's of the state, of the weighted values, of P^T), since states,
+// scores and products of tiny inputs leave its range.
 #include <algorithm>
 #include <cmath>
 
@@ -256,8 +257,13 @@ __device__ inline Run find_run(const fa_linear_args& a, int index) {
 template <int D, int kHeads>
 struct Lds {
   unsigned char bufs[(2 + kHeads) * kStages * kChunk * 2 * D];
+  float scales[kHeads > 0 ? kHeads : 1][D];  // of the state's columns, by wave: fp16
   float seen[1 + 2 * kChunk], left_of[2 * kChunk];
 };
+
+// bf16: s is kept times 2^-kLift.  Values are taken up to 16 times into it (by what s has yet to fall), and
+// the largest finite ones stay within fp32 so.
+constexpr int kLift = 5;
 
 // A run of one KV head, from its state through its chunks.  kStates: only the state that it makes, from
 // zeros, or the first run's from its sequence's.  kOne: groups of one query head.  kSplit: heads that are attended at once, by D / 32 waves
@@ -396,14 +402,15 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
   };
   floatx16 s[kTiles] = {};
   bool from_state = false;
+  constexpr float kInit = kHalf || kStates ? 1.f : 1.f / (1 << kLift);
   auto add_state = [&](const float* from, float fall) {
     const int state_at = state_place();
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        s[t][r] = __builtin_fmaf(s[t][r], fall,
-                                 from[state_at + (32 * t + 16 * (r >> 3) + (r & 7)) * D]);
+        s[t][r] = __builtin_fmaf(
+            s[t][r], fall, kInit * from[state_at + (32 * t + 16 * (r >> 3) + (r & 7)) * D]);
     from_state = true;
   };
   if (run.part == 0) {
@@ -436,7 +443,7 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
     const float e = decay(log_decay, max(kChunk - 1 - m, 0));
     seen[1 + m] = m < kChunk ? a.scale * e : 0.f;
     if (m == 0) seen[0] = a.scale * decay(log_decay, kChunk);
-    left_of[m] = e;
+    left_of[m] = kInit * e;
   }
   // The state is s times sigma = e^{a reset}, reset the tokens since s was last brought up: a product
   // of a whole state only where sigma has fallen by 16 (or grown, for a > 0), and no rounding of a
@@ -446,10 +453,12 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
   // States alone have their weights counted to the run's end instead, and are never brought up.
   int after = 0;
 
-  // fp16: s is kept times 2^-s_power, its largest at about 8 when it was last looked at: there is room
-  // for a growth by 2^12 (past it an output is not finite, and the chunk is taken again) and a fall
-  // by 2^17 (counted below) before its copies lose bits.
-  int s_power = 0, looked = -1;  // tokens since, -1: not yet
+  // s is kept times 2^-s_power.  fp16: a power for each column (a lane's), whose largest is at about 8
+  // when it was last looked at: there is room for a growth by 2^12 (past it an output is not finite,
+  // and the chunk is taken again) and a fall by 2^17 (counted below) before its copies lose bits.
+  int s_power = kHalf || kStates ? 0 : kLift;
+  int looked = -1;  // tokens since, -1: there was nothing yet
+  float* const scales = shared.scales[kStates ? 0 : part_of] + 32 * wave;
   auto look = [&]() {
     float most = 0.f;
 #pragma unroll
@@ -464,10 +473,10 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
         for (int r = 0; r < 16; ++r)
           most = fabsf(s[t][r]) < __builtin_inff() ? fmaxf(most, fabsf(s[t][r])) : most;
     }
+    most = max_xor32(most);
     // |s| 2^s_power is at most 2^128: both factors stay in range
-    most = wave_max(most);
-    const int by = uniform(most > 0.f ? max(power_of(most) - 3, -100 - s_power) : 0);
-    if (by < -2 || by > 2) {  // uniform
+    const int by = most > 0.f ? max(power_of(most) - 3, -100 - s_power) : 0;
+    if (__ballot(by < -2 || by > 2) != 0ull) {  // uniform
       const float x = two_to(-by);
 #pragma unroll
       for (int t = 0; t < kTiles; ++t)
@@ -475,9 +484,14 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
         for (int r = 0; r < 16; ++r) s[t][r] *= x;
       s_power += by;
     }
-    looked = 0;
+    looked = __ballot(most == 0.f) != 0ull ? -1 : 0;
+    scales[lane_id() & 31] = two_to(min(s_power, 127));
   };
-  if (kHalf && !kStates && from_state) look();
+  if (kHalf && !kStates) {
+    scales[lane_id() & 31] = 1.f;
+    if (from_state) look();
+  }
+
   // Token of register r in P^T's rows, and of element r of the values' operands, less 4h.
   auto token = [&](int r) { return 8 * (r >> 2) + (r & 3); };
   // dims 32t .. 32t + 31 of tokens token(8 ss) .. token(8 ss + 7), transposed
@@ -661,10 +675,13 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
           p_power = min(max(power_of(max_xor32(top)), kLeastPower), 100);
         }
         // O^T, relative to 2^p_power
-        const float by = kHalf ? __builtin_amdgcn_ldexpf(since, s_power - p_power) : since;
+        const float by = kHalf ? __builtin_amdgcn_ldexpf(since, -p_power) : since * (1 << kLift);
         const float p_by = two_to(-p_power), p_back = two_to(p_power);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[r] *= by;
+        for (int r = 0; r < 16; ++r) {  // token(r) + 4h is the column too
+          if (kHalf) o[r] *= scales[token(r) + 4 * h];
+          o[r] *= by;
+        }
 #pragma unroll
         for (int ss = 0; ss < 2; ++ss) {
           T8 pb, v8 = va[ss];
@@ -810,7 +827,7 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
   }
   if (to_state != nullptr) {
     const int state_at = state_place();
-    const float back = kHalf ? __builtin_amdgcn_ldexpf(sigma, s_power) : sigma;
+    const float back = __builtin_amdgcn_ldexpf(sigma, s_power);
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll

@@ -9,9 +9,9 @@ u is half a step of the output type (bf16 2^-8, fp16 2^-11).  Against the formul
   3 * 2^-24.  All in units of |x1| + |x2|: below 2^-18;
 * linear attention, output: rounded once, u |o|, or by half of the smallest step.  Scores and the
   state's copy are rounded to the type to meet v and q: u of every term, u M with M the sum of
-  magnitudes.  fp16 ones are taken relative to the largest of their column of 32 tokens or
-  tile of the state: off by 2^-24 of that instead where they are small, 2^-24 (32 max|p| max|v| +
-  sum|q| max|S| scale) in all.  Scores are sums of D products, sums run over up to 64 terms a chunk
+  magnitudes.  fp16 ones are taken relative to the largest of a token's 32 scores or of a
+  column of the state: off by 2^-24 of that instead where they are small, 2^-24 (32 max|p| max|v| +
+  sum|q| max|S| scale) in all, the maxima of v and S those of the output's column.  Scores are sums of D products, sums run over up to 64 terms a chunk
   and one per chunk, weights are off by (88 + 4) 2^-24 (an exponent above -88 and the function), two
   weights meet in a term;
 * linear attention, state: the weighted values are split in two numbers of the type, whose rest is
@@ -60,13 +60,13 @@ def small_out(q, k, v, state, scale):
         return 0.0
     q, k, v = q.double().abs(), k.double().abs(), v.double().abs()
     row = q.sum(-1, keepdim=True)
-    most_s = float((k.amax(0)[:, None] * v.amax(0)[None, :]).max()) * k.shape[0]
+    most_s = k.amax() * v.amax(0) * k.shape[0]  # of each column
     if state is not None:
-        most_s += float(state.abs().max())
-    return 2.0 ** -24 * abs(scale) * row * (32 * float(k.max()) * float(v.max()) + most_s)
+        most_s = most_s + state.double().abs().amax(0)
+    return 2.0 ** -24 * abs(scale) * row * (32 * k.max() * v.amax(0) + most_s)
 
 
 def small_state(k, v, dtype):
     if dtype != torch.float16:
         return 0.0
-    return 2.0 ** -24 * k.double().abs().sum(0)[:, None] * float(v.abs().max())
+    return 2.0 ** -24 * k.double().abs().sum(0)[:, None] * v.double().abs().amax(0)[None]

@@ -154,6 +154,43 @@ def test_fp16_outside_its_range(gain):
     check(q, k, v, a, cu, state, ids, scale=0.05 * gain ** -3 if gain < 1 else 1e-5)
 
 
+@pytest.mark.parametrize("h,hk,d", [(1, 1, 64), (3, 1, 128), (1, 1, 256)])
+def test_fp16_columns_of_different_sizes(h, hk, d):
+    """Dims of v from 2^-12 to 2^12, each within its own tolerance; and a state that is nothing for two
+    chunks, then tiny, then large."""
+    need_gpu()
+    say(f"linear fp16 columns h={h} d={d}")
+    q, k, v, a, cu, state, ids = make([150, 70], h, hk, d, torch.float16, seed=9)
+    sizes = 2.0 ** torch.linspace(-12, 12, d, device=DEV)
+    v = (v.float() * sizes[torch.randperm(d, device=DEV)]).half()
+    check(q, k, v, a, cu, scale=2.0 ** -10)
+    v2 = v.clone()
+    v2[:70] = 0
+    v2[70:110] *= 2.0 ** -8
+    check(q, k, v2, torch.full_like(a, -0.001), [0, 220], scale=2.0 ** -10)
+
+
+@pytest.mark.parametrize("d", DIMS)
+def test_largest_finite_values(d):
+    """One token of bf16's largest finite values behind slow decays: nothing on the way is larger."""
+    need_gpu()
+    say(f"linear largest values d={d}")
+    top = float(torch.finfo(torch.bfloat16).max)
+    q, k, v = (torch.zeros((200, 1, d), dtype=torch.bfloat16, device=DEV) for _ in range(3))
+    q[:, 0, 5] = 1.0
+    k[40, 0, 5], v[40] = 1.0, top
+    v[40, 0, ::2] = -top
+    for a in (-0.01, -0.08, 0.0):
+        decay = torch.full((1,), a, device=DEV)
+        state = torch.zeros((1, 1, d, d), device=DEV)
+        o = flag_attn.linear_attention_varlen(q, k, v, decay, i32([0, 200]), 200, state, sm_scale=1.0)
+        torch.cuda.synchronize()
+        ref, size, end, end_size = lo.attend(q, k[:, 0], v[:, 0], float(decay[0]), 1.0)
+        assert bool(torch.isfinite(o).all()) and bool(torch.isfinite(state).all())
+        assert_out(o, ref, size, 200)
+        assert_state(state[0, 0], end, end_size, 200, q.dtype)
+
+
 @pytest.mark.parametrize("d,dtype", [(64, torch.bfloat16), (128, torch.float16), (256, torch.bfloat16)])
 def test_strides(d, dtype):
     """Rows that are views: interleaved q, k and v, heads outermost, off the alignment, one row seen by
