@@ -960,6 +960,8 @@ double cost_of(const fa_linear_args& a, int segment, int max_seqlen, int cus) {
          std::max(std::max(longest, share) * each + starts, bytes / kBytesPerUs) + states;
 }
 
+constexpr int64_t kMaxWorkspace = int64_t{1} << 32;  // bytes
+
 // Tokens of a segment, 0 for whole sequences: the cheapest of powers of two and of what gives every slot
 // one segment.
 int choose_segment(const fa_linear_args& a, int max_seqlen, int cus) {
@@ -967,7 +969,8 @@ int choose_segment(const fa_linear_args& a, int max_seqlen, int cus) {
   int best = 0;
   double least = cost_of(a, 0, max_seqlen, cus);
   auto consider = [&](int64_t segment) {
-    if (segment >= max_seqlen) return;
+    const int64_t states = (a.total / segment + a.num_seqs) * static_cast<int64_t>(a.h_kv);
+    if (segment >= max_seqlen || states * a.d * a.d > kMaxWorkspace / 4) return;
     const double c = cost_of(a, static_cast<int>(segment), max_seqlen, cus);
     if (c < least) least = c, best = static_cast<int>(segment);
   };

@@ -1013,7 +1013,8 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!q || !k || !to_bool(args[7], &inplace) ||
       !rotary_of(*q, *k, args[2], args[3], args[4], args[5], args[6], &a))
     return none();
-  if (inplace && (!rows_apart(*q, 2) || !rows_apart(*k, 2))) return none();
+  if (inplace && (!rows_apart(*q, 2) || !rows_apart(*k, 2) || q->data_ptr() == k->data_ptr()))
+    return none();
   const c10::Device device = q->device();
   at::Tensor q_out, k_out;
   {
@@ -1053,7 +1054,7 @@ PyObject* rotary_cache(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       kc->size(3) != a.d || kc->scalar_type() != q->scalar_type() ||
       vc->scalar_type() != q->scalar_type() || kc->size(0) < 1 || kc->size(0) > INT32_MAX ||
       kc->size(2) < 1 || kc->size(2) > INT32_MAX || kc->stride(3) != 1 || vc->stride(3) != 1 ||
-      !rows_apart(*kc, 3) || !rows_apart(*vc, 3))
+      !rows_apart(*kc, 3) || !rows_apart(*vc, 3) || kc->data_ptr() == vc->data_ptr())
     return none();
   if ((slots->scalar_type() != at::kInt && slots->scalar_type() != at::kLong) || slots->dim() != 1 ||
       slots->size(0) != a.tokens || !slots->is_contiguous())

@@ -117,7 +117,8 @@ def rotary_embedding(
                ``i % axes`` as long as that axis has its number, and axis 0 from there on
     adjacent_pairs
                pairs are dims 2i and 2i + 1 instead of i and i + R/2
-    inplace    write into q and k themselves (their rows must not overlap)
+    inplace    write into q and k themselves (their rows must not overlap, nor the two each other: views of
+               one packed projection are fine)
 
     Returns ``(q, k)``, turned.
     """
@@ -132,6 +133,7 @@ def rotary_embedding(
     if inplace:
         _require(all(x.stride(2) == 1 and _apart(x, (0, 1)) for x in (q, k)),
                  "q and k must have contiguous rows that do not overlap")
+        _require(q.data_ptr() != k.data_ptr() or q.numel() == 0, "q and k overlap")
     _one_device(q, k, positions, inv_freq)
     if inplace:
         q_out, k_out = q, k
@@ -196,6 +198,7 @@ def rotary_cache_kv(
              "the cache is empty or has too many blocks")
     _require(all(c.stride(3) == 1 and _apart(c, (0, 1, 2)) for c in (key_cache, value_cache)),
              "rows of the cache must be contiguous and not overlap")
+    _require(key_cache.data_ptr() != value_cache.data_ptr(), "key_cache and value_cache overlap")
     _require(slot_mapping.dim() == 1 and slot_mapping.shape[0] == tokens
              and slot_mapping.dtype in (torch.int32, torch.int64),
              "slot_mapping must be int32 / int64 [num_tokens]")

@@ -72,6 +72,15 @@ def test_in_place_needs_rows_of_their_own(kw):
         flag_attn.rotary_embedding(**_rotary(**kw), inplace=True)
 
 
+def test_two_results_need_memory_of_their_own():
+    x = half(5, 2, 64)
+    with pytest.raises(ArgumentError, match="q and k overlap"):
+        flag_attn.rotary_embedding(**_rotary(q=x, k=x), inplace=True)
+    c = half(3, 2, 16, 64)
+    with pytest.raises(ArgumentError, match="key_cache and value_cache overlap"):
+        flag_attn.rotary_cache_kv(**_store(key_cache=c, value_cache=c))
+
+
 def _store(**kw):
     return {**_rotary(), **dict(v=half(5, 2, 64), key_cache=half(3, 2, 16, 64),
                                 value_cache=half(3, 2, 16, 64), slot_mapping=i32(5)), **kw}
@@ -231,6 +240,7 @@ def test_plans(d, h, hk):
         floats = lib.fa_linear_plan(ctypes.byref(args), most, 256)
         assert args.segment % 32 == 0 and 0 <= args.segment < max(most, 1)
         assert floats == (0 if not args.segment else (total // args.segment + seqs) * hk * d * d)
+        assert floats <= 1 << 30
         assert args.sorted == int(2 <= seqs <= 64 and most > 128)
         if most <= 64 or seqs == 0:
             assert args.segment == 0
