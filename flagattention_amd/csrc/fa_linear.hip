@@ -8,10 +8,13 @@
 // No factor is above 1 for a decay (a <= 0), however long the chunk or fast the decay.
 //
 // Wave w owns columns 32w .. 32w + 31 of S, in fp32 in its accumulators for the whole sequence, and the
-// same dims of the output; D / 32 waves.  All products are MFMA 32x32x16.  Nothing but the inputs goes
-// through LDS: S and P^T leave the accumulators as the operands of the next products (the rows of a
-// state tile are dealt to dims so that a lane's 8 registers are the 8 dims of its part of a step), and
-// every wave works the scores of a chunk out for itself, a fifth of its products.
+// same dims of the output; D / 32 waves.  Products are MFMA 32x32x16.  S leaves the accumulators as the
+// operands of the next products (the rows of a state tile are dealt to dims so that a lane's 8 registers
+// are the 8 dims of its part of a step).  Every wave needs the whole of P^T.  At head dim 256, and at 128
+// without groups, four waves work out 16 x 16 of it each and hand it round in LDS; each wave for itself
+// would make it a fifth of its products and read K and Q whole again (16 x 1,024 tokens of 16 heads,
+// D = 256: 200 us so, 179 shared; 32 heads, D = 128, fp16: 143 / 137; a lone sequence of one head waits
+// for the exchange, 410 / 441 at 8,192 tokens; two heads at once at D = 128: 227 / 233, so not there).
 //
 // Bound by q, k, v and out.  Inputs come three chunks deep into LDS.
 //
@@ -79,6 +82,13 @@ template <int C>
 __device__ inline int swizzle(int r) {
   return C >= 16 ? ((r & 3) << 2) | ((r >> 1) & 2) | ((r >> 3) & 1)
                  : ((r & 2) << 1) | ((r >> 1) & 2) | ((r >> 3) & 1);
+}
+
+__device__ inline floatx4 mfma_16x16x32(PVec<__bf16>::v8 a, PVec<__bf16>::v8 b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ inline floatx4 mfma_16x16x32(PVec<_Float16>::v8 a, PVec<_Float16>::v8 b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
 // A barrier that no access to memory passes.
@@ -251,12 +261,17 @@ __device__ inline Run find_run(const fa_linear_args& a, int index) {
   return run;
 }
 
-// LDS of a work-group: tiles of k, v and of q's kHeads heads, kStages of each, and weights by the place m
-// of a token before the chunk's last: at 1 + m scale e^{a (31 - m)}, 0 past 31 (tokens to come); and
-// e^{a (31 - m)}, 1 past 31.
-template <int D, int kHeads>
+// Whether the waves share a chunk's scores, or each works all of them out for itself.
+constexpr bool shares(int d, bool one) { return d == 256 || (d == 128 && one); }
+constexpr int kScoreRow = 36;  // floats of a row of shared scores: 16 rows lie in different banks
+
+// LDS of a work-group: tiles of k, v and of q's kHeads heads, kStages of each, P of each head, and weights
+// by the place m of a token before the chunk's last: at 1 + m scale e^{a (31 - m)}, 0 past 31 (tokens to
+// come); and e^{a (31 - m)}, 1 past 31.
+template <int D, int kHeads, bool kShare>
 struct Lds {
   unsigned char bufs[(2 + kHeads) * kStages * kChunk * 2 * D];
+  float scores[kShare ? kHeads * kChunk * kScoreRow : 4];  // P by [head][query][key]
   float scales[kHeads > 0 ? kHeads : 1][D];  // of the state's columns, by wave: fp16
   float seen[1 + 2 * kChunk], left_of[2 * kChunk];
 };
@@ -270,7 +285,7 @@ constexpr int kLift = 5;
 // each, which all keep the state.
 template <typename T, int D, bool kStates, bool kOne, int kSplit>
 __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
-                            Lds<D, kStates ? 0 : kSplit>& shared) {
+                            Lds<D, kStates ? 0 : kSplit, !kStates && shares(D, kOne)>& shared) {
   typedef typename PVec<T>::v8 T8;
   typedef typename PVec<T>::v4 T4;
   constexpr bool kHalf = !__is_same(T, __bf16);
@@ -287,6 +302,7 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
   constexpr int kGroupSteps = D == 256 ? 2 : 4;  // of a product of rows, read at once
   constexpr bool kEarly = kOne && D <= 128;  // values are split beside the scores' products
   constexpr bool kKeepQ = D == 64;  // from the scores to S^T Q^T, else it is read twice
+  constexpr bool kShare = !kStates && shares(D, kOne);
   static_assert(kCopies * kTiles * 1024 == kTileB, "whole copies per wave");
   unsigned char* const bufs = shared.bufs;  // [k, v, q][stage]
   float* const seen = shared.seen;
@@ -316,7 +332,8 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
   // Items are (chunk, kSplit query heads of the group), heads innermost; k and v come with the first.
   // States alone go through the chunks from the last one back: what they read last is what the next
   // launch reads first.  They end where e^{a n} is 0 in fp32 (below 2^-149): what lies before adds zeros
-  // (a third of the work at |a| = 0.1 and segments of 4,096: 131,001 tokens of 16 heads xxx -> xxx us).
+  // (a third of the work at |a| = 0.1 and segments of 4,096: 131,001 tokens of 16 heads,
+  // D = 128: 702 -> 638 us).
   const float log2_decay = log_decay * kLog2e;
   int chunks = cdiv(n, kChunk);
   const int begin = run.start + (kStates ? (chunks - 1) * kChunk : 0);
@@ -506,6 +523,7 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
   int q_stage = 0, kv_stage = 0, head = 0;
   int chunk = 0;
   bool first = true;
+  int turn = 0;  // the waves whose scores are next, at head dim 256
   T8 va[2];
   // the chunk's first row of the output
   unsigned char* out = static_cast<unsigned char*>(a.out) +
@@ -618,9 +636,33 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
       for (int ss = 0; ss < 2; ++ss) fold_bits(best, __builtin_bit_cast(uintx4, va[ss]));
       odd = __ballot(is_odd<T>(best)) != 0ull;
     } else {
-      int q_row = (2 * kStages + part_of) * kTileB + q_stage + row_at;
+      const int q_row_of_tile = (2 * kStages + part_of) * kTileB + q_stage;
+      int q_row = q_row_of_tile + row_at;
       asm volatile("" : "+v"(q_row));
       q_stage = q_stage == (kStages - 1) * kSplit * kTileB ? 0 : q_stage + kSplit * kTileB;
+      // A quarter of P^T for the head's waves, 16 keys by 16 queries; at head dim 256 those of four waves
+      // and of the other four in turn.
+      float* const scores = shared.scores + (kShare ? part_of * kChunk * kScoreRow : 0);
+      const bool sharing = kShare && mine && (D < 256 || (wave >> 2) == turn);  // uniform
+      turn ^= 1;
+      int quarter_at = 0;
+      floatx4 quarter = {};
+      auto share = [&]() {
+        const int in = lane_id(), row = in & 15, piece = in >> 4;
+        const int query = 16 * (wave & 1) + row, key = 16 * (wave >> 1 & 1) + row;
+        int key_at = kv_stage + key * kRowB + 16 * (piece ^ swizzle<C>(key));
+        int query_at = q_row_of_tile + query * kRowB + 16 * (piece ^ swizzle<C>(query));
+        asm volatile("" : "+v"(key_at), "+v"(query_at));
+        floatx4 p[2] = {};
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x)
+          p[x & 1] = mfma_16x16x32(*reinterpret_cast<const T8*>(bufs + (key_at ^ (64 * x))),
+                                   *reinterpret_cast<const T8*>(bufs + (query_at ^ (64 * x))), p[x & 1]);
+        const int key0 = key - row + 4 * piece;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) quarter[r] = (p[0][r] + p[1][r]) * seen[kChunk - query + key0 + r];
+        quarter_at = query * kScoreRow + key0;
+      };
       // O^T of the item.  kOdd: with weights of 0 for what is not finite and yet to come.
       auto attend = [&](auto tag) {
         constexpr bool kOdd = decltype(tag)::value != 0;
@@ -638,17 +680,22 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
                   *reinterpret_cast<const T8*>(bufs + (q_row ^ (32 * x)));
           }
         };
-        read(0, true);
+        if constexpr (!kShare) {
+          read(0, true);
 #pragma unroll
-        for (int i = 0; i < kKSteps / kGroupSteps; ++i) {
-          if (i + 1 < kKSteps / kGroupSteps) read(i + 1, true);
-          __builtin_amdgcn_sched_barrier(0);
+          for (int i = 0; i < kKSteps / kGroupSteps; ++i) {
+            if (i + 1 < kKSteps / kGroupSteps) read(i + 1, true);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int x = kGroupSteps * i; x < kGroupSteps * (i + 1); ++x)
-            p = mfma_32x32x16(ka[x % (2 * kGroupSteps)], qa[kKeepQ ? x : x % (2 * kGroupSteps)], p);
+            for (int x = kGroupSteps * i; x < kGroupSteps * (i + 1); ++x)
+              p = mfma_32x32x16(ka[x % (2 * kGroupSteps)], qa[kKeepQ ? x : x % (2 * kGroupSteps)], p);
+          }
+        }
+        if (!kKeepQ) read(0, false);
+        if constexpr (kShare && !kOdd) {
+          if (sharing) share();
         }
         if (kEarly && !kOdd) split();  // beside those products
-        if (!kKeepQ) read(0, false);
 #pragma unroll
         for (int i = 0; i < kKSteps / kGroupSteps; ++i) {
           if (!kKeepQ && i + 1 < kKSteps / kGroupSteps) read(i + 1, false);
@@ -663,9 +710,22 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
         }
         const float* const weight = seen + kChunk - c32 + 4 * h;
         const float since = seen[kChunk - 1 - c32] * sigma;  // scale e^{a (i + 1)} of the state
+        if constexpr (kShare) {
+          if (!kOdd) {
+            if (sharing) *reinterpret_cast<floatx4*>(scores + quarter_at) = quarter;
+            sync();
+          }
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const floatx4 four =
+                *reinterpret_cast<const floatx4*>(scores + c32 * kScoreRow + 8 * y + 4 * h);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) p[4 * y + x] = four[x];
+          }
+        }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          p[r] *= weight[token(r)];
+          if (!kShare) p[r] *= weight[token(r)];
           if (kOdd) p[r] = token(r) + 4 * h <= c32 ? p[r] : 0.f;
         }
         if constexpr (kHalf) {
@@ -717,7 +777,10 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
           }
         }
       };
-      if (mine) attend(IntTag<0>{});
+      if (mine)
+        attend(IntTag<0>{});
+      else if (kShare)
+        sync();
       // An infinity or a NaN among the scores or in v reaches the tokens before its own, through
       // weights of 0, and the outputs of its own: such a chunk is taken again.
       floatx4 trace = {0.f, 0.f, 0.f, 0.f};
@@ -839,7 +902,7 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
 template <typename T, int D, bool kOne, int kSplit>
 __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_linear_args a,
                                                                    const Divisor h_kv) {
-  __shared__ __attribute__((aligned(1024))) Lds<D, kSplit> shared;
+  __shared__ __attribute__((aligned(1024))) Lds<D, kSplit, shares(D, kOne)> shared;
   const int begins = sload(a.cu_seqlens), ends = sload(a.cu_seqlens + a.num_seqs);
   const int index = divide(blockIdx.x, h_kv);
   const int hk = blockIdx.x - index * a.h_kv;
@@ -864,7 +927,7 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
 template <typename T, int D>
 __global__ __launch_bounds__(2 * D, 2) void states_kernel(const fa_linear_args a,
                                                           const Divisor h_kv) {
-  __shared__ __attribute__((aligned(1024))) Lds<D, 0> shared;
+  __shared__ __attribute__((aligned(1024))) Lds<D, 0, false> shared;
   const int index = divide(blockIdx.x, h_kv);
   const int hk = blockIdx.x - index * a.h_kv;
   const Run run = find_run(a, index);
