@@ -988,10 +988,11 @@ int heads_at_once(int group, int d) {
   return group == 1 || d == 256 ? 1 : d == 128 || group == 2 ? 2 : 4;
 }
 
-// What a launch takes, in us, by segments of L tokens (0: whole sequences), from times of 36 shapes per
-// head dim (one sequence of 1,000 to 60 of up to 8,000, groups of 1 and 4 to 8; off by a tenth on average).  The
-// longest run's chunks or a slot's share of all, whichever is more; starts and ends of the work-groups;
-// the segments' states; no less than the bytes.
+// What a launch takes, in us, by segments of L tokens (0: whole sequences), from times of 12 shapes per
+// head dim (one sequence of 1,000 to 131,001 tokens, 3 to 40 of up to 8,000, groups of 1, 4 and 8), off by
+// a tenth on average; its choice is within 9% of the best in all but one (30 of up to 500, 32 heads of 8,
+// D = 128: 61 us for 55).  The longest run's chunks or a slot's share of all, whichever is more; starts
+// and ends of the work-groups; the segments' states; no less than the bytes.
 struct Cost {
   float chunk_one;          // a chunk, groups of one head
   float item, chunk_group;  // heads at once, a chunk beside them
@@ -1002,8 +1003,8 @@ struct Cost {
 };
 double cost_of(const fa_linear_args& a, int segment, int max_seqlen, int cus) {
   static const Cost kCost[3] = {{1.4f, 1.f, .9f, .42f, .01f, 5.2f, 4},
-                                {1.95f, 1.36f, .93f, .54f, .031f, 9.4f, 2},
-                                {4.4f, 1.95f, .7f, 2.8f, .11f, 23.f, 1}};
+                                {1.87f, 1.35f, .96f, .59f, .031f, 9.5f, 2},
+                                {4.16f, 1.77f, 1.81f, 1.74f, .086f, 23.7f, 1}};
   constexpr double kBytesPerUs = 5.1e6;
   const Cost& c = kCost[a.d == 64 ? 0 : a.d == 128 ? 1 : 2];
   const int group = a.h_q / a.h_kv, split = heads_at_once(group, a.d);
