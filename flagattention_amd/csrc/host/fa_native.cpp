@@ -1003,6 +1003,19 @@ bool rows_apart(const at::Tensor& t, int dims) {
   return true;
 }
 
+// Whether the bytes from the first element to the last of the two meet (rotary._reach_into).
+bool reach_into(const at::Tensor& x, const at::Tensor& y) {
+  uintptr_t at[2][2];
+  const at::Tensor* of[2] = {&x, &y};
+  for (int i = 0; i < 2; ++i) {
+    int64_t last = 0;
+    for (int64_t n = 0; n < of[i]->dim(); ++n) last += (of[i]->size(n) - 1) * of[i]->stride(n);
+    at[i][0] = reinterpret_cast<uintptr_t>(of[i]->data_ptr());
+    at[i][1] = at[i][0] + (of[i]->numel() > 0 ? (last + 1) * of[i]->element_size() : 0);
+  }
+  return at[0][0] < at[1][1] && at[1][0] < at[0][1];
+}
+
 // rotary(q, k, positions, inv_freq, sections, mixed_sections, adjacent_pairs, inplace): (q, k)
 PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -1062,6 +1075,8 @@ PyObject* rotary_cache(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const c10::Device device = q->device();
   for (const at::Tensor* t : {v, kc, vc, slots})
     if (t->device() != device) return none();
+  for (const at::Tensor* t : {q, k, v})
+    if (reach_into(*t, *kc) || reach_into(*t, *vc)) return none();
   at::Tensor q_out;
   {
     NoGil nogil;

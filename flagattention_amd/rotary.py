@@ -8,6 +8,7 @@ pair takes one axis, by the ``sections``.
 ``rotary_embedding`` turns q and k, for any of the attention operators here; ``rotary_cache_kv`` turns
 q and writes the turned k and v into the paged 16-bit cache that ``paged_attention`` reads.  Angles
 are worked out in 64 bits from the positions as they are, so there is no table and no last position.
+Forward only.
 
 Work is queued on the current stream; argument errors raise ``ArgumentError`` before any launch.
 """
@@ -61,6 +62,18 @@ def _apart(x, row_dims) -> bool:
                 return False
             reach += (size - 1) * stride
     return True
+
+
+def _span(x):
+    """The bytes from x's first element to its last."""
+    first = x.data_ptr()
+    last = sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
+    return (first, first + (last + 1) * x.element_size()) if x.numel() > 0 else (first, first)
+
+
+def _reach_into(x, y) -> bool:
+    a, b = _span(x), _span(y)
+    return a[0] < b[1] and b[0] < a[1]
 
 
 def _one_device(*tensors):
@@ -171,7 +184,8 @@ def rotary_cache_kv(
     q, k, positions, inv_freq, sections, mixed_sections, adjacent_pairs
                   as in ``rotary_embedding``; v [T, H_kv, D]
     key_cache, value_cache
-                  [num_blocks, H_kv, block_size, D] of q's type, as in ``paged_attention``
+                  [num_blocks, H_kv, block_size, D] of q's type, as in ``paged_attention``; they share no
+                  memory with each other, nor with q, k and v
     slot_mapping  int32 / int64 [T]: block * block_size + row of each token; negative slots (padding
                   tokens) and slots past the cache are skipped.  The slots of one call must differ:
                   rows that two tokens write are undefined
@@ -199,6 +213,8 @@ def rotary_cache_kv(
     _require(all(c.stride(3) == 1 and _apart(c, (0, 1, 2)) for c in (key_cache, value_cache)),
              "rows of the cache must be contiguous and not overlap")
     _require(key_cache.data_ptr() != value_cache.data_ptr(), "key_cache and value_cache overlap")
+    _require(not any(_reach_into(x, c) for x in (q, k, v) for c in (key_cache, value_cache)),
+             "q, k and v must not lie in the caches")
     _require(slot_mapping.dim() == 1 and slot_mapping.shape[0] == tokens
              and slot_mapping.dtype in (torch.int32, torch.int64),
              "slot_mapping must be int32 / int64 [num_tokens]")

@@ -148,6 +148,25 @@ def test_sizes_past_a_launch_are_left_to_python():
         flag_attn.linear_attention_varlen(*args[:4], cu, 1)
 
 
+@pytest.mark.parametrize("into", [0, 1, 2])
+def test_rows_that_lie_in_the_caches_are_refused(into):
+    """Before a launch: nothing is written."""
+    need_gpu()
+    fast = _lib.native()
+    kc, vc = half(3, 2, 16, 64), half(3, 2, 16, 64)
+    f, pos = torch.rand(32, device=DEV), torch.arange(5, device=DEV)
+    for cache in (kc, vc):
+        rows = [half(5, 2, 64) for _ in range(3)]
+        rows[into] = cache[1, :, 3:8].transpose(0, 1)
+        before = cache.clone()
+        assert fast.rotary_cache(*rows, pos, f, kc, vc, pos, None, False, False) is None
+        with pytest.raises(ArgumentError, match="must not lie in the caches"):
+            flag_attn.rotary_cache_kv(*rows, pos, f, kc, vc, pos)
+        assert torch.equal(cache, before)
+        rows[into] = rows[into].clone()
+        assert fast.rotary_cache(*rows, pos, f, kc, vc, pos, None, False, False) is not None
+
+
 def test_graph_rotary_and_store():
     """Both in one graph; the replays see new rows, positions and slots."""
     need_gpu()

@@ -106,6 +106,20 @@ def test_store_rejects(kw, msg):
         flag_attn.rotary_cache_kv(**_store(**kw))
 
 
+@pytest.mark.parametrize("into", ["q", "k", "v"])
+@pytest.mark.parametrize("cache", ["key_cache", "value_cache"])
+def test_store_rejects_rows_of_the_caches(into, cache):
+    whole = half(6 * 2 * 16 * 64)
+    rows = whole[2047:2047 + 5 * 2 * 64].view(5, 2, 64)
+    kw = _store(**{cache: whole[2048:2048 * 4].view(3, 2, 16, 64), into: rows, "q": half(5, 2, 64)}
+                if into != "q" else {cache: whole[2048:2048 * 4].view(3, 2, 16, 64), "q": rows})
+    with pytest.raises(ArgumentError, match="must not lie in the caches"):
+        flag_attn.rotary_cache_kv(**kw)
+    kw[into] = whole[2048 - 640:2048].view(5, 2, 64)  # up to the cache's first byte
+    with pytest.raises(ArgumentError, match="CUDA"):
+        flag_attn.rotary_cache_kv(**kw)
+
+
 def _prompt(**kw):
     return {**dict(q=half(9, 4, 64), k=half(9, 2, 64), v=half(9, 2, 64), log_decay=torch.zeros(2),
                    cu_seqlens=i32(3), max_seqlen=9, state=torch.zeros(4, 2, 64, 64),
