@@ -16,7 +16,11 @@
 // D = 256: 200 us so, 179 shared; 32 heads, D = 128, fp16: 143 / 137; a lone sequence of one head waits
 // for the exchange, 410 / 441 at 8,192 tokens; two heads at once at D = 128: 227 / 233, so not there).
 //
-// Bound by q, k, v and out.  Inputs come three chunks deep into LDS.
+// Bound by q, k, v and out where the card is full (16 x 1,024 tokens of 32 heads, D = 128: 129 us, 117
+// at the rate of a copy; of 64, D = 64: 145, 111), by a chunk's chain of products where it is not: 1.2,
+// 1.7 and 3.4 us in bf16 at D = 64, 128, 256 for a lone sequence of one head.  At D = 256 one work-group
+// fits a CU and the chain shows in full launches too (of 16: 179, 131).  Inputs come three chunks deep
+// into LDS, so that no chunk waits for memory.
 //
 // Rounding: scores, sums and states are fp32.  P and the state's copy are rounded to the input type to
 // meet V and Q, as the output is.  The weighted values that a state takes in are split in three bf16 or
@@ -922,8 +926,9 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
   walk<T, D, false, kOne, kSplit>(a, run, hk, shared);
 }
 
-// What every run but a sequence's last makes.  Without tiles of q three work-groups fit a CU (the first
-// runs' outputs in the same launch leave two: 131,001 tokens of 16 heads 638 -> 710 us).
+// What every run but a sequence's last makes.  Without tiles of q three work-groups fit a CU at D = 128
+// (the first runs' outputs in the same launch leave two: 131,001 tokens of 16 heads 638 -> 710 us).  That
+// sequence: 190 us here, for the half of k and v that is not skipped, then 441 for the outputs, 4.9 TB/s.
 template <typename T, int D>
 __global__ __launch_bounds__(2 * D, 2) void states_kernel(const fa_linear_args a,
                                                           const Divisor h_kv) {

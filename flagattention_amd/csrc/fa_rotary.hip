@@ -5,6 +5,10 @@
 // heads: it works the sines out once and uses them for each.  The angle of a pair is a product in
 // 64 bits, counted in revolutions, whose whole part is taken away there; what is left goes to the
 // hardware's sine and cosine (which count revolutions too) in 32.
+//
+// Bound by the rows, read and written once: 16,384 tokens of 64 heads and 8 of k and v, D = 128, into a
+// cache 131 us, 20,001 of 16 and 16, D = 256, 125 us, 5.1 and 5.3 TB/s (a large copy: 5.1); 8,192 of 32
+// and 8 35 us, 4.8.  A few tokens take 3 to 4.4 us, the launch and two trips to memory.
 #include "fa_common.h"
 #include "fa_divide.h"
 #include "flagattention_amd_linear.h"
