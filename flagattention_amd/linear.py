@@ -135,7 +135,8 @@ def linear_attention_varlen(
     Returns ``o`` shaped and typed like ``q``.  Rows of q that belong to no sequence get 0, a
     sequence without tokens leaves its slot as it is.  An infinity or a NaN in k or v makes the
     outputs that it reaches and the state not finite (not always the infinity that the sums
-    would have); tokens before it are not touched.
+    would have) while its weight is above 0 in float32, past which it may be forgotten; tokens before
+    it are not touched.
     """
     fast = _lib.native()
     if fast is not None:
