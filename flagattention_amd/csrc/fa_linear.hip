@@ -995,8 +995,8 @@ int heads_at_once(int group, int d) {
 
 // What a launch takes, in us, by segments of L tokens (0: whole sequences), from times of 12 shapes per
 // head dim (one sequence of 1,000 to 131,001 tokens, 3 to 40 of up to 8,000, groups of 1, 4 and 8), off by
-// a tenth on average; its choice is within 9% of the best in all but one (30 of up to 500, 32 heads of 8,
-// D = 128: 61 us for 55).  The longest run's chunks or a slot's share of all, whichever is more; starts
+// a tenth on average; its choice is within 5% of the best of the powers of two in all but one (20,000, 8
+// heads, D = 256, where what gives every slot a segment is better still).  The longest run's chunks or a slot's share of all, whichever is more; starts
 // and ends of the work-groups; the segments' states; no less than the bytes.
 struct Cost {
   float chunk_one;          // a chunk, groups of one head
@@ -1007,9 +1007,9 @@ struct Cost {
   int slots;                // work-groups per CU
 };
 double cost_of(const fa_linear_args& a, int segment, int max_seqlen, int cus) {
-  static const Cost kCost[3] = {{1.4f, 1.f, .9f, .42f, .01f, 5.2f, 4},
-                                {1.87f, 1.35f, .96f, .59f, .031f, 9.5f, 2},
-                                {4.16f, 1.77f, 1.81f, 1.74f, .086f, 23.7f, 1}};
+  static const Cost kCost[3] = {{1.29f, 1.12f, .7f, .56f, .0109f, 5.4f, 4},
+                                {1.98f, 1.4f, .31f, .63f, .056f, 5.4f, 2},
+                                {3.53f, 1.62f, 2.57f, 2.f, .165f, 21.f, 1}};
   constexpr double kBytesPerUs = 5.1e6;
   const Cost& c = kCost[a.d == 64 ? 0 : a.d == 128 ? 1 : 2];
   const int group = a.h_q / a.h_kv, split = heads_at_once(group, a.d);
@@ -1021,7 +1021,8 @@ double cost_of(const fa_linear_args& a, int segment, int max_seqlen, int cus) {
     runs = static_cast<double>(a.total) / segment + .6 * a.num_seqs;
     longest = segment / kChunk;
     each += c.chunk_state;
-    states = runs * a.h_kv * c.state;
+    // about half a segment of a sequence hands nothing on, or less where some are short
+    states = std::max(0., static_cast<double>(a.total) / segment - .3 * a.num_seqs) * a.h_kv * c.state;
   }
   const double starts = c.start * std::ceil(runs * a.h_kv / slots) * (segment > 0 ? 1. : .5);
   const double bytes = 4. * a.total * a.d * (a.h_q + a.h_kv * (segment > 0 ? 2. : 1.));
