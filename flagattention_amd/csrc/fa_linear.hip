@@ -1,32 +1,32 @@
 // Linear attention with a decay per head over packed sequences for gfx950: fp16 or bf16, head dim 64,
 // 128, 256.  Per KV head with log decay a, S_t = e^a S_{t-1} + k_t v_t^T, o_t = scale q_t S_t.
 //
-// A work-group takes one (sequence, KV head) through its tokens, 32 at a time. For such a chunk of
-// c tokens, counted from 0, with S the state before it: O^T = (S^T Q^T) diag(scale e^{a (i+1)}) +
-// V^T P^T,  P^T[j, i] = scale e^{a (i-j)} (K Q^T)[j, i], j <= i S'  = e^{a c} S + K^T diag(e^{a
-// (c-1-j)}) V No factor is above 1 for a decay (a <= 0), however long the chunk or fast the decay.
+// A work-group takes one (sequence, KV head) through its tokens, 32 at a time.  For such a chunk of c
+// tokens, counted from 0, with S the state before it:
+//   O^T = (S^T Q^T) diag(scale e^{a (i+1)}) + V^T P^T,  P^T[j, i] = scale e^{a (i-j)} (K Q^T)[j, i], j <= i
+//   S'  = e^{a c} S + K^T diag(e^{a (c-1-j)}) V
+// No factor is above 1 for a decay (a <= 0), however long the chunk or fast the decay.
 //
-// Wave w owns columns 32w .. 32w + 31 of S, in fp32 in its accumulators for the whole sequence, and
-// the same dims of the output; D / 32 waves. Products are MFMA 32x32x16. S leaves the
-// accumulators as the operands of the next products (the rows of a state tile are dealt to dims so
-// that a lane's 8 registers are the 8 dims of its part of a step). Every wave needs the whole of
-// P^T. At head dim 256, and at 128 without groups, four waves work out 16 x 16 of it each and hand
-// it round in LDS; each wave for itself would make it a fifth of its products and read K and Q
-// whole again (16 x 1,024 tokens of 16 heads, D = 256: 200 us so, 179 shared; 32 heads, D = 128,
-// fp16: 143 / 137; a lone sequence of one head waits for the exchange, 410 / 441 at 8,192 tokens;
-// two heads at once at D = 128: 227 / 233, so not there).
+// Wave w owns columns 32w .. 32w + 31 of S, in fp32 in its accumulators for the whole sequence, and the
+// same dims of the output; D / 32 waves.  Products are MFMA 32x32x16.  S leaves the accumulators as the
+// operands of the next products (the rows of a state tile are dealt to dims so that a lane's 8 registers
+// are the 8 dims of its part of a step).  Every wave needs the whole of P^T.  At head dim 256, and at 128
+// without groups, four waves work out 16 x 16 of it each and hand it round in LDS; each wave for itself
+// would make it a fifth of its products and read K and Q whole again (16 x 1,024 tokens of 16 heads,
+// D = 256: 200 us so, 179 shared; 32 heads, D = 128, fp16: 143 / 137; a lone sequence of one head waits
+// for the exchange, 410 / 441 at 8,192 tokens; two heads at once at D = 128: 227 / 233, so not there).
 //
-// Bound by q, k, v and out where the card is full (16 x 1,024 tokens of 32 heads, D = 128: 129 us,
-// 117 at the rate of a copy; of 64, D = 64: 145, 111), by a chunk's chain of products where it is
-// not: 1.2, 1.7 and 3.4 us in bf16 at D = 64, 128, 256 for a lone sequence of one head. At D = 256
-// one work-group fits a CU and the chain shows in full launches too (of 16: 179, 131). Inputs come
-// three chunks deep into LDS, so that no chunk waits for memory.
+// Bound by q, k, v and out where the card is full (16 x 1,024 tokens of 32 heads, D = 128: 129 us, 117
+// at the rate of a copy; of 64, D = 64: 145, 111), by a chunk's chain of products where it is not: 1.2,
+// 1.7 and 3.4 us in bf16 at D = 64, 128, 256 for a lone sequence of one head.  At D = 256 one work-group
+// fits a CU and the chain shows in full launches too (of 16: 179, 131).  Inputs come three chunks deep
+// into LDS, so that no chunk waits for memory.
 //
-// Rounding: scores, sums and states are fp32. P and the state's copy are rounded to the input type
-// to meet V and Q, as the output is. The weighted values that a state takes in are split in three
-// bf16 or two fp16 numbers, which hold 24 and 22 bits: the state is an output in fp32 (two bf16
-// numbers left it 2e-6 from 64 bits, three 2e-7). fp16 operands are taken relative to a power of
-// two of the largest (a column's of the state, of the weighted values, of P^T), since states,
+// Rounding: scores, sums and states are fp32.  P and the state's copy are rounded to the input type to
+// meet V and Q, as the output is.  The weighted values that a state takes in are split in three bf16 or
+// two fp16 numbers, which hold 24 and 22 bits: the state is an output in fp32 (two bf16 numbers left
+// it 2e-6 from 64 bits, three 2e-7).  fp16 operands are taken relative to a
+// power of two of the largest (a column's of the state, of the weighted values, of P^T), since states,
 // scores and products of tiny inputs leave its range.
 #include <algorithm>
 #include <cmath>
@@ -75,8 +75,8 @@ namespace {
 
 constexpr int kChunk = 32;
 constexpr int kStages = 3;
-// fp16: the least power of two that operands are relative to. What is below it by 2^-25 is below
-// half of the smallest step of the output for any q or v in range.
+// fp16: the least power of two that operands are relative to.  What is below it by 2^-25 is below half
+// of the smallest step of the output for any q or v in range.
 constexpr int kLeastPower = -40;
 
 // Where 16 bytes c of row r of a chunk lie in it: c ^ swizzle(r).  Rows are read 16 bytes a lane, one
@@ -171,15 +171,15 @@ __device__ inline bool has_of(const fa_linear_args& a, int s) {
   return a.has_state == nullptr || a.has_state[s] != 0;
 }
 
-// Run `index` of the launch. With segments of L tokens those of sequence s have the places start_s
-// / L + s and on: a sequence of n tokens has ceil(n / L) of them, and the next one's start is at
-// least that far on.
+// Run `index` of the launch.  With segments of L tokens those of sequence s have the places start_s / L + s
+// and on: a sequence of n tokens has ceil(n / L) of them, and the next one's start is at least that
+// far on.
 //
-// Sorted (up to 64 sequences, a lane each): whole segments first, then what is left of each
-// sequence, the longest first, so that the work-groups that run longest do not start last (60
-// sequences of up to 1,000 tokens, 16 heads, D = 128: 149 -> 110 us; 60 single tokens 23.5 -> 24.9,
-// so not for short ones). Otherwise in packed order, by their places; the sequence is the last one
-// whose first place is not past `index`, and a wave looks at 64 at a time.
+// Sorted (up to 64 sequences, a lane each): whole segments first, then what is left of each sequence, the
+// longest first, so that the work-groups that run longest do not start last (60 sequences of up to
+// 1,000 tokens, 16 heads, D = 128: 149 -> 110 us; 60 single tokens 23.5 -> 24.9, so not for short
+// ones).  Otherwise in packed order, by their places; the sequence is the last one whose first place
+// is not past `index`, and a wave looks at 64 at a time.
 __device__ inline Run find_run(const fa_linear_args& a, int index) {
   Run run = {-1, 0, 0, 0, 0, true, -1, false};
   const int lane = threadIdx.x & 63;
@@ -201,8 +201,8 @@ __device__ inline Run find_run(const fa_linear_args& a, int index) {
     if (index < wholes) {
       found = __ballot(upto > index);
     } else {
-      // by the upper bits of what is left as a float: the sequences that have more, or as much and
-      // come before
+      // by the upper bits of what is left as a float: the sequences that have more, or as much and come
+      // before
       const unsigned int key = __float_as_uint(static_cast<float>(rest)) >> 20;
       unsigned long long same = ~0ull;
       int longer = 0;
@@ -269,9 +269,9 @@ __device__ inline Run find_run(const fa_linear_args& a, int index) {
 constexpr bool shares(int d, bool one) { return d == 256 || (d == 128 && one); }
 constexpr int kScoreRow = 36;  // floats of a row of shared scores: 16 rows lie in different banks
 
-// LDS of a work-group: tiles of k, v and of q's kHeads heads, kStages of each, P of each head, and
-// weights by the place m of a token before the chunk's last: at 1 + m scale e^{a (31 - m)}, 0 past
-// 31 (tokens to come); and e^{a (31 - m)}, 1 past 31.
+// LDS of a work-group: tiles of k, v and of q's kHeads heads, kStages of each, P of each head, and weights
+// by the place m of a token before the chunk's last: at 1 + m scale e^{a (31 - m)}, 0 past 31 (tokens to
+// come); and e^{a (31 - m)}, 1 past 31.
 template <int D, int kHeads, bool kShare>
 struct Lds {
   unsigned char bufs[(2 + kHeads) * kStages * kChunk * 2 * D];
@@ -280,13 +280,13 @@ struct Lds {
   float seen[1 + 2 * kChunk], left_of[2 * kChunk];
 };
 
-// bf16: s is kept times 2^-kLift. Values are taken up to 16 times into it (by what s has yet to
-// fall), and the largest finite ones stay within fp32 so.
+// bf16: s is kept times 2^-kLift.  Values are taken up to 16 times into it (by what s has yet to fall), and
+// the largest finite ones stay within fp32 so.
 constexpr int kLift = 5;
 
-// A run of one KV head, from its state through its chunks. kStates: only the state that it makes,
-// from zeros, or the first run's from its sequence's. kOne: groups of one query head. kSplit:
-// heads that are attended at once, by D / 32 waves each, which all keep the state.
+// A run of one KV head, from its state through its chunks.  kStates: only the state that it makes, from
+// zeros, or the first run's from its sequence's.  kOne: groups of one query head.  kSplit: heads that
+// are attended at once, by D / 32 waves each, which all keep the state.
 template <typename T, int D, bool kStates, bool kOne, int kSplit>
 __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
                             Lds<D, kStates ? 0 : kSplit, !kStates && shares(D, kOne)>& shared) {
@@ -314,9 +314,8 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
 
   const int wave = uniform(wave_id() % kTiles);     // 32 columns of the state
   const int part_of = uniform(wave_id() / kTiles);  // of the heads at once
-  // At head dim 256 the state leaves few registers: what follows from the lane is worked out where
-  // it is used, and not kept (a wait for a register that comes back from memory waits for every
-  // copy too).
+  // At head dim 256 the state leaves few registers: what follows from the lane is worked out where it is
+  // used, and not kept (a wait for a register that comes back from memory waits for every copy too).
   auto lane_id = [&]() -> int { return D == 256 ? fresh_lane() : threadIdx.x & 63; };
   const int group = kStates || kOne ? 1 : a.h_q / a.h_kv;
 
@@ -327,18 +326,18 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
           ? a.state + run.slot * a.state_stride_s + hk * a.state_stride_h
           : nullptr;
 
-  // Of a sequence of several runs, part has what each makes at the place of the next, and at the
-  // first's a copy of what that starts from: the last run may write the sequence's state while the
-  // first has not read it yet.
+  // Of a sequence of several runs, part has what each makes at the place of the next, and at the first's
+  // a copy of what that starts from: the last run may write the sequence's state while the first
+  // has not read it yet.
   const long long part_step = static_cast<long long>(a.h_kv) * (D * D);
   float* const part = a.part + run.place * part_step + hk * (D * D);
   float* const to_state = kStates ? part + part_step : run.last ? slot_state : nullptr;
 
-  // Items are (chunk, kSplit query heads of the group), heads innermost; k and v come with the
-  // first. States alone go through the chunks from the last one back: what they read last is what
-  // the next launch reads first. They end where e^{a n} is 0 in fp32 (below 2^-149): what lies
-  // before adds zeros (a third of the work at |a| = 0.1 and segments of 4,096: 131,001 tokens of 16
-  // heads, D = 128: 702 -> 638 us).
+  // Items are (chunk, kSplit query heads of the group), heads innermost; k and v come with the first.
+  // States alone go through the chunks from the last one back: what they read last is what the next
+  // launch reads first.  They end where e^{a n} is 0 in fp32 (below 2^-149): what lies before adds zeros
+  // (a third of the work at |a| = 0.1 and segments of 4,096: 131,001 tokens of 16 heads,
+  // D = 128: 702 -> 638 us).
   const float log2_decay = log_decay * kLog2e;
   int chunks = cdiv(n, kChunk);
   const int begin = run.start + (kStates ? (chunks - 1) * kChunk : 0);
@@ -415,9 +414,8 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
   int ahead = fetch();  // copies on their way after those of the item at hand
   int stored = 0;       // stores of the last item
 
-  // Row rho of a 32-row tile of the state (or of O^T) is dim 16 (rho / 16) + 8 ((rho / 4) % 2) + 4
-  // ((rho / 8) % 2) + rho % 4: accumulator register r of half h is then dim 16 (r / 8) + 8h + r %
-  // 8.
+  // Row rho of a 32-row tile of the state (or of O^T) is dim 16 (rho / 16) + 8 ((rho / 4) % 2) +
+  // 4 ((rho / 8) % 2) + rho % 4: accumulator register r of half h is then dim 16 (r / 8) + 8h + r % 8.
   auto state_place = [&]() -> int {
     const int lane = lane_id(), c32 = lane & 31;
     const int pi = (c32 & 16) + 8 * ((c32 >> 2) & 1) + 4 * ((c32 >> 3) & 1) + (c32 & 3);
@@ -476,10 +474,9 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
   // States alone have their weights counted to the run's end instead, and are never brought up.
   int after = 0;
 
-  // s is kept times 2^-s_power. fp16: a power for each column (a lane's), whose largest is at
-  // about 8 when it was last looked at: there is room for a growth by 2^12 (past it an output is
-  // not finite, and the chunk is taken again) and a fall by 2^17 (counted below) before its copies
-  // lose bits.
+  // s is kept times 2^-s_power.  fp16: a power for each column (a lane's), whose largest is at about 8
+  // when it was last looked at: there is room for a growth by 2^12 (past it an output is not finite,
+  // and the chunk is taken again) and a fall by 2^17 (counted below) before its copies lose bits.
   int s_power = kHalf || kStates ? 0 : kLift;
   int looked = -1;  // tokens since, -1: there was nothing yet
   float* const scales = shared.scales[kStates ? 0 : part_of] + 32 * wave;
@@ -647,8 +644,8 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
       int q_row = q_row_of_tile + row_at;
       asm volatile("" : "+v"(q_row));
       q_stage = q_stage == (kStages - 1) * kSplit * kTileB ? 0 : q_stage + kSplit * kTileB;
-      // A quarter of P^T for the head's waves, 16 keys by 16 queries; at head dim 256 those of four
-      // waves and of the other four in turn.
+      // A quarter of P^T for the head's waves, 16 keys by 16 queries; at head dim 256 those of four waves
+      // and of the other four in turn.
       float* const scores = shared.scores + (kShare ? part_of * kChunk * kScoreRow : 0);
       const bool sharing = kShare && mine && (D < 256 || (wave >> 2) == turn);  // uniform
       turn ^= 1;
@@ -929,10 +926,9 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
   walk<T, D, false, kOne, kSplit>(a, run, hk, shared);
 }
 
-// What every run but a sequence's last makes. Without tiles of q three work-groups fit a CU at D =
-// 128 (the first runs' outputs in the same launch leave two: 131,001 tokens of 16 heads 638 -> 710
-// us). That sequence: 190 us here, for the half of k and v that is not skipped, then 441 for the
-// outputs, 4.9 TB/s.
+// What every run but a sequence's last makes.  Without tiles of q three work-groups fit a CU at D = 128
+// (the first runs' outputs in the same launch leave two: 131,001 tokens of 16 heads 638 -> 710 us).  That
+// sequence: 190 us here, for the half of k and v that is not skipped, then 441 for the outputs, 4.9 TB/s.
 template <typename T, int D>
 __global__ __launch_bounds__(2 * D, 2) void states_kernel(const fa_linear_args a,
                                                           const Divisor h_kv) {
@@ -944,8 +940,8 @@ __global__ __launch_bounds__(2 * D, 2) void states_kernel(const fa_linear_args a
   walk<T, D, true, false, 1>(a, run, hk, shared);
 }
 
-// The states that runs start from, but for the first two: each what its predecessor made on top of
-// what that one started from, part[i] += e^{a L} part[i - 1].
+// The states that runs start from, but for the first two: each what its predecessor made on top of what
+// that one started from, part[i] += e^{a L} part[i - 1].
 template <int D>
 __global__ __launch_bounds__(256) void join_kernel(const fa_linear_args a, const Divisor h_kv) {
   constexpr int kAhead = 8;
@@ -985,25 +981,25 @@ int runs_of(const fa_linear_args& a) {
   return a.segment > 0 ? a.total / a.segment + seqs : seqs;
 }
 
-// Runs of a sequence from which on their states are joined in a launch of their own, which takes 6
-// to 24 us; below, each run adds up what those before it made, 3 us a state at head dim 128, 13 at
-// 256 (8 prompts of up to 2,048 tokens, 16 KV heads, in segments of 416: 299 us so, 192 joined; one
-// of 131,001 at 128 684 / 637, of 2,560 in five segments 58 both ways).
+// Runs of a sequence from which on their states are joined in a launch of their own, which takes 6 to 24
+// us; below, each run adds up what those before it made, 3 us a state at head dim 128, 13 at 256
+// (8 prompts of up to 2,048 tokens, 16 KV heads, in segments of 416: 299 us so, 192 joined; one of
+// 131,001 at 128 684 / 637, of 2,560 in five segments 58 both ways).
 int join_runs(int d) { return d == 256 ? 3 : 5; }
 
-// Heads that a work-group attends at once: as many as the registers of two waves per SIMD keep the
-// state for (8 sequences of 1,024 tokens, 64 heads of 8, D = 128: 136 us with one, 97 with two;
-// three of up to 48, 8 heads of 2, D = 64: 10.8 with one, 8.1 with four).
+// Heads that a work-group attends at once: as many as the registers of two waves per SIMD keep the state
+// for (8 sequences of 1,024 tokens, 64 heads of 8, D = 128: 136 us with one, 97 with two; three of up to
+// 48, 8 heads of 2, D = 64: 10.8 with one, 8.1 with four).
 int heads_at_once(int group, int d) {
   return group == 1 || d == 256 ? 1 : d == 128 || group == 2 ? 2 : 4;
 }
 
-// What a launch takes, in us, by segments of L tokens (0: whole sequences), from times of 12 shapes
-// per head dim (one sequence of 1,000 to 131,001 tokens, 3 to 40 of up to 8,000, groups of 1, 4 and
-// 8), off by a tenth on average; its choice is within 5% of the best of the powers of two in all
-// but one (20,000, 8 heads, D = 256, where what gives every slot a segment is better still). The
-// longest run's chunks or a slot's share of all, whichever is more; starts and ends of the
-// work-groups; the segments' states; no less than the bytes.
+// What a launch takes, in us, by segments of L tokens (0: whole sequences), from times of 12 shapes per
+// head dim (one sequence of 1,000 to 131,001 tokens, 3 to 40 of up to 8,000, groups of 1, 4 and 8), off by
+// a tenth on average; its choice is within 5% of the best of the powers of two in all but one (20,000, 8
+// heads, D = 256, where what gives every slot a segment is better still).  The longest run's chunks or a
+// slot's share of all, whichever is more; starts and ends of the work-groups; the segments' states; no
+// less than the bytes.
 struct Cost {
   float chunk_one;          // a chunk, groups of one head
   float item, chunk_group;  // heads at once, a chunk beside them
@@ -1038,8 +1034,8 @@ double cost_of(const fa_linear_args& a, int segment, int max_seqlen, int cus) {
 
 constexpr int64_t kMaxWorkspace = int64_t{1} << 32;  // bytes
 
-// Tokens of a segment, 0 for whole sequences: the cheapest of powers of two and of what gives every
-// slot one segment.
+// Tokens of a segment, 0 for whole sequences: the cheapest of powers of two and of what gives every slot
+// one segment.
 int choose_segment(const fa_linear_args& a, int max_seqlen, int cus) {
   if (a.num_seqs == 0 || max_seqlen <= 2 * kChunk) return 0;
   int best = 0;
