@@ -252,6 +252,45 @@ def test_what_is_not_finite_reaches_later_tokens_only(which, dtype, bad):
     assert not bool(torch.isfinite(state2[~rest]).any())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("h,hk,d", [(2, 2, 64), (6, 2, 64), (2, 2, 128), (6, 2, 128), (2, 2, 256), (6, 2, 256)])
+@pytest.mark.parametrize("which", ["q", "k", "v", "state"])
+def test_what_is_not_finite_in_every_layout(which, h, hk, d, dtype):
+    """An infinity in the second KV head (or its last query head) of token 41 of the middle sequence, or in
+    its state: what it does not reach keeps its bits."""
+    need_gpu()
+    say(f"linear infinity in {which} h={h} hk={hk} d={d} {dtype}")
+    lens, g = [40, 100, 40], h // hk
+    q, k, v, a, cu, state, ids = make(lens, h, hk, d, dtype, seed=8)
+    a[:] = -0.05
+    state2, slot, col = state.clone(), int(ids[1]), d - 27
+    o = flag_attn.linear_attention_varlen(q, k, v, a, i32(cu), 100, state, ids)
+    t = cu[1] + 41
+    reached = torch.zeros(o.shape, dtype=torch.bool, device=DEV)
+    rest = torch.ones(state.shape, dtype=torch.bool, device=DEV)
+    if which == "q":
+        q[t, h - 1, col] = math.inf
+        reached[t, h - 1] = True
+    elif which == "k":
+        k[t, 1, col] = math.inf
+        reached[t:cu[2], g:] = True
+        rest[slot, 1, col] = False
+    elif which == "v":
+        v[t, 1, col] = -math.inf
+        reached[t:cu[2], g:, col] = True
+        rest[slot, 1, :, col] = False
+    else:
+        state2[slot, 1, 5, col] = math.inf
+        reached[cu[1]:cu[2], g:, col] = True
+        rest[slot, 1, 5, col] = False
+    o2 = flag_attn.linear_attention_varlen(q, k, v, a, i32(cu), 100, state2, ids)
+    torch.cuda.synchronize()
+    assert torch.equal(o2[~reached], o[~reached])
+    assert not bool(torch.isfinite(o2[reached]).any())
+    assert torch.equal(state2[rest], state[rest])
+    assert not bool(torch.isfinite(state2[~rest]).any())
+
+
 def test_a_last_token_that_is_not_finite():
     """Rows past the end of a chunk repeat no such value into the state's other dims."""
     need_gpu()

@@ -120,6 +120,24 @@ def test_a_wrong_bound_changes_the_launch_only(most):
             assert_state(state[int(ids[s]), j], end, end_size, 2 * (e - b) + 64, q.dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("h,hk,d", [(16, 16, 64), (24, 8, 64), (16, 16, 128), (24, 8, 128), (8, 8, 256), (24, 8, 256)])
+def test_the_same_call_gives_the_same_bits(h, hk, d, dtype):
+    """Of a full card, twenty times over: nothing depends on which wave or work-group comes first."""
+    need_gpu()
+    say(f"linear repeats h={h} hk={hk} d={d} {dtype}")
+    lens = [1500, 3, 700, 33, 900, 0, 64, 1, 400, 1023]
+    q, k, v, a, cu, state, ids = make(lens, h, hk, d, dtype, seed=d + h, behind=5)
+    first = None
+    for _ in range(20):
+        end = state.clone()
+        o = flag_attn.linear_attention_varlen(q, k, v, a, i32(cu), 1500, end, ids)
+        if first is None:
+            first = o, end
+        else:
+            assert torch.equal(o, first[0]) and torch.equal(end, first[1])
+
+
 @pytest.mark.parametrize("segment", [0, 32])
 @pytest.mark.parametrize("order", [False, True])
 def test_starts_that_fall_or_leave_the_rows_stay_in_bounds(segment, order):
