@@ -445,6 +445,38 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
     for (int i = run.part - 1; i >= 0; --i)
       add_state(part - i * part_step, i == run.part - 1 ? 0.f : fall);
   }
+  // s is kept times 2^-s_power.  fp16: a power for each column (a lane's).
+  int s_power = kHalf || kStates ? 0 : kLift;
+  // The largest of the lane's column that is finite.
+  auto most_of = [&]() -> float {
+    float most = 0.f;
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(s[t][r]));
+    if (__ballot(most == __builtin_inff()) != 0ull) {  // uniform
+      most = 0.f;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          most = fabsf(s[t][r]) < __builtin_inff() ? fmaxf(most, fabsf(s[t][r])) : most;
+    }
+    return max_xor32(most);
+  };
+  auto scale_down = [&](int by) {
+    const float x = two_to(-by);
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[t][r] *= x;
+    s_power += by;
+  };
+  // fp16 states alone take the values in units of s, whose power follows the largest of them, 2^11 units or
+  // more: 2^-25 of a unit is lost.  It starts so low that what the run starts from is at 2^30.  (Products
+  // of their own power, added to s: 131,001 tokens of 16 heads, D = 256, 1,867 us for 1,775.)
+  constexpr int kLowest = -126;
+  if constexpr (kStates && kHalf) s_power = kLowest;
   if constexpr (kStates) {
     if (from_state) {
       const int state_at = state_place();
@@ -456,6 +488,11 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
           part[state_at + (32 * t + 16 * (r >> 3) + (r & 7)) * D] = s[t][r];
           s[t][r] *= fall;
         }
+      if constexpr (kHalf) {
+        s_power = 0;
+        const float most = most_of();
+        scale_down(most > 0.f ? max(power_of(most) - 30, kLowest) : kLowest);
+      }
     }
   }
 
@@ -474,37 +511,16 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
   // States alone have their weights counted to the run's end instead, and are never brought up.
   int after = 0;
 
-  // s is kept times 2^-s_power.  fp16: a power for each column (a lane's), whose largest is at about 8
-  // when it was last looked at: there is room for a growth by 2^12 (past it an output is not finite,
-  // and the chunk is taken again) and a fall by 2^17 (counted below) before its copies lose bits.
-  int s_power = kHalf || kStates ? 0 : kLift;
+  // fp16: a column's largest is at about 8 when it was last looked at: there is room for a growth by 2^12
+  // (past it an output is not finite, and the chunk is taken again) and a fall by 2^17 (counted below)
+  // before its copies lose bits.
   int looked = -1;  // tokens since, -1: there was nothing yet
   float* const scales = shared.scales[kStates ? 0 : part_of] + 32 * wave;
   auto look = [&]() {
-    float most = 0.f;
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(s[t][r]));
-    if (__ballot(most == __builtin_inff()) != 0ull) {  // uniform: of those that are finite
-      most = 0.f;
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          most = fabsf(s[t][r]) < __builtin_inff() ? fmaxf(most, fabsf(s[t][r])) : most;
-    }
-    most = max_xor32(most);
+    const float most = most_of();
     // |s| 2^s_power is at most 2^128: both factors stay in range
     const int by = most > 0.f ? max(power_of(most) - 3, -100 - s_power) : 0;
-    if (__ballot(by < -2 || by > 2) != 0ull) {  // uniform
-      const float x = two_to(-by);
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[t][r] *= x;
-      s_power += by;
-    }
+    if (__ballot(by < -2 || by > 2) != 0ull) scale_down(by);  // uniform
     looked = __ballot(most == 0.f) != 0ull ? -1 : 0;
     scales[lane_id() & 31] = two_to(min(s_power, 127));
   };
@@ -586,7 +602,8 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
     va[0] = transposed(kStages * kTileB + k_tr, wave, 0);
     va[1] = transposed(kStages * kTileB + k_tr, wave, 1);
 
-    // The weighted values, each as a sum of kTerms numbers of the type (relative to 2^v_power).
+    // The weighted values, each as a sum of kTerms numbers of the type (relative to 2^v_power: their column's
+    // largest, so that what an infinity does to s elsewhere changes no bit of them; of states alone s_power).
     T8 terms[kTerms][2];
     int v_power = 0;
     auto split = [&]() {
@@ -604,6 +621,11 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(f[r]));
         v_power = min(max(power_of(max_xor32(top)), -100), 100);
+        if constexpr (kStates) {
+          if (__ballot(v_power > s_power + 15) != 0ull)  // uniform: the values' parts leave fp16's range
+            scale_down(v_power > s_power + 15 ? v_power - 12 - s_power : 0);
+          v_power = s_power;
+        }
         const float by = two_to(-v_power);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -856,7 +878,7 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
     }
     after += taken;
     // of the products in units of s
-    const float add_by = kHalf ? two_to(min(max(v_power - s_power, -126), 127)) : 1.f;
+    const float add_by = kHalf && !kStates ? two_to(min(max(v_power - s_power, -126), 127)) : 1.f;
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
       if (t + 1 < kTiles) {
@@ -869,13 +891,13 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
       for (int ss = 0; ss < 2; ++ss) {
 #pragma unroll
         for (int x = 0; x < kTerms; ++x) {
-          if (kHalf)
+          if (kHalf && !kStates)
             add = mfma_32x32x16(kt[t & 1][ss], terms[x][ss], add);
           else
             s[t] = mfma_32x32x16(kt[t & 1][ss], terms[x][ss], s[t]);
         }
       }
-      if constexpr (kHalf) {
+      if constexpr (kHalf && !kStates) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[t][r] = __builtin_fmaf(add[r], add_by, s[t][r]);
       }

@@ -120,6 +120,36 @@ def test_a_wrong_bound_changes_the_launch_only(most):
             assert_state(state[int(ids[s]), j], end, end_size, 2 * (e - b) + 64, q.dtype)
 
 
+@pytest.mark.parametrize("joined", [False, True])
+@pytest.mark.parametrize("steps", [(14, 0), (0, 14), (0, 7, 14, 3)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_fp16_segments_of_values_that_rise_and_fall(d, steps, joined):
+    """Values of 2^-12 to 2 in their dims, up to 2^14 times larger from one part of a sequence to the next,
+    behind states of nothing, tiny and large ones: the power that a segment's state is taken in follows."""
+    need_gpu()
+    say(f"linear fp16 segments d={d} {steps} joined={joined}")
+    lens, dtype = [400, 350, 290], torch.float16
+    q, k, v, a, cu, state, ids = make(lens, 2, 1, d, dtype, seed=d)
+    q *= 2.0 ** -10
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    v *= (2.0 ** torch.linspace(-12, 1, d, device=DEV))[torch.randperm(d, generator=gen, device=DEV)]
+    for b, e in zip(cu, cu[1:]):
+        for i, step in enumerate(steps):
+            v[b + (e - b) * i // len(steps):b + (e - b) * (i + 1) // len(steps)] *= 2.0 ** (step - 7)
+    state[int(ids[1])] *= 2.0 ** -24
+    state[int(ids[2])] *= 2.0 ** 12
+    for decay in (torch.full_like(a, -0.0005), torch.full_like(a, -0.2)):
+        has, before, now = torch.tensor([0, 1, 1], device=DEV, dtype=torch.uint8), state.clone(), state.clone()
+        o = launch(q, k, v, decay, i32(cu), now, ids, has, 96, joined, True)
+        for s, (b, e) in enumerate(zip(cu, cu[1:])):
+            s0 = before[int(ids[s]), 0] if s > 0 else None
+            rows = q[b:e], k[b:e, 0], v[b:e, 0]
+            ref, size, end, end_size = lo.attend(*rows, float(decay[0]), d ** -0.5, s0)
+            n = 2 * (e - b) + 64
+            assert_out(o[b:e], ref, size, n, small_out(*rows, s0, d ** -0.5))
+            assert_state(now[int(ids[s]), 0], end, end_size, n, dtype, small_state(k[b:e, 0], v[b:e, 0], dtype))
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("h,hk,d", [(16, 16, 64), (24, 8, 64), (16, 16, 128), (24, 8, 128), (8, 8, 256), (24, 8, 256)])
 def test_the_same_call_gives_the_same_bits(h, hk, d, dtype):
