@@ -1005,7 +1005,7 @@ int runs_of(const fa_linear_args& a) {
 
 // Runs of a sequence from which on their states are joined in a launch of their own, which takes 6 to 24
 // us; below, each run adds up what those before it made, 3 us a state at head dim 128, 13 at 256
-// (8 prompts of up to 2,048 tokens, 16 KV heads, in segments of 416: 299 us so, 192 joined; one of
+// (8 prompts of up to 2,048 tokens, 16 KV heads, in segments of 416: 299 us so, 190 joined; one of
 // 131,001 at 128 684 / 637, of 2,560 in five segments 58 both ways).
 int join_runs(int d) { return d == 256 ? 3 : 5; }
 
