@@ -514,7 +514,7 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
   // fp16: a column's largest is at about 8 when it was last looked at: there is room for a growth by 2^12
   // (past it an output is not finite, and the chunk is taken again) and a fall by 2^17 (counted below)
   // before its copies lose bits.
-  int looked = -1;  // tokens since, -1: there was nothing yet
+  int looked = -1;  // tokens since, -1: to be looked at behind this chunk
   float* const scales = shared.scales[kStates ? 0 : part_of] + 32 * wave;
   auto look = [&]() {
     const float most = most_of();
@@ -621,7 +621,9 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(f[r]));
         v_power = min(max(power_of(max_xor32(top)), -100), 100);
-        if constexpr (kStates) {
+        if constexpr (!kStates) {
+          v_power = max_xor32(top) > 0.f ? v_power : -100;
+        } else {
           if (__ballot(v_power > s_power + 15) != 0ull)  // uniform: the values' parts leave fp16's range
             scale_down(v_power > s_power + 15 ? v_power - 12 - s_power : 0);
           v_power = s_power;
@@ -877,6 +879,14 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
       sigma = sigma_then;
     }
     after += taken;
+    if constexpr (kHalf && !kStates) {
+      // A column that was next to nothing when it was last looked at may be 2^121 below these products
+      // (of at most 2^21): s takes their unit then, or they would leave fp32.
+      if (__ballot(v_power - s_power > 64) != 0ull) {  // uniform
+        scale_down(v_power - s_power > 64 ? v_power - s_power : 0);
+        looked = -1;
+      }
+    }
     // of the products in units of s
     const float add_by = kHalf && !kStates ? two_to(min(max(v_power - s_power, -126), 127)) : 1.f;
 #pragma unroll

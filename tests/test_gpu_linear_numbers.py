@@ -1,0 +1,60 @@
+"""Linear attention where its numbers are hard: fp16 states from tiny to large, states over many tokens
+and segments, each against the formula in 64 bits."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from flagattention_amd import _lib, linear
+from oracle import linear_oracle as lo
+from tests._helpers import DEV, need_gpu, say
+from tests._linear import assert_out, assert_state, small_out, small_state
+from tests.test_gpu_linear import i32
+
+pytestmark = pytest.mark.gpu
+
+
+def rows(n, h, d, dtype, seed, gain=1.0):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    return (gain * torch.randn((n, h, d), generator=gen, device=DEV)).to(dtype)
+
+
+def prompt(q, k, v, a, state, scale, segment, joined=True):
+    """One sequence through fa_linear_prompt, in segments of so many tokens; the output."""
+    n, _, d = q.shape
+    hk = k.shape[1]
+    o = torch.full_like(q, math.nan)
+    cu = i32([0, n])
+    args = linear._args(q, k, v, a, state, None, o, 1, scale, int(q.dtype == torch.bfloat16))
+    args.cu_seqlens, args.segment, args.joined = cu.data_ptr(), segment, int(joined)
+    part = torch.full(((n // segment + 1 if segment else 1) * hk * d * d,), math.nan, device=DEV)
+    args.part = part.data_ptr()
+    _lib.check(_lib.load().fa_linear_prompt(ctypes.byref(args),
+                                            torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    return o
+
+
+@pytest.mark.parametrize("segment", [0, 32, 96])
+@pytest.mark.parametrize("h,d", [(1, 64), (4, 64), (1, 128), (2, 128), (1, 256), (2, 256)])
+@pytest.mark.parametrize("a,first", [(-1.0, 1.0), (-0.65, 1.0), (-0.01, 1e-30), (-0.3, 0.0)])
+def test_fp16_large_values_behind_next_to_nothing(a, first, h, d, segment):
+    """A state that falls to nothing, that starts next to nothing, or that is nothing; 96 tokens without
+    values in half of the columns; then one of 20,000 times 20,000, and ordinary ones."""
+    need_gpu()
+    say(f"linear fp16 from nothing a={a} first={first} h={h} d={d} segment={segment}")
+    n, scale = 150, 2.0 ** -20  # brings outputs of 4e8 back into fp16
+    q, k, v = (rows(n, x, d, torch.float16, i) for i, x in enumerate((h, 1, 1)))
+    q *= 2.0 ** -10
+    v[:96, :, ::2] = 0
+    k[96], v[96] = 20000.0, 20000.0
+    state = rows(1, d, d, torch.float32, 3, first)[None]
+    decay = torch.full((1,), a, device=DEV)
+    s0 = state[0, 0].clone()
+    args = q, k[:, 0], v[:, 0]
+    ref, size, end, end_size = lo.attend(*args, float(decay[0]), scale, s0)
+    o = prompt(q, k, v, decay, state, scale, segment)
+    assert bool(torch.isfinite(state).all()), "a state of 4e8 is finite"
+    assert_out(o, ref, size, 2 * n + 64, small_out(*args, s0, scale))
+    assert_state(state[0, 0], end, end_size, 2 * n + 64, q.dtype, small_state(k[:, 0], v[:, 0], q.dtype))
