@@ -620,10 +620,10 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
         float top = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(f[r]));
-        v_power = min(max(power_of(max_xor32(top)), -100), 100);
-        if constexpr (!kStates) {
-          v_power = max_xor32(top) > 0.f ? v_power : -100;
-        } else {
+        top = max_xor32(top);
+        // a column without values asks for no unit
+        v_power = top > 0.f ? min(max(power_of(top), -100), 100) : -120;
+        if constexpr (kStates) {
           if (__ballot(v_power > s_power + 15) != 0ull)  // uniform: the values' parts leave fp16's range
             scale_down(v_power > s_power + 15 ? v_power - 12 - s_power : 0);
           v_power = s_power;

@@ -58,3 +58,22 @@ def test_fp16_large_values_behind_next_to_nothing(a, first, h, d, segment):
     assert bool(torch.isfinite(state).all()), "a state of 4e8 is finite"
     assert_out(o, ref, size, 2 * n + 64, small_out(*args, s0, scale))
     assert_state(state[0, 0], end, end_size, 2 * n + 64, q.dtype, small_state(k[:, 0], v[:, 0], q.dtype))
+
+
+@pytest.mark.parametrize("segment", [0, 64, 96])
+@pytest.mark.parametrize("a", [-0.05, -0.5])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_fp16_values_before_tokens_without_any(d, a, segment):
+    """The last 90 tokens have no values in half of the columns: what the first 60 leave there is small, and
+    as exact as any (the weighted values are held in 22 bits, the rest in fp32)."""
+    need_gpu()
+    say(f"linear fp16 before nothing d={d} a={a} segment={segment}")
+    n = 150
+    q, k, v = (rows(n, 1, d, torch.float16, i) for i in range(3))
+    v[60:, :, ::2] = 0
+    state = torch.zeros((1, 1, d, d), device=DEV)
+    decay = torch.full((1,), a, device=DEV)
+    ref, size, end, end_size = lo.attend(q, k[:, 0], v[:, 0], float(decay[0]), 0.1)
+    o = prompt(q, k, v, decay, state, 0.1, segment)
+    assert_out(o, ref, size, 2 * n + 64, small_out(q, k[:, 0], v[:, 0], None, 0.1))
+    assert_state(state[0, 0], end, end_size, 2 * n + 64, q.dtype)
