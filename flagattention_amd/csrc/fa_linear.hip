@@ -26,7 +26,7 @@
 // meet V and Q, as the output is.  The weighted values that a state takes in are split in three bf16 or
 // two fp16 numbers, which hold 24 and 22 bits: the state is an output in fp32 (two bf16 numbers left
 // it 2e-6 from 64 bits, three 2e-7).  fp16 operands are taken relative to a
-// power of two of the largest (a column's of the state, of the weighted values, of P^T), since states,
+// power of two by the largest (a column's of the state, of the weighted values, of P^T), since states,
 // scores and products of tiny inputs leave its range.
 #include <algorithm>
 #include <cmath>
@@ -75,7 +75,10 @@ namespace {
 
 constexpr int kChunk = 32;
 constexpr int kStages = 3;
-// fp16: the least power of two that operands are relative to.  What is below it by 2^-25 is below half
+// fp16: operands are below 2^kHalfBits of the power of two that they are relative to: its whole range holds
+// what is small beside them (2^-25 of that power is lost, 2^-39 of the largest).
+constexpr int kHalfBits = 15;
+// The least power of two that they are relative to.  What is below it by 2^-25 is below half
 // of the smallest step of the output for any q or v in range.
 constexpr int kLeastPower = -40;
 
@@ -602,8 +605,9 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
     va[0] = transposed(kStages * kTileB + k_tr, wave, 0);
     va[1] = transposed(kStages * kTileB + k_tr, wave, 1);
 
-    // The weighted values, each as a sum of kTerms numbers of the type (relative to 2^v_power: their column's
-    // largest, so that what an infinity does to s elsewhere changes no bit of them; of states alone s_power).
+    // The weighted values, each as a sum of kTerms numbers of the type (fp16: relative to 2^v_power, which
+    // their column's largest is 2^14 of, so that what an infinity does to s elsewhere changes no bit of them;
+    // of states alone s_power).
     T8 terms[kTerms][2];
     int v_power = 0;
     auto split = [&]() {
@@ -622,10 +626,10 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
         for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(f[r]));
         top = max_xor32(top);
         // a column without values asks for no unit
-        v_power = top > 0.f ? min(max(power_of(top), -100), 100) : -120;
+        v_power = top > 0.f ? min(max(power_of(top) - (kStates ? 0 : kHalfBits), -100), 100) : -120;
         if constexpr (kStates) {
-          if (__ballot(v_power > s_power + 15) != 0ull)  // uniform: the values' parts leave fp16's range
-            scale_down(v_power > s_power + 15 ? v_power - 12 - s_power : 0);
+          if (__ballot(v_power > s_power + kHalfBits) != 0ull)  // uniform: the parts leave fp16's range
+            scale_down(v_power > s_power + kHalfBits ? v_power - 12 - s_power : 0);
           v_power = s_power;
         }
         const float by = two_to(-v_power);
@@ -760,7 +764,7 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
           float top = 0.f;
 #pragma unroll
           for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(p[r]));
-          p_power = min(max(power_of(max_xor32(top)), kLeastPower), 100);
+          p_power = min(max(power_of(max_xor32(top)) - kHalfBits, kLeastPower), 100);
         }
         // O^T, relative to 2^p_power
         const float by = kHalf ? __builtin_amdgcn_ldexpf(since, -p_power) : since * (1 << kLift);
@@ -880,8 +884,8 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
     }
     after += taken;
     if constexpr (kHalf && !kStates) {
-      // A column that was next to nothing when it was last looked at may be 2^121 below these products
-      // (of at most 2^21): s takes their unit then, or they would leave fp32.
+      // A column that was next to nothing when it was last looked at may be far below the unit of these
+      // products (of at most 2^37 units): s takes it then, or they would leave fp32.
       if (__ballot(v_power - s_power > 64) != 0ull) {  // uniform
         scale_down(v_power - s_power > 64 ? v_power - s_power : 0);
         looked = -1;

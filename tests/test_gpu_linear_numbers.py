@@ -77,3 +77,47 @@ def test_fp16_values_before_tokens_without_any(d, a, segment):
     o = prompt(q, k, v, decay, state, 0.1, segment)
     assert_out(o, ref, size, 2 * n + 64, small_out(q, k[:, 0], v[:, 0], None, 0.1))
     assert_state(state[0, 0], end, end_size, 2 * n + 64, q.dtype)
+
+
+@pytest.mark.parametrize("segment", [0, 64])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_fp16_small_values_beside_large_ones(d, segment):
+    """Values of 2^-8 between values of up to 2^15, the former with keys of their own: what they leave in the
+    state is off by no more than 2^-36 of the largest value.  (The parts of a weighted value are off by
+    2^-25 of a unit, which the largest is 2^11 of, at least.)"""
+    need_gpu()
+    say(f"linear fp16 small beside large d={d} segment={segment}")
+    n = 150
+    q, k, v = (rows(n, 1, d, torch.float16, i) for i in range(3))
+    k[::2, :, ::2] = 0
+    k[1::2, :, 1::2] = 0
+    v[::2] *= 2.0 ** 12
+    v[1::2] *= 2.0 ** -8
+    state = torch.zeros((1, 1, d, d), device=DEV)
+    decay = torch.full((1,), -0.02, device=DEV)
+    _, _, end, end_size = lo.attend(q, k[:, 0], v[:, 0], float(decay[0]), 1e-4)
+    prompt(q, k, v, decay, state, 1e-4, segment)
+    assert_state(state[0, 0], end, end_size, 2 * n + 64, q.dtype,
+                 2.0 ** -12 * small_state(k[:, 0], v[:, 0], q.dtype))
+
+
+@pytest.mark.parametrize("h,d", [(1, 64), (1, 128), (3, 128), (1, 256)])
+def test_fp16_small_scores_of_large_values(h, d):
+    """Keys of 2^10 with values of 2^-10 between keys of 2^-14 with values of 2^13, which make most of the
+    output: scores are off by 2^-11 of themselves, or by 2^-39 of the largest (2^-25 of a unit, which
+    that is 2^14 of, at least)."""
+    need_gpu()
+    say(f"linear fp16 small scores h={h} d={d}")
+    n = 64
+    q, k, v = (rows(n, x, d, torch.float16, i) for i, x in enumerate((h, 1, 1)))
+    k[::2] *= 2.0 ** 10
+    v[::2] *= 2.0 ** -10
+    k[1::2] *= 2.0 ** -14
+    v[1::2] *= 2.0 ** 13
+    decay = torch.full((1,), -0.02, device=DEV)
+    # chunk after chunk from nothing, so that no state has a part
+    for b in (0, 32):
+        args = q[b:b + 32], k[b:b + 32], v[b:b + 32]
+        ref, size, _, _ = lo.attend(args[0], args[1][:, 0], args[2][:, 0], float(decay[0]), 2.0 ** -3)
+        o = prompt(*args, decay, None, 2.0 ** -3, 0)
+        assert_out(o, ref, size, 32, 2.0 ** -14 * small_out(args[0], args[1][:, 0], args[2][:, 0], None, 2.0 ** -3))
