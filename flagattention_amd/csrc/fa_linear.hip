@@ -448,7 +448,8 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
     for (int i = run.part - 1; i >= 0; --i)
       add_state(part - i * part_step, i == run.part - 1 ? 0.f : fall);
   }
-  // s is kept times 2^-s_power.  fp16: a power for each column (a lane's).
+  // s is kept times 2^-s_power.  fp16: a power for each column (a lane's), kLowest or more.
+  constexpr int kLowest = -126;
   int s_power = kHalf || kStates ? 0 : kLift;
   // The largest of the lane's column that is finite.
   auto most_of = [&]() -> float {
@@ -478,7 +479,6 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
   // fp16 states alone take the values in units of s, whose power follows the largest of them, 2^11 units or
   // more: 2^-25 of a unit is lost.  It starts so low that what the run starts from is at 2^30.  (Products
   // of their own power, added to s: 131,001 tokens of 16 heads, D = 256, 1,867 us for 1,775.)
-  constexpr int kLowest = -126;
   if constexpr (kStates && kHalf) s_power = kLowest;
   if constexpr (kStates) {
     if (from_state) {
@@ -524,7 +524,11 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
     // |s| 2^s_power is at most 2^128: both factors stay in range
     const int by = most > 0.f ? max(power_of(most) - 3, -100 - s_power) : 0;
     if (__ballot(by < -2 || by > 2) != 0ull) scale_down(by);  // uniform
-    looked = __ballot(most == 0.f) != 0ull ? -1 : 0;
+    // A column of zeros is far below its first values, which have it looked at again.  (One that stays so,
+    // as the dims that a head is padded by, costs nothing: 8,192 tokens of one head, 96 of D = 128 filled,
+    // 539 us where such a column was looked at behind every chunk, 504 now.)
+    if (most == 0.f) s_power = kLowest;
+    looked = 0;
     scales[lane_id() & 31] = two_to(min(s_power, 127));
   };
   if (kHalf && !kStates) {
@@ -621,12 +625,11 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
       for (int r = 0; r < 16; ++r)
         f[r] = static_cast<float>(va[r >> 3][r & 7]) * (weight[token(r)] * against);
       if constexpr (kHalf) {
-        float top = 0.f;
+        float top = two_to(kLowest);
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(f[r]));
-        top = max_xor32(top);
-        // a column without values asks for no unit
-        v_power = top > 0.f ? min(max(power_of(top) - (kStates ? 0 : kHalfBits), -100), 100) : -120;
+        // (a column without values asks for no unit: kLowest + kHalfBits is above none)
+        v_power = min(max(power_of(max_xor32(top)) - (kStates ? 0 : kHalfBits), kLowest + kHalfBits), 100);
         if constexpr (kStates) {
           if (__ballot(v_power > s_power + kHalfBits) != 0ull)  // uniform: the parts leave fp16's range
             scale_down(v_power > s_power + kHalfBits ? v_power - 12 - s_power : 0);
@@ -884,8 +887,8 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
     }
     after += taken;
     if constexpr (kHalf && !kStates) {
-      // A column that was next to nothing when it was last looked at may be far below the unit of these
-      // products (of at most 2^37 units): s takes it then, or they would leave fp32.
+      // A column that was next to nothing when it was last looked at, or nothing, may be far below the unit
+      // of these products (of at most 2^37 units): s takes it then, or they would leave fp32.
       if (__ballot(v_power - s_power > 64) != 0ull) {  // uniform
         scale_down(v_power - s_power > 64 ? v_power - s_power : 0);
         looked = -1;

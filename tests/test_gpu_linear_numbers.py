@@ -121,3 +121,25 @@ def test_fp16_small_scores_of_large_values(h, d):
         ref, size, _, _ = lo.attend(args[0], args[1][:, 0], args[2][:, 0], float(decay[0]), 2.0 ** -3)
         o = prompt(*args, decay, None, 2.0 ** -3, 0)
         assert_out(o, ref, size, 32, 2.0 ** -14 * small_out(args[0], args[1][:, 0], args[2][:, 0], None, 2.0 ** -3))
+
+
+@pytest.mark.parametrize("segment", [0, 64])
+@pytest.mark.parametrize("h,d,used", [(2, 64, 48), (1, 128, 96), (4, 128, 80), (1, 256, 192)])
+def test_fp16_heads_padded_with_zeros(h, d, used, segment):
+    """Dims that have nothing keep nothing, and the others are what they are without them; one of them gets
+    its first, tiny value late."""
+    need_gpu()
+    say(f"linear fp16 padded h={h} d={d} used={used} segment={segment}")
+    n, scale = 300, used ** -0.5
+    q, k, v = (rows(n, x, d, torch.float16, i) for i, x in enumerate((h, 1, 1)))
+    for x in (q, k, v):
+        x[..., used:] = 0
+    v[200:, 0, used] = 2.0 ** -12 * v[200:, 0, 0]
+    state = torch.zeros((1, 1, d, d), device=DEV)
+    decay = torch.full((1,), -0.02, device=DEV)
+    ref, size, end, end_size = lo.attend(q, k[:, 0], v[:, 0], float(decay[0]), scale)
+    o = prompt(q, k, v, decay, state, scale, segment)
+    assert_out(o, ref, size, 2 * n + 64, 2.0 ** -10 * small_out(q, k[:, 0], v[:, 0], None, scale))
+    assert_state(state[0, 0], end, end_size, 2 * n + 64, q.dtype, 2.0 ** -12 * small_state(k[:, 0], v[:, 0], q.dtype))
+    assert not bool(o[..., used + 1:].any()) and not bool(state[0, 0, :, used + 1:].any())
+    assert not bool(o[:200, :, used].any()) and not bool(state[0, 0, used:].any())
