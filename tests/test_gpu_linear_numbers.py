@@ -143,3 +143,34 @@ def test_fp16_heads_padded_with_zeros(h, d, used, segment):
     assert_state(state[0, 0], end, end_size, 2 * n + 64, q.dtype, 2.0 ** -12 * small_state(k[:, 0], v[:, 0], q.dtype))
     assert not bool(o[..., used + 1:].any()) and not bool(state[0, 0, :, used + 1:].any())
     assert not bool(o[:200, :, used].any()) and not bool(state[0, 0, used:].any())
+
+
+def long_state(n, d, dtype, a, first, segment, joined):
+    """(error, size) of the state that n tokens of one sign leave behind one of `first`, in 64 bits."""
+    q, k, v = (rows(n, 1, d, dtype, i).abs() for i in range(3))
+    state = rows(1, d, d, torch.float32, 3, first).abs()[None]
+    decay = torch.full((1,), a, device=DEV)
+    left = lo.powers(float(decay[0]), n - 1 - torch.arange(n, device=DEV))[:, None]
+    fall = lo.powers(float(decay[0]), torch.full((1,), n, device=DEV))
+    end = fall * state[0, 0].double() + k[:, 0].double().t() @ (left * v[:, 0].double())
+    prompt(q, k, v, decay, state, 1e-6, segment, joined)
+    return state[0, 0].double() - end, end
+
+
+@pytest.mark.parametrize("segment,joined", [(0, False)])
+@pytest.mark.parametrize("d,dtype", [(64, torch.bfloat16), (64, torch.float16), (128, torch.bfloat16),
+                                     (256, torch.bfloat16), (256, torch.float16)])
+@pytest.mark.parametrize("a", [0.0, -1e-6, -1e-5, -1e-4])
+@pytest.mark.parametrize("first", [1.0, 1e6])
+def test_states_of_many_tokens(first, a, d, dtype, segment, joined):
+    """131,001 tokens of one sign, slow decays, behind a state like them or far above them: every sum is
+    rounded to nearest, so errors of 2^-25 each grow by the square root of their number (6 sigma:
+    2 sqrt(sums) 2^-24 where the state is as large throughout), and nothing is lost always the same
+    way but what the weights are off by (eight roundings or last bits of an exponential)."""
+    need_gpu()
+    say(f"linear long states d={d} {dtype} a={a} first={first} segment={segment} joined={joined}")
+    n = 131001
+    err, end = long_state(n, d, dtype, a, first, segment, joined)
+    sums = n / 32 if segment == 0 else segment / 32 + n / segment
+    assert float((err / end).abs().max()) <= (2 * math.sqrt(sums) + 16) * 2.0 ** -24
+    assert abs(float((err / end).mean())) <= 8 * 2.0 ** -24
