@@ -448,7 +448,8 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
     for (int i = run.part - 1; i >= 0; --i)
       add_state(part - i * part_step, i == run.part - 1 ? 0.f : fall);
   }
-  // s is kept times 2^-s_power.  fp16: a power for each column (a lane's), kLowest or more.
+  // s is kept times 2^-s_power.  fp16: a power for each column (a lane's), kLowest or more; states alone
+  // have no copies in fp16, and 0.
   constexpr int kLowest = -126;
   int s_power = kHalf || kStates ? 0 : kLift;
   // The largest of the lane's column that is finite.
@@ -476,10 +477,6 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
       for (int r = 0; r < 16; ++r) s[t][r] *= x;
     s_power += by;
   };
-  // fp16 states alone take the values in units of s, whose power follows the largest of them, 2^11 units or
-  // more: 2^-25 of a unit is lost.  It starts so low that what the run starts from is at 2^30.  (Products
-  // of their own power, added to s: 131,001 tokens of 16 heads, D = 256, 1,867 us for 1,775.)
-  if constexpr (kStates && kHalf) s_power = kLowest;
   if constexpr (kStates) {
     if (from_state) {
       const int state_at = state_place();
@@ -491,11 +488,6 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
           part[state_at + (32 * t + 16 * (r >> 3) + (r & 7)) * D] = s[t][r];
           s[t][r] *= fall;
         }
-      if constexpr (kHalf) {
-        s_power = 0;
-        const float most = most_of();
-        scale_down(most > 0.f ? max(power_of(most) - 30, kLowest) : kLowest);
-      }
     }
   }
 
@@ -610,8 +602,7 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
     va[1] = transposed(kStages * kTileB + k_tr, wave, 1);
 
     // The weighted values, each as a sum of kTerms numbers of the type (fp16: relative to 2^v_power, which
-    // their column's largest is 2^14 of, so that what an infinity does to s elsewhere changes no bit of them;
-    // of states alone s_power).
+    // their column's largest is 2^14 of, so that what an infinity does to s elsewhere changes no bit of them).
     T8 terms[kTerms][2];
     int v_power = 0;
     auto split = [&]() {
@@ -628,13 +619,7 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
         float top = two_to(kLowest);
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(f[r]));
-        // (a column without values asks for no unit: kLowest + kHalfBits is above none)
-        v_power = min(max(power_of(max_xor32(top)) - (kStates ? 0 : kHalfBits), kLowest + kHalfBits), 100);
-        if constexpr (kStates) {
-          if (__ballot(v_power > s_power + kHalfBits) != 0ull)  // uniform: the parts leave fp16's range
-            scale_down(v_power > s_power + kHalfBits ? v_power - 12 - s_power : 0);
-          v_power = s_power;
-        }
+        v_power = min(max(power_of(max_xor32(top)) - kHalfBits, kLowest + kHalfBits), 100);
         const float by = two_to(-v_power);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -895,7 +880,7 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
       }
     }
     // of the products in units of s
-    const float add_by = kHalf && !kStates ? two_to(min(max(v_power - s_power, -126), 127)) : 1.f;
+    const float add_by = kHalf ? two_to(min(max(v_power - s_power, -126), 127)) : 1.f;
     // A chunk's products are summed by themselves, the least terms first: each added to s alone, what is
     // below its last bit would be lost, and always the same way (bf16, values of one sign behind a state of
     // 1e6, 131,001 tokens: 1.5e-4 of it).  A tile's sums are added while the next tile's are made.
@@ -903,7 +888,7 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
     auto take = [&](int t) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        s[t][r] = kHalf && !kStates ? __builtin_fmaf(add[t & 1][r], add_by, s[t][r]) : s[t][r] + add[t & 1][r];
+        s[t][r] = kHalf ? __builtin_fmaf(add[t & 1][r], add_by, s[t][r]) : s[t][r] + add[t & 1][r];
     };
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {

@@ -174,3 +174,24 @@ def test_states_of_many_tokens(first, a, d, dtype, segment, joined):
     sums = n / 32 if segment == 0 else segment / 32 + n / segment
     assert float((err / end).abs().max()) <= (2 * math.sqrt(sums) + 16) * 2.0 ** -24
     assert abs(float((err / end).mean())) <= 8 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("segment,joined", [(0, False), (96, False), (96, True), (32, True)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_fp16_small_values_before_large_ones(d, segment, joined):
+    """Values of 2^-12, 32 large ones and small ones again, each kind with keys of its own: 22 bits of all."""
+    need_gpu()
+    say(f"linear fp16 small before large d={d} segment={segment} joined={joined}")
+    n = 320
+    q, k, v = (rows(n, 1, d, torch.float16, i) for i in range(3))
+    large = torch.zeros(n, dtype=torch.bool, device=DEV)
+    large[160:192] = True
+    k[large, :, ::2] = 0
+    k[~large, :, 1::2] = 0
+    v[large] *= 2.0 ** 13
+    v[~large] *= 2.0 ** -12
+    state = torch.zeros((1, 1, d, d), device=DEV)
+    decay = torch.full((1,), -0.02, device=DEV)
+    _, _, end, end_size = lo.attend(q, k[:, 0], v[:, 0], float(decay[0]), 1e-4)
+    prompt(q, k, v, decay, state, 1e-4, segment, joined)
+    assert_state(state[0, 0], end, end_size, n, q.dtype)
