@@ -14,13 +14,16 @@ __device__ inline float decay(float a, int n) {
 // 2^-25 of S a step and always the same way (1e-4 after 4,000 steps).  A fast one is a product: there
 // the difference would lose them.
 struct Fall {
-  float by;
-  bool slow;
+  float by, keep;  // S keep + S by, keep is 1 or 0
 };
 __device__ inline Fall fall_of(float a, int n) {
   const float x = a * static_cast<float>(n);
   const bool slow = x > -0.5f;
-  return Fall{n == 0 ? 0.f : slow ? expm1f(x) : expf(x), slow || n == 0};
+  return Fall{n == 0 ? 0.f : slow ? expm1f(x) : expf(x), slow || n == 0 ? 1.f : 0.f};
+}
+// more + S e^(a n): rounded at S's size once.
+__device__ inline float add_fallen(float s, Fall fall, float more) {
+  return __builtin_fmaf(s, fall.keep, __builtin_fmaf(s, fall.by, more));
 }
 
 int check_linear_shape(const fa_linear_args& a);

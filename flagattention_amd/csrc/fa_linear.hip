@@ -425,28 +425,44 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
     return 8 * (lane >> 5) * D + 32 * wave + pi;
   };
   floatx16 s[kTiles] = {};
-  bool from_state = false;
   constexpr float kInit = kHalf || kStates ? 1.f : 1.f / (1 << kLift);
-  auto add_state = [&](const float* from, float fall) {
+  // What the run starts from: its sequence's state, the joined state in front of it, or what every run
+  // before it made.
+  const float* from = part;
+  int states = 0;
+  if (run.part == 0) {
+    states = slot_state && run.has;
+    if (kStates || run.last) from = slot_state;
+  } else if (!kStates) {
+    states = a.joined ? 1 : run.part;
+    from -= (states - 1) * part_step;
+  }
+  const bool from_state = states > 0;
+  if (from_state) {
     const int state_at = state_place();
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        s[t][r] = __builtin_fmaf(
-            s[t][r], fall, kInit * from[state_at + (32 * t + 16 * (r >> 3) + (r & 7)) * D]);
-    from_state = true;
-  };
-  if (run.part == 0) {
-    if (slot_state && run.has)
-      add_state(kStates || run.last ? slot_state : part, 0.f);
-  } else if (kStates) {
-  } else if (a.joined) {
-    add_state(part, 0.f);
-  } else {  // what every run before it made
-    const float fall = decay(log_decay, a.segment);
-    for (int i = run.part - 1; i >= 0; --i)
-      add_state(part - i * part_step, i == run.part - 1 ? 0.f : fall);
+        s[t][r] = kInit * from[state_at + (32 * t + 16 * (r >> 3) + (r & 7)) * D];
+  }
+  if (states > 1) {
+    constexpr int kAtOnce = D == 256 ? 1 : kTiles;  // tiles: more would be spilled
+    const Fall fall = fall_of(log_decay, a.segment);
+    const int state_at = state_place();
+#pragma unroll
+    for (int t0 = 0; t0 < kTiles; t0 += kAtOnce) {
+      const float* next = from;
+      for (int i = 1; i < states; ++i) {
+        next += part_step;
+#pragma unroll
+        for (int t = t0; t < t0 + kAtOnce; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            s[t][r] = add_fallen(s[t][r], fall,
+                                 kInit * next[state_at + (32 * t + 16 * (r >> 3) + (r & 7)) * D]);
+      }
+    }
   }
   // s is kept times 2^-s_power.  fp16: a power for each column (a lane's), kLowest or more; states alone
   // have no copies in fp16, and 0.
@@ -984,22 +1000,23 @@ __global__ __launch_bounds__(256) void join_kernel(const fa_linear_args a, const
   floatx4* at = reinterpret_cast<floatx4*>(a.part) +
                 (static_cast<long long>(start / a.segment + seq + 1) * a.h_kv + hk) * (D * D / 4) +
                 blockIdx.y * 256 + threadIdx.x;
-  const float fall = decay(sload(a.log_decay + hk), a.segment);
-  if (fall == 0.f) return;
+  const Fall fall = fall_of(sload(a.log_decay + hk), a.segment);
+  if (fall.by == 0.f && fall.keep == 0.f) return;
   floatx4 sum = *at;
   for (int i = 1; i < states; i += kAhead) {
-    floatx4 next[kAhead];
+    floatx4 next[kAhead] = {};
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
       if (i + j < states) next[j] = at[(j + 1) * step];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-      if (i + j < states) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) sum[x] = __builtin_fmaf(sum[x], fall, next[j][x]);
-        at[(j + 1) * step] = sum;
-      }
+      for (int x = 0; x < 4; ++x) next[j][x] = add_fallen(j > 0 ? next[j - 1][x] : sum[x], fall, next[j][x]);
     }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (i + j < states) at[(j + 1) * step] = next[j];
+    sum = next[kAhead - 1];  // (another round follows only if all were there)
     at += kAhead * step;
   }
 }

@@ -157,7 +157,7 @@ def long_state(n, d, dtype, a, first, segment, joined):
     return state[0, 0].double() - end, end
 
 
-@pytest.mark.parametrize("segment,joined", [(0, False)])
+@pytest.mark.parametrize("segment,joined", [(0, False), (256, True), (4096, True), (1024, False)])
 @pytest.mark.parametrize("d,dtype", [(64, torch.bfloat16), (64, torch.float16), (128, torch.bfloat16),
                                      (256, torch.bfloat16), (256, torch.float16)])
 @pytest.mark.parametrize("a", [0.0, -1e-6, -1e-5, -1e-4])
