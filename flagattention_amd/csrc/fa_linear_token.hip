@@ -76,7 +76,7 @@ __global__ __launch_bounds__(kThreads) void linear_token_kernel(const fa_linear_
         const float kr = ks[row0 + i * kRows];
 #pragma unroll
         for (int x = 0; x < 4; ++x)
-          s[i][x] = __builtin_fmaf(kr, vs[x], __builtin_fmaf(s[i][x], fall.by, fall.keep * s[i][x]));
+          s[i][x] = add_fallen(s[i][x], fall, kr * vs[x]);  // (an exact product)
         *reinterpret_cast<floatx4*>(state + (row0 + i * kRows) * D) = s[i];
       }
     }

@@ -6,6 +6,7 @@ import math
 import pytest
 import torch
 
+import flag_attn
 from flagattention_amd import _lib, linear
 from oracle import linear_oracle as lo
 from tests._helpers import DEV, need_gpu, say
@@ -195,3 +196,24 @@ def test_fp16_small_values_before_large_ones(d, segment, joined):
     _, _, end, end_size = lo.attend(q, k[:, 0], v[:, 0], float(decay[0]), 1e-4)
     prompt(q, k, v, decay, state, 1e-4, segment, joined)
     assert_state(state[0, 0], end, end_size, n, q.dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("a", [0.0, -1e-6, -1e-5, -1e-3])
+def test_states_of_many_single_tokens(a, dtype):
+    """4,000 steps of decode, k and v of one sign behind states of 1000: a step rounds a state once at its
+    size (to nearest: 2^-24 of it at most, an error of 2^-24 / sqrt(3) each, 6 sigma over the steps), and
+    nothing drifts."""
+    need_gpu()
+    say(f"linear many single tokens a={a} {dtype}")
+    n, d = 4000, 64
+    q, k, v = (rows(n, 1, d, dtype, i).abs() for i in range(3))
+    state = torch.full((1, 1, d, d), 1000.0, device=DEV)
+    ref, decay = state[0, 0].double(), torch.full((1,), a, device=DEV)
+    step = torch.exp(decay.double())
+    for t in range(n):
+        flag_attn.linear_attention_decode(q[t:t + 1], k[t:t + 1], v[t:t + 1], decay, state)
+        ref = ref * step + k[t, 0].double()[:, None] * v[t, 0].double()
+    err = (state[0, 0].double() - ref) / ref
+    assert float(err.abs().max()) <= 6 / math.sqrt(3) * math.sqrt(n) * 2.0 ** -24
+    assert abs(float(err.mean())) <= 8 * 2.0 ** -24
