@@ -1003,6 +1003,38 @@ bool rows_apart(const at::Tensor& t, int dims) {
   return true;
 }
 
+// The rows of a view: (stride, size) of the dims in front of the last, the largest stride first, those of
+// one row left out.
+struct Rows {
+  int64_t stride[3], size[3], width;
+  int first = 0, last = 0;
+  explicit Rows(const at::Tensor& t) : width(t.size(t.dim() - 1)) {
+    for (int64_t i = 0; i + 1 < t.dim(); ++i) {
+      if (t.size(i) <= 1) continue;
+      int at = last++;
+      for (; at > 0 && stride[at - 1] < t.stride(i); --at)
+        stride[at] = stride[at - 1], size[at] = size[at - 1];
+      stride[at] = t.stride(i), size[at] = t.size(i);
+    }
+  }
+  int64_t reach() const {
+    int64_t sum = width;
+    for (int i = first; i < last; ++i) sum += (size[i] - 1) * stride[i];
+    return sum;
+  }
+  int64_t step() const { return first < last ? stride[first] : 0; }
+};
+bool rows_meet(int64_t delta, Rows x, Rows y) {
+  if (delta >= x.reach() || delta + y.reach() <= 0) return false;
+  const int64_t step = std::max(x.step(), y.step());
+  if (step == 0) return true;
+  if (x.step() == step) ++x.first;
+  if (y.step() == step) ++y.first;
+  if (x.reach() > step || y.reach() > step) return true;
+  delta = (delta % step + step) % step;
+  return rows_meet(delta, x, y) || rows_meet(delta - step, x, y);
+}
+
 // Whether the bytes from the first element to the last of the two meet (rotary._reach_into).
 bool reach_into(const at::Tensor& x, const at::Tensor& y) {
   uintptr_t at[2][2];
@@ -1016,6 +1048,13 @@ bool reach_into(const at::Tensor& x, const at::Tensor& y) {
   return at[0][0] < at[1][1] && at[1][0] < at[0][1];
 }
 
+// Whether two views of one type, each of rows that lie apart, may share an element (rotary._meet).
+bool meet(const at::Tensor& x, const at::Tensor& y) {
+  if (!reach_into(x, y)) return false;
+  const int64_t bytes = static_cast<const char*>(y.data_ptr()) - static_cast<const char*>(x.data_ptr());
+  return bytes % x.element_size() != 0 || rows_meet(bytes / x.element_size(), Rows(x), Rows(y));
+}
+
 // rotary(q, k, positions, inv_freq, sections, mixed_sections, adjacent_pairs, inplace): (q, k)
 PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -1026,7 +1065,7 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!q || !k || !to_bool(args[7], &inplace) ||
       !rotary_of(*q, *k, args[2], args[3], args[4], args[5], args[6], &a))
     return none();
-  if (inplace && (!rows_apart(*q, 2) || !rows_apart(*k, 2) || q->data_ptr() == k->data_ptr()))
+  if (inplace && (!rows_apart(*q, 2) || !rows_apart(*k, 2) || meet(*q, *k)))
     return none();
   const c10::Device device = q->device();
   at::Tensor q_out, k_out;
@@ -1067,7 +1106,7 @@ PyObject* rotary_cache(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       kc->size(3) != a.d || kc->scalar_type() != q->scalar_type() ||
       vc->scalar_type() != q->scalar_type() || kc->size(0) < 1 || kc->size(0) > INT32_MAX ||
       kc->size(2) < 1 || kc->size(2) > INT32_MAX || kc->stride(3) != 1 || vc->stride(3) != 1 ||
-      !rows_apart(*kc, 3) || !rows_apart(*vc, 3) || kc->data_ptr() == vc->data_ptr())
+      !rows_apart(*kc, 3) || !rows_apart(*vc, 3) || meet(*kc, *vc))
     return none();
   if ((slots->scalar_type() != at::kInt && slots->scalar_type() != at::kLong) || slots->dim() != 1 ||
       slots->size(0) != a.tokens || !slots->is_contiguous())

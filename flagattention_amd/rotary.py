@@ -76,6 +76,35 @@ def _reach_into(x, y) -> bool:
     return a[0] < b[1] and b[0] < a[1]
 
 
+def _meet(x, y) -> bool:
+    """Whether two views of one type may share an element: no where their spans lie apart, or their rows
+    within every stride that they have in common (heads of one packed row, caches block by block).  Each
+    view's own rows lie apart (_apart)."""
+    if not _reach_into(x, y):
+        return False
+    delta, off = divmod(y.data_ptr() - x.data_ptr(), x.element_size())
+    if off != 0:
+        return True
+
+    def reach(dims):
+        return x.shape[-1] + sum((n - 1) * s for s, n in dims)
+
+    def meet(delta, xs, ys):  # y starts delta elements behind x; (stride, size) of the rows, outermost first
+        if delta >= reach(xs) or delta + reach(ys) <= 0:
+            return False
+        if not xs and not ys:
+            return True
+        step = max(d[0][0] for d in (xs, ys) if d)
+        xs, ys = (d[1:] if d and d[0][0] == step else d for d in (xs, ys))
+        if max(reach(xs), reach(ys)) > step:
+            return True
+        # what is left of each fits a step: only the copies next to each other can meet
+        return meet(delta % step, xs, ys) or meet(delta % step - step, xs, ys)
+
+    return meet(delta, *(sorted(((s, n) for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1),
+                                reverse=True) for t in (x, y)))
+
+
 def _one_device(*tensors):
     _require(all(t.is_cuda and t.device == tensors[0].device for t in tensors),
              "all tensors must be CUDA (HIP) tensors on one device")
@@ -146,7 +175,7 @@ def rotary_embedding(
     if inplace:
         _require(all(x.stride(2) == 1 and _apart(x, (0, 1)) for x in (q, k)),
                  "q and k must have contiguous rows that do not overlap")
-        _require(q.data_ptr() != k.data_ptr() or q.numel() == 0, "q and k overlap")
+        _require(not _meet(q, k), "q and k overlap")
     _one_device(q, k, positions, inv_freq)
     if inplace:
         q_out, k_out = q, k
@@ -212,7 +241,7 @@ def rotary_cache_kv(
              "the cache is empty or has too many blocks")
     _require(all(c.stride(3) == 1 and _apart(c, (0, 1, 2)) for c in (key_cache, value_cache)),
              "rows of the cache must be contiguous and not overlap")
-    _require(key_cache.data_ptr() != value_cache.data_ptr(), "key_cache and value_cache overlap")
+    _require(not _meet(key_cache, value_cache), "key_cache and value_cache overlap")
     _require(not any(_reach_into(x, c) for x in (q, k, v) for c in (key_cache, value_cache)),
              "q, k and v must not lie in the caches")
     _require(slot_mapping.dim() == 1 and slot_mapping.shape[0] == tokens
