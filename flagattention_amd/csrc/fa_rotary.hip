@@ -1,5 +1,5 @@
 // Rotary positions for gfx950: q and k turned by the angles of their tokens' positions (of up to four
-// axes), into new rows, in place, or k and v into a paged cache.
+// axes), into new rows, in place, or k and v into a paged cache (and k into new rows beside it).
 //
 // A thread takes one unit of a token -- kVec pairs, whose two pieces are kVec dims each -- over a few
 // heads: it works the sines out once and uses them for each.  The angle of a pair is a product in
@@ -8,7 +8,10 @@
 //
 // Bound by the rows, read and written once: 16,384 tokens of 64 heads and 8 of k and v, D = 128, into a
 // cache 131 us, 20,001 of 16 and 16, D = 256, 125 us, 5.1 and 5.3 TB/s (a large copy: 5.1); 8,192 of 32
-// and 8 35 us, 4.8.  A few tokens take 3 to 4.4 us, the launch and two trips to memory.
+// and 8 35 to 39 us, 4.8 to 4.3.  A few tokens take 3 to 4.4 us, the launch and two trips to memory.  The turned k beside the cache is
+// k's rows once more (16,384 tokens of 64 heads and 8: 129 us without it, 135 with it, 244 by two calls).
+#include <algorithm>
+
 #include "fa_common.h"
 #include "fa_divide.h"
 #include "flagattention_amd_linear.h"
@@ -22,7 +25,7 @@ struct RotaryPlan {
   Divisor units, chunks;  // units of a row; threads that share a token's rows
   Divisor axes, block;    // block: where a slot fits 31 bits
   bool small_slots;
-  int rows;               // rows of a token: q's heads, k's, and with caches v's
+  int rows;               // rows of a token: q's heads, k's, with caches v's, and k's for k_out
   int threads;
 };
 
@@ -83,6 +86,10 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const fa_rotary_args a
       } else {
         dst[n] = static_cast<T*>(a.k_out) + t * a.k_out_stride_t + h * a.k_out_stride_h;
       }
+    } else if (row >= a.h_q + 2 * a.h_kv) {
+      const int h = row - a.h_q - 2 * a.h_kv;
+      src[n] = static_cast<const T*>(a.k) + t * a.k_stride_t + h * a.k_stride_h;
+      dst[n] = static_cast<T*>(a.k_out) + t * a.k_out_stride_t + h * a.k_out_stride_h;
     } else {
       const int h = row - a.h_q - a.h_kv;
       src[n] = static_cast<const T*>(a.v) + t * a.v_stride_t + h * a.v_stride_h;
@@ -181,6 +188,10 @@ bool rows_of_16(const void* p, int64_t s0, int64_t s1) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s0 % 8 == 0 && s1 % 8 == 0;
 }
 
+int rows_of(const fa_rotary_args& a) {
+  return a.h_q + a.h_kv * (!a.key_cache ? 1 : a.k_out ? 3 : 2);
+}
+
 // Rows of a thread: one while the launch leaves the card idle, four to share the sines then.  A thread's
 // rows come one after the other (three of 10 heads, D = 64: 4.8 us with four, 3.0 with one).
 constexpr int kFewThreads = 1 << 18;
@@ -201,7 +212,7 @@ void launch(const fa_rotary_args& a, hipStream_t stream) {
   // in place the dims that do not turn are there already
   const bool rest = a.key_cache || (a.h_q > 0 ? a.q != a.q_out : a.k != a.k_out);
   const int units = a.pairs / kVec + (rest ? cdiv(a.d - 2 * a.pairs, 2 * kVec) : 0);
-  plan.rows = a.h_q + a.h_kv * (a.key_cache ? 2 : 1);
+  plan.rows = rows_of(a);
   plan.units = divisor(units);
   plan.axes = divisor(a.axes);
   plan.small_slots = a.key_cache && a.num_blocks * a.block_size <= INT32_MAX;
@@ -249,6 +260,7 @@ extern "C" int fa_rotary(const fa_rotary_args* args, void* stream) {
                  "NULL pointer");
     FA_CHECK_ARG(a.num_blocks >= 1 && a.num_blocks <= INT32_MAX && a.block_size >= 1,
                  "the cache has no blocks or too many");
+    FA_CHECK_ARG(!a.k_out || a.k_out != a.k, "k is read for the cache while it is turned in place");
   } else {
     FA_CHECK_ARG(a.tokens == 0 || a.h_kv == 0 || (a.k && a.k_out), "NULL pointer");
     FA_CHECK_ARG(a.h_q == 0 || a.h_kv == 0 || (a.q == a.q_out) == (a.k == a.k_out),
@@ -256,9 +268,10 @@ extern "C" int fa_rotary(const fa_rotary_args* args, void* stream) {
   }
   if (a.tokens == 0) return FA_OK;
   // a thread per unit and heads: ids of 31 bits
-  FA_CHECK_ARG(static_cast<int64_t>(a.tokens) * (a.h_q + 2 * a.h_kv) * a.d < int64_t{1} << 40 &&
-                   static_cast<int64_t>(a.tokens) * ((a.h_q + 2 * a.h_kv + 3) / 4) *
-                           (a.d / 2 + 1) < INT32_MAX - fa::kThreads,
+  const int rows = std::max(fa::rows_of(a), a.h_q + 2 * a.h_kv);
+  FA_CHECK_ARG(static_cast<int64_t>(a.tokens) * rows * a.d < int64_t{1} << 40 &&
+                   static_cast<int64_t>(a.tokens) * ((rows + 3) / 4) * (a.d / 2 + 1) <
+                       INT32_MAX - fa::kThreads,
                "too many tokens or heads");
   bool wide = a.pairs % 8 == 0 && a.d % 8 == 0;
   if (a.h_q > 0)
@@ -269,7 +282,7 @@ extern "C" int fa_rotary(const fa_rotary_args* args, void* stream) {
     wide = wide && fa::rows_of_16(a.v, a.v_stride_t, a.v_stride_h) &&
            fa::rows_of_16(a.key_cache, a.kc_stride_h, a.kc_stride_t) && a.kc_stride_0 % 8 == 0 &&
            fa::rows_of_16(a.value_cache, a.vc_stride_h, a.vc_stride_t) && a.vc_stride_0 % 8 == 0;
-  if (a.h_kv > 0 && !cache)
+  if (a.h_kv > 0 && a.k_out)
     wide = wide && fa::rows_of_16(a.k_out, a.k_out_stride_t, a.k_out_stride_h);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (a.dtype == 1)

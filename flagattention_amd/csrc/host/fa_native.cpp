@@ -987,6 +987,19 @@ void rotary_out(fa_rotary_args* a, const at::Tensor& q) {
   a->q_out_stride_t = q.stride(0);
   a->q_out_stride_h = q.stride(1);
 }
+void rotary_key_out(fa_rotary_args* a, const at::Tensor& k) {
+  a->k_out = k.data_ptr();
+  a->k_out_stride_t = k.stride(0);
+  a->k_out_stride_h = k.stride(1);
+}
+PyObject* both_of(at::Tensor first, at::Tensor second) {
+  PyObject* const x = THPVariable_Wrap(std::move(first));
+  PyObject* const y = THPVariable_Wrap(std::move(second));
+  PyObject* const both = x && y ? PyTuple_Pack(2, x, y) : nullptr;
+  Py_XDECREF(x);
+  Py_XDECREF(y);
+  return both;
+}
 // No two rows share an element (rotary._apart): the last dim is contiguous.
 bool rows_apart(const at::Tensor& t, int dims) {
   int order[3] = {0, 1, 2};
@@ -1075,26 +1088,19 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     q_out = inplace ? *q : make(q->sizes(), q->scalar_type(), device);
     k_out = inplace ? *k : make(k->sizes(), k->scalar_type(), device);
     rotary_out(&a, q_out);
-    a.k_out = k_out.data_ptr();
-    a.k_out_stride_t = k_out.stride(0);
-    a.k_out_stride_h = k_out.stride(1);
+    rotary_key_out(&a, k_out);
     check(fa_rotary(&a, stream_of(device)));
   }
-  if (inplace) return PyTuple_Pack(2, args[0], args[1]);
-  PyObject* const x = THPVariable_Wrap(std::move(q_out));
-  PyObject* const y = THPVariable_Wrap(std::move(k_out));
-  PyObject* const both = x && y ? PyTuple_Pack(2, x, y) : nullptr;
-  Py_XDECREF(x);
-  Py_XDECREF(y);
-  return both;
+  return inplace ? PyTuple_Pack(2, args[0], args[1]) : both_of(std::move(q_out), std::move(k_out));
   END_HANDLE_TH_ERRORS
 }
 
 // rotary_cache(q, k, v, positions, inv_freq, key_cache, value_cache, slot_mapping, sections,
-//              mixed_sections, adjacent_pairs): q
+//              mixed_sections, adjacent_pairs[, return_key]): q, or (q, k)
 PyObject* rotary_cache(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 11) return none();
+  bool with_key = false;
+  if (nargs != 11 && (nargs != 12 || !to_bool(args[11], &with_key))) return none();
   const at::Tensor *q = plain(args[0]), *k = plain(args[1]), *v = plain(args[2]),
                    *kc = plain(args[5]), *vc = plain(args[6]), *slots = plain(args[7]);
   fa_rotary_args a = {};
@@ -1111,17 +1117,24 @@ PyObject* rotary_cache(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if ((slots->scalar_type() != at::kInt && slots->scalar_type() != at::kLong) || slots->dim() != 1 ||
       slots->size(0) != a.tokens || !slots->is_contiguous())
     return none();
+  if (with_key && static_cast<int64_t>(a.tokens) * cdiv(a.h_q + 3 * a.h_kv, 4) * (a.d / 2 + 1) >=
+                      (int64_t{1} << 31) - 1024)
+    return none();
   const c10::Device device = q->device();
   for (const at::Tensor* t : {v, kc, vc, slots})
     if (t->device() != device) return none();
   for (const at::Tensor* t : {q, k, v})
     if (reach_into(*t, *kc) || reach_into(*t, *vc)) return none();
-  at::Tensor q_out;
+  at::Tensor q_out, k_out;
   {
     NoGil nogil;
     c10::DeviceGuard guard(device);
     q_out = make(q->sizes(), q->scalar_type(), device);
     rotary_out(&a, q_out);
+    if (with_key) {
+      k_out = make(k->sizes(), k->scalar_type(), device);
+      rotary_key_out(&a, k_out);
+    }
     a.v = v->data_ptr();
     a.v_stride_t = v->stride(0);
     a.v_stride_h = v->stride(1);
@@ -1139,7 +1152,7 @@ PyObject* rotary_cache(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     a.slots64 = slots->scalar_type() == at::kLong;
     check(fa_rotary(&a, stream_of(device)));
   }
-  return THPVariable_Wrap(std::move(q_out));
+  return with_key ? both_of(std::move(q_out), std::move(k_out)) : THPVariable_Wrap(std::move(q_out));
   END_HANDLE_TH_ERRORS
 }
 

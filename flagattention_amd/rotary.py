@@ -6,7 +6,8 @@ has one position, or one on each of up to four axes (time, height, width of imag
 pair takes one axis, by the ``sections``.
 
 ``rotary_embedding`` turns q and k, for any of the attention operators here; ``rotary_cache_kv`` turns
-q and writes the turned k and v into the paged 16-bit cache that ``paged_attention`` reads.  Angles
+q and writes the turned k and v into the paged 16-bit cache that ``paged_attention`` reads (and returns
+the turned k for attention over a packed prompt).  Angles
 are worked out in 64 bits from the positions as they are, so there is no table and no last position.
 Forward only.
 
@@ -15,7 +16,7 @@ Work is queued on the current stream; argument errors raise ``ArgumentError`` be
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Sequence, Tuple
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -127,14 +128,14 @@ def _args(q, k, q_out, positions, inv_freq, sections, mixed_sections, adjacent_p
         adjacent=int(bool(adjacent_pairs)), pos64=int(positions.dtype == torch.int64), dtype=code)
 
 
-def _check_heads(q, k):
+def _check_heads(q, k, kv_rows=2):
     _require(q.dim() == 3 and k.dim() == 3 and k.shape[0] == q.shape[0]
              and k.shape[2] == q.shape[2], "q and k must be [num_tokens, heads, head_dim]")
     _require(1 <= q.shape[1] <= 65535 and 1 <= k.shape[1] <= 65535, "no heads or too many")
     code = _dtype_code(q.dtype)
     _require(k.dtype == q.dtype, "q and k dtypes differ")
     # a thread for at least a pair of four rows; what is taken 16 bytes at a time needs an eighth
-    _require(q.shape[0] * -(-(q.shape[1] + 2 * k.shape[1] + 3) // 4) * (q.shape[2] // 2 + 1)
+    _require(q.shape[0] * -(-(q.shape[1] + kv_rows * k.shape[1] + 3) // 4) * (q.shape[2] // 2 + 1)
              < (1 << 31) - 1024, "too many tokens or heads")
     return code
 
@@ -207,7 +208,8 @@ def rotary_cache_kv(
     sections: Optional[Sequence[int]] = None,
     mixed_sections: bool = False,
     adjacent_pairs: bool = False,
-) -> torch.Tensor:
+    return_key: bool = False,
+) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """Turn q and k by their tokens' positions, and write k and v into the paged cache (in place).
 
     q, k, positions, inv_freq, sections, mixed_sections, adjacent_pairs
@@ -218,17 +220,18 @@ def rotary_cache_kv(
     slot_mapping  int32 / int64 [T]: block * block_size + row of each token; negative slots (padding
                   tokens) and slots past the cache are skipped.  The slots of one call must differ:
                   rows that two tokens write are undefined
+    return_key    return the turned k too, also of tokens without a slot
 
-    Returns the turned ``q``, ready for ``paged_attention`` or, with the packed k and v of a prompt,
-    ``flash_attention_varlen``.
+    Returns the turned ``q``, ready for ``paged_attention``; with ``return_key`` ``(q, k)``, both turned,
+    as ``flash_attention_varlen`` takes them with the packed v of a prompt.
     """
     fast = _lib.native()
     if fast is not None:
         done = fast.rotary_cache(q, k, v, positions, inv_freq, key_cache, value_cache, slot_mapping,
-                                 sections, mixed_sections, adjacent_pairs)
+                                 sections, mixed_sections, adjacent_pairs, return_key)
         if done is not None:
             return done
-    code = _check_heads(q, k)
+    code = _check_heads(q, k, 3 if return_key else 2)
     _require(v.shape == k.shape and v.dtype == k.dtype, "k and v shapes or dtypes differ")
     tokens, _, d = q.shape
     _, sections = _check_turn(tokens, d, positions, inv_freq, sections, mixed_sections)
@@ -250,10 +253,14 @@ def rotary_cache_kv(
     _one_device(q, k, v, positions, inv_freq, key_cache, value_cache, slot_mapping)
     q, k, v = _dense(q), _dense(k), _dense(v)
     q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if return_key else None
     if tokens > 0:
         slots = slot_mapping.contiguous()
         args = _args(q, k, q_out, positions, inv_freq, sections, mixed_sections, adjacent_pairs,
                      code)
+        if return_key:
+            args.k_out, args.k_out_stride_t, args.k_out_stride_h = (k_out.data_ptr(), k_out.stride(0),
+                                                                    k_out.stride(1))
         args.v, args.v_stride_t, args.v_stride_h = v.data_ptr(), v.stride(0), v.stride(1)
         args.key_cache, args.value_cache = key_cache.data_ptr(), value_cache.data_ptr()
         args.kc_stride_0, args.kc_stride_h, args.kc_stride_t = key_cache.stride()[:3]
@@ -264,4 +271,4 @@ def rotary_cache_kv(
         with torch.cuda.device(q.device):
             _lib.check(lib.fa_rotary(ctypes.byref(args),
                                      torch.cuda.current_stream(q.device).cuda_stream))
-    return q_out
+    return (q_out, k_out) if return_key else q_out

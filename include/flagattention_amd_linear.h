@@ -24,8 +24,8 @@ extern "C" {
  * q and k (and v) are [tokens][heads][d], element strides, last dimension contiguous; k may be NULL
  * with h_kv 0.  Outputs may be the inputs themselves (the same pointer and strides), but may not
  * overlap them otherwise.  With key_cache, k and v go to row slots[t] % block_size of block
- * slots[t] / block_size of caches [num_blocks][h_kv][block_size][d] instead of k_out; tokens
- * whose slot is negative or past the cache are skipped.  fp16 or bf16; any alignment (rows
+ * slots[t] / block_size of caches [num_blocks][h_kv][block_size][d], and k to k_out only where
+ * that is not NULL (nor k itself); tokens whose slot is negative or past the cache are skipped there.  fp16 or bf16; any alignment (rows
  * and strides of 16 bytes with pairs and d multiples of 8 are taken 16 bytes at a time).
  */
 typedef struct fa_rotary_args {
@@ -35,7 +35,7 @@ typedef struct fa_rotary_args {
   int64_t k_stride_t, k_stride_h;
   void* q_out;
   int64_t q_out_stride_t, q_out_stride_h;
-  void* k_out; /* without caches */
+  void* k_out; /* with caches NULL, or where k goes too */
   int64_t k_out_stride_t, k_out_stride_h;
   const void* v; /* with caches */
   int64_t v_stride_t, v_stride_h;
