@@ -137,20 +137,6 @@ __device__ inline unsigned int upper_halves(float x, float y) {
   return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
 }
 
-// Largest of a wave's values.
-template <int kCtrl>
-__device__ inline float dpp_f32(float x) {
-  return __uint_as_float(static_cast<unsigned int>(__builtin_amdgcn_update_dpp(
-      0, static_cast<int>(__float_as_uint(x)), kCtrl, 0xF, 0xF, false)));
-}
-__device__ inline float wave_max(float x) {
-  x = fmaxf(x, dpp_f32<0xB1>(x));   // quad_perm [1, 0, 3, 2]
-  x = fmaxf(x, dpp_f32<0x4E>(x));   // quad_perm [2, 3, 0, 1]
-  x = fmaxf(x, dpp_f32<0x141>(x));  // row_half_mirror
-  x = fmaxf(x, dpp_f32<0x140>(x));  // row_mirror
-  return max_xor32(max_xor16(x));
-}
-
 // Power of two above |x|, 0 for 0, infinities and NaN.
 __device__ inline int power_of(float x) { return __builtin_amdgcn_frexp_expf(x); }
 __device__ inline float two_to(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
@@ -311,6 +297,7 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
   constexpr bool kKeepQ = D == 64;  // from the scores to S^T Q^T, else it is read twice
   constexpr bool kShare = !kStates && shares(D, kOne);
   static_assert(kCopies * kTiles * 1024 == kTileB, "whole copies per wave");
+  static_assert(!kShare || kSplit == 1, "the waves that share scores meet at a barrier in each item");
   unsigned char* const bufs = shared.bufs;  // [k, v, q][stage]
   float* const seen = shared.seen;
   float* const left_of = shared.left_of;
@@ -813,10 +800,7 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
           }
         }
       };
-      if (mine)
-        attend(IntTag<0>{});
-      else if (kShare)
-        sync();
+      if (mine) attend(IntTag<0>{});  // (the waves that share scores are of one head)
       // An infinity or a NaN among the scores or in v reaches the tokens before its own, through
       // weights of 0, and the outputs of its own: such a chunk is taken again.
       floatx4 trace = {0.f, 0.f, 0.f, 0.f};
