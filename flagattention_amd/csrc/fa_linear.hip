@@ -5,7 +5,8 @@
 // tokens, counted from 0, with S the state before it:
 //   O^T = (S^T Q^T) diag(scale e^{a (i+1)}) + V^T P^T,  P^T[j, i] = scale e^{a (i-j)} (K Q^T)[j, i], j <= i
 //   S'  = e^{a c} S + K^T diag(e^{a (c-1-j)}) V
-// No factor is above 1 for a decay (a <= 0), however long the chunk or fast the decay.
+// No weight is above 1 for a decay (a <= 0), however long the chunk or fast the decay; S is kept by what
+// it has fallen since it was last brought up, at most 16, and what meets it is taken that much larger.
 //
 // Wave w owns columns 32w .. 32w + 31 of S, in fp32 in its accumulators for the whole sequence, and the
 // same dims of the output; D / 32 waves.  Products are MFMA 32x32x16.  S leaves the accumulators as the
@@ -13,21 +14,25 @@
 // are the 8 dims of its part of a step).  Every wave needs the whole of P^T.  At head dim 256, and at 128
 // without groups, four waves work out 16 x 16 of it each and hand it round in LDS; each wave for itself
 // would make it a fifth of its products and read K and Q whole again (16 x 1,024 tokens of 16 heads,
-// D = 256: 200 us so, 179 shared; 32 heads, D = 128, fp16: 143 / 137; a lone sequence of one head waits
-// for the exchange, 410 / 441 at 8,192 tokens; two heads at once at D = 128: 227 / 233, so not there).
+// D = 256: 200 us so, 179 shared, when it was made so; 32 heads, D = 128, fp16: 143 / 137; a lone sequence
+// of one head waits for the exchange, 410 / 441 at 8,192 tokens; two heads at once at D = 128: 227 / 233,
+// so not there).
 //
-// Bound by q, k, v and out where the card is full (16 x 1,024 tokens of 32 heads, D = 128: 129 us, 117
-// at the rate of a copy; of 64, D = 64: 145, 111), by a chunk's chain of products where it is not: 1.2,
-// 1.7 and 3.4 us in bf16 at D = 64, 128, 256 for a lone sequence of one head.  At D = 256 one work-group
-// fits a CU and the chain shows in full launches too (of 16: 179, 131).  Inputs come three chunks deep
+// Bound by q, k, v and out where the card is full (16 x 1,024 tokens of 32 heads, D = 128: 132 us, 117
+// at the rate of a copy; of 64, D = 64: 145, 111), by a chunk's chain of products where it is not: 1.3,
+// 1.8 and 3.7 us in bf16 at D = 64, 128, 256 for a lone sequence of one head.  At D = 256 one work-group
+// fits a CU and the chain shows in full launches too (of 16: 190, 131).  Inputs come three chunks deep
 // into LDS, so that no chunk waits for memory.
 //
 // Rounding: scores, sums and states are fp32.  P and the state's copy are rounded to the input type to
-// meet V and Q, as the output is.  The weighted values that a state takes in are split in three bf16 or
-// two fp16 numbers, which hold 24 and 22 bits: the state is an output in fp32 (two bf16 numbers left
-// it 2e-6 from 64 bits, three 2e-7).  fp16 operands are taken relative to a
-// power of two by the largest (a column's of the state, of the weighted values, of P^T), since states,
-// scores and products of tiny inputs leave its range.
+// meet V and Q, which costs as much as rounding the output does: 2.1e-3 from 64 bits in bf16 and 2.5e-4 to
+// 2.9e-4 in fp16, 1.7e-3 and 2.1e-4 without.  (Two numbers of the type for each would save that: 10 to
+// 14% more time at D = 128, 20 to 26% at 256, where the state's are 360 instructions of a lane and chunk
+// more; for P alone 1 to 4%.)  The weighted values that a state takes in are split in three bf16 or two
+// fp16 numbers, which hold 24 and 22 bits: the state is an output in fp32 (two bf16 numbers left it 2e-6
+// from 64 bits, three 2e-7).  fp16 operands are taken relative to a power of two by the largest (a
+// column's of the state, of the weighted values, of P^T), since states, scores and products of tiny inputs
+// leave its range.
 #include <algorithm>
 #include <cmath>
 
@@ -75,8 +80,8 @@ namespace {
 
 constexpr int kChunk = 32;
 constexpr int kStages = 3;
-// fp16: operands are below 2^kHalfBits of the power of two that they are relative to: its whole range holds
-// what is small beside them (2^-25 of that power is lost, 2^-39 of the largest).
+// fp16: weighted values and scores are below 2^kHalfBits of the power of two that they are relative to: its
+// whole range holds what is small beside them (2^-25 of that power is lost, 2^-39 of the largest).
 constexpr int kHalfBits = 15;
 // The least power of two that they are relative to.  What is below it by 2^-25 is below half
 // of the smallest step of the output for any q or v in range.
@@ -165,9 +170,10 @@ __device__ inline bool has_of(const fa_linear_args& a, int s) {
 // far on.
 //
 // Sorted (up to 64 sequences, a lane each): whole segments first, then what is left of each sequence, the
-// longest first, so that the work-groups that run longest do not start last (60 sequences of up to
-// 1,000 tokens, 16 heads, D = 128: 149 -> 110 us; 60 single tokens 23.5 -> 24.9, so not for short
-// ones).  Otherwise in packed order, by their places; the sequence is the last one whose first place
+// longest first, so that the work-groups that run longest do not start last (64 sequences of up to
+// 1,000 tokens, 16 heads, D = 128: 131 -> 108 us; up to 3,900, 8 heads, D = 256: 814 -> 567; 60 single
+// tokens 23.5 -> 24.9, so not for short ones; the 65th sequence costs such a batch what the order gives).
+// Otherwise in packed order, by their places; the sequence is the last one whose first place
 // is not past `index`, and a wave looks at 64 at a time.
 __device__ inline Run find_run(const fa_linear_args& a, int index) {
   Run run = {-1, 0, 0, 0, 0, true, -1, false};
@@ -327,7 +333,7 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
   // States alone go through the chunks from the last one back: what they read last is what the next
   // launch reads first.  They end where e^{a n} is 0 in fp32 (below 2^-149): what lies before adds zeros
   // (a third of the work at |a| = 0.1 and segments of 4,096: 131,001 tokens of 16 heads,
-  // D = 128: 702 -> 638 us).
+  // D = 128: 702 -> 638 us when it was made so).
   const float log2_decay = log_decay * kLog2e;
   int chunks = cdiv(n, kChunk);
   const int begin = run.start + (kStates ? (chunks - 1) * kChunk : 0);
@@ -956,8 +962,9 @@ __global__ __launch_bounds__(2 * D * kSplit, 2) void linear_kernel(const fa_line
 }
 
 // What every run but a sequence's last makes.  Without tiles of q three work-groups fit a CU at D = 128
-// (the first runs' outputs in the same launch leave two: 131,001 tokens of 16 heads 638 -> 710 us).  That
-// sequence: 190 us here, for the half of k and v that is not skipped, then 441 for the outputs, 4.9 TB/s.
+// (the first runs' outputs in the same launch leave two: 131,001 tokens of 16 heads 638 -> 710 us; not
+// measured for ragged batches, where first runs are half of the launch).  That sequence: 207 us here, for
+// the half of k and v that is not skipped, then 458 for the outputs, 4.7 TB/s.
 template <typename T, int D>
 __global__ __launch_bounds__(2 * D, 2) void states_kernel(const fa_linear_args a,
                                                           const Divisor h_kv) {
@@ -1012,9 +1019,10 @@ int runs_of(const fa_linear_args& a) {
 }
 
 // Runs of a sequence from which on their states are joined in a launch of their own, which takes 6 to 24
-// us; below, each run adds up what those before it made, 3 us a state at head dim 128, 13 at 256
-// (8 prompts of up to 2,048 tokens, 16 KV heads, in segments of 416: 299 us so, 190 joined; one of
-// 131,001 at 128 684 / 637, of 2,560 in five segments 58 both ways).
+// us; below, each run adds up what those before it made (one sequence of 16 heads, D = 128, in three
+// segments of 512 59.0 us so, 60.5 joined, in five 62.3 / 61.9, in seven 64.8 / 62.8, 131,001 tokens in
+// segments of 4,096 710 / 661; D = 256 in three 121 / 124, in four 128 / 126, 8 prompts of up to 2,048
+// in segments of 416 197 / 194).
 int join_runs(int d) { return d == 256 ? 3 : 5; }
 
 // Heads that a work-group attends at once: as many as the registers of two waves per SIMD keep the state
@@ -1026,10 +1034,12 @@ int heads_at_once(int group, int d) {
 
 // What a launch takes, in us, by segments of L tokens (0: whole sequences), from times of 12 shapes per
 // head dim (one sequence of 1,000 to 131,001 tokens, 3 to 40 of up to 8,000, groups of 1, 4 and 8), off by
-// a tenth on average; its choice is within 5% of the best of the powers of two in all but one (20,000, 8
-// heads, D = 256, where what gives every slot a segment is better still).  The longest run's chunks or a
-// slot's share of all, whichever is more; starts and ends of the work-groups; the segments' states; no
-// less than the bytes.
+// a tenth on average.  Of another 12 its choice is within 4% of the best of the powers of two in ten, 8% off
+// in three of 8,000, 64 heads of 8, D = 128, and 11% in 12 of 4,000, 16 of 4, D = 64; lengths that it does
+// not try can be better still (8 prompts at D = 256: 416 or 448 194 us, 480 182).
+//
+// The longest run's chunks or a slot's share of all, whichever is more; starts and ends of the
+// work-groups; the segments' states; no less than the bytes.
 struct Cost {
   float chunk_one;          // a chunk, groups of one head
   float item, chunk_group;  // heads at once, a chunk beside them

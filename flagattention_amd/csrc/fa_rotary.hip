@@ -8,8 +8,9 @@
 //
 // Bound by the rows, read and written once: 16,384 tokens of 64 heads and 8 of k and v, D = 128, into a
 // cache 131 us, 20,001 of 16 and 16, D = 256, 125 us, 5.1 and 5.3 TB/s (a large copy: 5.1); 8,192 of 32
-// and 8 35 to 39 us, 4.8 to 4.3.  A few tokens take 3 to 4.4 us, the launch and two trips to memory.  The turned k beside the cache is
-// k's rows once more (16,384 tokens of 64 heads and 8: 129 us without it, 135 with it, 244 by two calls).
+// and 8 35 to 39 us, 4.8 to 4.3.  A few tokens take 3 to 4.4 us, the launch and two trips to memory.  The
+// turned k beside the cache is k's rows once more (16,384 tokens of 64 heads and 8: 129 us without it, 135
+// with it, 244 by two calls).
 #include <algorithm>
 
 #include "fa_common.h"

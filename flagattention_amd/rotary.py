@@ -7,9 +7,10 @@ pair takes one axis, by the ``sections``.
 
 ``rotary_embedding`` turns q and k, for any of the attention operators here; ``rotary_cache_kv`` turns
 q and writes the turned k and v into the paged 16-bit cache that ``paged_attention`` reads (and returns
-the turned k for attention over a packed prompt).  Angles
-are worked out in 64 bits from the positions as they are, so there is no table and no last position.
-Forward only.
+the turned k for attention over a packed prompt).  Angles are worked out in 64 bits from
+the positions as they are, so there is no table and no last position; with frequencies up to 1 they are
+off by 2^-20 of a radian at most up to positions of 2^31, and twice as much for every doubling past
+that.  Forward only.
 
 Work is queued on the current stream; argument errors raise ``ArgumentError`` before any launch.
 """
@@ -160,8 +161,8 @@ def rotary_embedding(
                ``i % axes`` as long as that axis has its number, and axis 0 from there on
     adjacent_pairs
                pairs are dims 2i and 2i + 1 instead of i and i + R/2
-    inplace    write into q and k themselves (their rows must not overlap, nor the two each other: views of
-               one packed projection are fine)
+    inplace    write into q and k themselves (their rows must not overlap, nor the two each other, which
+               is refused: views of one packed projection are fine)
 
     Returns ``(q, k)``, turned.
     """
@@ -216,7 +217,7 @@ def rotary_cache_kv(
                   as in ``rotary_embedding``; v [T, H_kv, D]
     key_cache, value_cache
                   [num_blocks, H_kv, block_size, D] of q's type, as in ``paged_attention``; they share no
-                  memory with each other, nor with q, k and v
+                  element with each other (views of one pool are fine), and no memory with q, k and v
     slot_mapping  int32 / int64 [T]: block * block_size + row of each token; negative slots (padding
                   tokens) and slots past the cache are skipped.  The slots of one call must differ:
                   rows that two tokens write are undefined
