@@ -515,15 +515,16 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
   // States alone have their weights counted to the run's end instead, and are never brought up.
   int after = 0;
 
-  // fp16: a column's largest is at about 8 when it was last looked at: there is room for a growth by 2^12
-  // (past it an output is not finite, and the chunk is taken again) and a fall by 2^17 (counted below)
-  // before its copies lose bits.
+  // fp16: a column's largest is 2^7 to 2^12 when it was last looked at: there is room for a growth by 2^4
+  // (past it an output is not finite, and the chunk is taken again) and a fall by 2^kFall (counted below),
+  // before which 2^-32 of it or less is lost in its copies, and 2^-20 behind it.
+  constexpr int kFall = 12;
   int looked = -1;  // tokens since, -1: to be looked at behind this chunk
   float* const scales = shared.scales[kStates ? 0 : part_of] + 32 * wave;
   auto look = [&]() {
     const float most = most_of();
     // |s| 2^s_power is at most 2^128: both factors stay in range
-    const int by = most > 0.f ? max(power_of(most) - 3, -100 - s_power) : 0;
+    const int by = most > 0.f ? max(power_of(most) - 10, -100 - s_power) : 0;
     if (__ballot(by < -2 || by > 2) != 0ull) scale_down(by);  // uniform
     // A column of zeros is far below its first values, which have it looked at again.  (One that stays so,
     // as the dims that a head is padded by, costs nothing: 8,192 tokens of one head, 96 of D = 128 filled,
@@ -919,7 +920,7 @@ __device__ inline void walk(const fa_linear_args& a, const Run run, int hk,
     if (++chunk == chunks) break;
     if constexpr (kHalf && !kStates) {
       if (looked >= 0) looked += taken;
-      if (looked < 0 || !(log2_decay * static_cast<float>(looked) > -16.f)) look();  // uniform
+      if (looked < 0 || !(log2_decay * static_cast<float>(looked) > -kFall)) look();  // uniform
     }
   }
 

@@ -217,3 +217,26 @@ def test_states_of_many_single_tokens(a, dtype):
     err = (state[0, 0].double() - ref) / ref
     assert float(err.abs().max()) <= 6 / math.sqrt(3) * math.sqrt(n) * 2.0 ** -24
     assert abs(float(err.mean())) <= 8 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("h,d", [(1, 64), (4, 64), (1, 128), (2, 128), (1, 256)])
+@pytest.mark.parametrize("a", [-0.02, -0.1, -0.2, -0.6])
+def test_fp16_small_rows_of_a_state_that_falls(a, h, d):
+    """A state that only falls, q along rows that are 2^-10 of the others: a state's copy is off by 2^-11 of
+    itself, or by 2^-20 of the largest of its column (2^-25 of a unit, which that is 2^-5 of, at least)."""
+    need_gpu()
+    say(f"linear fp16 falling state a={a} h={h} d={d}")
+    n = min(400, int(40 / -a))
+    q = rows(n, h, d, torch.float16, 1)
+    q[..., ::2] = 0
+    k = v = torch.zeros((n, 1, d), dtype=torch.float16, device=DEV)
+    s0 = rows(1, d, d, torch.float32, 2)[0]
+    s0[1::2] *= 2.0 ** -10
+    decay = torch.full((1,), a, device=DEV)
+    fall = torch.exp(float(decay[0]) * (1 + torch.arange(n, device=DEV).double()))[:, None, None]
+    scale = 2.0 ** 10
+    o = prompt(q, k, v, decay, s0[None, None].clone(), scale, 0)
+    x = scale * q.double()
+    ref, size = x @ s0.double() * fall, x.abs() @ s0.double().abs() * fall
+    small = 2.0 ** -20 * x.abs().sum(-1, keepdim=True) * s0.double().abs().amax(0) * fall
+    assert_out(o, ref, size, n, small)
