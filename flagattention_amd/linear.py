@@ -135,7 +135,8 @@ def linear_attention_varlen(
     Returns ``o`` shaped and typed like ``q``.  States are float32 throughout.  Scores, and the copy of
     a state that meets q, are rounded to q's type for their products with v and q, so that an output is
     off by that beside its own rounding (in all 2.1e-3 of its size in bf16, 2.5e-4 to 2.9e-4 in fp16,
-    for 1.7e-3 and 2.1e-4); ``linear_attention_decode`` keeps both in float32.
+    for 1.7e-3 and 2.1e-4); ``linear_attention_decode`` keeps both in float32.  What a decay leaves below
+    2^-126, and in fp16 weighted values below 2^-39 of the largest of their 32 tokens and dim, count as 0.
 
     Rows of q that belong to no sequence get 0, a
     sequence without tokens leaves its slot as it is.  An infinity or a NaN in k or v makes the
